@@ -61,6 +61,14 @@ class DecoderScratch(ctypes.Structure):
         "gate_up_fused")]
 
 
+class KVPages(ctypes.Structure):
+    """The fields of a page pool's handle (include/kv_pages.h)."""
+
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "table", "len", "ref")] + [
+        (n, ctypes.c_int) for n in ("num_layers", "num_pages", "page_size", "kv_heads", "head_dim", "max_seqs",
+                                    "max_pages", "kv_dtype")]
+
+
 _F32P = ctypes.POINTER(ctypes.c_float)
 _VP = ctypes.c_void_p
 
@@ -137,6 +145,25 @@ _SIGNATURES = {
                                                            ctypes.c_int, ctypes.c_int, ctypes.c_float, ctypes.c_float,
                                                            _VP]),
     "attention_decode_append_gqa_sharded": (ctypes.c_int, [_VP, _VP, _VP, _VP, _VP, ctypes.c_int, ctypes.c_float]),
+    # include/kv_pages.h
+    "kv_pages_alloc": (_VP, [ctypes.c_int] * 8),
+    "kv_pages_attach": (_VP, [_VP] * 5 + [ctypes.c_int] * 8),
+    "kv_pages_release": (None, [_VP]),
+    "kv_pages_extend": (ctypes.c_int, [_VP, _VP, _VP, ctypes.c_int]),
+    "kv_pages_write": (ctypes.c_int, [_VP, ctypes.c_int, _VP, _VP, ctypes.c_int, ctypes.c_int, _VP, _VP, ctypes.c_int,
+                                      ctypes.c_longlong]),
+    "kv_pages_import": (ctypes.c_int, [_VP, ctypes.c_int, _VP]),
+    "kv_pages_fork": (ctypes.c_int, [_VP, _VP, _VP, ctypes.c_int]),
+    "kv_pages_copy": (ctypes.c_int, [_VP, _VP, _VP, ctypes.c_int]),
+    "kv_pages_free": (ctypes.c_int, [_VP, _VP, ctypes.c_int]),
+    "kv_pages_trim": (ctypes.c_int, [_VP, _VP, ctypes.c_int, ctypes.c_int, ctypes.c_int]),
+    "kv_pages_compact": (ctypes.c_int, [_VP, _VP]),
+    "attention_pages_prefix_gqa": (ctypes.c_int, [_VP, ctypes.c_longlong, _VP, ctypes.c_int, _VP, ctypes.c_int,
+                                                  ctypes.c_int, ctypes.c_int, ctypes.c_int, _VP, ctypes.c_int,
+                                                  ctypes.c_float]),
+    "attention_pages_window_gqa": (ctypes.c_int, [_VP, ctypes.c_longlong, _VP, ctypes.c_int, _VP, _VP, ctypes.c_int,
+                                                  ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int,
+                                                  ctypes.c_int, _VP, ctypes.c_int, ctypes.c_float]),
 }
 
 # The all-gather callback of attn_shard_init: (send, recv, bytes, user) -> 0 on success.
@@ -169,6 +196,11 @@ def cache_struct(handle) -> KVCache:
 def scratch_struct(handle) -> DecoderScratch:
     """The fields of a DecoderScratch handle from decoder_scratch_alloc."""
     return DecoderScratch.from_address(handle)
+
+
+def pages_struct(handle) -> KVPages:
+    """The fields of a KVPages handle from kv_pages_alloc or kv_pages_attach."""
+    return KVPages.from_address(handle)
 
 
 def last_error(lib) -> str:

@@ -23,6 +23,7 @@ enum { TYB_F32 = 0, TYB_BF16 = 1 };
 /* Bits of the device status word (tyb_status_fetch). */
 #define TYB_STATUS_WAIT_TIMEOUT 0x1u /* an mbarrier wait ran past its time limit */
 #define TYB_STATUS_BAD_ARGUMENT 0x2u /* a kernel found an index outside its buffers */
+#define TYB_STATUS_OUT_OF_PAGES 0x4u /* a page pool had too few free pages for a call */
 
 /* One sequence's K and V rows for ONE layer, head-first:
  * element (kv_head h, row r, dim d) at base + ((size_t)h * row_capacity + r) * 128 + d. */

@@ -1,0 +1,437 @@
+/*
+ * pages.c -- the paged KV cache and its attention (kv_pages.h): handles, argument checks and the
+ * workspace of the launches (pages.cu, pages_attn.cu, pages_attn_tc.cu).
+ *
+ * The reference's cache is one block per request (kernel/kv_cache.c:15-34) and is copied whole where
+ * two requests share a document; here requests name the same pages.  All of it is queued work on
+ * device memory: nothing here reads the device back.
+ */
+#include <cuda_runtime_api.h>
+#include <pthread.h>
+#include <stdlib.h>
+#include <string.h>
+
+#include "attn_ext.h"
+#include "host_internal.h"
+#include "kv_pages.h"
+#include "pages_shim.h"
+
+#define TYB_PAGES_MAGIC 0x54594250u /* "TYBP" */
+
+typedef struct {
+    KVPages pub; /* first: the KVPages* handed out converts back */
+    uint32_t magic;
+    int device;
+    int owned;
+} tyb_pages;
+
+/* ---- workspace ----------------------------------------------------------------------------
+ * One buffer per (device, stream), so that calls on different streams never share one; work on one
+ * stream uses it in turn.  Grown on demand (after waiting for the device), kept until exit. */
+#define TYB_PAGES_STREAMS 32
+static pthread_mutex_t g_lock = PTHREAD_MUTEX_INITIALIZER;
+static struct {
+    int used, device;
+    void *stream, *p;
+    size_t bytes;
+} g_ws[TYB_PAGES_STREAMS];
+static int g_next;
+
+static void *workspace(int device, size_t bytes, const char *what)
+{
+    void *st = tyb_stream(), *p = NULL;
+    int at = -1;
+    pthread_mutex_lock(&g_lock);
+    for (int i = 0; i < TYB_PAGES_STREAMS && at < 0; i++)
+        if (g_ws[i].used && g_ws[i].device == device && g_ws[i].stream == st) at = i;
+    if (at >= 0 && g_ws[at].bytes >= bytes) {
+        p = g_ws[at].p;
+    } else {
+        if (at < 0) { /* a slot of its own: a free one, else the one taken longest ago on this device */
+            for (int i = 0; i < TYB_PAGES_STREAMS && at < 0; i++)
+                if (!g_ws[i].used) at = i;
+            for (int i = 0; i < TYB_PAGES_STREAMS && at < 0; i++, g_next++)
+                if (g_ws[g_next % TYB_PAGES_STREAMS].device == device) at = g_next % TYB_PAGES_STREAMS;
+        }
+        if (at < 0) {
+            tyb_set_error("%s: workspaces of %d streams in use on other devices", what, TYB_PAGES_STREAMS);
+        } else {
+            if (g_ws[at].used) {
+                cudaDeviceSynchronize(); /* it may still be in use */
+                cudaFree(g_ws[at].p);
+                g_ws[at].used = 0;
+            }
+            size_t want = 1 << 20;
+            while (want < bytes) want += want / 2;
+            if (tyb_dev_alloc(&p, want, what)) {
+                g_ws[at].used = 1;
+                g_ws[at].device = device;
+                g_ws[at].stream = st;
+                g_ws[at].p = p;
+                g_ws[at].bytes = want;
+            }
+        }
+    }
+    pthread_mutex_unlock(&g_lock);
+    return p;
+}
+
+/* ---- handles ------------------------------------------------------------------------------- */
+
+/* The pool behind a KVPages*, with its device current; NULL (error set) otherwise. */
+static tyb_pages *pages_from(const KVPages *p, const char *what)
+{
+    tyb_pages *t = (tyb_pages *)p;
+    if (!p) {
+        tyb_set_error("%s: KVPages is NULL", what);
+        return NULL;
+    }
+    if (t->magic != TYB_PAGES_MAGIC) {
+        tyb_set_error("%s: KVPages was not made by kv_pages_alloc or kv_pages_attach", what);
+        return NULL;
+    }
+    int dev = -1;
+    if (!tyb_cuda_ok(cudaGetDevice(&dev), what)) return NULL;
+    if (dev != t->device) {
+        tyb_set_error("%s: the pool is on device %d, the current device is %d", what, t->device, dev);
+        return NULL;
+    }
+    return t;
+}
+
+/* Device memory, `align` bytes aligned; 1 when so. */
+static int on_device(const void *p, size_t align, const char *name, const char *what)
+{
+    if (!p) {
+        tyb_set_error("%s: NULL %s", what, name);
+        return 0;
+    }
+    if ((uintptr_t)p % align) {
+        tyb_set_error("%s: %s %p is not %zu-byte aligned", what, name, p, align);
+        return 0;
+    }
+    const int d = tyb_is_device_ptr(p);
+    if (d == 0) tyb_set_error("%s: %s is not device memory", what, name);
+    return d == 1;
+}
+
+static int check_dims(const KVPages *p, const char *what)
+{
+    const char *bad = NULL;
+    if (p->num_layers < 1) bad = "num_layers";
+    else if (p->num_pages < 1 || p->num_pages > 1 << 20) bad = "num_pages";
+    else if (p->page_size != 16 && p->page_size != 32 && p->page_size != 64 && p->page_size != 128) bad = "page_size";
+    else if (p->kv_heads < 1 || p->kv_heads > 1024) bad = "kv_heads";
+    else if (p->head_dim != 64 && p->head_dim != 128) bad = "head_dim";
+    else if (p->max_seqs < 1 || p->max_seqs > TYB_PAGES_MAX_SEQS) bad = "max_seqs";
+    else if (p->max_pages < 1 || p->max_pages > 1 << 20) bad = "max_pages";
+    else if (p->kv_dtype != ATTN_KV_F32 && p->kv_dtype != ATTN_KV_BF16) bad = "kv_dtype";
+    else if ((long long)p->num_layers * p->num_pages > (1LL << 31) / ((long long)p->kv_heads * p->page_size) - 1)
+        bad = "num_layers * num_pages * kv_heads * page_size";
+    if (bad) tyb_set_error("%s: %s is outside the supported range", what, bad);
+    return !bad;
+}
+
+static size_t slab_bytes(const KVPages *p)
+{
+    return (size_t)p->num_layers * p->num_pages * p->kv_heads * p->page_size * p->head_dim *
+           (p->kv_dtype == ATTN_KV_BF16 ? 2 : 4);
+}
+
+static tyb_pages *make(const KVPages *dims, int owned, const char *what)
+{
+    tyb_pages *t = (tyb_pages *)calloc(1, sizeof *t);
+    if (!t) {
+        tyb_set_error("%s: out of host memory", what);
+        return NULL;
+    }
+    t->pub = *dims;
+    t->magic = TYB_PAGES_MAGIC;
+    t->owned = owned;
+    if (!tyb_cuda_ok(cudaGetDevice(&t->device), what)) {
+        free(t);
+        return NULL;
+    }
+    if (tyb_status_mirror_setup() != 0) cudaGetLastError(); /* as in kv_cache_alloc_ex */
+    return t;
+}
+
+static void destroy(tyb_pages *t)
+{
+    if (t->owned) {
+        cudaFree(t->pub.k);
+        cudaFree(t->pub.v);
+        cudaFree(t->pub.table); /* table, len and ref are one allocation */
+    }
+    t->magic = 0;
+    free(t);
+}
+
+KVPages *kv_pages_alloc(int num_layers, int num_pages, int page_size, int kv_heads, int head_dim, int max_seqs,
+                        int max_pages, int kv_dtype)
+{
+    const char *what = "kv_pages_alloc";
+    const KVPages d = {NULL, NULL, NULL, NULL, NULL, num_layers, num_pages, page_size, kv_heads, head_dim, max_seqs,
+                       max_pages, kv_dtype};
+    if (!check_dims(&d, what)) return NULL;
+    tyb_pages *t = make(&d, 1, what);
+    if (!t) return NULL;
+    const size_t entries = (size_t)max_seqs * max_pages, ints = entries + max_seqs + num_pages;
+    int ok = tyb_dev_alloc(&t->pub.k, slab_bytes(&d), what) && tyb_dev_alloc(&t->pub.v, slab_bytes(&d), what) &&
+             tyb_dev_alloc((void **)&t->pub.table, ints * sizeof(int), what);
+    if (ok) {
+        t->pub.len = t->pub.table + entries;
+        t->pub.ref = t->pub.len + max_seqs;
+        ok = tyb_cuda_ok(cudaMemset(t->pub.table, 0xff, entries * sizeof(int)), what) &&
+             tyb_cuda_ok(cudaMemset(t->pub.len, 0, (ints - entries) * sizeof(int)), what) &&
+             tyb_cuda_ok(cudaDeviceSynchronize(), what); /* the pool may be used on any stream next */
+    }
+    if (!ok) {
+        destroy(t);
+        return NULL;
+    }
+    return &t->pub;
+}
+
+KVPages *kv_pages_attach(void *k, void *v, int *table, int *len, int *ref, int num_layers, int num_pages, int page_size,
+                         int kv_heads, int head_dim, int max_seqs, int max_pages, int kv_dtype)
+{
+    const char *what = "kv_pages_attach";
+    const KVPages d = {k, v, table, len, ref, num_layers, num_pages, page_size, kv_heads, head_dim, max_seqs, max_pages,
+                       kv_dtype};
+    if (!check_dims(&d, what) || !on_device(k, 16, "k", what) || !on_device(v, 16, "v", what) ||
+        !on_device(table, 4, "table", what) || !on_device(len, 4, "len", what) || !on_device(ref, 4, "ref", what))
+        return NULL;
+    tyb_pages *t = make(&d, 0, what);
+    return t ? &t->pub : NULL;
+}
+
+void kv_pages_release(KVPages *p)
+{
+    if (!p) return;
+    tyb_pages *t = pages_from(p, "kv_pages_release");
+    if (!t) return;
+    cudaStreamSynchronize((cudaStream_t)tyb_stream());
+    destroy(t);
+}
+
+/* ---- maintenance --------------------------------------------------------------------------- */
+
+/* A list of n device ints; 1 when there is one to work on, 0 when the call is done (*rc says how). */
+static int list_ready(const int *list, int n, const char *name, int *rc, const char *what)
+{
+    *rc = 1;
+    if (n < 0) {
+        tyb_set_error("%s: negative count %d", what, n);
+        return 0;
+    }
+    if (n == 0) {
+        *rc = 0;
+        return 0;
+    }
+    return on_device(list, 4, name, what);
+}
+
+static int launched(int err, const char *what)
+{
+    if (!tyb_cuda_ok(err, what)) return 1;
+    return 0;
+}
+
+int kv_pages_extend(KVPages *p, const int *seqs, const int *counts, int n)
+{
+    const char *what = "kv_pages_extend";
+    int rc;
+    tyb_pages *t = pages_from(p, what);
+    if (!t) return 1;
+    if (!list_ready(seqs, n, "seqs", &rc, what)) return rc;
+    if (!on_device(counts, 4, "counts", what)) return 1;
+    void *ws = workspace(t->device, tyb_pages_plan_bytes(p, n), what);
+    return ws ? launched(tyb_pages_extend_launch(p, seqs, counts, n, ws, tyb_stream()), what) : 1;
+}
+
+static int fork_or_copy(KVPages *p, const int *src, const int *dst, int n, int deep, const char *what)
+{
+    int rc;
+    tyb_pages *t = pages_from(p, what);
+    if (!t) return 1;
+    if (!list_ready(src, n, "src", &rc, what)) return rc;
+    if (!on_device(dst, 4, "dst", what)) return 1;
+    void *ws = workspace(t->device, tyb_pages_plan_bytes(p, n), what);
+    return ws ? launched(tyb_pages_fork_launch(p, src, dst, n, deep, ws, tyb_stream()), what) : 1;
+}
+
+int kv_pages_fork(KVPages *p, const int *src, const int *dst, int n) { return fork_or_copy(p, src, dst, n, 0, "kv_pages_fork"); }
+
+int kv_pages_copy(KVPages *p, const int *src, const int *dst, int n) { return fork_or_copy(p, src, dst, n, 1, "kv_pages_copy"); }
+
+int kv_pages_free(KVPages *p, const int *seqs, int n)
+{
+    const char *what = "kv_pages_free";
+    int rc;
+    if (!pages_from(p, what)) return 1;
+    if (!list_ready(seqs, n, "seqs", &rc, what)) return rc;
+    return launched(tyb_pages_free_launch(p, seqs, n, tyb_stream()), what);
+}
+
+int kv_pages_trim(KVPages *p, const int *seqs, int n, int window, int sinks)
+{
+    const char *what = "kv_pages_trim";
+    int rc;
+    if (!pages_from(p, what)) return 1;
+    if (window < 1 || sinks < 0) {
+        tyb_set_error("%s: window %d must be at least 1 and sinks %d not negative", what, window, sinks);
+        return 1;
+    }
+    if (!list_ready(seqs, n, "seqs", &rc, what)) return rc;
+    return launched(tyb_pages_trim_launch(p, seqs, n, window, sinks, tyb_stream()), what);
+}
+
+int kv_pages_compact(KVPages *p, int *live_out)
+{
+    const char *what = "kv_pages_compact";
+    tyb_pages *t = pages_from(p, what);
+    if (!t || (live_out && !on_device(live_out, 4, "live_out", what))) return 1;
+    void *ws = workspace(t->device, tyb_pages_plan_bytes(p, 0), what);
+    return ws ? launched(tyb_pages_compact_launch(p, live_out, ws, tyb_stream()), what) : 1;
+}
+
+static int check_layer(const KVPages *p, int layer, const char *what)
+{
+    if (layer >= 0 && layer < p->num_layers) return 1;
+    tyb_set_error("%s: layer %d out of range [0, %d)", what, layer, p->num_layers);
+    return 0;
+}
+
+/* Rows of `width` elements, `stride` apart, in dtype: 16-byte accesses have to fit. */
+static int check_rows(const void *x, int dtype, long long stride, long long width, const char *name, const char *what)
+{
+    if (dtype != ATTN_DT_F32 && dtype != ATTN_DT_BF16) {
+        tyb_set_error("%s: unknown element type %d", what, dtype);
+        return 0;
+    }
+    if (stride < width || stride % (dtype == ATTN_DT_BF16 ? 8 : 4)) {
+        tyb_set_error("%s: %s rows are %lld elements apart: at least %lld, and a multiple of 16 bytes, are wanted", what, name,
+                      stride, width);
+        return 0;
+    }
+    return on_device(x, 16, name, what);
+}
+
+int kv_pages_write(KVPages *p, int layer, const int *seqs, const int *starts, int n, int rows, const void *k_new,
+                   const void *v_new, int in_dtype, long long stride)
+{
+    const char *what = "kv_pages_write";
+    int rc;
+    if (!pages_from(p, what) || !check_layer(p, layer, what)) return 1;
+    if (rows < 0 || rows > 1 << 28) {
+        tyb_set_error("%s: rows %d out of range", what, rows);
+        return 1;
+    }
+    if (!list_ready(seqs, n, "seqs", &rc, what)) return rc;
+    if (rows == 0) return 0;
+    const long long width = (long long)p->kv_heads * p->head_dim;
+    if (!on_device(starts, 4, "starts", what) || !check_rows(k_new, in_dtype, stride, width, "k_new", what) ||
+        !check_rows(v_new, in_dtype, stride, width, "v_new", what))
+        return 1;
+    return launched(tyb_pages_write_launch(p, layer, seqs, starts, n, rows, k_new, v_new, in_dtype == ATTN_DT_BF16, stride,
+                                           tyb_stream()),
+                    what);
+}
+
+int kv_pages_import(KVPages *p, int seq, const KVCache *cache)
+{
+    const char *what = "kv_pages_import";
+    tyb_pages *t = pages_from(p, what);
+    if (!t) return 1;
+    tyb_cache *c = tyb_cache_from(cache);
+    if (!c) return 1;
+    if (p->num_layers != KV_NUM_LAYERS || p->kv_heads != KV_NUM_KV_HEADS || p->head_dim != KV_HEAD_DIM ||
+        p->kv_dtype != kv_cache_dtype(cache) || c->device != t->device) {
+        tyb_set_error("%s: the pool's layers, heads, element type and device have to be the cache's", what);
+        return 1;
+    }
+    if (seq < 0 || seq >= p->max_seqs) {
+        tyb_set_error("%s: sequence %d out of range [0, %d)", what, seq, p->max_seqs);
+        return 1;
+    }
+    const int rows = cache->seq_len;
+    if (rows < 0 || rows > cache->max_seq_len) {
+        tyb_set_error("%s: seq_len %d out of range [0, %d]", what, rows, cache->max_seq_len);
+        return 1;
+    }
+    for (int l = 0; l < KV_NUM_LAYERS; l++)
+        if (!tyb_flush_pending(c, l, what)) return 1;
+    if (rows == 0) return 0;
+    void *ws = workspace(t->device, tyb_pages_plan_bytes(p, 1), what);
+    if (!ws) return 1;
+    return launched(tyb_pages_import_launch(p, seq, c->k_slab, c->v_slab, cache->max_seq_len, rows, ws, tyb_stream()), what);
+}
+
+/* ---- attention ------------------------------------------------------------------------------ */
+
+static int attend(const KVPages *p, tyb_pages_attn *a, const char *what)
+{
+    tyb_pages *t = pages_from(p, what);
+    if (!t || !check_layer(p, a->layer, what)) return 1;
+    if (a->q_heads < 1 || a->q_heads % p->kv_heads || a->q_heads / p->kv_heads > TYB_PAGES_MAX_GROUP) {
+        tyb_set_error("%s: q_heads %d is not 1 .. %d times the %d KV heads", what, a->q_heads, TYB_PAGES_MAX_GROUP, p->kv_heads);
+        return 1;
+    }
+    if (a->batch < 0 || a->batch > 65535 || a->rows < 0 || a->rows > (1 << 30) / a->q_heads) {
+        tyb_set_error("%s: batch %d or rows %d out of range", what, a->batch, a->rows);
+        return 1;
+    }
+    if (a->max_new < 0 || a->max_len < 0 || a->window < 0 || a->sinks < 0) {
+        tyb_set_error("%s: negative max_new, max_len, window or sinks", what);
+        return 1;
+    }
+    if (a->batch == 0 || a->rows == 0) return 0;
+    if (!check_rows(a->q, a->io_bf16 ? ATTN_DT_BF16 : ATTN_DT_F32, a->q_stride, (long long)a->q_heads * p->head_dim, "q", what) ||
+        !on_device(a->out, 16, "output", what) || !on_device(a->seqs, 4, "seqs", what))
+        return 1;
+    a->p = *p;
+    const size_t bytes = tyb_pages_attn_bytes(a);
+    void *ws = bytes ? workspace(t->device, bytes, what) : NULL;
+    if (bytes && !ws) return 1;
+    return launched(tyb_pages_attn_launch(a, ws, tyb_stream()), what);
+}
+
+static int io_type(int io_dtype, const char *what)
+{
+    if (io_dtype == ATTN_DT_F32 || io_dtype == ATTN_DT_BF16) return 1;
+    tyb_set_error("%s: unknown element type %d", what, io_dtype);
+    return 0;
+}
+
+int attention_pages_prefix_gqa(const void *q, long long q_stride, const KVPages *p, int layer, const int *seqs, int batch,
+                               int q_heads, int prefix_len, int max_len, void *output, int io_dtype, float scale)
+{
+    const char *what = "attention_pages_prefix_gqa";
+    if (!io_type(io_dtype, what)) return 1;
+    if (prefix_len < 0 || prefix_len > max_len) {
+        tyb_set_error("%s: prefix_len %d out of range [0, max_len = %d]", what, prefix_len, max_len);
+        return 1;
+    }
+    tyb_pages_attn a = {.layer = layer, .q = q, .q_stride = q_stride, .out = output, .io_bf16 = io_dtype == ATTN_DT_BF16,
+                        .q_heads = q_heads, .seqs = seqs, .batch = batch, .rows = batch, .max_new = 1, .max_len = max_len,
+                        .scale = scale};
+    /* The shared pass takes whole pages: each sequence has its own copy of a partly filled one. */
+    if (pages_from(p, what)) a.prefix = prefix_len / p->page_size * p->page_size;
+    if (batch == 1) a.prefix = 0; /* nothing to share */
+    return attend(p, &a, what);
+}
+
+int attention_pages_window_gqa(const void *q, long long q_stride, const KVPages *p, int layer, const int *seqs,
+                               const int *starts, int batch, int rows, int q_heads, int max_new, int max_len, int window,
+                               int sinks, void *output, int io_dtype, float scale)
+{
+    const char *what = "attention_pages_window_gqa";
+    if (!io_type(io_dtype, what)) return 1;
+    const int tokens = max_new == 1 && rows == batch;
+    if (!tokens && batch > 0 && rows > 0 && !on_device(starts, 4, "starts", what)) return 1;
+    tyb_pages_attn a = {.layer = layer, .q = q, .q_stride = q_stride, .out = output, .io_bf16 = io_dtype == ATTN_DT_BF16,
+                        .q_heads = q_heads, .seqs = seqs, .starts = starts, .batch = batch, .rows = rows,
+                        .max_new = max_new, .max_len = max_len, .window = window, .sinks = sinks, .scale = scale};
+    return attend(p, &a, what);
+}

@@ -1,0 +1,101 @@
+// pages_attn.cuh -- what the attention kernels over the paged cache share: the visibility of a query
+// row, the list of key tiles a set of rows can see, and the layout of the split records.
+#pragma once
+
+#include "common.cuh"
+#include "pages_shim.h"
+
+namespace tyb {
+
+struct Status {
+    unsigned int* word;
+    unsigned int* mirror;
+};
+
+__device__ __forceinline__ void raise(const Status& s, unsigned int bits)
+{
+    atomicOr(s.word, bits);
+    flag_mirror(s.mirror);
+}
+
+// A query row at position `pos` sees key j when j <= pos and (j >= lo or j < sinks).  The four uses:
+//   prefix      pos = P - 1,   lo = 0
+//   own rows    pos = len - 1, lo = P
+//   window      pos = its position, lo = max(0, pos - window + 1)
+//   causal      the same with lo = 0
+// A row that is not there has pos = -1: it sees nothing.
+
+// The key tiles (of `kt` rows) that rows with positions up to pos_max and lower bounds from lo_min
+// on can see: [0, na) for the sinks, then [b0, b0 + nb).
+struct Tiles {
+    int na, b0, nb;
+    __device__ __forceinline__ int count() const { return na + nb; }
+    __device__ __forceinline__ int at(int i) const { return i < na ? i : b0 + i - na; }
+};
+
+__device__ __forceinline__ Tiles tiles_of(int pos_max, int lo_min, int sinks, int kt)
+{
+    Tiles t;
+    pos_max = max(pos_max, -1);
+    const int end = (pos_max + kt) / kt;  // tiles up to pos_max
+    t.na = (min(sinks, pos_max + 1) + kt - 1) / kt;
+    t.b0 = max(lo_min / kt, t.na);
+    t.nb = max(0, end - t.b0);
+    return t;
+}
+
+// Split record s of output row R (= token * q_heads + head): the unnormalised output in FP32 at
+// o[(s * rows + R) * D], the running maximum (base-2 exponent) and sum at ml[s * rows + R].
+struct Records {
+    float* o;
+    float2* ml;
+    int rows;
+    int slots;
+};
+
+// Length of sequence s as the kernels may use it: within its table, 0 when s is no sequence.
+__device__ __forceinline__ int checked_len(const KVPages& p, int s, const Status& st)
+{
+    if (s < 0 || s >= p.max_seqs) {
+        raise(st, TYB_STATUS_BAD_ARGUMENT);
+        return 0;
+    }
+    const int len = p.len[s];
+    if (len < 0 || len > p.max_pages * p.page_size) {
+        raise(st, TYB_STATUS_BAD_ARGUMENT);
+        return 0;
+    }
+    return len;
+}
+
+struct AttnArgs {
+    KVPages p;
+    const void* k;  // the layer's pages
+    const void* v;
+    const void* q;
+    long long q_stride;
+    void* out;
+    int io_bf16;
+    int q_heads, group;
+    const int* seqs;
+    const int* starts;
+    int batch, rows;
+    int prefix;      // leading rows left to (or handled by) the shared pass
+    int window, sinks;
+    float scale_log2;
+    int splits, slot0;  // this launch's splits, and the record slot of its first
+    Records rec;        // slots == 1: the output is written directly
+    Status st;
+};
+
+// log2 of the page size (16 .. 128)
+__device__ __forceinline__ int page_shift(int page_size) { return __ffs(page_size) - 1; }
+
+__device__ __forceinline__ float fast_exp2(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+}  // namespace tyb

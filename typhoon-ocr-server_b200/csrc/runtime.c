@@ -305,9 +305,10 @@ int tyb_finish(void *stream, const char *what)
     if (!tyb_cuda_ok(e, what)) return 0;
     if (g_last_write.stream == stream) g_last_write.valid = 0; /* everything queued is done */
     if (bits) {
-        tyb_set_error("%s: device status 0x%x (%s%s)", what, bits,
+        tyb_set_error("%s: device status 0x%x (%s%s%s)", what, bits,
                       (bits & TYB_STATUS_WAIT_TIMEOUT) ? "wait timed out " : "",
-                      (bits & TYB_STATUS_BAD_ARGUMENT) ? "index check failed" : "");
+                      (bits & TYB_STATUS_BAD_ARGUMENT) ? "index check failed " : "",
+                      (bits & TYB_STATUS_OUT_OF_PAGES) ? "out of pages" : "");
         return 0;
     }
     return 1;
