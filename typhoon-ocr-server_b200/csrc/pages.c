@@ -23,6 +23,7 @@ typedef struct {
     uint32_t magic;
     int device;
     int owned;
+    _Alignas(64) unsigned char maps[TYB_PAGES_MAPS_BYTES];
 } tyb_pages;
 
 /* ---- workspace ----------------------------------------------------------------------------
@@ -140,11 +141,12 @@ static size_t slab_bytes(const KVPages *p)
 
 static tyb_pages *make(const KVPages *dims, int owned, const char *what)
 {
-    tyb_pages *t = (tyb_pages *)calloc(1, sizeof *t);
+    tyb_pages *t = (tyb_pages *)aligned_alloc(64, sizeof *t); /* the maps' alignment */
     if (!t) {
         tyb_set_error("%s: out of host memory", what);
         return NULL;
     }
+    memset(t, 0, sizeof *t);
     t->pub = *dims;
     t->magic = TYB_PAGES_MAGIC;
     t->owned = owned;
@@ -184,7 +186,8 @@ KVPages *kv_pages_alloc(int num_layers, int num_pages, int page_size, int kv_hea
         t->pub.ref = t->pub.len + max_seqs;
         ok = tyb_cuda_ok(cudaMemset(t->pub.table, 0xff, entries * sizeof(int)), what) &&
              tyb_cuda_ok(cudaMemset(t->pub.len, 0, (ints - entries) * sizeof(int)), what) &&
-             tyb_cuda_ok(cudaDeviceSynchronize(), what); /* the pool may be used on any stream next */
+             tyb_cuda_ok(cudaDeviceSynchronize(), what) && /* the pool may be used on any stream next */
+             tyb_cuda_ok(tyb_pages_maps(&t->pub, t->maps), what);
     }
     if (!ok) {
         destroy(t);
@@ -203,6 +206,10 @@ KVPages *kv_pages_attach(void *k, void *v, int *table, int *len, int *ref, int n
         !on_device(table, 4, "table", what) || !on_device(len, 4, "len", what) || !on_device(ref, 4, "ref", what))
         return NULL;
     tyb_pages *t = make(&d, 0, what);
+    if (t && !tyb_cuda_ok(tyb_pages_maps(&t->pub, t->maps), what)) {
+        destroy(t);
+        t = NULL;
+    }
     return t ? &t->pub : NULL;
 }
 
@@ -391,6 +398,7 @@ static int attend(const KVPages *p, tyb_pages_attn *a, const char *what)
         !on_device(a->out, 16, "output", what) || !on_device(a->seqs, 4, "seqs", what))
         return 1;
     a->p = *p;
+    a->maps = t->maps;
     const size_t bytes = tyb_pages_attn_bytes(a);
     void *ws = bytes ? workspace(t->device, bytes, what) : NULL;
     if (bytes && !ws) return 1;

@@ -634,9 +634,11 @@ constexpr int kSms = 148;
 
 // How a call is laid out: its row tiles and splits.
 struct Layout {
-    bool tokens;     // the token kernel handles (all or the own rows of) the call
-    bool shared;     // the rows kernel handles a shared prefix
-    int token_splits, row_tiles, row_splits, slots;
+    bool tokens;  // the token kernel handles (all or the own rows of) the call
+    bool shared;  // the row tiles are the shared pass over a prefix
+    bool tc;      // the row tiles run on the tcgen05 form
+    bool tall;
+    int token_splits, row_tiles, row_splits, row_slots, slots;
 };
 
 static int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
@@ -657,15 +659,26 @@ static Layout layout_of(const tyb_pages_attn* c)
         l.token_splits = s < 1 ? 1 : s;
     }
     if (!l.tokens || l.shared) {
-        const int per = kRowsCta / group;
-        l.row_tiles = l.shared ? ceil_div(c->batch, per) : ceil_div(c->rows, per) + c->batch;
+        l.tc = c->p.kv_dtype == TYB_BF16;
+        l.tall = l.tc && (long long)(l.shared ? c->batch : c->max_new) * group <= kTcTall;
+        const int per = (l.tall ? kTcTall : l.tc ? kTcWide : kRowsCta) / group;
+        // Each of the sequences of a call ends in a tile of its own; no list has more tiles than this.
+        l.row_tiles = l.shared ? ceil_div(c->batch, per) : (int)((c->rows + (long long)c->batch * (per - 1)) / per);
         const long long keys = l.shared ? c->prefix : c->window && c->window < c->max_len ? c->window + c->sinks : c->max_len;
-        const int tiles = ceil_div(keys, kt);
-        int s = ceil_div(3LL * kSms, (long long)l.row_tiles * c->p.kv_heads);
-        if (s > ceil_div(tiles, 8)) s = ceil_div(tiles, 8);
+        const int tiles = ceil_div(keys, l.tc ? 128 : kt);
+        const long long ctas = (long long)l.row_tiles * c->p.kv_heads;
+        int s;
+        if (l.tc) {
+            s = (int)(kSms / ctas);  // one CTA fits an SM; a split has at least two tiles
+            if (s > tiles / 2) s = tiles / 2;
+        } else {
+            s = ceil_div(3LL * kSms, ctas);
+            if (s > ceil_div(tiles, 8)) s = ceil_div(tiles, 8);
+        }
         l.row_splits = s < 1 ? 1 : s;
     }
-    l.slots = l.token_splits + l.row_splits;
+    l.row_slots = l.row_splits * (l.tall ? 2 : 1);
+    l.slots = l.token_splits + l.row_slots;
     return l;
 }
 
@@ -726,7 +739,7 @@ static int launch(const tyb_pages_attn* c, void* ws, cudaStream_t stream)
     }
     if (l.tokens) {
         a.splits = l.token_splits;
-        a.slot0 = l.row_splits;
+        a.slot0 = l.row_slots;
         pages_token_kernel<T, D><<<dim3(l.token_splits, c->p.kv_heads, c->batch), kThreads, solo, stream>>>(a);
         if ((e = cudaGetLastError()) != cudaSuccess) return (int)e;
     }
@@ -734,7 +747,10 @@ static int launch(const tyb_pages_attn* c, void* ws, cudaStream_t stream)
         a.splits = l.row_splits;
         a.slot0 = 0;
         const dim3 grid(l.row_tiles, c->p.kv_heads, l.row_splits);
-        if (l.shared) pages_rows_kernel<T, D, true><<<grid, kThreads, rows, stream>>>(a);
+        if (l.tc) {
+            const int rc = tc_launch(a, c->layer, l.tall, l.shared, l.row_tiles, c->maps, stream);
+            if (rc) return rc;
+        } else if (l.shared) pages_rows_kernel<T, D, true><<<grid, kThreads, rows, stream>>>(a);
         else pages_rows_kernel<T, D, false><<<grid, kThreads, rows, stream>>>(a);
         if ((e = cudaGetLastError()) != cudaSuccess) return (int)e;
     }

@@ -88,6 +88,11 @@ struct AttnArgs {
     Status st;
 };
 
+// The tcgen05 form (pages_attn_tc.cu) for the query rows of a BF16 pool, `items` row tiles: tall, of at
+// most 128 rows each, with two record slots a split; else of 256 rows.
+constexpr int kTcTall = 128, kTcWide = 256;
+int tc_launch(const AttnArgs& a, int layer, bool tall, bool shared_pass, int items, const void* maps, cudaStream_t stream);
+
 // log2 of the page size (16 .. 128)
 __device__ __forceinline__ int page_shift(int page_size) { return __ffs(page_size) - 1; }
 

@@ -1,0 +1,605 @@
+// pages_attn_tc.cu -- attention of many query rows over the paged BF16 cache on the 5th-generation
+// tensor cores (tcgen05 + TMEM): prompt chunks through a window with sinks, and the shared prefix of a
+// decode batch.
+//
+// A CTA has query rows of one KV head (its q_heads / kv_heads query heads folded into the rows, so
+// that one K/V tile feeds them all) and a run of key tiles of 128.  Two streams of 128 rows alternate
+// on the tensor core, one's softmax overlapping the other's products:
+//   wide   256 rows, both streams take every tile (each K/V tile is loaded once for 256 rows);
+//   tall   at most 128 rows: the streams have the same rows and take the tiles in turn, and their
+//          results are joined like those of two splits.  Half the tensor work of a wide item that
+//          would be half empty, and twice the streams' tiles in flight.
+// A tile comes page by page: one TMA tensor copy per page and 64 columns, the 128-byte-swizzled
+// layout building up in shared memory as if it were one copy; the pages of a tile are issued by as
+// many lanes of the producer warp.  Rows of the tile that no row of the item sees (behind the
+// sequence's end, a page that is not there, before the window) may hold anything: their scores are
+// masked, and their V rows are cleared in shared memory before P.V, since 0 * NaN is not 0.
+//
+// Roles (12 warps): 0-3 and 4-7 the streams' softmax (one row per thread), 8 issues the MMAs, 9 the
+// copies, 10 clears V rows.  TMEM: S (128 columns, the streams in turn) | P0 | P1 (64 each) | O0 | O1.
+// Every wait is bounded; a CTA whose wait ran out raises the status word, leaves its loops, frees its
+// TMEM and returns.
+#define TYB_WHOLE_PROGRAM
+#include "pages_attn.cuh"
+#include "tcgen05.cuh"
+
+namespace tyb {
+
+constexpr int kRows = 128;   // rows of a stream (tensor-core M)
+constexpr int kKeys = 128;   // keys of a tile
+constexpr int kSoftThreads = 256;
+constexpr int kTcThreads = kSoftThreads + 128;
+// Register split, as in the fused prefill: launched at kLaunchRegs, the issue warpgroup drops to
+// kIssueRegs and the softmax warpgroups rise to kSoftRegs; the shares fit the launch's registers.
+constexpr int kLaunchRegs = 168, kIssueRegs = 112, kSoftRegs = 192;
+static_assert(kSoftThreads * kSoftRegs + 128 * kIssueRegs <= kTcThreads * kLaunchRegs, "register split");
+static_assert(2 * kSoftRegs + kIssueRegs <= 512, "register split of a sub-partition");
+constexpr int kBox = kTcBox;  // 128 rows x 64 columns of BF16
+constexpr int kStages = 2;
+constexpr int kSeen = 8;  // ring of page masks, one per tile: more than the tiles in flight
+
+struct TcArgs {
+    AttnArgs a;
+    int layer;
+    int tall;        // the streams share their rows
+    int shared_pass; // the rows are the batch's single tokens against the first sequence's leading rows
+    unsigned long long wait_ns;
+};
+
+template <int D>
+struct Smem {
+    static constexpr int kTile = (D / 64) * kBox;
+    static constexpr int kQ = 0, kK = 2 * kTile, kV = kK + kStages * kTile, kBars = kV + kStages * kTile;
+    static constexpr size_t kBytes = (size_t)kBars + 512 + 1024;  // + barriers + alignment slack
+};
+
+// Instruction descriptor, kind::f16: BF16 operands, FP32 accumulator, M = 128.
+__host__ __device__ constexpr uint32_t idesc(int n, bool b_mn_major)
+{
+    return (1u << 4) | (1u << 7) | (1u << 10) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
+}
+
+__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int c0, int c1, uint64_t* bar)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(smem_u32(bar))
+        : "memory");
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c)
+{
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+// Columns [0, n) of 32, n clamped.
+__device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
+
+// Which of a tile's columns a row sees, 32 per word.
+struct Mask {
+    uint32_t w[4];
+};
+
+template <bool kMask>
+__device__ __forceinline__ float row_max(const float (&s)[kKeys], const Mask& mk)
+{
+    float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (int c = 0; c < kKeys; c += 2) {
+        const float a = (!kMask || (mk.w[c >> 5] >> (c & 31) & 1u)) ? s[c] : -INFINITY;
+        const float b = (!kMask || (mk.w[c >> 5] >> ((c + 1) & 31) & 1u)) ? s[c + 1] : -INFINITY;
+        m[(c >> 1) & 3] = max3(m[(c >> 1) & 3], a, b);
+    }
+    return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+}
+
+// p = exp2(s * scale + neg) on the visible columns (0 on the others) as BF16 pairs into the row's TMEM
+// columns at p_addr; returns the FP32 sum.  kTrack: *top receives the largest exponent.
+template <bool kMask, bool kTrack>
+__device__ __forceinline__ float row_exp(const float (&s)[kKeys], const Mask& mk, float scale, float neg, uint32_t p_addr, float* top)
+{
+    const float2 sc = make_float2(scale, scale), nm = make_float2(neg, neg);
+    float2 acc0 = make_float2(0.f, 0.f), acc1 = make_float2(0.f, 0.f);
+    float t0 = -INFINITY, t1 = -INFINITY;
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+        uint32_t pk[16];
+#pragma unroll
+        for (int c = 0; c < 32; c += 4) {
+            const int k = q * 32 + c;
+            float2 x0 = __ffma2_rn(make_float2(s[k], s[k + 1]), sc, nm);
+            float2 x1 = __ffma2_rn(make_float2(s[k + 2], s[k + 3]), sc, nm);
+            if (kMask) {
+                if (!(mk.w[q] >> c & 1u)) x0.x = -INFINITY;
+                if (!(mk.w[q] >> (c + 1) & 1u)) x0.y = -INFINITY;
+                if (!(mk.w[q] >> (c + 2) & 1u)) x1.x = -INFINITY;
+                if (!(mk.w[q] >> (c + 3) & 1u)) x1.y = -INFINITY;
+            }
+            if (kTrack) {
+                t0 = max3(t0, x0.x, x0.y);
+                t1 = max3(t1, x1.x, x1.y);
+            }
+            const float2 e0 = make_float2(pt_exp2(x0.x), pt_exp2(x0.y)), e1 = make_float2(pt_exp2(x1.x), pt_exp2(x1.y));
+            acc0 = __fadd2_rn(acc0, e0);
+            acc1 = __fadd2_rn(acc1, e1);
+            pk[c / 2] = pack_bf16x2(e0.x, e0.y);
+            pk[c / 2 + 1] = pack_bf16x2(e1.x, e1.y);
+        }
+        tmem_st16u(p_addr + q * 16, pk);
+    }
+    tmem_wait_st();
+    if (kTrack) *top = fmaxf(t0, t1);
+    return (acc0.x + acc0.y) + (acc1.x + acc1.y);
+}
+
+template <int D>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    pages_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const TcArgs ta)
+{
+    using S = Smem<D>;
+    const AttnArgs& a = ta.a;
+    extern __shared__ __align__(1024) unsigned char raw[];
+    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+    unsigned char *sQ = smem + S::kQ, *sK = smem + S::kK, *sV = smem + S::kV;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBars);
+    uint64_t *k_full = bars, *k_free = bars + 2, *v_full = bars + 4, *v_free = bars + 6, *s_full = bars + 8, *s_free = bars + 10,
+             *p_full = bars + 12, *pv_done = bars + 14, *v_clear = bars + 16, *q_full = bars + 18, *drain = bars + 19;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 20);
+    int* found = reinterpret_cast<int*>(bars + 21);                      // [4]
+    volatile uint32_t* present = reinterpret_cast<uint32_t*>(bars + 23);  // [kSeen] a bit per 16 rows of the tile
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int kvh = blockIdx.y, split = blockIdx.z;
+    const int rows_item = ta.tall ? kRows : 2 * kRows;
+    const int per = rows_item / a.group;  // tokens of an item
+
+    // Which tokens: item x of the batch (the last items, with the most keys to see, first).
+    if (warp == 0 && !ta.shared_pass) {
+        const int x = (int)(gridDim.x - 1 - blockIdx.x);
+        int before = 0;
+        if (lane == 0) found[0] = -1;
+        __syncwarp();
+        for (int base = 0; base < a.batch && before <= x; base += 32) {
+            const int b = base + lane;
+            const int q0 = b < a.batch ? a.starts[b] : 0, q1 = b < a.batch ? a.starts[b + 1] : 0;
+            const int cnt = q1 > q0 ? (q1 - q0 + per - 1) / per : 0;
+            int sum = cnt;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= o) sum += y;
+            }
+            const int lo = before + sum - cnt;
+            if (x >= lo && x < lo + cnt) {
+                if (q0 < 0 || q1 > a.rows) {
+                    raise(a.st, TYB_STATUS_BAD_ARGUMENT);
+                } else {
+                    found[0] = b;
+                    found[1] = q0 + (x - lo) * per;
+                    found[2] = min(per, q1 - q0 - (x - lo) * per);
+                    found[3] = (x - lo) * per - (q1 - q0);
+                }
+            }
+            before += __shfl_sync(0xffffffffu, sum, 31);
+        }
+    }
+    if (warp == 8) {
+        if (lane == 0) {
+            for (int i = 0; i < 2; i++) {
+                mbar_init(&k_full[i], 1);
+                mbar_init(&k_free[i], 1);
+                mbar_init(&v_full[i], 1);
+                mbar_init(&v_free[i], 1);
+                mbar_init(&v_clear[i], 32);
+                mbar_init(&s_full[i], 1);
+                mbar_init(&s_free[i], kRows);
+                mbar_init(&p_full[i], kRows);
+                mbar_init(&pv_done[i], 1);
+            }
+            mbar_init(q_full, kSoftThreads);
+            mbar_init(drain, 1);
+            fence_barrier_init();
+            fence_proxy_async_smem();
+        }
+        __syncwarp();
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        tc_fence_before();
+    }
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    int seq = -1, tok0 = 0, ntok = 0, pos0 = -1;
+    if (ta.shared_pass) {
+        tok0 = (int)blockIdx.x * per;
+        ntok = min(per, a.batch - tok0);
+        seq = a.seqs[0];
+        pos0 = min(a.prefix, checked_len(a.p, seq, a.st)) - 1;
+    } else if (found[0] >= 0) {
+        seq = a.seqs[found[0]];
+        tok0 = found[1];
+        ntok = found[2];
+        pos0 = checked_len(a.p, seq, a.st) + found[3];
+        if (pos0 < 0 && tid == 0) raise(a.st, TYB_STATUS_BAD_ARGUMENT);  // more queries than tokens
+    }
+    const int sinks = ta.shared_pass ? 0 : a.sinks;
+    const bool windowed = !ta.shared_pass && a.window;
+    const int pos_max = ta.shared_pass ? pos0 : pos0 + ntok - 1;
+    const int lo_min = windowed ? max(0, pos0 - a.window + 1) : 0, lo_max = windowed ? max(0, pos_max - a.window + 1) : 0;
+    const Tiles tiles = tiles_of(ntok > 0 ? pos_max : -1, lo_min, sinks, kKeys);
+    const int all = tiles.count();
+    const int first = (int)((long long)all * split / a.splits), nt = (int)((long long)all * (split + 1) / a.splits) - first;
+    const int steps = ta.tall ? nt : 2 * nt;  // softmax steps of both streams; step i: stream i & 1
+    // Whether some row of the item does not see the whole tile (its pages aside), and whether the tile
+    // has rows that none sees.
+    auto edge = [&](int k0) { return k0 + kKeys - 1 > pos0 || (k0 < lo_max && k0 + kKeys > sinks); };
+    auto loose = [&](int k0) { return k0 + kKeys - 1 > pos_max || (k0 < lo_min && k0 + kKeys > sinks); };
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+        return mbar_wait_bounded_to(bar, parity & 1u, ta.wait_ns, TYB_STATUS_WAIT_TIMEOUT, a.st.word, a.st.mirror);
+    };
+
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
+        if (warp == 9) {
+            // ---- copies: lane l < pages of a tile has page l
+            const int ps = a.p.page_size, shift = page_shift(ps), per_tile = kKeys >> shift;
+            const int* table = a.p.table + (size_t)max(0, min(seq, a.p.max_seqs - 1)) * a.p.max_pages;
+            const uint32_t all_seen = 0xffu, page_bits = (1u << (ps / 16)) - 1u;
+            const int page_bytes = ps * 128;  // of a 64-column box
+            bool ok = true;
+            int k_sent = 0, v_sent = 0;  // tiles requested
+            for (int t = 0; t < nt && ok; t++) {
+                const int st = t & 1, entry = (tiles.at(first + t) * kKeys >> shift) + lane;
+                int page = -1;
+                if (lane < per_tile && entry <= pos_max >> shift) {
+                    page = table[entry];
+                    if (page >= a.p.num_pages) {
+                        raise(a.st, TYB_STATUS_BAD_ARGUMENT);
+                        page = -1;
+                    }
+                }
+                const uint32_t have = __ballot_sync(0xffffffffu, page >= 0);
+                const int row = page < 0 ? 0 : ((ta.layer * a.p.num_pages + page) * a.p.kv_heads + kvh) * ps;
+                const uint32_t bytes = (uint32_t)__popc(have) * (uint32_t)(page_bytes * (D / 64));
+                if (t >= kStages) ok = wait(&k_free[st], (uint32_t)((t - kStages) >> 1));
+                if (__any_sync(0xffffffffu, !ok)) break;
+                if (lane == 0) {
+                    uint32_t seen = 0;
+                    for (int l = 0; l < per_tile; l++)
+                        if (have >> l & 1u) seen |= page_bits << (l * (ps / 16));
+                    present[t & (kSeen - 1)] = seen & all_seen;
+                    mbar_arrive_expect_tx(&k_full[st], bytes);
+                }
+                __syncwarp();
+                if (page >= 0)
+#pragma unroll
+                    for (int c = 0; c < D / 64; c++)
+                        tma_load_2d(sK + st * S::kTile + c * kBox + lane * page_bytes, &map_k, 64 * c, row, &k_full[st]);
+                k_sent = t + 1;
+                if (t >= kStages) ok = wait(&v_free[st], (uint32_t)((t - kStages) >> 1));
+                if (__any_sync(0xffffffffu, !ok)) break;
+                if (lane == 0) mbar_arrive_expect_tx(&v_full[st], bytes);
+                __syncwarp();
+                if (page >= 0)
+#pragma unroll
+                    for (int c = 0; c < D / 64; c++)
+                        tma_load_2d(sV + st * S::kTile + c * kBox + lane * page_bytes, &map_v, 64 * c, row, &v_full[st]);
+                v_sent = t + 1;
+            }
+            if (__any_sync(0xffffffffu, !ok)) {  // a wait ran out: the copies requested still land in this CTA
+                for (int t = max(0, k_sent - kStages); t < k_sent; t++) wait(&k_full[t & 1], (uint32_t)(t >> 1));
+                for (int t = max(0, v_sent - kStages); t < v_sent; t++) wait(&v_full[t & 1], (uint32_t)(t >> 1));
+            }
+        } else if (warp == 8) {
+            // ---- MMA issue (one thread): QK runs two steps ahead of P.V
+            if (lane == 0 && steps > 0) {
+                const uint64_t dq[2] = {umma_desc(smem_u32(sQ), 16), umma_desc(smem_u32(sQ) + (ta.tall ? 0 : S::kTile), 16)};
+                const uint64_t dk[2] = {umma_desc(smem_u32(sK), 16), umma_desc(smem_u32(sK) + S::kTile, 16)};
+                const uint64_t dv[2] = {umma_desc(smem_u32(sV), kBox), umma_desc(smem_u32(sV) + S::kTile, kBox)};
+                auto tile = [&](int i) { return ta.tall ? i : i >> 1; };
+                auto last_use = [&](int i) { return ta.tall || (i & 1); };
+                auto qk = [&](int i) {
+                    const int h = i & 1, t = tile(i), st = t & 1;
+#pragma unroll
+                    for (int kk = 0; kk < D / 16; kk++) {
+                        const uint32_t off = ((kk >> 2) * kBox + (kk & 3) * 32) >> 4;
+                        tc_mma(tmem, (h ? dq[1] : dq[0]) + off, (st ? dk[1] : dk[0]) + off, idesc(kKeys, false), kk > 0);
+                    }
+                    tc_commit(&s_full[h]);
+                    if (last_use(i)) tc_commit(&k_free[st]);
+                };
+                auto pv = [&](int i) {
+                    const int h = i & 1, t = tile(i), st = t & 1;
+#pragma unroll
+                    for (int kk = 0; kk < kKeys / 16; kk++)
+                        tc_mma_ts(tmem + 256 + h * D, tmem + 128 + h * 64 + kk * 8, (st ? dv[1] : dv[0]) + ((kk * 16 * 128) >> 4),
+                                  idesc(D, true), i > 1 || kk > 0);
+                    tc_commit(&pv_done[h]);
+                    if (last_use(i)) tc_commit(&v_free[st]);
+                };
+                auto step_ready = [&](int i) {  // S free (step i - 1 has read it) and K there
+                    const bool ok = (i == 0 || wait(&s_free[(i - 1) & 1], (uint32_t)((i - 1) >> 1))) &&
+                                    wait(&k_full[tile(i) & 1], (uint32_t)(tile(i) >> 1));
+                    tc_fence_after();
+                    return ok;
+                };
+                auto v_ready = [&](int i) {
+                    const int t = tile(i), st = t & 1;
+                    return wait(&v_full[st], (uint32_t)(t >> 1)) && wait(&v_clear[st], (uint32_t)(t >> 1));
+                };
+                bool ok = wait(q_full, 0) && step_ready(0);
+                if (ok) qk(0);
+                if (ok && steps > 1) {
+                    ok = step_ready(1);
+                    if (ok) qk(1);
+                }
+                for (int i = 0; i < steps && ok; i++) {
+                    if (i + 2 < steps) {
+                        ok = step_ready(i + 2);
+                        if (!ok) break;
+                        qk(i + 2);
+                    }
+                    ok = wait(&p_full[i & 1], (uint32_t)(i >> 1)) && v_ready(i);
+                    tc_fence_after();
+                    if (ok) pv(i);
+                }
+                if (!ok) {  // the products issued end before TMEM is given back
+                    tc_commit(drain);
+                    wait(drain, 0);
+                }
+            }
+            __syncwarp();
+        } else if (warp == 10) {
+            // ---- V rows that no row of the item sees.  Every tile passes here, so that this warp and the MMAs
+            // stay within one phase of each other.
+            for (int t = 0; t < nt; t++) {
+                const int st = t & 1, k0 = tiles.at(first + t) * kKeys;
+                if (__any_sync(0xffffffffu, !wait(&v_full[st], (uint32_t)(t >> 1)))) break;
+                const uint32_t seen = present[t & (kSeen - 1)];
+                if (loose(k0) || seen != 0xffu) {
+                    for (int r = 0; r < kKeys; r++) {
+                        const int j = k0 + r;
+                        if ((seen >> (r >> 4) & 1u) && j <= pos_max && (j >= lo_min || j < sinks)) continue;
+                        if (lane < 8 * (D / 64))
+                            *reinterpret_cast<uint4*>(sV + st * S::kTile + (lane >> 3) * kBox + r * 128 + (lane & 7) * 16) =
+                                make_uint4(0, 0, 0, 0);
+                    }
+                    fence_proxy_async_smem();
+                }
+                mbar_arrive(&v_clear[st]);
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
+        // Row r of stream h is flat row 2 r + h of the item (r when tall), token-major: both streams reach
+        // over the same tokens.
+        const int h = warp >> 2, r = 32 * (warp & 3) + lane;
+        // ---- queries, BF16, into the swizzled layout: a warp per 32 rows, D / 8 lanes a row
+        if (!ta.tall || h == 0) {
+            constexpr int kLanes = D / 8, kAtOnce = 32 / kLanes;
+            unsigned char* tile = sQ + h * S::kTile;
+#pragma unroll 8
+            for (int i = 0; i < 32; i += kAtOnce) {
+                const int row = 32 * (warp & 3) + i + lane / kLanes, c = lane % kLanes * 8;
+                const int flat = ta.tall ? row : 2 * row + h;
+                const int tk = flat / a.group, hh = flat - tk * a.group;
+                float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                uint4 packed = make_uint4(0, 0, 0, 0);
+                if (tk < ntok) {
+                    const size_t off = (size_t)(tok0 + tk) * a.q_stride + (size_t)(kvh * a.group + hh) * D + c;
+                    if (a.io_bf16) {
+                        packed = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) + off);
+                    } else {
+                        load8(static_cast<const float*>(a.q) + off, x);
+                        packed = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
+                    }
+                }
+                *reinterpret_cast<uint4*>(tile + sw128_offset(row, c)) = packed;
+            }
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(q_full);
+
+        // ---- softmax: a row per thread
+        const int flat = ta.tall ? r : 2 * r + h;
+        const int tk = flat / a.group, hh = flat - tk * a.group;
+        const bool here = tk < ntok;
+        const int pos = ta.shared_pass ? pos0 : pos0 + min(tk, ntok - 1);
+        const int lo = windowed ? max(0, pos - a.window + 1) : 0;
+        const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+        const uint32_t s_addr = tmem + lanes, p_addr = tmem + lanes + 128 + h * 64, o_addr = tmem + lanes + 256 + h * D;
+        const int mine = ta.tall ? (nt + 1 - h) >> 1 : nt;  // steps of this stream
+        float m_run = -INFINITY, l_run = 0.f;
+        bool ok = true;
+        auto warp_wait = [&](uint64_t* bar, uint32_t parity) { return !__any_sync(0xffffffffu, !wait(bar, parity)); };
+        for (int j = 0; j < mine; j++) {
+            const int t = ta.tall ? 2 * j + h : j;
+            if (!warp_wait(&s_full[h], (uint32_t)j)) {
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+            float sv[kKeys];
+            tmem_ld128(s_addr, sv);
+            tc_fence_before();
+            const uint32_t seen = present[t & (kSeen - 1)];
+            mbar_arrive(&s_free[h]);
+            if (j > 0) {  // P is the previous P.V's operand until that is done
+                if (!warp_wait(&pv_done[h], (uint32_t)(j - 1))) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+            }
+            const int k0 = tiles.at(first + t) * kKeys;
+            const bool masked = edge(k0) || seen != 0xffu;
+            Mask mk;
+            if (masked) {
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const int c0 = k0 + 32 * q;
+                    const uint32_t pages = (seen >> (2 * q) & 1u ? 0xffffu : 0u) | (seen >> (2 * q) & 2u ? 0xffff0000u : 0u);
+                    mk.w[q] = below(pos + 1 - c0) & (~below(lo - c0) | below(sinks - c0)) & pages;
+                }
+            }
+            // The running maximum moves only when a tile's exceeds it by more than 2^8 (P stays within BF16's
+            // range and the FP32 sums do not mind), which spares most rescalings of O: exponentials against the
+            // running maximum, tracking the largest exponent, and again if some row's passed 8.  Rows that have
+            // seen nothing yet take their tile's maximum first.
+            float rowsum, alpha = 1.f;
+            if (__any_sync(0xffffffffu, m_run == -INFINITY)) {
+                float m_new = m_run;
+                const float top = (masked ? row_max<true>(sv, mk) : row_max<false>(sv, mk)) * a.scale_log2;
+                if (m_run == -INFINITY) m_new = top;
+                else if (top > m_run + 8.f) m_new = top;
+                alpha = m_run == -INFINITY ? 1.f : pt_exp2(m_run - m_new);  // nothing gathered: nothing to scale
+                m_run = m_new;
+                const float neg = m_run == -INFINITY ? 0.f : -m_run;
+                rowsum = masked ? row_exp<true, false>(sv, mk, a.scale_log2, neg, p_addr, nullptr)
+                                : row_exp<false, false>(sv, mk, a.scale_log2, neg, p_addr, nullptr);
+            } else {
+                float top;
+                rowsum = masked ? row_exp<true, true>(sv, mk, a.scale_log2, -m_run, p_addr, &top)
+                                : row_exp<false, true>(sv, mk, a.scale_log2, -m_run, p_addr, &top);
+                const bool move = top > 8.f;
+                if (__any_sync(0xffffffffu, move)) {
+                    float m_new = m_run;
+                    if (move) {
+                        m_new = m_run + top;
+                        alpha = pt_exp2(m_run - m_new);
+                    }
+                    m_run = m_new;
+                    rowsum = masked ? row_exp<true, false>(sv, mk, a.scale_log2, -m_run, p_addr, nullptr)
+                                    : row_exp<false, false>(sv, mk, a.scale_log2, -m_run, p_addr, nullptr);
+                }
+            }
+            if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+#pragma unroll
+                for (int q = 0; q < D / 32; q++) {
+                    float ov[32];
+                    tmem_ld32(o_addr + q * 32, ov);
+#pragma unroll
+                    for (int c = 0; c < 32; c++) ov[c] *= alpha;
+                    tmem_st32(o_addr + q * 32, ov);
+                }
+                tmem_wait_st();
+            }
+            l_run = l_run * alpha + rowsum;
+            tc_fence_before();
+            mbar_arrive(&p_full[h]);
+        }
+        // ---- the row's output, or its record
+        const int slot = a.slot0 + (ta.tall ? 2 * split + h : split);
+        const size_t R = (size_t)(tok0 + tk) * a.q_heads + kvh * a.group + hh;
+        const bool direct = a.rec.slots == 1;
+        if (ok && mine > 0) ok = warp_wait(&pv_done[h], (uint32_t)(mine - 1));
+        if (ok) {
+            tc_fence_after();
+            const float mul = !direct ? 1.f : l_run == 0.f ? 0.f : 1.f / l_run;
+#pragma unroll
+            for (int c = 0; c < D / 32; c++) {
+                float v[32];
+                if (mine > 0) {
+                    tmem_ld32(o_addr + c * 32, v);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; i++) v[i] = 0.f;
+                }
+                if (!here) continue;
+#pragma unroll
+                for (int i = 0; i < 32; i++) v[i] = mul == 0.f ? 0.f : v[i] * mul;
+                if (direct && a.io_bf16) {
+                    __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.out) + R * D + c * 32;
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8)
+                        *reinterpret_cast<uint4*>(dst + i) = make_uint4(pack_bf16x2(v[i], v[i + 1]), pack_bf16x2(v[i + 2], v[i + 3]),
+                                                                       pack_bf16x2(v[i + 4], v[i + 5]), pack_bf16x2(v[i + 6], v[i + 7]));
+                } else {
+                    float* dst = direct ? static_cast<float*>(a.out) + R * D + c * 32 : a.rec.o + ((size_t)slot * a.rec.rows + R) * D + c * 32;
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(dst + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                }
+            }
+            if (!direct && here) a.rec.ml[(size_t)slot * a.rec.rows + R] = make_float2(m_run, l_run);
+        }
+        tc_fence_before();
+    }
+    __syncthreads();
+    if (warp == 8) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+}
+
+// ---- host --------------------------------------------------------------------------------------
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+template <int D>
+static int launch_tc(const TcArgs& ta, const void* maps, dim3 grid, cudaStream_t stream)
+{
+    static bool ready[64];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return (int)e;
+    if (dev < 0 || dev >= 64) return (int)cudaErrorInvalidDevice;
+    if (!ready[dev]) {
+        // a register split above the launch's registers would never be granted
+        cudaFuncAttributes fa;
+        e = cudaFuncGetAttributes(&fa, pages_tc_kernel<D>);
+        if (e != cudaSuccess) return (int)e;
+        if (fa.numRegs != kLaunchRegs || fa.maxThreadsPerBlock < kTcThreads) return (int)cudaErrorInvalidConfiguration;
+        e = cudaFuncSetAttribute(pages_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Smem<D>::kBytes);
+        if (e != cudaSuccess) return (int)e;
+        ready[dev] = true;
+    }
+    const CUtensorMap* m = static_cast<const CUtensorMap*>(maps);
+    pages_tc_kernel<D><<<grid, kTcThreads, Smem<D>::kBytes, stream>>>(m[0], m[1], ta);
+    return (int)cudaGetLastError();
+}
+
+int tc_launch(const AttnArgs& a, int layer, bool tall, bool shared_pass, int items, const void* maps, cudaStream_t stream)
+{
+    TcArgs ta;
+    ta.a = a;
+    ta.layer = layer;
+    ta.tall = tall;
+    ta.shared_pass = shared_pass;
+    ta.wait_ns = tyb_wait_limit();
+    const dim3 grid(items, a.p.kv_heads, a.splits);
+    return a.p.head_dim == 128 ? launch_tc<128>(ta, maps, grid, stream) : launch_tc<64>(ta, maps, grid, stream);
+}
+
+}  // namespace tyb
+
+using namespace tyb;
+
+extern "C" int tyb_pages_maps(const KVPages* p, void* maps)
+{
+    memset(maps, 0, TYB_PAGES_MAPS_BYTES);
+    if (p->kv_dtype != TYB_BF16) return 0;
+    static EncodeTiledFn fn = nullptr;
+    if (!fn) {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess)
+            return (int)cudaErrorNotSupported;
+        fn = reinterpret_cast<EncodeTiledFn>(f);
+    }
+    // Every row of every layer, page and head as a 2-D tensor; a box is a page's rows by 64 columns.
+    const cuuint64_t dims[2] = {(cuuint64_t)p->head_dim, (cuuint64_t)p->num_layers * p->num_pages * p->kv_heads * p->page_size};
+    const cuuint64_t strides[1] = {(cuuint64_t)p->head_dim * 2};
+    const cuuint32_t box[2] = {64, (cuuint32_t)p->page_size};
+    const cuuint32_t estr[2] = {1, 1};
+    for (int i = 0; i < 2; i++)
+        if (fn(static_cast<CUtensorMap*>(maps) + i, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, i ? p->v : p->k, dims, strides, box, estr,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+            return (int)cudaErrorInvalidValue;
+    return 0;
+}

@@ -36,8 +36,13 @@ int tyb_pages_import_launch(const KVPages *p, int seq, const void *k_slab, const
                             int rows, void *ws, void *stream);
 
 /* ---- attention ---------------------------------------------------------------------------- */
+/* TMA tensor maps of a BF16 pool's K and V (64-byte aligned room), built once per handle. */
+#define TYB_PAGES_MAPS_BYTES 256
+int tyb_pages_maps(const KVPages *p, void *maps);
+
 typedef struct {
     KVPages p;
+    const void *maps;
     int layer;
     const void *q;
     long long q_stride;
