@@ -31,45 +31,63 @@ typedef struct {
  * stream uses it in turn.  Grown on demand (after waiting for the device), kept until exit. */
 #define TYB_PAGES_STREAMS 32
 static pthread_mutex_t g_lock = PTHREAD_MUTEX_INITIALIZER;
+enum { WS_SCRATCH, WS_TICKETS, WS_KINDS };
 static struct {
     int used, device;
-    void *stream, *p;
-    size_t bytes;
+    void *stream, *p[WS_KINDS];
+    size_t bytes[WS_KINDS];
+    unsigned int timeouts; /* tyb_timeouts() when the tickets were last known to be zero */
 } g_ws[TYB_PAGES_STREAMS];
 static int g_next;
 
-static void *workspace(int device, size_t bytes, const char *what)
+/* The calling stream's buffer of a kind; tickets are zero when handed out.  NULL on failure (error set). */
+static void *workspace(int device, int kind, size_t bytes, const char *what)
 {
     void *st = tyb_stream(), *p = NULL;
     int at = -1;
     pthread_mutex_lock(&g_lock);
     for (int i = 0; i < TYB_PAGES_STREAMS && at < 0; i++)
         if (g_ws[i].used && g_ws[i].device == device && g_ws[i].stream == st) at = i;
-    if (at >= 0 && g_ws[at].bytes >= bytes) {
-        p = g_ws[at].p;
-    } else {
-        if (at < 0) { /* a slot of its own: a free one, else the one taken longest ago on this device */
-            for (int i = 0; i < TYB_PAGES_STREAMS && at < 0; i++)
-                if (!g_ws[i].used) at = i;
-            for (int i = 0; i < TYB_PAGES_STREAMS && at < 0; i++, g_next++)
-                if (g_ws[g_next % TYB_PAGES_STREAMS].device == device) at = g_next % TYB_PAGES_STREAMS;
+    if (at < 0) { /* a slot of its own: a free one, else the one taken longest ago on this device */
+        for (int i = 0; i < TYB_PAGES_STREAMS && at < 0; i++)
+            if (!g_ws[i].used) at = i;
+        for (int i = 0; i < TYB_PAGES_STREAMS && at < 0; i++, g_next++)
+            if (g_ws[g_next % TYB_PAGES_STREAMS].device == device) at = g_next % TYB_PAGES_STREAMS;
+        if (at >= 0 && g_ws[at].used) {
+            cudaDeviceSynchronize(); /* it may still be in use */
+            for (int k = 0; k < WS_KINDS; k++) cudaFree(g_ws[at].p[k]);
         }
-        if (at < 0) {
-            tyb_set_error("%s: workspaces of %d streams in use on other devices", what, TYB_PAGES_STREAMS);
-        } else {
-            if (g_ws[at].used) {
-                cudaDeviceSynchronize(); /* it may still be in use */
-                cudaFree(g_ws[at].p);
-                g_ws[at].used = 0;
+        if (at >= 0) {
+            memset(&g_ws[at], 0, sizeof g_ws[at]);
+            g_ws[at].used = 1;
+            g_ws[at].device = device;
+            g_ws[at].stream = st;
+        }
+    }
+    if (at < 0) {
+        tyb_set_error("%s: workspaces of %d streams in use on other devices", what, TYB_PAGES_STREAMS);
+    } else {
+        if (g_ws[at].bytes[kind] < bytes) {
+            if (g_ws[at].p[kind]) {
+                cudaDeviceSynchronize();
+                cudaFree(g_ws[at].p[kind]);
+                g_ws[at].p[kind] = NULL;
+                g_ws[at].bytes[kind] = 0;
             }
-            size_t want = 1 << 20;
+            size_t want = 1 << 18;
             while (want < bytes) want += want / 2;
-            if (tyb_dev_alloc(&p, want, what)) {
-                g_ws[at].used = 1;
-                g_ws[at].device = device;
-                g_ws[at].stream = st;
-                g_ws[at].p = p;
-                g_ws[at].bytes = want;
+            if (tyb_dev_alloc(&g_ws[at].p[kind], want, what)) {
+                g_ws[at].bytes[kind] = want;
+                if (kind == WS_TICKETS) g_ws[at].timeouts = tyb_timeouts() - 1; /* not zero yet */
+            }
+        }
+        p = g_ws[at].p[kind];
+        if (p && kind == WS_TICKETS && g_ws[at].timeouts != tyb_timeouts()) {
+            /* new, or a kernel gave up in mid-call since: it may not have put its tickets back */
+            g_ws[at].timeouts = tyb_timeouts();
+            if (!tyb_cuda_ok(cudaMemsetAsync(p, 0, g_ws[at].bytes[kind], (cudaStream_t)st), what)) {
+                g_ws[at].timeouts--;
+                p = NULL;
             }
         }
     }
@@ -253,7 +271,7 @@ int kv_pages_extend(KVPages *p, const int *seqs, const int *counts, int n)
     if (!t) return 1;
     if (!list_ready(seqs, n, "seqs", &rc, what)) return rc;
     if (!on_device(counts, 4, "counts", what)) return 1;
-    void *ws = workspace(t->device, tyb_pages_plan_bytes(p, n), what);
+    void *ws = workspace(t->device, WS_SCRATCH, tyb_pages_plan_bytes(p, n), what);
     return ws ? launched(tyb_pages_extend_launch(p, seqs, counts, n, ws, tyb_stream()), what) : 1;
 }
 
@@ -264,7 +282,7 @@ static int fork_or_copy(KVPages *p, const int *src, const int *dst, int n, int d
     if (!t) return 1;
     if (!list_ready(src, n, "src", &rc, what)) return rc;
     if (!on_device(dst, 4, "dst", what)) return 1;
-    void *ws = workspace(t->device, tyb_pages_plan_bytes(p, n), what);
+    void *ws = workspace(t->device, WS_SCRATCH, tyb_pages_plan_bytes(p, n), what);
     return ws ? launched(tyb_pages_fork_launch(p, src, dst, n, deep, ws, tyb_stream()), what) : 1;
 }
 
@@ -299,7 +317,7 @@ int kv_pages_compact(KVPages *p, int *live_out)
     const char *what = "kv_pages_compact";
     tyb_pages *t = pages_from(p, what);
     if (!t || (live_out && !on_device(live_out, 4, "live_out", what))) return 1;
-    void *ws = workspace(t->device, tyb_pages_plan_bytes(p, 0), what);
+    void *ws = workspace(t->device, WS_SCRATCH, tyb_pages_plan_bytes(p, 0), what);
     return ws ? launched(tyb_pages_compact_launch(p, live_out, ws, tyb_stream()), what) : 1;
 }
 
@@ -370,7 +388,7 @@ int kv_pages_import(KVPages *p, int seq, const KVCache *cache)
     for (int l = 0; l < KV_NUM_LAYERS; l++)
         if (!tyb_flush_pending(c, l, what)) return 1;
     if (rows == 0) return 0;
-    void *ws = workspace(t->device, tyb_pages_plan_bytes(p, 1), what);
+    void *ws = workspace(t->device, WS_SCRATCH, tyb_pages_plan_bytes(p, 1), what);
     if (!ws) return 1;
     return launched(tyb_pages_import_launch(p, seq, c->k_slab, c->v_slab, cache->max_seq_len, rows, ws, tyb_stream()), what);
 }
@@ -393,16 +411,22 @@ static int attend(const KVPages *p, tyb_pages_attn *a, const char *what)
         tyb_set_error("%s: negative max_new, max_len, window or sinks", what);
         return 1;
     }
+    if (!(a->scale > 0.f) || a->scale > 3.0e38f) {
+        tyb_set_error("%s: scale %g is not a positive number", what, (double)a->scale);
+        return 1;
+    }
     if (a->batch == 0 || a->rows == 0) return 0;
     if (!check_rows(a->q, a->io_bf16 ? ATTN_DT_BF16 : ATTN_DT_F32, a->q_stride, (long long)a->q_heads * p->head_dim, "q", what) ||
         !on_device(a->out, 16, "output", what) || !on_device(a->seqs, 4, "seqs", what))
         return 1;
     a->p = *p;
     a->maps = t->maps;
-    const size_t bytes = tyb_pages_attn_bytes(a);
-    void *ws = bytes ? workspace(t->device, bytes, what) : NULL;
-    if (bytes && !ws) return 1;
-    return launched(tyb_pages_attn_launch(a, ws, tyb_stream()), what);
+    size_t bytes, ticket_bytes;
+    tyb_pages_attn_bytes(a, &bytes, &ticket_bytes);
+    void *ws = bytes ? workspace(t->device, WS_SCRATCH, bytes, what) : NULL;
+    void *tickets = ticket_bytes ? workspace(t->device, WS_TICKETS, ticket_bytes, what) : NULL;
+    if ((bytes && !ws) || (ticket_bytes && !tickets)) return 1;
+    return launched(tyb_pages_attn_launch(a, ws, tickets, tyb_stream()), what);
 }
 
 static int io_type(int io_dtype, const char *what)

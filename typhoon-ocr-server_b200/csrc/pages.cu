@@ -18,7 +18,7 @@ namespace tyb {
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanWarps = kPlanThreads / 32;
 constexpr int kApplyThreads = 256;
-constexpr int kSms = 148;
+
 
 // One copy of a plan: the first `rows` rows of page `from` (every layer, K and V) go to page `to`.
 struct Move {

@@ -16,7 +16,7 @@
 // Decode is bound by memory (each K and V element is used by q_heads / kv_heads rows once), so what
 // matters is bytes in flight: four warps a CTA, each with one tile of K and of V (8 KB) requested.
 #define TYB_WHOLE_PROGRAM
-#include "pages_attn.cuh"
+#include "pages_mma.cuh"
 
 namespace tyb {
 
@@ -28,35 +28,6 @@ __device__ __forceinline__ uint4 ldg16(const void* p)
     uint4 v;
     asm("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
     return v;
-}
-
-__device__ __forceinline__ uint32_t pack2(float lo, float hi)
-{
-    __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<uint32_t*>(&h);
-}
-__device__ __forceinline__ float lo_of(uint32_t x) { return __uint_as_float(x << 16); }
-__device__ __forceinline__ float hi_of(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
-
-__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
-{
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
-__device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
-{
-    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// x = hi + lo in TF32, the remainder below 2^-22 |x|.
-__device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo)
-{
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(x - __uint_as_float(hi)));
 }
 
 // Where key row `tile * KT` lies, as an element offset into the layer's pages of KV head h; -1 when the
@@ -136,43 +107,6 @@ template <typename T, int D>
 struct Query;
 
 template <int D>
-struct Query<__nv_bfloat16, D> {
-    static constexpr int kSharedFloats = 0;
-    uint32_t a[D / 16][4];
-    // Row r of the warp at q[r] (NULL: absent, zeros), FP32 or BF16.
-    __device__ __forceinline__ void load(const void* row0, const void* row1, bool bf16, int t, float*, int)
-    {
-#pragma unroll
-        for (int j = 0; j < D / 32; j++)
-#pragma unroll
-            for (int r = 0; r < 2; r++) {
-                const void* row = r ? row1 : row0;
-                float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                const int at = (4 * j + t) * 8;
-                if (row && bf16) load8(static_cast<const __nv_bfloat16*>(row) + at, x);
-                else if (row) load8(static_cast<const float*>(row) + at, x);
-                a[2 * j][r] = pack2(x[0], x[1]);
-                a[2 * j][2 + r] = pack2(x[2], x[3]);
-                a[2 * j + 1][r] = pack2(x[4], x[5]);
-                a[2 * j + 1][2 + r] = pack2(x[6], x[7]);
-            }
-    }
-    // Scores of the 16 rows against the tile: s[e] keys 8e .. 8e + 8 (rows g, g + 8; keys 2t, 2t + 1).
-    __device__ __forceinline__ void scores(const Warp<__nv_bfloat16, D>& w, float (&s)[2][4], int, int) const
-    {
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-            s[e][0] = s[e][1] = s[e][2] = s[e][3] = 0.f;
-#pragma unroll
-            for (int j = 0; j < D / 32; j++) {
-                mma_bf16(s[e], a[2 * j][0], a[2 * j][1], a[2 * j][2], a[2 * j][3], w.k[e][j].x, w.k[e][j].y);
-                mma_bf16(s[e], a[2 * j + 1][0], a[2 * j + 1][1], a[2 * j + 1][2], a[2 * j + 1][3], w.k[e][j].z, w.k[e][j].w);
-            }
-        }
-    }
-};
-
-template <int D>
 struct Query<float, D> {
     static constexpr int kPitch = D + 16;
     static constexpr int kSharedFloats = 16 * kPitch;
@@ -221,31 +155,6 @@ struct Query<float, D> {
 };
 
 // O += P . V for the tile; P in the score layout.
-template <int D>
-__device__ __forceinline__ void accumulate(Warp<__nv_bfloat16, D>& w, const float (&p)[2][4])
-{
-    uint32_t h[4], r[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const float x = p[i >> 1][2 * (i & 1)], y = p[i >> 1][2 * (i & 1) + 1];
-        h[i] = pack2(x, y);
-        r[i] = pack2(x - lo_of(h[i]), y - hi_of(h[i]));
-    }
-    const uint32_t(&v)[4][Warp<__nv_bfloat16, D>::kChunkV][4] =
-        reinterpret_cast<const uint32_t(&)[4][Warp<__nv_bfloat16, D>::kChunkV][4]>(w.v);
-#pragma unroll
-    for (int j = 0; j < Warp<__nv_bfloat16, D>::kChunkV; j++)
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            // element i of the chunk of two key rows as a pair
-            const uint32_t sel = i & 1 ? 0x7632 : 0x5410;
-            const uint32_t b0 = __byte_perm(v[0][j][i / 2], v[1][j][i / 2], sel);
-            const uint32_t b1 = __byte_perm(v[2][j][i / 2], v[3][j][i / 2], sel);
-            mma_bf16(w.o[8 * j + i], h[0], h[1], h[2], h[3], b0, b1);
-            mma_bf16(w.o[8 * j + i], r[0], r[1], r[2], r[3], b0, b1);
-        }
-}
-
 template <int D>
 __device__ __forceinline__ void accumulate(Warp<float, D>& w, const float (&p)[1][4])
 {
@@ -397,96 +306,12 @@ __device__ __forceinline__ void put4(const AttnArgs& a, int D, int slot, size_t 
     }
 }
 
-template <typename T, int D>
-constexpr size_t solo_shared_floats()
-{
-    const size_t join = (size_t)kWarps * 16 * (D + 4) + 2 * kWarps * 16;
-    return Query<T, D>::kSharedFloats > join ? Query<T, D>::kSharedFloats : join;
-}
-
-// Single tokens: CTA (split, KV head, sequence); the four warps share the head's query rows and deal
-// out the split's tiles in turn; their results are joined in shared memory.
-template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) pages_token_kernel(const AttnArgs a)
-{
-    using W = Warp<T, D>;
-    extern __shared__ float4 shared4[];
-    float* shared = reinterpret_cast<float*>(shared4);
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    const int split = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
-    const int s = a.seqs[b];
-    const int len = checked_len(a.p, s, a.st);
-    View view;
-    view.table = a.p.table + (size_t)(len ? s : 0) * a.p.max_pages;
-    view.kvh = kvh;
-    view.sinks = a.sinks;
-    view.pos_min = view.pos_max = len - 1;
-    view.lo_min = view.lo_max = a.window ? max(0, len - a.window) : min(a.prefix, len);
-    view.pos[0] = view.pos[1] = view.pos_max;
-    view.lo[0] = view.lo[1] = view.lo_min;
-    const Tiles tiles = tiles_of(view.pos_max, view.lo_min, view.sinks, W::kTile);
-    const int n = tiles.count();
-    const int first = (int)((long long)n * split / a.splits), end = (int)((long long)n * (split + 1) / a.splits);
-
-    Query<T, D> q;
-    const size_t esize = a.io_bf16 ? 2 : 4;
-    const char* q0 = static_cast<const char*>(a.q) + ((size_t)b * a.q_stride + (size_t)kvh * a.group * D) * esize;
-    q.load(g < a.group ? q0 + (size_t)g * D * esize : nullptr, g + 8 < a.group ? q0 + (size_t)(g + 8) * D * esize : nullptr, a.io_bf16, t,
-           shared, g);
-    if (Query<T, D>::kSharedFloats) __syncthreads();  // every warp wrote the same rows
-
-    W w;
-    w.clear();
-    walk(w, q, a, view, tiles, first + warp, end, kWarps, g, t, lane);
-
-    // Join the warps: maximum, then everything scaled to it.
-    if (Query<T, D>::kSharedFloats) __syncthreads();  // the query rows are no longer needed
-    constexpr int kPitch = D + 4;
-    float* so = shared;                          // [warp][16][kPitch]
-    float* sm = shared + kWarps * 16 * kPitch;   // [warp][16]
-    float* sl = sm + kWarps * 16;
-    if (t == 0)
-        for (int r = 0; r < 2; r++) {
-            sm[warp * 16 + g + 8 * r] = w.m[r];
-            sl[warp * 16 + g + 8 * r] = w.l[r];
-        }
-#pragma unroll
-    for (int r = 0; r < 2; r++) {
-        if (g + 8 * r >= a.group) continue;
-#pragma unroll
-        for (int c = 0; c < W::kOut; c++) {
-            so[(warp * 16 + g + 8 * r) * kPitch + W::column(c, 0, t)] = w.o[c][2 * r];
-            so[(warp * 16 + g + 8 * r) * kPitch + W::column(c, 1, t)] = w.o[c][2 * r + 1];
-        }
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < a.group * (D / 4); i += kThreads) {
-        const int row = i / (D / 4), c = i % (D / 4) * 4;
-        float top = -INFINITY, l = 0.f;
-        for (int x = 0; x < kWarps; x++) top = fmaxf(top, sm[x * 16 + row]);
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int x = 0; x < kWarps; x++) {
-            const float mx = sm[x * 16 + row];
-            const float f = mx == -INFINITY ? 0.f : fast_exp2(mx - top);
-            const float4 y = *reinterpret_cast<const float4*>(so + (x * 16 + row) * kPitch + c);
-            l += sl[x * 16 + row] * f;
-            o.x = fmaf(y.x, f, o.x);
-            o.y = fmaf(y.y, f, o.y);
-            o.z = fmaf(y.z, f, o.z);
-            o.w = fmaf(y.w, f, o.w);
-        }
-        const size_t R = (size_t)b * a.q_heads + kvh * a.group + row;
-        put4(a, D, a.slot0 + split, R, c, o, l);
-        if (a.rec.slots > 1 && c == 0) a.rec.ml[(size_t)(a.slot0 + split) * a.rec.rows + R] = make_float2(top, l);
-    }
-}
-
 // Rows of a CTA tile: `per` tokens x `group` heads, token-major.  The prefix pass takes the batch's
 // single tokens as its rows.
 constexpr int kRowsCta = 16 * kWarps;
 
 // CTA (row tile, KV head, split): each warp has 16 rows of its own and walks all the split's tiles.
-template <typename T, int D, bool kPrefix>
+template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) pages_rows_kernel(const AttnArgs a)
 {
     using W = Warp<T, D>;
@@ -496,13 +321,7 @@ __global__ void __launch_bounds__(kThreads) pages_rows_kernel(const AttnArgs a)
     const int per = kRowsCta / a.group;
     int seq = 0, tok0, ntok, pos0;  // first token (row of q) of the tile, tokens, position of the first
     __shared__ int found[4];
-    if (kPrefix) {
-        tok0 = blockIdx.x * per;
-        ntok = min(per, a.batch - tok0);
-        seq = a.seqs[0];
-        const int len = checked_len(a.p, seq, a.st);
-        pos0 = min(a.prefix, len) - 1;
-    } else {
+    {
         // which sequence's tile this is: a warp scans the sequences' tile counts
         if (warp == 0) {
             int before = 0;
@@ -545,10 +364,10 @@ __global__ void __launch_bounds__(kThreads) pages_rows_kernel(const AttnArgs a)
     View view;
     view.table = a.p.table + (size_t)(seq < 0 || seq >= a.p.max_seqs ? 0 : seq) * a.p.max_pages;
     view.kvh = kvh;
-    view.sinks = kPrefix ? 0 : a.sinks;
-    auto lo_of_pos = [&](int pos) { return !kPrefix && a.window ? max(0, pos - a.window + 1) : 0; };
+    view.sinks = a.sinks;
+    auto lo_of_pos = [&](int pos) { return a.window ? max(0, pos - a.window + 1) : 0; };
     view.pos_min = pos0;
-    view.pos_max = kPrefix ? pos0 : pos0 + ntok - 1;
+    view.pos_max = pos0 + ntok - 1;
     view.lo_min = lo_of_pos(view.pos_min);
     view.lo_max = lo_of_pos(view.pos_max);
     const char* qrow[2];
@@ -559,7 +378,7 @@ __global__ void __launch_bounds__(kThreads) pages_rows_kernel(const AttnArgs a)
     for (int r = 0; r < 2; r++) {
         const int row = 16 * warp + g + 8 * r, tk = row / a.group, hh = row - tk * a.group;
         here[r] = tk < ntok;
-        view.pos[r] = !here[r] ? -1 : kPrefix ? pos0 : pos0 + tk;
+        view.pos[r] = here[r] ? pos0 + tk : -1;
         view.lo[r] = lo_of_pos(view.pos[r]);
         qrow[r] = here[r] ? static_cast<const char*>(a.q) + ((size_t)(tok0 + tk) * a.q_stride + (size_t)(kvh * a.group + hh) * D) * esize : nullptr;
         R[r] = (size_t)(tok0 + tk) * a.q_heads + kvh * a.group + hh;
@@ -630,78 +449,58 @@ __global__ void __launch_bounds__(kThreads) pages_join_kernel(const AttnArgs a)
 
 // ---- launches ----------------------------------------------------------------------------------
 
-constexpr int kSms = 148;
+static int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
 
-// How a call is laid out: its row tiles and splits.
+// How a call is laid out.
 struct Layout {
-    bool tokens;  // the token kernel handles (all or the own rows of) the call
-    bool shared;  // the row tiles are the shared pass over a prefix
-    bool tc;      // the row tiles run on the tcgen05 form
-    bool tall;
-    int token_splits, row_tiles, row_splits, row_slots, slots;
+    bool tokens;  // single tokens: the streaming form
+    bool tiles;   // row tiles: prompt chunks, or a shared prefix on the tcgen05 form
+    bool shared;  // the streaming form takes the shared prefix along
+    bool tc, tall;
+    int row_tiles, splits, slots;
 };
 
-static int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
+// Query rows of a KV head from which the shared prefix runs on the tcgen05 form.
+constexpr int kTcSharedRows = 65;
 
 static Layout layout_of(const tyb_pages_attn* c)
 {
     Layout l = {};
-    const int kt = c->p.kv_dtype == TYB_BF16 ? 16 : 8;
+    const bool bf16 = c->p.kv_dtype == TYB_BF16;
     const int group = c->q_heads / c->p.kv_heads;
     l.tokens = c->max_new == 1 && c->rows == c->batch;
-    l.shared = l.tokens && c->prefix > 0;
-    if (l.tokens) {
-        long long own = c->window && c->window < c->max_len ? c->window + c->sinks : c->max_len - c->prefix;
-        const int tiles = ceil_div(own, kt) + 1;
-        // enough CTAs for four on every SM, and at least a tile for each warp of a split
-        int s = ceil_div(4LL * kSms, (long long)c->batch * c->p.kv_heads);
-        if (s > ceil_div(tiles, kWarps)) s = ceil_div(tiles, kWarps);
-        l.token_splits = s < 1 ? 1 : s;
+    const bool prefix = l.tokens && c->prefix > 0;
+    l.tiles = !l.tokens || (prefix && bf16 && (long long)c->batch * group >= kTcSharedRows);
+    l.shared = prefix && !l.tiles;
+    if (!l.tiles) return l;
+    l.tc = bf16;
+    l.tall = l.tc && (long long)(l.tokens ? c->batch : c->max_new) * group <= kTcTall;
+    const int per = (l.tall ? kTcTall : l.tc ? kTcWide : kRowsCta) / group;
+    // Each of the sequences of a call ends in a tile of its own; no list has more tiles than this.
+    l.row_tiles = l.tokens ? ceil_div(c->batch, per) : (int)((c->rows + (long long)c->batch * (per - 1)) / per);
+    const long long keys = l.tokens ? c->prefix : c->window && c->window < c->max_len ? c->window + c->sinks : c->max_len;
+    const int tiles = ceil_div(keys, l.tc ? 128 : 8);
+    const long long ctas = (long long)l.row_tiles * c->p.kv_heads;
+    if (l.tc) {
+        l.splits = (int)(kSms / ctas);  // one CTA fits an SM; a split has at least two tiles
+        if (l.splits > tiles / 2) l.splits = tiles / 2;
+    } else {
+        l.splits = ceil_div(3LL * kSms, ctas);
+        if (l.splits > ceil_div(tiles, 8)) l.splits = ceil_div(tiles, 8);
     }
-    if (!l.tokens || l.shared) {
-        l.tc = c->p.kv_dtype == TYB_BF16;
-        l.tall = l.tc && (long long)(l.shared ? c->batch : c->max_new) * group <= kTcTall;
-        const int per = (l.tall ? kTcTall : l.tc ? kTcWide : kRowsCta) / group;
-        // Each of the sequences of a call ends in a tile of its own; no list has more tiles than this.
-        l.row_tiles = l.shared ? ceil_div(c->batch, per) : (int)((c->rows + (long long)c->batch * (per - 1)) / per);
-        const long long keys = l.shared ? c->prefix : c->window && c->window < c->max_len ? c->window + c->sinks : c->max_len;
-        const int tiles = ceil_div(keys, l.tc ? 128 : kt);
-        const long long ctas = (long long)l.row_tiles * c->p.kv_heads;
-        int s;
-        if (l.tc) {
-            s = (int)(kSms / ctas);  // one CTA fits an SM; a split has at least two tiles
-            if (s > tiles / 2) s = tiles / 2;
-        } else {
-            s = ceil_div(3LL * kSms, ctas);
-            if (s > ceil_div(tiles, 8)) s = ceil_div(tiles, 8);
-        }
-        l.row_splits = s < 1 ? 1 : s;
-    }
-    l.row_slots = l.row_splits * (l.tall ? 2 : 1);
-    l.slots = l.token_splits + l.row_slots;
+    if (l.splits < 1) l.splits = 1;
+    l.slots = l.splits * (l.tall ? 2 : 1) + l.tokens;  // the last one of a shared pass's call: the own rows
     return l;
 }
 
-}  // namespace tyb
-
-extern "C" size_t tyb_pages_attn_bytes(const tyb_pages_attn* c)
+static AttnArgs args_of(const tyb_pages_attn* c, const Layout& l)
 {
-    const tyb::Layout l = tyb::layout_of(c);
-    if (l.slots <= 1) return 0;
-    return (size_t)l.slots * c->rows * c->q_heads * (c->p.head_dim * sizeof(float) + sizeof(float2));
-}
-
-namespace tyb {
-
-template <typename T, int D>
-static int launch(const tyb_pages_attn* c, void* ws, cudaStream_t stream)
-{
-    const Layout l = layout_of(c);
     AttnArgs a = {};
     a.p = c->p;
-    const size_t layer = (size_t)c->layer * c->p.num_pages * c->p.kv_heads * c->p.page_size * D;
-    a.k = static_cast<const T*>(c->p.k) + layer;
-    a.v = static_cast<const T*>(c->p.v) + layer;
+    const size_t layer = (size_t)c->layer * c->p.num_pages * c->p.kv_heads * c->p.page_size * c->p.head_dim *
+                         (c->p.kv_dtype == TYB_BF16 ? 2 : 4);
+    a.k = static_cast<const char*>(c->p.k) + layer;
+    a.v = static_cast<const char*>(c->p.v) + layer;
     a.q = c->q;
     a.q_stride = c->q_stride;
     a.out = c->out;
@@ -716,59 +515,81 @@ static int launch(const tyb_pages_attn* c, void* ws, cudaStream_t stream)
     a.window = c->window;
     a.sinks = c->window ? c->sinks : 0;
     a.scale_log2 = c->scale * kLog2e;
+    a.splits = l.splits;
     a.rec.rows = c->rows * c->q_heads;
     a.rec.slots = l.slots;
-    a.rec.o = static_cast<float*>(ws);
-    a.rec.ml = reinterpret_cast<float2*>(static_cast<float*>(ws) + (size_t)l.slots * a.rec.rows * D);
-    a.st.word = tyb_status_word();
-    a.st.mirror = tyb_status_mirror_device();
-    if (!a.st.word) return (int)cudaErrorInvalidSymbol;
+    return a;
+}
+
+static bool records(const Layout& l) { return l.slots > 1; }
+static size_t record_bytes(const AttnArgs& a, const Layout& l)
+{
+    return records(l) ? (size_t)l.slots * a.rec.rows * (a.p.head_dim * sizeof(float) + sizeof(float2)) : 0;
+}
+
+template <int D>
+static int launch_rows(const AttnArgs& a, int row_tiles, cudaStream_t stream)
+{
     static bool ready[64];
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return (int)e;
     if (dev < 0 || dev >= 64) return (int)cudaErrorInvalidDevice;
-    const size_t solo = solo_shared_floats<T, D>() * sizeof(float);
     const size_t rows = kWarps * (size_t)Query<float, D>::kSharedFloats * sizeof(float);
     if (!ready[dev]) {
-        e = cudaFuncSetAttribute(pages_token_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)solo);
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(pages_rows_kernel<T, D, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)rows);
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(pages_rows_kernel<T, D, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)rows);
+        e = cudaFuncSetAttribute(pages_rows_kernel<float, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)rows);
         if (e != cudaSuccess) return (int)e;
         ready[dev] = true;
     }
-    if (l.tokens) {
-        a.splits = l.token_splits;
-        a.slot0 = l.row_slots;
-        pages_token_kernel<T, D><<<dim3(l.token_splits, c->p.kv_heads, c->batch), kThreads, solo, stream>>>(a);
-        if ((e = cudaGetLastError()) != cudaSuccess) return (int)e;
-    }
-    if (l.row_splits) {
-        a.splits = l.row_splits;
-        a.slot0 = 0;
-        const dim3 grid(l.row_tiles, c->p.kv_heads, l.row_splits);
-        if (l.tc) {
-            const int rc = tc_launch(a, c->layer, l.tall, l.shared, l.row_tiles, c->maps, stream);
-            if (rc) return rc;
-        } else if (l.shared) pages_rows_kernel<T, D, true><<<grid, kThreads, rows, stream>>>(a);
-        else pages_rows_kernel<T, D, false><<<grid, kThreads, rows, stream>>>(a);
-        if ((e = cudaGetLastError()) != cudaSuccess) return (int)e;
-    }
-    if (l.slots > 1) {
-        pages_join_kernel<D><<<ceil_div(a.rec.rows, kWarps), kThreads, 0, stream>>>(a);
-        if ((e = cudaGetLastError()) != cudaSuccess) return (int)e;
-    }
-    return 0;
+    pages_rows_kernel<float, D><<<dim3(row_tiles, a.p.kv_heads, a.splits), kThreads, rows, stream>>>(a);
+    return (int)cudaGetLastError();
 }
 
 }  // namespace tyb
 
 using namespace tyb;
 
-extern "C" int tyb_pages_attn_launch(const tyb_pages_attn* c, void* ws, void* stream)
+extern "C" void tyb_pages_attn_bytes(const tyb_pages_attn* c, size_t* ws, size_t* tickets)
+{
+    const Layout l = layout_of(c);
+    const AttnArgs a = args_of(c, l);
+    const int count = c->batch < kStreamSeqs ? c->batch : kStreamSeqs;
+    *ws = (record_bytes(a, l) + 255) / 256 * 256 + (l.tokens ? stream_bytes(a, count, l.shared) : 0);
+    *tickets = l.tokens ? (size_t)count * c->p.kv_heads * sizeof(unsigned int) : 0;
+}
+
+extern "C" int tyb_pages_attn_launch(const tyb_pages_attn* c, void* ws, void* tickets, void* stream)
 {
     cudaStream_t st = (cudaStream_t)stream;
-    if (c->p.kv_dtype == TYB_BF16)
-        return c->p.head_dim == 128 ? launch<__nv_bfloat16, 128>(c, ws, st) : launch<__nv_bfloat16, 64>(c, ws, st);
-    return c->p.head_dim == 128 ? launch<float, 128>(c, ws, st) : launch<float, 64>(c, ws, st);
+    const Layout l = layout_of(c);
+    AttnArgs a = args_of(c, l);
+    a.st.word = tyb_status_word();
+    a.st.mirror = tyb_status_mirror_device();
+    if (!a.st.word) return (int)cudaErrorInvalidSymbol;
+    const int D = a.p.head_dim;
+    if (records(l)) {
+        a.rec.o = static_cast<float*>(ws);
+        a.rec.ml = reinterpret_cast<float2*>(a.rec.o + (size_t)l.slots * a.rec.rows * D);
+    }
+    void* more = static_cast<char*>(ws) + (record_bytes(a, l) + 255) / 256 * 256;
+    if (l.tiles) {
+        const int e = l.tc ? tc_launch(a, c->layer, l.tall, l.tokens, l.row_tiles, c->maps, st)
+                           : D == 128 ? launch_rows<128>(a, l.row_tiles, st) : launch_rows<64>(a, l.row_tiles, st);
+        if (e) return e;
+    }
+    if (l.tokens) {
+        for (int first = 0; first < c->batch; first += kStreamSeqs) {
+            const int count = c->batch - first < kStreamSeqs ? c->batch - first : kStreamSeqs;
+            const int e = launch_stream(a, c->layer, first, count, l.shared, l.tiles ? l.slots - 1 : -1, c->max_len, c->maps, more,
+                                        static_cast<unsigned int*>(tickets), st);
+            if (e) return e;
+        }
+    }
+    if (records(l)) {
+        const int grid = ceil_div(a.rec.rows, kWarps);
+        if (D == 128) pages_join_kernel<128><<<grid, kThreads, 0, st>>>(a);
+        else pages_join_kernel<64><<<grid, kThreads, 0, st>>>(a);
+        return (int)cudaGetLastError();
+    }
+    return 0;
 }

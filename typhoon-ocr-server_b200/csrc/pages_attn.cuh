@@ -18,6 +18,23 @@ __device__ __forceinline__ void raise(const Status& s, unsigned int bits)
     flag_mirror(s.mirror);
 }
 
+// Waits for phase `parity` of an mbarrier, at most limit_ns; false (and the status raised) when that ran
+// out.
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, uint64_t limit_ns, const Status& s)
+{
+    if (mbar_try_wait(bar, parity)) return true;
+    const uint64_t t0 = globaltimer_ns();
+    while (true) {
+#pragma unroll 1
+        for (int i = 0; i < 64; i++)
+            if (mbar_try_wait(bar, parity)) return true;
+        if (globaltimer_ns() - t0 > limit_ns) {
+            raise(s, TYB_STATUS_WAIT_TIMEOUT);
+            return false;
+        }
+    }
+}
+
 // A query row at position `pos` sees key j when j <= pos and (j >= lo or j < sinks).  The four uses:
 //   prefix      pos = P - 1,   lo = 0
 //   own rows    pos = len - 1, lo = P
@@ -93,8 +110,34 @@ struct AttnArgs {
 constexpr int kTcTall = 128, kTcWide = 256;
 int tc_launch(const AttnArgs& a, int layer, bool tall, bool shared_pass, int items, const void* maps, cudaStream_t stream);
 
+// The streaming form (pages_stream.cu): the single tokens of sequences first .. first + count (at most
+// kStreamSeqs) of the call, with the shared pass over a.prefix rows in the same launch (`shared`); the
+// results are the output, or (out_slot >= 0) record slot out_slot of a.rec.  ws: stream_bytes; tickets: count * kv_heads words, zero (and left
+// so).
+constexpr int kStreamSeqs = 1024;
+size_t stream_bytes(const AttnArgs& a, int count, bool shared);
+int launch_stream(const AttnArgs& a, int layer, int first, int count, bool shared, int out_slot, int max_len, const void* maps, void* ws,
+                  unsigned int* tickets, cudaStream_t stream);
+
+constexpr int kSms = 148;
+// Rows of a TMA box of the pool's maps: a page, or the part of it that a stage holds.
+__host__ __device__ inline int box_rows(const KVPages& p)
+{
+    const int most = p.kv_dtype == TYB_BF16 ? 64 : 32;
+    return p.page_size < most ? p.page_size : most;
+}
+
 // log2 of the page size (16 .. 128)
 __device__ __forceinline__ int page_shift(int page_size) { return __ffs(page_size) - 1; }
+
+// A box of a page pool's map: columns from c0, rows from c1.
+__device__ __forceinline__ void tma_load_2d(void* dst, const void* map, int c0, int c1, uint64_t* bar)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(smem_u32(bar))
+        : "memory");
+}
 
 __device__ __forceinline__ float fast_exp2(float x)
 {

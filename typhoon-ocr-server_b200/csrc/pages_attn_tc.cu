@@ -59,14 +59,6 @@ __host__ __device__ constexpr uint32_t idesc(int n, bool b_mn_major)
     return (1u << 4) | (1u << 7) | (1u << 10) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
 }
 
-__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int c0, int c1, uint64_t* bar)
-{
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(dst)),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(smem_u32(bar))
-        : "memory");
-}
-
 __device__ __forceinline__ float max3(float a, float b, float c)
 {
     float d;
@@ -238,46 +230,47 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     auto edge = [&](int k0) { return k0 + kKeys - 1 > pos0 || (k0 < lo_max && k0 + kKeys > sinks); };
     auto loose = [&](int k0) { return k0 + kKeys - 1 > pos_max || (k0 < lo_min && k0 + kKeys > sinks); };
     auto wait = [&](uint64_t* bar, uint32_t parity) {
-        return mbar_wait_bounded_to(bar, parity & 1u, ta.wait_ns, TYB_STATUS_WAIT_TIMEOUT, a.st.word, a.st.mirror);
+        return wait_for(bar, parity & 1u, ta.wait_ns, a.st);
     };
 
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
         if (warp == 9) {
-            // ---- copies: lane l < pages of a tile has page l
-            const int ps = a.p.page_size, shift = page_shift(ps), per_tile = kKeys >> shift;
+            // ---- copies: lane l < parts of a tile has the page, or the half page, at its rows l * part
+            const int part = box_rows(a.p), shift = page_shift(a.p.page_size), per_tile = kKeys / part;
             const int* table = a.p.table + (size_t)max(0, min(seq, a.p.max_seqs - 1)) * a.p.max_pages;
-            const uint32_t all_seen = 0xffu, page_bits = (1u << (ps / 16)) - 1u;
-            const int page_bytes = ps * 128;  // of a 64-column box
+            const uint32_t part_bits = (1u << (part / 16)) - 1u;
+            const int part_bytes = part * 128;  // of a 64-column box
             bool ok = true;
             int k_sent = 0, v_sent = 0;  // tiles requested
             for (int t = 0; t < nt && ok; t++) {
-                const int st = t & 1, entry = (tiles.at(first + t) * kKeys >> shift) + lane;
+                const int st = t & 1, key = tiles.at(first + t) * kKeys + lane * part;
                 int page = -1;
-                if (lane < per_tile && entry <= pos_max >> shift) {
-                    page = table[entry];
+                if (lane < per_tile && key <= pos_max) {
+                    page = table[key >> shift];
                     if (page >= a.p.num_pages) {
                         raise(a.st, TYB_STATUS_BAD_ARGUMENT);
                         page = -1;
                     }
                 }
                 const uint32_t have = __ballot_sync(0xffffffffu, page >= 0);
-                const int row = page < 0 ? 0 : ((ta.layer * a.p.num_pages + page) * a.p.kv_heads + kvh) * ps;
-                const uint32_t bytes = (uint32_t)__popc(have) * (uint32_t)(page_bytes * (D / 64));
+                const int row = page < 0 ? 0
+                                         : ((ta.layer * a.p.num_pages + page) * a.p.kv_heads + kvh) * a.p.page_size + (key & (a.p.page_size - 1));
+                const uint32_t bytes = (uint32_t)__popc(have) * (uint32_t)(part_bytes * (D / 64));
                 if (t >= kStages) ok = wait(&k_free[st], (uint32_t)((t - kStages) >> 1));
                 if (__any_sync(0xffffffffu, !ok)) break;
                 if (lane == 0) {
                     uint32_t seen = 0;
                     for (int l = 0; l < per_tile; l++)
-                        if (have >> l & 1u) seen |= page_bits << (l * (ps / 16));
-                    present[t & (kSeen - 1)] = seen & all_seen;
+                        if (have >> l & 1u) seen |= part_bits << (l * (part / 16));
+                    present[t & (kSeen - 1)] = seen;
                     mbar_arrive_expect_tx(&k_full[st], bytes);
                 }
                 __syncwarp();
                 if (page >= 0)
 #pragma unroll
                     for (int c = 0; c < D / 64; c++)
-                        tma_load_2d(sK + st * S::kTile + c * kBox + lane * page_bytes, &map_k, 64 * c, row, &k_full[st]);
+                        tma_load_2d(sK + st * S::kTile + c * kBox + lane * part_bytes, &map_k, 64 * c, row, &k_full[st]);
                 k_sent = t + 1;
                 if (t >= kStages) ok = wait(&v_free[st], (uint32_t)((t - kStages) >> 1));
                 if (__any_sync(0xffffffffu, !ok)) break;
@@ -286,7 +279,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 if (page >= 0)
 #pragma unroll
                     for (int c = 0; c < D / 64; c++)
-                        tma_load_2d(sV + st * S::kTile + c * kBox + lane * page_bytes, &map_v, 64 * c, row, &v_full[st]);
+                        tma_load_2d(sV + st * S::kTile + c * kBox + lane * part_bytes, &map_v, 64 * c, row, &v_full[st]);
                 v_sent = t + 1;
             }
             if (__any_sync(0xffffffffu, !ok)) {  // a wait ran out: the copies requested still land in this CTA
@@ -581,8 +574,6 @@ using namespace tyb;
 
 extern "C" int tyb_pages_maps(const KVPages* p, void* maps)
 {
-    memset(maps, 0, TYB_PAGES_MAPS_BYTES);
-    if (p->kv_dtype != TYB_BF16) return 0;
     static EncodeTiledFn fn = nullptr;
     if (!fn) {
         void* f = nullptr;
@@ -591,13 +582,14 @@ extern "C" int tyb_pages_maps(const KVPages* p, void* maps)
             return (int)cudaErrorNotSupported;
         fn = reinterpret_cast<EncodeTiledFn>(f);
     }
-    // Every row of every layer, page and head as a 2-D tensor; a box is a page's rows by 64 columns.
+    // Every row of every layer, page and head as a 2-D tensor; a box is 128 bytes of a page's rows.
+    const bool bf16 = p->kv_dtype == TYB_BF16;
     const cuuint64_t dims[2] = {(cuuint64_t)p->head_dim, (cuuint64_t)p->num_layers * p->num_pages * p->kv_heads * p->page_size};
-    const cuuint64_t strides[1] = {(cuuint64_t)p->head_dim * 2};
-    const cuuint32_t box[2] = {64, (cuuint32_t)p->page_size};
+    const cuuint64_t strides[1] = {(cuuint64_t)p->head_dim * (bf16 ? 2 : 4)};
+    const cuuint32_t box[2] = {bf16 ? 64u : 32u, (cuuint32_t)box_rows(*p)};
     const cuuint32_t estr[2] = {1, 1};
     for (int i = 0; i < 2; i++)
-        if (fn(static_cast<CUtensorMap*>(maps) + i, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, i ? p->v : p->k, dims, strides, box, estr,
+        if (fn(static_cast<CUtensorMap*>(maps) + i, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, i ? p->v : p->k, dims, strides, box, estr,
                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
             return (int)cudaErrorInvalidValue;

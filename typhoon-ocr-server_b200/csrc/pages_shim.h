@@ -61,9 +61,10 @@ typedef struct {
     float scale;
 } tyb_pages_attn;
 
-/* Workspace of a call (0: none). */
-size_t tyb_pages_attn_bytes(const tyb_pages_attn *a);
-int tyb_pages_attn_launch(const tyb_pages_attn *a, void *ws, void *stream);
+/* Bytes of workspace and of tickets (words that are zero between launches; a launch that ended in a
+ * status may leave them otherwise) of a call. */
+void tyb_pages_attn_bytes(const tyb_pages_attn *a, size_t *ws, size_t *tickets);
+int tyb_pages_attn_launch(const tyb_pages_attn *a, void *ws, void *tickets, void *stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,581 @@
+// pages_stream.cu -- single-token attention over the paged cache: every sequence's own rows (all of
+// them, those behind a shared prefix, or those in a window with sinks) and, for batches too small for
+// the tcgen05 form, the shared prefix itself.
+//
+// The work is memory traffic: each K and V element meets q_heads / kv_heads query rows (a prefix
+// element at most 16) once.  So the kernel is two CTAs per SM that stream equal shares of all the call's
+// rows, whatever the lengths: the key tiles of all (sequence, KV head) items, laid end to end,
+// are cut into gridDim.x equal runs.  One warp requests a run's tiles with TMA into a ring of stages,
+// crossing from item to item without a pause (item starts bring their query rows along).  Four warps
+// take 16 (BF16) or 8 (FP32) rows of each stage, with the running maximum and sum of an online softmax in
+// base 2, and at the item's end are joined through shared memory, while the SM's other CTA streams on.  An item that a run boundary cuts
+// is joined by the CTA that finishes it last (records in the workspace, a ticket per item); the order
+// of that sum is by run, not by arrival, so results repeat exactly.
+//
+//   BF16: mma.sync m16n8k16 from ldmatrix; P as a BF16 pair (value and remainder), so that the only
+//         roundings are the operands' own and the output's.  The products are far from the bound.
+//   FP32: mma.sync m16n8k8 on TF32 halves, x = hi + lo: hi.hi + hi.lo + lo.hi, a relative error of about
+//         2^-21 per product; sums in FP32.
+#define TYB_WHOLE_PROGRAM
+#include "pages_attn.cuh"
+#include "pages_mma.cuh"
+#include "tcgen05.cuh"
+
+namespace tyb {
+
+constexpr int kTakers = 4;                       // warps that consume stages
+constexpr int kTakerThreads = 32 * kTakers;
+constexpr int kStreamThreads = kTakerThreads + 32;  // + the requesting warp
+constexpr int kMaxStages = 10;
+constexpr int kStreamRuns = 2 * kSms;            // CTAs, at most
+
+template <typename T, int D>
+struct Stream {
+    static constexpr int kKeys = sizeof(T) == 2 ? 16 : 8;   // of a warp
+    static constexpr int kRows = kTakers * kKeys;           // of a stage
+    static constexpr int kBoxCols = 128 / (int)sizeof(T);   // columns of a 128-byte box
+    static constexpr int kBoxes = D / kBoxCols;
+    static constexpr int kBox = kRows * 128;                // bytes
+    static constexpr int kHalf = kBoxes * kBox;             // K (or V) of a stage
+    static constexpr int kStage = 2 * kHalf;
+    static constexpr int kPitch = D + 4;                    // floats; joins and FP32 queries
+};
+
+// What the requesting warp tells the takers about a stage.
+struct Tile {
+    int first, last;  // of its item (in this CTA)
+    int k0;           // key of the stage's first row
+    unsigned int seen;  // a bit per 8 rows: the page is there
+    int shared;       // an item of the shared pass
+    int tok0, ntok, kvh;
+    int pos, lo, sinks;
+    int c0, c1, s0;   // the runs that have part of the item, and which record of run c0 is its
+};
+
+struct StreamArgs {
+    AttnArgs a;
+    int layer;
+    int tok_base;      // token (row of q) of this launch's first sequence
+    int shared_tiles;  // row tiles of the shared pass in this launch (0: none)
+    int shared_units;  // stages of its rows
+    int out_slot;      // record slot of a.rec that receives the results; -1: they are the output
+    int max_len;
+    int stages, q_bytes, item_rows, buffers;
+    // Records of this launch: [2 * kStreamRuns][16] rows of items cut by a run boundary; with a shared pass, uncut
+    // items too: [batch * q_heads] own rows, then [shared_tiles * kv_heads][16] shared ones.
+    float* rec_o;
+    float2* rec_ml;
+    unsigned int* tickets;  // [batch * kv_heads], zero between launches
+    unsigned long long wait_ns;
+};
+
+// `total` units in `runs` runs whose sizes differ by at most one (runs <= total < 2^31: no run is empty,
+// and 32-bit arithmetic will do).
+struct Runs {
+    unsigned int runs, base, more;  // the first `more` runs have base + 1
+    __device__ __forceinline__ Runs(unsigned int total, unsigned int n) : runs(n), base(total / n), more(total % n) {}
+    __device__ __forceinline__ unsigned int start(unsigned int run) const { return run * base + min(run, more); }
+    __device__ __forceinline__ unsigned int of(unsigned int u) const
+    {
+        const unsigned int split = more * (base + 1);
+        return u < split ? u / (base + 1) : more + (u - split) / base;
+    }
+    // The runs c0 .. c1 that units [u0, u1) lie in, and which record of run c0 is theirs (0: its first item's,
+    // 1: its last's; in the later runs they are the first item).
+    __device__ __forceinline__ void span(unsigned int u0, unsigned int u1, int& c0, int& c1, int& s0) const
+    {
+        c0 = (int)of(u0);
+        c1 = (int)of(u1 - 1);
+        s0 = start(c0) < u0;
+    }
+};
+
+// Four output columns joined over several records: maximum (base 2), sum, values.
+struct Gather {
+    float m = -INFINITY, l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    __device__ __forceinline__ void add(float2 ml, float4 x)
+    {
+        // a record that saw nothing has l = 0, o = 0 and m = -inf: its factor is 0
+        const float top = fmaxf(m, ml.x), f = m == -INFINITY ? 0.f : fast_exp2(m - top), e = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - top);
+        m = top;
+        l = l * f + ml.y * e;
+        o.x = o.x * f + x.x * e;
+        o.y = o.y * f + x.y * e;
+        o.z = o.z * f + x.z * e;
+        o.w = o.w * f + x.w * e;
+    }
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kStreamThreads, 2)
+    pages_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const StreamArgs sa)
+{
+    using S = Stream<T, D>;
+    const AttnArgs& a = sa.a;
+    extern __shared__ __align__(1024) unsigned char raw[];
+    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+    unsigned char* ring = smem;
+    float* joins = reinterpret_cast<float*>(ring + sa.stages * S::kStage);  // [buffers][kTakers][item_rows][kPitch]
+    float* split_q = joins + sa.buffers * kTakers * sa.item_rows * S::kPitch;  // FP32: hi and lo, [split_rows][kPitch] each
+    const int split_rows = sa.item_rows <= 8 ? 8 : 16;
+    unsigned char* qs = reinterpret_cast<unsigned char*>(split_q + (sizeof(T) == 4 ? 2 * split_rows * S::kPitch : 0));  // [stages][q_bytes]
+    int* cum = reinterpret_cast<int*>(qs + sa.stages * sa.q_bytes);        // units before each sequence
+    int* lens = cum + a.batch + 1;
+
+    __shared__ uint64_t full[kMaxStages], empty[kMaxStages], met;
+    __shared__ Tile tiles_of_stage[kMaxStages];
+    __shared__ float2 join_mls[2][kTakers][16];
+    __shared__ int scan[kStreamThreads / 32];
+    __shared__ unsigned int last_of;  // tokens whose join is this CTA's
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int heads = a.p.kv_heads, run = blockIdx.x;
+
+    if (tid == 0) {
+        for (int i = 0; i < sa.stages; i++) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], kTakers);
+        }
+        mbar_init(&met, kTakers);
+        fence_barrier_init();
+    }
+    // Units (stages) of each sequence's own rows: at least one, so that every output row has an owner.
+    auto own_lo = [&](int len) { return a.window ? max(0, len - a.window) : min(a.prefix, len); };
+    long long before = 0;
+    for (int base = 0; base < a.batch; base += kStreamThreads) {
+        const int b = base + tid;
+        int len = 0, n = 0;
+        if (b < a.batch) {
+            len = checked_len(a.p, a.seqs[b], a.st);
+            if (len > sa.max_len) {
+                raise(a.st, TYB_STATUS_BAD_ARGUMENT);
+                len = 0;
+            }
+            n = max(1, tiles_of(len - 1, own_lo(len), a.sinks, S::kRows).count());
+        }
+        int sum = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += y;
+        }
+        if (lane == 31) scan[warp] = sum;
+        __syncthreads();
+        int add = (int)before;
+        for (int w = 0; w < kStreamThreads / 32; w++) {
+            if (w < warp) add += scan[w];
+            before += scan[w];
+        }
+        if (b < a.batch) {
+            cum[b] = add + sum - n;
+            lens[b] = len;
+        }
+        __syncthreads();
+    }
+    if (tid == 0) cum[a.batch] = (int)before;
+    __syncthreads();
+    const unsigned long long all = ((unsigned long long)sa.shared_tiles * sa.shared_units + before) * heads;
+    if (all >= 1ull << 31) {  // only tables that name pages over and over
+        if (tid == 0) raise(a.st, TYB_STATUS_BAD_ARGUMENT);
+        return;
+    }
+    const Runs cuts((unsigned int)all, min(gridDim.x, (unsigned int)all));
+    if (run >= (int)cuts.runs) return;
+    const unsigned int shared_all = (unsigned int)sa.shared_tiles * sa.shared_units * heads;
+    const unsigned int begin = cuts.start(run), end = cuts.start(run + 1);
+    const int per = 16 / a.group;  // tokens of a shared row tile
+
+    if (warp == kTakers) {
+        // ---- requests
+        const int sub = min(a.p.page_size, S::kRows), subs = S::kRows / sub, shift = page_shift(a.p.page_size);
+        const unsigned int sub_bits = (1u << (sub / 8)) - 1u;
+        const size_t esize = a.io_bf16 ? 2 : 4;
+        Tile tile = {};
+        Tiles list = {};
+        const int* table = a.p.table;
+        unsigned int u = begin, u0 = 0, u1 = 0;  // the current item's units
+        int b = 0, st = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (; u < end; u++) {
+            const bool start = u == begin || u >= u1;
+            if (start) {  // the item that unit u lies in
+                if (u < shared_all) {
+                    const unsigned int item = u / sa.shared_units;
+                    u0 = item * sa.shared_units;
+                    u1 = u0 + sa.shared_units;
+                    tile.shared = 1;
+                    tile.kvh = (int)(item % heads);
+                    tile.tok0 = (int)(item / heads) * per;
+                    tile.ntok = min(per, a.batch - tile.tok0);
+                    tile.sinks = 0;
+                    tile.lo = 0;
+                    tile.pos = min(a.prefix, lens[0]) - 1;
+                    const int s = a.seqs[0];
+                    table = a.p.table + (size_t)(lens[0] ? s : 0) * a.p.max_pages;
+                } else {
+                    if (u == begin) {  // which sequence: cum[b] * heads <= u - shared_all
+                        int lo = 0, hi = a.batch;
+                        while (hi - lo > 1) {
+                            const int mid = (lo + hi) >> 1;
+                            if ((unsigned int)(cum[mid] * heads) <= u - shared_all) lo = mid;
+                            else hi = mid;
+                        }
+                        b = lo;
+                    } else if (u - shared_all >= (unsigned int)(cum[b + 1] * heads)) {
+                        b++;
+                    }
+                    const unsigned int units = cum[b + 1] - cum[b], at = u - shared_all - cum[b] * heads;
+                    tile.kvh = (int)(at / units);
+                    u0 = u - at % units;
+                    u1 = u0 + units;
+                    tile.shared = 0;
+                    tile.tok0 = b;
+                    tile.ntok = 1;
+                    tile.sinks = a.sinks;
+                    tile.pos = lens[b] - 1;
+                    tile.lo = own_lo(lens[b]);
+                    table = a.p.table + (size_t)(lens[b] ? a.seqs[b] : 0) * a.p.max_pages;
+                }
+                cuts.span(u0, u1, tile.c0, tile.c1, tile.s0);
+                list = tiles_of(tile.pos, tile.lo, tile.sinks, S::kRows);
+            }
+            tile.first = start;
+            tile.last = u + 1 == u1 || u + 1 == end;
+            const int i = (int)(u - u0);
+            tile.k0 = i < list.count() ? list.at(i) * S::kRows : tile.pos + 1;
+            // lane l < subs: the page (or part of one) at rows l * sub of the stage
+            int page = -1;
+            const int key = tile.k0 + lane * sub;
+            if (lane < subs && i < list.count() && key <= tile.pos) {
+                page = table[key >> shift];
+                if (page >= a.p.num_pages) {
+                    raise(a.st, TYB_STATUS_BAD_ARGUMENT);
+                    page = -1;
+                }
+            }
+            const unsigned int have = __ballot_sync(0xffffffffu, page >= 0);
+            tile.seen = 0;
+            for (int l = 0; l < subs; l++)
+                if (have >> l & 1u) tile.seen |= sub_bits << (l * (sub / 8));
+            if (u - begin >= (unsigned int)sa.stages) {
+                ok = wait_for(&empty[st], phase ^ 1u, sa.wait_ns, a.st);
+                if (__any_sync(0xffffffffu, !ok)) break;
+            }
+            const uint32_t q_row = (uint32_t)(a.group * D * esize);
+            if (lane == 0) {
+                tiles_of_stage[st] = tile;
+                mbar_arrive_expect_tx(&full[st], (uint32_t)__popc(have) * (uint32_t)(sub * 128 * S::kBoxes * 2) +
+                                                     (start ? q_row * (uint32_t)tile.ntok : 0u));
+            }
+            __syncwarp();
+            unsigned char* to = ring + st * S::kStage;
+            if (page >= 0) {
+                const int row = ((sa.layer * a.p.num_pages + page) * heads + tile.kvh) * a.p.page_size + (key & (a.p.page_size - 1));
+#pragma unroll
+                for (int c = 0; c < S::kBoxes; c++) {
+                    tma_load_2d(to + c * S::kBox + lane * sub * 128, &map_k, c * S::kBoxCols, row, &full[st]);
+                    tma_load_2d(to + S::kHalf + c * S::kBox + lane * sub * 128, &map_v, c * S::kBoxCols, row, &full[st]);
+                }
+            }
+            if (start && lane < tile.ntok)
+                bulk_g2s(qs + st * sa.q_bytes + lane * q_row,
+                         static_cast<const char*>(a.q) +
+                             ((size_t)(sa.tok_base + tile.tok0 + lane) * a.q_stride + (size_t)tile.kvh * a.group * D) * esize,
+                         q_row, &full[st]);
+            if (++st == sa.stages) {
+                st = 0;
+                phase ^= 1u;
+            }
+        }
+        if (__any_sync(0xffffffffu, !ok)) {  // a wait ran out: the copies requested still land in this CTA
+            const unsigned int sent = u - begin, stages = sa.stages;
+            for (unsigned int n = sent > stages ? sent - stages : 0; n < sent; n++)
+                wait_for(&full[n % stages], n / stages & 1u, sa.wait_ns, a.st);
+        }
+        return;
+    }
+
+    // ---- takers
+    const int g = lane >> 2, t = lane & 3, r0 = warp * S::kKeys;
+    Rows<T, D> w;
+    w.clear();
+    int st = 0;
+    uint32_t phase = 0;
+    bool one_item = true;  // no item has ended in this run yet
+    int buffer = 0;        // of the join rows: two, used in turn
+    // Rows of the records: of a cut item's part in a run, of uncut own rows, of an uncut shared item.
+    auto part_row = [&](int run_of, int second) { return (size_t)(2 * run_of + second) * 16; };
+    auto own_row = [&](int tok, int kvh) { return (size_t)2 * kStreamRuns * 16 + (size_t)tok * a.q_heads + kvh * a.group; };
+    auto shared_row = [&](int tok, int kvh) {
+        return (size_t)2 * kStreamRuns * 16 + (size_t)a.batch * a.q_heads + ((size_t)(tok / per) * heads + kvh) * 16;
+    };
+    // The takers meet at an mbarrier rather than a CTA barrier: its wait is bounded, so that a warp whose
+    // wait ran out and left does not leave the others waiting.
+    uint32_t meeting = 0;
+    auto meet = [&]() {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&met);
+        const bool ok = wait_for(&met, meeting, sa.wait_ns, a.st);
+        meeting ^= 1u;
+        return !__any_sync(0xffffffffu, !ok);
+    };
+    // A finished row block: the output, or its record for the join kernel.
+    auto deliver = [&](size_t R, int c, const Gather& x) {
+        if (sa.out_slot < 0) {
+            put_out(a, R * D + c, x.o, x.l);
+        } else {
+            const size_t at = (size_t)sa.out_slot * a.rec.rows + R;
+            *reinterpret_cast<float4*>(a.rec.o + at * D + c) = x.o;
+            if (c == 0) a.rec.ml[at] = make_float2(x.m, x.l);
+        }
+    };
+    // Four columns of a row, joined over the warps' shares in shared memory.
+    auto over_warps = [&](int row, int c) {
+        const float* join = joins + buffer * kTakers * sa.item_rows * S::kPitch;
+        const float2(*join_ml)[16] = join_mls[buffer];
+        Gather sum;
+#pragma unroll
+        for (int x = 0; x < kTakers; x++)
+            sum.add(join_ml[x][row], *reinterpret_cast<const float4*>(join + (x * sa.item_rows + row) * S::kPitch + c));
+        return sum;
+    };
+    for (unsigned int u = begin; u < end; u++) {
+        const bool here = wait_for(&full[st], phase, sa.wait_ns, a.st);
+        if (__any_sync(0xffffffffu, !here)) return;
+        const Tile tile = tiles_of_stage[st];
+        const int nrows = tile.ntok * a.group;
+        if (tile.first) {
+            w.load_q(qs + st * sa.q_bytes, nrows, a.io_bf16, g, t, split_q, split_rows, tid, kTakerThreads);
+            if (sizeof(T) == 4 && !meet()) return;
+        }
+        const int j0 = tile.k0 + r0;
+        unsigned char* rows_k = ring + st * S::kStage;
+        unsigned char* rows_v = rows_k + S::kHalf;
+        const unsigned int want = (1u << (S::kKeys / 8)) - 1u, seen = tile.seen >> (r0 / 8) & want;
+        // none of the warp's rows in sight: nothing to do
+        const bool any = seen && j0 <= tile.pos && (j0 + S::kKeys > tile.lo || j0 < tile.sinks);
+        if (any) {
+            unsigned int see = (1u << S::kKeys) - 1u;  // bit i: row j0 + i
+            if (seen != want || j0 + S::kKeys - 1 > tile.pos || (j0 < tile.lo && j0 + S::kKeys > tile.sinks)) {
+                auto under = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; };
+                unsigned int pages = seen & 1u ? 0xffu : 0u;
+                if (seen & 2u) pages |= 0xff00u;
+                see &= pages & under(tile.pos + 1 - j0) & (~under(tile.lo - j0) | under(tile.sinks - j0));
+                // what lies in rows out of sight may be anything, and 0 * NaN is not 0
+                for (int i = 0; i < S::kKeys; i++)
+                    if (!(see >> i & 1u) && lane < D * (int)sizeof(T) / 16)
+                        *reinterpret_cast<uint4*>(rows_v + (lane >> 3) * S::kBox + (r0 + i) * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+                fence_proxy_async_smem();
+                __syncwarp();
+            }
+            w.step(rows_k, rows_v, S::kBox, r0, see, a.scale_log2, split_q, g, t, lane);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[st]);
+        if (++st == sa.stages) {
+            st = 0;
+            phase ^= 1u;
+        }
+        if (!tile.last) continue;
+
+        // ---- the item's end in this run: join the warps.  With two buffers the next item's join rows are the
+        // other one's, and these are written again only after all have met there; with one, they meet first.
+        if (sa.buffers == 2) buffer ^= 1;
+        else if (!meet()) return;
+        float* join = joins + buffer * kTakers * sa.item_rows * S::kPitch;
+        float2(*join_ml)[16] = join_mls[buffer];
+        w.finish();
+        if (t == 0) {
+            join_ml[warp][g] = make_float2(w.m[0], w.l[0]);
+            join_ml[warp][g + 8] = make_float2(w.m[1], w.l[1]);
+        }
+#pragma unroll
+        for (int r = 0; r < 2; r++)
+            if (g + 8 * r < nrows)
+#pragma unroll
+                for (int c = 0; c < D / 8; c++)
+                    *reinterpret_cast<float2*>(join + (warp * sa.item_rows + g + 8 * r) * S::kPitch + 8 * c + 2 * t) =
+                        make_float2(w.o[c][2 * r], w.o[c][2 * r + 1]);
+        w.clear();  // (and so not kept through what follows)
+        if (!meet()) return;
+        const bool cut = tile.c0 != tile.c1, direct = !cut && !sa.shared_tiles;
+        const size_t record = cut ? part_row(run, one_item ? 0 : 1) : tile.shared ? shared_row(tile.tok0, tile.kvh) : own_row(tile.tok0, tile.kvh);
+        one_item = false;
+        for (int i = tid; i < nrows * (D / 4); i += kTakerThreads) {
+            const int row = i / (D / 4), c = i % (D / 4) * 4;
+            const Gather sum = over_warps(row, c);
+            if (direct) {
+                deliver((size_t)(sa.tok_base + tile.tok0) * a.q_heads + tile.kvh * a.group + row, c, sum);
+            } else {
+                *reinterpret_cast<float4*>(sa.rec_o + (record + row) * D + c) = sum.o;
+                if (c == 0) sa.rec_ml[record + row] = make_float2(sum.m, sum.l);
+            }
+        }
+        if (direct) continue;
+
+        // Tickets: of each sequence that the item has rows of, this run's record is there; the last to come
+        // joins that sequence's rows.
+        __threadfence();
+        if (tid == 0) last_of = 0;
+        if (!meet()) return;
+        // the records of (token, KV head): where its shared ones and its own ones lie
+        auto spans = [&](int tok, Tile& sh, Tile& ow) {
+            ow = sh = tile;
+            if (tile.shared) {
+                const unsigned int units = cum[tok + 1] - cum[tok], v0 = shared_all + cum[tok] * heads + tile.kvh * units;
+                cuts.span(v0, v0 + units, ow.c0, ow.c1, ow.s0);
+            } else if (sa.shared_tiles) {
+                const unsigned int v0 = ((unsigned int)(tok / per) * heads + tile.kvh) * sa.shared_units;
+                cuts.span(v0, v0 + sa.shared_units, sh.c0, sh.c1, sh.s0);
+            }
+            if (!sa.shared_tiles) sh.c0 = 0, sh.c1 = -1;
+        };
+        if (tid < tile.ntok) {
+            Tile sh, ow;
+            spans(tile.tok0 + tid, sh, ow);
+            const unsigned int count = (unsigned int)(ow.c1 - ow.c0 + 1 + sh.c1 - sh.c0 + 1);
+            unsigned int* ticket = sa.tickets + (size_t)(tile.tok0 + tid) * heads + tile.kvh;
+            if (atomicAdd(ticket, 1u) == count - 1u) {
+                *ticket = 0u;
+                atomicOr(&last_of, 1u << tid);
+            }
+        }
+        if (!meet()) return;
+        const unsigned int mine = last_of;
+        if (!mine) continue;
+        __threadfence();
+        // The rows of all those sequences at once: `teams` warps a row, each with some of its records, eight
+        // requested at a time; then the warps are joined.
+        const int rows = __popc(mine) * a.group, teams = rows >= kTakers ? 1 : kTakers / rows;
+        auto token_of = [&](int k) {  // of the k-th sequence to join
+            unsigned int left = mine;
+            for (; k > 0; k--) left &= left - 1;
+            return __ffs(left) - 1;
+        };
+        for (int j = warp; j < rows * teams; j += kTakers) {
+            const int row = j / teams, part = j % teams, k = token_of(row / a.group), in_head = row % a.group, tok = tile.tok0 + k;
+            Tile sh, ow;
+            spans(tok, sh, ow);
+            const int ns = sh.c1 - sh.c0 + 1, n = ns + ow.c1 - ow.c0 + 1;
+            auto row_of = [&](int x) {
+                if (x < ns) return (ns == 1 ? shared_row(tok, tile.kvh) : part_row(sh.c0 + x, x ? 0 : sh.s0)) + tok % per * a.group + in_head;
+                x -= ns;
+                return (ow.c0 == ow.c1 ? own_row(tok, tile.kvh) : part_row(ow.c0 + x, x ? 0 : ow.s0)) + in_head;
+            };
+            const int c = lane % (D / 4) * 4;  // D = 64: two lanes have the same columns
+            Gather sum;
+            for (int x = part; x < n; x += 8 * teams) {
+                float2 ml[8];
+                float4 o[8];
+#pragma unroll
+                for (int y = 0; y < 8; y++) {
+                    const size_t at = row_of(min(x + y * teams, n - 1));
+                    ml[y] = __ldcg(&sa.rec_ml[at]);
+                    o[y] = __ldcg(reinterpret_cast<const float4*>(sa.rec_o + at * D + c));
+                }
+#pragma unroll
+                for (int y = 0; y < 8; y++)
+                    if (x + y * teams < n) sum.add(ml[y], o[y]);
+            }
+            const size_t R = (size_t)(sa.tok_base + tok) * a.q_heads + tile.kvh * a.group + in_head;
+            if (teams == 1) {
+                if (lane < D / 4) deliver(R, c, sum);
+            } else if (lane < D / 4) {
+                *reinterpret_cast<float4*>(join + (part * sa.item_rows + row) * S::kPitch + c) = sum.o;
+                if (c == 0) join_ml[part][row] = make_float2(sum.m, sum.l);
+            }
+        }
+        if (teams > 1) {
+            if (!meet()) return;
+            for (int i = tid; i < rows * (D / 4); i += kTakerThreads) {
+                const int row = i / (D / 4), c = i % (D / 4) * 4, tok = tile.tok0 + token_of(row / a.group);
+                Gather sum;
+                for (int x = 0; x < teams; x++)
+                    sum.add(join_ml[x][row], *reinterpret_cast<const float4*>(join + (x * sa.item_rows + row) * S::kPitch + c));
+                deliver((size_t)(sa.tok_base + tok) * a.q_heads + tile.kvh * a.group + row % a.group, c, sum);
+            }
+        }
+        // (the next item's meeting comes before these join rows are written again)
+    }
+}
+
+// ---- host --------------------------------------------------------------------------------------
+
+constexpr int kSmemMax = 227 * 1024, kSmemSm = 228 * 1024, kStaticMax = 2048;  // the kernel's own shared arrays: at most this
+
+static int shared_tiles_of(const AttnArgs& a, int count) { return (count + 16 / a.group - 1) / (16 / a.group); }
+
+template <typename T, int D>
+static int launch_stream_t(StreamArgs sa, const void* maps, cudaStream_t stream)
+{
+    using S = Stream<T, D>;
+    static bool ready[64];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return (int)e;
+    if (dev < 0 || dev >= 64) return (int)cudaErrorInvalidDevice;
+    const int tokens = sa.shared_tiles ? 16 / sa.a.group : 1;  // of an item, at most
+    sa.q_bytes = (tokens * sa.a.group * D * (sa.a.io_bf16 ? 2 : 4) + 127) / 128 * 128;
+    sa.item_rows = tokens * sa.a.group;
+    // Two CTAs per SM where that leaves each two stages or more, else one.
+    sa.buffers = sa.item_rows <= 4 ? 2 : 1;
+    const int fixed = sa.buffers * kTakers * sa.item_rows * S::kPitch * 4 + (2 * sa.a.batch + 1) * 4 + 1024 +  // + alignment
+                      (sizeof(T) == 4 ? 2 * (sa.item_rows <= 8 ? 8 : 16) * S::kPitch * 4 : 0);
+    int ctas = 2, most = kSmemSm / 2 - 1024 - kStaticMax;
+    if ((most - fixed) / (S::kStage + sa.q_bytes) < 2) {
+        ctas = 1;
+        most = kSmemMax - kStaticMax;
+    }
+    sa.stages = (most - fixed) / (S::kStage + sa.q_bytes);
+    if (sa.stages > kMaxStages) sa.stages = kMaxStages;
+    const int bytes = sa.stages * (S::kStage + sa.q_bytes) + fixed;
+    if (!ready[dev]) {
+        e = cudaFuncSetAttribute(pages_stream_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax - kStaticMax);
+        if (e == cudaSuccess)
+            e = cudaFuncSetAttribute(pages_stream_kernel<T, D>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+        if (e != cudaSuccess) return (int)e;
+        ready[dev] = true;
+    }
+    const CUtensorMap* m = static_cast<const CUtensorMap*>(maps);
+    pages_stream_kernel<T, D><<<ctas * kSms, kStreamThreads, bytes, stream>>>(m[0], m[1], sa);
+    return (int)cudaGetLastError();
+}
+
+// Record rows of one launch for `count` sequences.
+static size_t record_rows(const AttnArgs& a, int count, bool shared)
+{
+    return (size_t)2 * kStreamRuns * 16 + (shared ? (size_t)count * a.q_heads + (size_t)shared_tiles_of(a, count) * a.p.kv_heads * 16 : 0);
+}
+
+size_t stream_bytes(const AttnArgs& a, int count, bool shared)
+{
+    return record_rows(a, count, shared) * (a.p.head_dim * sizeof(float) + sizeof(float2));
+}
+
+int launch_stream(const AttnArgs& a, int layer, int first, int count, bool shared, int out_slot, int max_len, const void* maps, void* ws,
+                  unsigned int* tickets, cudaStream_t stream)
+{
+    const int D = a.p.head_dim;
+    StreamArgs sa = {};
+    sa.a = a;
+    sa.a.seqs = a.seqs + first;
+    sa.a.batch = count;
+    sa.layer = layer;
+    sa.tok_base = first;
+    const int rows = a.p.kv_dtype == TYB_BF16 ? 64 : 32;  // of a stage
+    sa.shared_tiles = shared ? shared_tiles_of(a, count) : 0;
+    sa.shared_units = shared ? (a.prefix + rows - 1) / rows : 0;
+    sa.out_slot = out_slot;
+    sa.max_len = max_len;
+    sa.rec_o = static_cast<float*>(ws);
+    sa.rec_ml = reinterpret_cast<float2*>(sa.rec_o + record_rows(a, count, shared) * D);
+    sa.tickets = tickets;
+    sa.wait_ns = tyb_wait_limit();
+    if (a.p.kv_dtype == TYB_BF16)
+        return D == 128 ? launch_stream_t<__nv_bfloat16, 128>(sa, maps, stream) : launch_stream_t<__nv_bfloat16, 64>(sa, maps, stream);
+    return D == 128 ? launch_stream_t<float, 128>(sa, maps, stream) : launch_stream_t<float, 64>(sa, maps, stream);
+}
+
+}  // namespace tyb
