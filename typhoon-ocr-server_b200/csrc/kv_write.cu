@@ -188,9 +188,13 @@ extern "C" int tyb_set_wait_limit(unsigned long long ns)
     return 0;
 }
 
+extern "C" unsigned long long tyb_wait_limit_of(int dev)
+{
+    return dev < 0 || dev >= 64 || !g_wait_limit_host[dev] ? kWaitLimitNs : g_wait_limit_host[dev];
+}
+
 extern "C" unsigned long long tyb_wait_limit(void)
 {
     int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64 || !g_wait_limit_host[dev]) return kWaitLimitNs;
-    return g_wait_limit_host[dev];
+    return tyb_wait_limit_of(cudaGetDevice(&dev) == cudaSuccess ? dev : -1);
 }

@@ -21,8 +21,8 @@
 typedef struct {
     KVPages pub; /* first: the KVPages* handed out converts back */
     uint32_t magic;
-    int device;
     int owned;
+    tyb_pages_env env;
     _Alignas(64) unsigned char maps[TYB_PAGES_MAPS_BYTES];
 } tyb_pages;
 
@@ -111,8 +111,8 @@ static tyb_pages *pages_from(const KVPages *p, const char *what)
     }
     int dev = -1;
     if (!tyb_cuda_ok(cudaGetDevice(&dev), what)) return NULL;
-    if (dev != t->device) {
-        tyb_set_error("%s: the pool is on device %d, the current device is %d", what, t->device, dev);
+    if (dev != t->env.device) {
+        tyb_set_error("%s: the pool is on device %d, the current device is %d", what, t->env.device, dev);
         return NULL;
     }
     return t;
@@ -168,11 +168,18 @@ static tyb_pages *make(const KVPages *dims, int owned, const char *what)
     t->pub = *dims;
     t->magic = TYB_PAGES_MAGIC;
     t->owned = owned;
-    if (!tyb_cuda_ok(cudaGetDevice(&t->device), what)) {
+    if (!tyb_cuda_ok(cudaGetDevice(&t->env.device), what)) {
         free(t);
         return NULL;
     }
     if (tyb_status_mirror_setup() != 0) cudaGetLastError(); /* as in kv_cache_alloc_ex */
+    t->env.status = tyb_status_word();
+    t->env.mirror = tyb_status_mirror_device();
+    if (!t->env.status) {
+        tyb_set_error("%s: no status word on device %d", what, t->env.device);
+        free(t);
+        return NULL;
+    }
     return t;
 }
 
@@ -271,8 +278,8 @@ int kv_pages_extend(KVPages *p, const int *seqs, const int *counts, int n)
     if (!t) return 1;
     if (!list_ready(seqs, n, "seqs", &rc, what)) return rc;
     if (!on_device(counts, 4, "counts", what)) return 1;
-    void *ws = workspace(t->device, WS_SCRATCH, tyb_pages_plan_bytes(p, n), what);
-    return ws ? launched(tyb_pages_extend_launch(p, seqs, counts, n, ws, tyb_stream()), what) : 1;
+    void *ws = workspace(t->env.device, WS_SCRATCH, tyb_pages_plan_bytes(p, n), what);
+    return ws ? launched(tyb_pages_extend_launch(p, &t->env, seqs, counts, n, ws, tyb_stream()), what) : 1;
 }
 
 static int fork_or_copy(KVPages *p, const int *src, const int *dst, int n, int deep, const char *what)
@@ -282,8 +289,8 @@ static int fork_or_copy(KVPages *p, const int *src, const int *dst, int n, int d
     if (!t) return 1;
     if (!list_ready(src, n, "src", &rc, what)) return rc;
     if (!on_device(dst, 4, "dst", what)) return 1;
-    void *ws = workspace(t->device, WS_SCRATCH, tyb_pages_plan_bytes(p, n), what);
-    return ws ? launched(tyb_pages_fork_launch(p, src, dst, n, deep, ws, tyb_stream()), what) : 1;
+    void *ws = workspace(t->env.device, WS_SCRATCH, tyb_pages_plan_bytes(p, n), what);
+    return ws ? launched(tyb_pages_fork_launch(p, &t->env, src, dst, n, deep, ws, tyb_stream()), what) : 1;
 }
 
 int kv_pages_fork(KVPages *p, const int *src, const int *dst, int n) { return fork_or_copy(p, src, dst, n, 0, "kv_pages_fork"); }
@@ -294,22 +301,24 @@ int kv_pages_free(KVPages *p, const int *seqs, int n)
 {
     const char *what = "kv_pages_free";
     int rc;
-    if (!pages_from(p, what)) return 1;
+    tyb_pages *t = pages_from(p, what);
+    if (!t) return 1;
     if (!list_ready(seqs, n, "seqs", &rc, what)) return rc;
-    return launched(tyb_pages_free_launch(p, seqs, n, tyb_stream()), what);
+    return launched(tyb_pages_free_launch(p, &t->env, seqs, n, tyb_stream()), what);
 }
 
 int kv_pages_trim(KVPages *p, const int *seqs, int n, int window, int sinks)
 {
     const char *what = "kv_pages_trim";
     int rc;
-    if (!pages_from(p, what)) return 1;
+    tyb_pages *t = pages_from(p, what);
+    if (!t) return 1;
     if (window < 1 || sinks < 0) {
         tyb_set_error("%s: window %d must be at least 1 and sinks %d not negative", what, window, sinks);
         return 1;
     }
     if (!list_ready(seqs, n, "seqs", &rc, what)) return rc;
-    return launched(tyb_pages_trim_launch(p, seqs, n, window, sinks, tyb_stream()), what);
+    return launched(tyb_pages_trim_launch(p, &t->env, seqs, n, window, sinks, tyb_stream()), what);
 }
 
 int kv_pages_compact(KVPages *p, int *live_out)
@@ -317,7 +326,7 @@ int kv_pages_compact(KVPages *p, int *live_out)
     const char *what = "kv_pages_compact";
     tyb_pages *t = pages_from(p, what);
     if (!t || (live_out && !on_device(live_out, 4, "live_out", what))) return 1;
-    void *ws = workspace(t->device, WS_SCRATCH, tyb_pages_plan_bytes(p, 0), what);
+    void *ws = workspace(t->env.device, WS_SCRATCH, tyb_pages_plan_bytes(p, 0), what);
     return ws ? launched(tyb_pages_compact_launch(p, live_out, ws, tyb_stream()), what) : 1;
 }
 
@@ -348,7 +357,8 @@ int kv_pages_write(KVPages *p, int layer, const int *seqs, const int *starts, in
 {
     const char *what = "kv_pages_write";
     int rc;
-    if (!pages_from(p, what) || !check_layer(p, layer, what)) return 1;
+    tyb_pages *t = pages_from(p, what);
+    if (!t || !check_layer(p, layer, what)) return 1;
     if (rows < 0 || rows > 1 << 28) {
         tyb_set_error("%s: rows %d out of range", what, rows);
         return 1;
@@ -359,7 +369,7 @@ int kv_pages_write(KVPages *p, int layer, const int *seqs, const int *starts, in
     if (!on_device(starts, 4, "starts", what) || !check_rows(k_new, in_dtype, stride, width, "k_new", what) ||
         !check_rows(v_new, in_dtype, stride, width, "v_new", what))
         return 1;
-    return launched(tyb_pages_write_launch(p, layer, seqs, starts, n, rows, k_new, v_new, in_dtype == ATTN_DT_BF16, stride,
+    return launched(tyb_pages_write_launch(p, &t->env, layer, seqs, starts, n, rows, k_new, v_new, in_dtype == ATTN_DT_BF16, stride,
                                            tyb_stream()),
                     what);
 }
@@ -372,7 +382,7 @@ int kv_pages_import(KVPages *p, int seq, const KVCache *cache)
     tyb_cache *c = tyb_cache_from(cache);
     if (!c) return 1;
     if (p->num_layers != KV_NUM_LAYERS || p->kv_heads != KV_NUM_KV_HEADS || p->head_dim != KV_HEAD_DIM ||
-        p->kv_dtype != kv_cache_dtype(cache) || c->device != t->device) {
+        p->kv_dtype != kv_cache_dtype(cache) || c->device != t->env.device) {
         tyb_set_error("%s: the pool's layers, heads, element type and device have to be the cache's", what);
         return 1;
     }
@@ -388,9 +398,9 @@ int kv_pages_import(KVPages *p, int seq, const KVCache *cache)
     for (int l = 0; l < KV_NUM_LAYERS; l++)
         if (!tyb_flush_pending(c, l, what)) return 1;
     if (rows == 0) return 0;
-    void *ws = workspace(t->device, WS_SCRATCH, tyb_pages_plan_bytes(p, 1), what);
+    void *ws = workspace(t->env.device, WS_SCRATCH, tyb_pages_plan_bytes(p, 1), what);
     if (!ws) return 1;
-    return launched(tyb_pages_import_launch(p, seq, c->k_slab, c->v_slab, cache->max_seq_len, rows, ws, tyb_stream()), what);
+    return launched(tyb_pages_import_launch(p, &t->env, seq, c->k_slab, c->v_slab, cache->max_seq_len, rows, ws, tyb_stream()), what);
 }
 
 /* ---- attention ------------------------------------------------------------------------------ */
@@ -419,12 +429,15 @@ static int attend(const KVPages *p, tyb_pages_attn *a, const char *what)
     if (!check_rows(a->q, a->io_bf16 ? ATTN_DT_BF16 : ATTN_DT_F32, a->q_stride, (long long)a->q_heads * p->head_dim, "q", what) ||
         !on_device(a->out, 16, "output", what) || !on_device(a->seqs, 4, "seqs", what))
         return 1;
+    /* The shared pass takes whole pages: each sequence has its own copy of a partly filled one. */
+    a->prefix -= a->prefix % p->page_size;
     a->p = *p;
     a->maps = t->maps;
+    a->env = t->env;
     size_t bytes, ticket_bytes;
     tyb_pages_attn_bytes(a, &bytes, &ticket_bytes);
-    void *ws = bytes ? workspace(t->device, WS_SCRATCH, bytes, what) : NULL;
-    void *tickets = ticket_bytes ? workspace(t->device, WS_TICKETS, ticket_bytes, what) : NULL;
+    void *ws = bytes ? workspace(t->env.device, WS_SCRATCH, bytes, what) : NULL;
+    void *tickets = ticket_bytes ? workspace(t->env.device, WS_TICKETS, ticket_bytes, what) : NULL;
     if ((bytes && !ws) || (ticket_bytes && !tickets)) return 1;
     return launched(tyb_pages_attn_launch(a, ws, tickets, tyb_stream()), what);
 }
@@ -448,9 +461,7 @@ int attention_pages_prefix_gqa(const void *q, long long q_stride, const KVPages 
     tyb_pages_attn a = {.layer = layer, .q = q, .q_stride = q_stride, .out = output, .io_bf16 = io_dtype == ATTN_DT_BF16,
                         .q_heads = q_heads, .seqs = seqs, .batch = batch, .rows = batch, .max_new = 1, .max_len = max_len,
                         .scale = scale};
-    /* The shared pass takes whole pages: each sequence has its own copy of a partly filled one. */
-    if (pages_from(p, what)) a.prefix = prefix_len / p->page_size * p->page_size;
-    if (batch == 1) a.prefix = 0; /* nothing to share */
+    a.prefix = batch == 1 ? 0 : prefix_len; /* one alone has nothing to share */
     return attend(p, &a, what);
 }
 

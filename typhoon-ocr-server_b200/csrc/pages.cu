@@ -449,12 +449,7 @@ __global__ void __launch_bounds__(kApplyThreads)
 
 static int row_bytes_of(const KVPages* p) { return p->head_dim * (p->kv_dtype == TYB_BF16 ? 2 : 4); }
 
-static int status_of(Status* st)
-{
-    st->word = tyb_status_word();
-    st->mirror = tyb_status_mirror_device();
-    return st->word ? 0 : (int)cudaErrorInvalidSymbol;
-}
+static Status status_of(const tyb_pages_env* env) { return {env->status, env->mirror}; }
 
 // Shared memory of the duplicate check, above the default limit for pools of many sequences.
 template <typename K>
@@ -471,23 +466,21 @@ using namespace tyb;
 
 extern "C" size_t tyb_pages_plan_bytes(const KVPages* p, int n) { return plan_bytes(n, p->num_pages); }
 
-extern "C" int tyb_pages_extend_launch(const KVPages* p, const int* seqs, const int* counts, int n, void* ws, void* stream)
+extern "C" int tyb_pages_extend_launch(const KVPages* p, const tyb_pages_env* env, const int* seqs, const int* counts, int n, void* ws, void* stream)
 {
-    Status st;
+    const Status st = status_of(env);
     size_t marks;
-    int e = status_of(&st);
-    if (!e) e = marks_bytes(pages_extend_kernel, p, &marks);
+    int e = marks_bytes(pages_extend_kernel, p, &marks);
     if (e) return e;
     pages_extend_kernel<<<1, kPlanThreads, marks, (cudaStream_t)stream>>>(*p, seqs, counts, n, 0, 0, ws, st);
     return (int)cudaGetLastError();
 }
 
-extern "C" int tyb_pages_fork_launch(const KVPages* p, const int* src, const int* dst, int n, int deep, void* ws, void* stream)
+extern "C" int tyb_pages_fork_launch(const KVPages* p, const tyb_pages_env* env, const int* src, const int* dst, int n, int deep, void* ws, void* stream)
 {
-    Status st;
+    const Status st = status_of(env);
     size_t marks;
-    int e = status_of(&st);
-    if (!e) e = marks_bytes(pages_fork_plan_kernel, p, &marks);
+    int e = marks_bytes(pages_fork_plan_kernel, p, &marks);
     if (e) return e;
     pages_fork_plan_kernel<<<1, kPlanThreads, marks, (cudaStream_t)stream>>>(*p, src, dst, n, deep, ws, st);
     e = (int)cudaGetLastError();
@@ -496,20 +489,16 @@ extern "C" int tyb_pages_fork_launch(const KVPages* p, const int* src, const int
     return (int)cudaGetLastError();
 }
 
-extern "C" int tyb_pages_free_launch(const KVPages* p, const int* seqs, int n, void* stream)
+extern "C" int tyb_pages_free_launch(const KVPages* p, const tyb_pages_env* env, const int* seqs, int n, void* stream)
 {
-    Status st;
-    const int e = status_of(&st);
-    if (e) return e;
+    const Status st = status_of(env);
     pages_free_kernel<<<n, 128, 0, (cudaStream_t)stream>>>(*p, seqs, 0, 0, 0, st);
     return (int)cudaGetLastError();
 }
 
-extern "C" int tyb_pages_trim_launch(const KVPages* p, const int* seqs, int n, int window, int sinks, void* stream)
+extern "C" int tyb_pages_trim_launch(const KVPages* p, const tyb_pages_env* env, const int* seqs, int n, int window, int sinks, void* stream)
 {
-    Status st;
-    const int e = status_of(&st);
-    if (e) return e;
+    const Status st = status_of(env);
     pages_free_kernel<<<n, 128, 0, (cudaStream_t)stream>>>(*p, seqs, 1, window, sinks, st);
     return (int)cudaGetLastError();
 }
@@ -523,12 +512,10 @@ extern "C" int tyb_pages_compact_launch(const KVPages* p, int* live_out, void* w
     return (int)cudaGetLastError();
 }
 
-extern "C" int tyb_pages_write_launch(const KVPages* p, int layer, const int* seqs, const int* starts, int n, int rows,
+extern "C" int tyb_pages_write_launch(const KVPages* p, const tyb_pages_env* env, int layer, const int* seqs, const int* starts, int n, int rows,
                                       const void* k_new, const void* v_new, int in_bf16, long long stride, void* stream)
 {
-    Status st;
-    const int e = status_of(&st);
-    if (e) return e;
+    const Status st = status_of(env);
     const int per_cta = kApplyThreads / 32;
     const long long ctas = (2LL * rows + per_cta - 1) / per_cta;
     const unsigned grid = (unsigned)(ctas < kSms * 16 ? ctas : kSms * 16);
@@ -549,13 +536,12 @@ extern "C" int tyb_pages_write_launch(const KVPages* p, int layer, const int* se
     return (int)cudaGetLastError();
 }
 
-extern "C" int tyb_pages_import_launch(const KVPages* p, int seq, const void* k_slab, const void* v_slab, int row_capacity,
+extern "C" int tyb_pages_import_launch(const KVPages* p, const tyb_pages_env* env, int seq, const void* k_slab, const void* v_slab, int row_capacity,
                                        int rows, void* ws, void* stream)
 {
-    Status st;
+    const Status st = status_of(env);
     size_t marks;
-    int e = status_of(&st);
-    if (!e) e = marks_bytes(pages_extend_kernel, p, &marks);
+    int e = marks_bytes(pages_extend_kernel, p, &marks);
     if (e) return e;
     pages_extend_kernel<<<1, kPlanThreads, marks, (cudaStream_t)stream>>>(*p, nullptr, nullptr, 1, seq, rows, ws, st);
     e = (int)cudaGetLastError();

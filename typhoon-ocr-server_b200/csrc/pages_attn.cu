@@ -531,10 +531,9 @@ template <int D>
 static int launch_rows(const AttnArgs& a, int row_tiles, cudaStream_t stream)
 {
     static bool ready[64];
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return (int)e;
+    const int dev = a.device;
     if (dev < 0 || dev >= 64) return (int)cudaErrorInvalidDevice;
+    cudaError_t e;
     const size_t rows = kWarps * (size_t)Query<float, D>::kSharedFloats * sizeof(float);
     if (!ready[dev]) {
         e = cudaFuncSetAttribute(pages_rows_kernel<float, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)rows);
@@ -563,9 +562,9 @@ extern "C" int tyb_pages_attn_launch(const tyb_pages_attn* c, void* ws, void* ti
     cudaStream_t st = (cudaStream_t)stream;
     const Layout l = layout_of(c);
     AttnArgs a = args_of(c, l);
-    a.st.word = tyb_status_word();
-    a.st.mirror = tyb_status_mirror_device();
-    if (!a.st.word) return (int)cudaErrorInvalidSymbol;
+    a.st.word = c->env.status;
+    a.st.mirror = c->env.mirror;
+    a.device = c->env.device;
     const int D = a.p.head_dim;
     if (records(l)) {
         a.rec.o = static_cast<float*>(ws);

@@ -103,6 +103,7 @@ struct AttnArgs {
     int splits, slot0;  // this launch's splits, and the record slot of its first
     Records rec;        // slots == 1: the output is written directly
     Status st;
+    int device;
 };
 
 // The tcgen05 form (pages_attn_tc.cu) for the query rows of a BF16 pool, `items` row tiles: tall, of at

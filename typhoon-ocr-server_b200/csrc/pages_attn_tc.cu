@@ -537,10 +537,9 @@ template <int D>
 static int launch_tc(const TcArgs& ta, const void* maps, dim3 grid, cudaStream_t stream)
 {
     static bool ready[64];
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return (int)e;
+    const int dev = ta.a.device;
     if (dev < 0 || dev >= 64) return (int)cudaErrorInvalidDevice;
+    cudaError_t e;
     if (!ready[dev]) {
         // a register split above the launch's registers would never be granted
         cudaFuncAttributes fa;
@@ -563,7 +562,7 @@ int tc_launch(const AttnArgs& a, int layer, bool tall, bool shared_pass, int ite
     ta.layer = layer;
     ta.tall = tall;
     ta.shared_pass = shared_pass;
-    ta.wait_ns = tyb_wait_limit();
+    ta.wait_ns = tyb_wait_limit_of(a.device);
     const dim3 grid(items, a.p.kv_heads, a.splits);
     return a.p.head_dim == 128 ? launch_tc<128>(ta, maps, grid, stream) : launch_tc<64>(ta, maps, grid, stream);
 }

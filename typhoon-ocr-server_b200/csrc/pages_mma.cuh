@@ -1,6 +1,17 @@
-// pages_mma.cuh -- 16 query rows of one warp against key tiles in shared memory, on warp-level matrix
-// products (mma.sync): the running softmax and output of pages_stream.cu.  Tiles lie as TMA writes
-// them with the 128-byte swizzle: boxes of 128-byte rows, 16-byte chunks XORed with row % 8.
+// pages_mma.cuh -- a few query rows of one warp against key tiles in shared memory, on warp-level matrix
+// products (mma.sync): the running softmax and output of pages_stream.cu.  Tiles lie as TMA writes them
+// with the 128-byte swizzle: boxes of 128-byte rows, 16-byte chunks XORed with row % 8.
+//
+// Few rows meet many keys, so the keys (and in P.V the head dimensions) are the 16 rows of the product and
+// the queries its 8 columns: S^T = K Q^T, O^T = V^T P^T.  A product costs the same whether its columns are
+// used or not, and for at most four query rows the other four columns carry what would be a second product:
+//   BF16  the weights' remainders: columns 0-3 of P^T the weights rounded to BF16, columns 4-7 what that
+//         left (the queries are repeated, so those lanes have the scores as well); O is the columns' sum.
+//         So the only roundings are the operands' own and the output's.
+//   FP32  the TF32 remainders: x = hi + lo in every operand; columns 0-3 of Q^T and P^T hi, 4-7 lo; two
+//         products (hi and lo of K or V) give all four terms.  A relative error of about 2^-21 per product.
+// That makes 32 products for 32 BF16 keys of 128 dimensions, against 96 of the usual form (queries as rows,
+// remainders by a second product): mma.sync issues one per 16 cycles here, and the usual form was bound by it.
 #pragma once
 
 #include "pages_attn.cuh"
@@ -51,6 +62,14 @@ __device__ __forceinline__ void ldsm_t(uint32_t (&r)[4], uint32_t at)
                  : "memory");
 }
 
+// The 8x8 matrix of 16-bit values whose row g lane (g, t) has columns 2 t, 2 t + 1 of, transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x)
+{
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
 // Four finished output values at element `at`.
 __device__ __forceinline__ void put_out(const AttnArgs& a, size_t at, float4 x, float l)
 {
@@ -61,231 +80,318 @@ __device__ __forceinline__ void put_out(const AttnArgs& a, size_t at, float4 x, 
         *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
 }
 
-// Output fragments and statistics; lane (g, t) = (lane / 4, lane % 4) has columns 8 c + 2 t, + 1 of rows g
-// (o[c][0..1]) and g + 8 (o[c][2..3]).
-template <int D>
+// Column q of block n of the products is query row 8 n + q; with kDup (rows up to 4, one block) columns 4-7
+// are rows 0-3 again.  Lane (g, t) = (lane / 4, lane % 4).
+// O^T fragments: o[n][i][c] is dimension 16 i + g + 8 (c / 2) of column 2 t + c % 2; statistics per column.
+template <int D, int kBlocks, bool kDup>
 struct Running {
-    float o[D / 8][4];
-    float m[2], l[2];
+    float o[kBlocks][D / 16][4];
+    float m[kBlocks][2], l[kBlocks][2];
 
     __device__ __forceinline__ void clear()
     {
 #pragma unroll
-        for (int c = 0; c < D / 8; c++) o[c][0] = o[c][1] = o[c][2] = o[c][3] = 0.f;
-        m[0] = m[1] = -INFINITY;
-        l[0] = l[1] = 0.f;
+        for (int n = 0; n < kBlocks; n++) {
+#pragma unroll
+            for (int i = 0; i < D / 16; i++) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
+            m[n][0] = m[n][1] = -INFINITY;
+            l[n][0] = l[n][1] = 0.f;
+        }
     }
 
-    // Scores s[e][..] (keys 8 e + 2 t, + 1 of rows g and g + 8) become weights; bit i of `see`: key i is in
-    // sight of the rows.
+    // Scores s[n][e][c] (key 16 e + g + 8 (c / 2) of column 2 t + c % 2) become weights; bit i of `see`: key i
+    // is in sight of the rows.
     template <int E>
-    __device__ __forceinline__ void weigh(float (&s)[E][4], unsigned int see, float scale, int t)
+    __device__ __forceinline__ void weigh(float (&s)[kBlocks][E][4], unsigned int see, float scale, int g)
     {
-        if (see != (1u << (8 * E)) - 1u) {
+        if (see != 0xffffffffu >> (32 - 16 * E)) {
 #pragma unroll
             for (int e = 0; e < E; e++)
 #pragma unroll
-                for (int r = 0; r < 2; r++)
-                    if (!(see >> (8 * e + 2 * t + r) & 1u)) s[e][r] = s[e][2 + r] = -INFINITY;
+                for (int hf = 0; hf < 2; hf++)
+                    if (!(see >> (16 * e + g + 8 * hf) & 1u)) {
+#pragma unroll
+                        for (int n = 0; n < kBlocks; n++) s[n][e][2 * hf] = s[n][e][2 * hf + 1] = -INFINITY;
+                    }
         }
-        float top[2];
+        float top[kBlocks][2];
+        bool rise = false;
 #pragma unroll
-        for (int r = 0; r < 2; r++) {
-            top[r] = fmaxf(s[0][2 * r], s[0][2 * r + 1]);
+        for (int n = 0; n < kBlocks; n++)
 #pragma unroll
-            for (int e = 1; e < E; e++) top[r] = fmaxf(top[r], fmaxf(s[e][2 * r], s[e][2 * r + 1]));
-            top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-            top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-            top[r] = fmaxf(m[r], top[r] * scale);
-        }
-        if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {
+            for (int c = 0; c < 2; c++) {
+                float x = fmaxf(s[n][0][c], s[n][0][2 + c]);
 #pragma unroll
-            for (int r = 0; r < 2; r++) {
-                const float f = m[r] == -INFINITY ? 0.f : fast_exp2(m[r] - top[r]);
-                l[r] *= f;
-                m[r] = top[r];
+                for (int e = 1; e < E; e++) x = fmaxf(x, fmaxf(s[n][e][c], s[n][e][2 + c]));
 #pragma unroll
-                for (int c = 0; c < D / 8; c++) {
-                    o[c][2 * r] *= f;
-                    o[c][2 * r + 1] *= f;
-                }
+                for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+                top[n][c] = fmaxf(m[n][c], x * scale);
+                rise |= top[n][c] > m[n][c];
             }
+        if (__any_sync(0xffffffffu, rise)) {
+#pragma unroll
+            for (int n = 0; n < kBlocks; n++)
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    const float f = m[n][c] == -INFINITY ? 0.f : fast_exp2(m[n][c] - top[n][c]);
+                    l[n][c] *= f;
+                    m[n][c] = top[n][c];
+#pragma unroll
+                    for (int i = 0; i < D / 16; i++) {
+                        o[n][i][c] *= f;
+                        o[n][i][2 + c] *= f;
+                    }
+                }
         }
-        const float neg[2] = {m[0] == -INFINITY ? 0.f : -m[0], m[1] == -INFINITY ? 0.f : -m[1]};
 #pragma unroll
-        for (int e = 0; e < E; e++)
+        for (int n = 0; n < kBlocks; n++)
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                s[e][r] = fast_exp2(fmaf(s[e][r], scale, neg[r >> 1]));
-                l[r >> 1] += s[e][r];
+            for (int c = 0; c < 2; c++) {
+                const float neg = m[n][c] == -INFINITY ? 0.f : -m[n][c];
+#pragma unroll
+                for (int e = 0; e < E; e++)
+#pragma unroll
+                    for (int hf = 0; hf < 2; hf++) {
+                        float& x = s[n][e][2 * hf + c];
+                        x = fast_exp2(fmaf(x, scale, neg));
+                        l[n][c] += x;
+                    }
             }
     }
 
-    // The lanes' shares of the row sums.
-    __device__ __forceinline__ void finish()
+    // The warp's rows, to be joined: output rows at rows[r * pitch], statistics at ml[r].
+    __device__ __forceinline__ void put(float* rows, int pitch, float2* ml, int nrows, int g, int t)
     {
 #pragma unroll
-        for (int r = 0; r < 2; r++) {
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+        for (int n = 0; n < kBlocks; n++)
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], d);
+                const int row = 8 * n + 2 * t + c;
+                if (g == 0 && row < nrows) ml[row] = make_float2(m[n][c], l[n][c]);
+#pragma unroll
+                for (int i = 0; i < D / 16; i++)
+#pragma unroll
+                    for (int hf = 0; hf < 2; hf++) {
+                        float x = o[n][i][2 * hf + c];
+                        if (kDup) x += __shfl_xor_sync(0xffffffffu, x, 2);
+                        if (row < nrows) rows[row * pitch + 16 * i + g + 8 * hf] = x;
+                    }
+            }
+    }
+};
+
+template <typename T, int D, int kBlocks, bool kDup>
+struct Rows;
+
+template <int D, int kBlocks, bool kDup>
+struct Rows<__nv_bfloat16, D, kBlocks, kDup> : Running<D, kBlocks, kDup> {
+    uint32_t q[kBlocks][D / 16][2];
+
+    // n >= 1 query rows at `at` (shared memory, [n][D] BF16 or FP32); further columns repeat the last one:
+    // theirs are results that nobody takes.
+    __device__ __forceinline__ void load_q(const unsigned char* at, int n, bool bf16, int g, int t, float*, int, int)
+    {
+#pragma unroll
+        for (int b = 0; b < kBlocks; b++) {
+            const int first = min(8 * b + (kDup ? g & 3 : g), n - 1) * D + 2 * t;
+            if (bf16) {
+#pragma unroll
+                for (int k = 0; k < D / 16; k++)
+#pragma unroll
+                    for (int i = 0; i < 2; i++) q[b][k][i] = *reinterpret_cast<const uint32_t*>(at + (first + 16 * k + 8 * i) * 2);
+            } else {
+#pragma unroll
+                for (int k = 0; k < D / 16; k++)
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        const float2 f = *reinterpret_cast<const float2*>(at + (first + 16 * k + 8 * i) * 4);
+                        q[b][k][i] = pack2(f.x, f.y);
+                    }
+            }
+        }
+    }
+
+    // Rows r0 .. r0 + 32 of the tile.
+    __device__ __forceinline__ void step(const unsigned char* kt, const unsigned char* vt, int box, int r0, unsigned int see, float scale,
+                                         const float*, int g, int t, int lane)
+    {
+        float s[kBlocks][2][4];
+#pragma unroll
+        for (int b = 0; b < kBlocks; b++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) s[b][e][0] = s[b][e][1] = s[b][e][2] = s[b][e][3] = 0.f;
+        {
+            const int row = r0 + (lane & 15), half = lane >> 4;
+            const uint32_t at = smem_u32(kt) + row * 128;
+#pragma unroll
+            for (int k = 0; k < D / 16; k++) {
+                const int chunk = 2 * k + half;
+                const uint32_t off = at + (chunk >> 3) * box + (((chunk & 7) ^ (row & 7)) << 4);
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    uint32_t x[4];
+                    ldsm(x, off + e * 16 * 128);
+#pragma unroll
+                    for (int b = 0; b < kBlocks; b++) mma_bf16(s[b][e], x, q[b][k][0], q[b][k][1]);
+                }
+            }
+        }
+        this->template weigh<2>(s, see, scale, g);
+        const int row = r0 + (lane & 7) + (lane >> 4) * 8, half = lane >> 3 & 1;
+        const uint32_t at = smem_u32(vt) + row * 128;
+#pragma unroll
+        for (int e = 0; e < 2; e++) {  // 16 keys
+            uint32_t h[kBlocks][2], r[kBlocks][2];
+#pragma unroll
+            for (int b = 0; b < kBlocks; b++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const float x = s[b][e][2 * i], y = s[b][e][2 * i + 1];
+                    h[b][i] = pack2(x, y);
+                    r[b][i] = pack2(x - lo_of(h[b][i]), y - hi_of(h[b][i]));
+                    if (kDup) h[b][i] = t < 2 ? h[b][i] : r[b][i];
+                    h[b][i] = transpose8(h[b][i]);
+                    if (!kDup) r[b][i] = transpose8(r[b][i]);
+                }
+#pragma unroll
+            for (int i = 0; i < D / 16; i++) {
+                const int chunk = 2 * i + half;
+                uint32_t x[4];
+                ldsm_t(x, at + e * 16 * 128 + (chunk >> 3) * box + (((chunk & 7) ^ (row & 7)) << 4));
+#pragma unroll
+                for (int b = 0; b < kBlocks; b++) {
+                    mma_bf16(this->o[b][i], x, h[b][0], h[b][1]);
+                    if (!kDup) mma_bf16(this->o[b][i], x, r[b][0], r[b][1]);
+                }
+            }
         }
     }
 };
 
-template <typename T, int D>
-struct Rows;
+template <int D, int kBlocks, bool kDup>
+struct Rows<float, D, kBlocks, kDup> : Running<D, kBlocks, kDup> {
+    static constexpr int kPitch = D + 4;
+    uint32_t q[kDup ? D / 8 : 1][2];  // kDup: hi of rows 0-3 in columns 0-3, lo in columns 4-7
 
-template <int D>
-struct Rows<__nv_bfloat16, D> : Running<D> {
-    uint32_t q[D / 16][4];
-
-    // n query rows at `at` (shared memory, [n][D] BF16 or FP32; the others are zeros).
-    __device__ __forceinline__ void load_q(const unsigned char* at, int n, bool bf16, int g, int t, float*, int, int, int)
+    // The rows as TF32 halves: into registers (kDup), or by `threads` threads together into `split` (hi, then
+    // lo: [8 kBlocks][kPitch] each).
+    __device__ __forceinline__ void load_q(const unsigned char* at, int n, bool bf16, int g, int t, float* split, int tid, int threads)
     {
+        auto value = [&](int row, int c) {
+            const int i = min(row, n - 1) * D + c;
+            return bf16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(at)[i]) : reinterpret_cast<const float*>(at)[i];
+        };
+        if constexpr (kDup) {
 #pragma unroll
-        for (int k = 0; k < D / 16; k++)
+            for (int k = 0; k < D / 8; k++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int row = g + 8 * (i & 1), c = 16 * k + 8 * (i >> 1) + 2 * t;
-                uint32_t x = 0;
-                if (row < n) {
-                    if (bf16) {
-                        x = *reinterpret_cast<const uint32_t*>(at + (row * D + c) * 2);
-                    } else {
-                        const float2 f = *reinterpret_cast<const float2*>(at + (row * D + c) * 4);
-                        x = pack2(f.x, f.y);
-                    }
+                for (int i = 0; i < 2; i++) {
+                    uint32_t hi, lo;
+                    split_tf32(value(g & 3, 8 * k + 4 * i + t), hi, lo);
+                    q[k][i] = g < 4 ? hi : lo;
                 }
-                q[k][i] = x;
+        } else {
+            for (int i = tid; i < 8 * kBlocks * D; i += threads) {
+                const int row = i / D, c = i % D;
+                uint32_t hi, lo;
+                split_tf32(value(row, c), hi, lo);
+                split[row * kPitch + c] = __uint_as_float(hi);
+                split[(8 * kBlocks + row) * kPitch + c] = __uint_as_float(lo);
             }
+        }
     }
 
     // Rows r0 .. r0 + 16 of the tile.
     __device__ __forceinline__ void step(const unsigned char* kt, const unsigned char* vt, int box, int r0, unsigned int see, float scale,
-                                         const float*, int, int t, int lane)
-    {
-        const uint32_t kb = smem_u32(kt), vb = smem_u32(vt);
-        float s[2][4], s2[2][4];
-#pragma unroll
-        for (int e = 0; e < 2; e++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) s[e][i] = s2[e][i] = 0.f;
-        {
-            const int row = r0 + (lane & 7) + (lane >> 4) * 8, half = lane >> 3 & 1;
-            const uint32_t at = kb + row * 128;
-#pragma unroll
-            for (int k = 0; k < D / 16; k++) {
-                uint32_t b[4];
-                const int chunk = 2 * k + half;
-                ldsm(b, at + (chunk >> 3) * box + (((chunk & 7) ^ (row & 7)) << 4));
-                mma_bf16(k & 1 ? s2[0] : s[0], q[k], b[0], b[1]);
-                mma_bf16(k & 1 ? s2[1] : s[1], q[k], b[2], b[3]);
-            }
-        }
-#pragma unroll
-        for (int e = 0; e < 2; e++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) s[e][i] += s2[e][i];
-        this->template weigh<2>(s, see, scale, t);
-        uint32_t h[4], r[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float x = s[i >> 1][2 * (i & 1)], y = s[i >> 1][2 * (i & 1) + 1];
-            h[i] = pack2(x, y);
-            r[i] = pack2(x - lo_of(h[i]), y - hi_of(h[i]));
-        }
-        const int row = r0 + (lane & 7) + (lane >> 3 & 1) * 8, half = lane >> 4;
-        const uint32_t at = vb + row * 128;
-#pragma unroll
-        for (int c = 0; c < D / 16; c++) {
-            uint32_t b[4];
-            const int chunk = 2 * c + half;
-            ldsm_t(b, at + (chunk >> 3) * box + (((chunk & 7) ^ (row & 7)) << 4));
-            mma_bf16(this->o[2 * c], h, b[0], b[1]);
-            mma_bf16(this->o[2 * c + 1], h, b[2], b[3]);
-            mma_bf16(this->o[2 * c], r, b[0], b[1]);
-            mma_bf16(this->o[2 * c + 1], r, b[2], b[3]);
-        }
-    }
-};
-
-template <int D>
-struct Rows<float, D> : Running<D> {
-    static constexpr int kPitch = D + 4;
-
-    // The rows as TF32 halves into `split` (hi, then lo: [rows][kPitch] each, rows 8 or 16), by `threads`
-    // threads together.
-    int rows;
-    __device__ __forceinline__ void load_q(const unsigned char* at, int n, bool bf16, int, int, float* split, int padded, int tid, int threads)
-    {
-        rows = padded;
-        for (int i = tid; i < rows * D; i += threads) {
-            const int row = i / D, c = i % D;
-            float x = 0.f;
-            if (row < n) x = bf16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(at)[row * D + c]) : reinterpret_cast<const float*>(at)[row * D + c];
-            uint32_t hi, lo;
-            split_tf32(x, hi, lo);
-            split[row * kPitch + c] = __uint_as_float(hi);
-            split[(rows + row) * kPitch + c] = __uint_as_float(lo);
-        }
-    }
-
-    // Rows r0 .. r0 + 8 of the tile.
-    __device__ __forceinline__ void step(const unsigned char* kt, const unsigned char* vt, int box, int r0, unsigned int see, float scale,
                                          const float* split, int g, int t, int lane)
     {
-        const uint32_t kb = smem_u32(kt);
-        const uint32_t* qh = reinterpret_cast<const uint32_t*>(split) + g * kPitch + t;
-        const uint32_t* ql = qh + rows * kPitch;
-        const int low = rows == 16 ? 8 * kPitch : 0;  // of 8 rows, g + 8 repeats g: not used
-        // hi.hi and the cross terms in accumulators of their own: shorter chains, and the small terms are
-        // not rounded away one by one
-        float c0[4] = {}, c1[4] = {}, c2[4] = {};
-        const int row = r0 + (lane & 7);
+        // Even and odd steps, and the small terms, in accumulators of their own: shorter chains, and the small
+        // terms are not rounded away one by one.
+        float s[kBlocks][1][4], s2[kBlocks][4];
 #pragma unroll
-        for (int k = 0; k < D / 16; k++) {
-            uint32_t b[4];
-            const int chunk = 4 * k + (lane >> 3);
-            ldsm(b, kb + (chunk >> 3) * box + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
+        for (int b = 0; b < kBlocks; b++)
 #pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const int d = 16 * k + 8 * u;
-                const uint32_t ah[4] = {qh[d], qh[d + low], qh[d + 4], qh[d + 4 + low]};
-                const uint32_t al[4] = {ql[d], ql[d + low], ql[d + 4], ql[d + 4 + low]};
-                uint32_t bh[2], bl[2];
-                split_tf32(__uint_as_float(b[2 * u]), bh[0], bl[0]);
-                split_tf32(__uint_as_float(b[2 * u + 1]), bh[1], bl[1]);
-                mma_tf32(c0, ah, bh[0], bh[1]);
-                mma_tf32(c1, al, bh[0], bh[1]);
-                mma_tf32(c2, ah, bl[0], bl[1]);
+            for (int i = 0; i < 4; i++) s[b][0][i] = s2[b][i] = 0.f;
+        {
+            const int row = r0 + (lane & 15), half = lane >> 4;
+            const uint32_t at = smem_u32(kt) + row * 128;
+            const uint32_t* qh = reinterpret_cast<const uint32_t*>(split) + g * kPitch + t;
+#pragma unroll
+            for (int k = 0; k < D / 8; k++) {
+                const int chunk = 2 * k + half;
+                uint32_t x[4], hi[4], lo[4];
+                ldsm(x, at + (chunk >> 3) * box + (((chunk & 7) ^ (row & 7)) << 4));
+#pragma unroll
+                for (int i = 0; i < 4; i++) split_tf32(__uint_as_float(x[i]), hi[i], lo[i]);
+#pragma unroll
+                for (int b = 0; b < kBlocks; b++) {
+                    if constexpr (kDup) {
+                        mma_tf32(s[b][0], hi, q[k][0], q[k][1]);
+                        mma_tf32(s2[b], lo, q[k][0], q[k][1]);
+                    } else {
+                        const uint32_t* p = qh + 8 * b * kPitch + 8 * k;
+                        const uint32_t h0 = p[0], h1 = p[4], l0 = p[8 * kBlocks * kPitch], l1 = p[8 * kBlocks * kPitch + 4];
+                        mma_tf32(s[b][0], hi, h0, h1);
+                        mma_tf32(s2[b], lo, h0, h1);
+                        mma_tf32(s2[b], hi, l0, l1);
+                    }
+                }
             }
         }
-        float s[1][4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) s[0][i] = c0[i] + (c1[i] + c2[i]);
-        this->template weigh<1>(s, see, scale, t);
-        // columns k = t and t + 4 of the P operand are keys 2 t and 2 t + 1
-        uint32_t ph[4], pl[4];
-        split_tf32(s[0][0], ph[0], pl[0]);
-        split_tf32(s[0][2], ph[1], pl[1]);
-        split_tf32(s[0][1], ph[2], pl[2]);
-        split_tf32(s[0][3], ph[3], pl[3]);
-        const int v0 = r0 + 2 * t, v1 = v0 + 1;
+        for (int b = 0; b < kBlocks; b++)
 #pragma unroll
-        for (int c = 0; c < D / 8; c++) {
-            const int chunk = 2 * c + (g >> 2);
-            const unsigned char* at = vt + (chunk >> 3) * box + (g & 3) * 4;
-            uint32_t bh[2], bl[2];
-            split_tf32(*reinterpret_cast<const float*>(at + v0 * 128 + (((chunk & 7) ^ (v0 & 7)) << 4)), bh[0], bl[0]);
-            split_tf32(*reinterpret_cast<const float*>(at + v1 * 128 + (((chunk & 7) ^ (v1 & 7)) << 4)), bh[1], bl[1]);
-            // The tile's contribution in an accumulator of its own, joined by an FP32 addition: the tensor
-            // core's own sums round towards zero, which over thousands of keys would add up.
-            float x[4] = {};
-            mma_tf32(x, pl, bh[0], bh[1]);
-            mma_tf32(x, ph, bl[0], bl[1]);
-            mma_tf32(x, ph, bh[0], bh[1]);
+            for (int i = 0; i < 4; i++) {
+                s[b][0][i] += s2[b][i];
+                if (kDup) s[b][0][i] += __shfl_xor_sync(0xffffffffu, s[b][0][i], 2);  // the columns of hi and of lo
+            }
+        this->template weigh<1>(s, see, scale, g);
+        // P^T as the products' second operand: lane (g, t) has column g of keys 2 t and 2 t + 1 (of 8; the
+        // order of the keys is the same in V^T).
+        uint32_t ph[kBlocks][2][2], pl[kBlocks][2][2];
 #pragma unroll
-            for (int i = 0; i < 4; i++) this->o[c][i] += x[i];
+        for (int b = 0; b < kBlocks; b++)
+#pragma unroll
+            for (int e = 0; e < 2; e++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const int from = (2 * t + i) * 4 + (g >> 1);
+                    const float x = __shfl_sync(0xffffffffu, s[b][0][2 * e], from), y = __shfl_sync(0xffffffffu, s[b][0][2 * e + 1], from);
+                    split_tf32(g & 1 ? y : x, ph[b][e][i], pl[b][e][i]);
+                    if (kDup && g >= 4) ph[b][e][i] = pl[b][e][i];
+                }
+        const unsigned char* v0 = vt + (r0 + 2 * t) * 128 + (g & 3) * 4;
+#pragma unroll
+        for (int i = 0; i < D / 16; i++) {
+            // The tile's contribution in accumulators of its own, joined by an FP32 addition: the tensor core's
+            // own sums round towards zero, which over thousands of keys would add up.
+            float x[kBlocks][4], y[kBlocks][4];
+#pragma unroll
+            for (int b = 0; b < kBlocks; b++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) x[b][c] = y[b][c] = 0.f;
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                uint32_t hi[4], lo[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {  // dimension + 8 (j & 1), key 2 t + (j >> 1)
+                    const int chunk = 4 * i + 2 * (j & 1) + (g >> 2), key = 2 * t + (j >> 1);
+                    split_tf32(*reinterpret_cast<const float*>(v0 + (chunk >> 3) * box + (8 * e + (j >> 1)) * 128 + (((chunk & 7) ^ key) << 4)),
+                               hi[j], lo[j]);
+                }
+#pragma unroll
+                for (int b = 0; b < kBlocks; b++) {
+                    mma_tf32(x[b], hi, ph[b][e][0], ph[b][e][1]);
+                    mma_tf32(y[b], lo, ph[b][e][0], ph[b][e][1]);
+                    if (!kDup) mma_tf32(y[b], hi, pl[b][e][0], pl[b][e][1]);
+                }
+            }
+#pragma unroll
+            for (int b = 0; b < kBlocks; b++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) this->o[b][i][c] += x[b][c] + y[b][c];
         }
     }
 };

@@ -21,18 +21,24 @@ extern "C" {
 /* Largest q_heads / kv_heads: the query rows of one tensor-core row tile. */
 #define TYB_PAGES_MAX_GROUP 16
 
+/* What a handle looks up once for its launches: its device, and there the status word and its mirror. */
+typedef struct {
+    int device;
+    unsigned int *status, *mirror;
+} tyb_pages_env;
+
 /* ---- maintenance (pages.cu); ws: tyb_pages_plan_bytes bytes of workspace ----------------- */
 size_t tyb_pages_plan_bytes(const KVPages *p, int n);
-int tyb_pages_extend_launch(const KVPages *p, const int *seqs, const int *counts, int n, void *ws, void *stream);
-int tyb_pages_fork_launch(const KVPages *p, const int *src, const int *dst, int n, int deep, void *ws, void *stream);
-int tyb_pages_free_launch(const KVPages *p, const int *seqs, int n, void *stream);
-int tyb_pages_trim_launch(const KVPages *p, const int *seqs, int n, int window, int sinks, void *stream);
+int tyb_pages_extend_launch(const KVPages *p, const tyb_pages_env *env, const int *seqs, const int *counts, int n, void *ws, void *stream);
+int tyb_pages_fork_launch(const KVPages *p, const tyb_pages_env *env, const int *src, const int *dst, int n, int deep, void *ws, void *stream);
+int tyb_pages_free_launch(const KVPages *p, const tyb_pages_env *env, const int *seqs, int n, void *stream);
+int tyb_pages_trim_launch(const KVPages *p, const tyb_pages_env *env, const int *seqs, int n, int window, int sinks, void *stream);
 int tyb_pages_compact_launch(const KVPages *p, int *live_out, void *ws, void *stream);
-int tyb_pages_write_launch(const KVPages *p, int layer, const int *seqs, const int *starts, int n, int rows,
+int tyb_pages_write_launch(const KVPages *p, const tyb_pages_env *env, int layer, const int *seqs, const int *starts, int n, int rows,
                            const void *k_new, const void *v_new, int in_bf16, long long stride, void *stream);
 /* Sequence `seq` (a host number) takes `rows` tokens: kv_pages_extend's plan for one sequence, then
  * the rows of a static cache (k_slab, v_slab: [28][8][row_capacity][128] of the pool's type). */
-int tyb_pages_import_launch(const KVPages *p, int seq, const void *k_slab, const void *v_slab, int row_capacity,
+int tyb_pages_import_launch(const KVPages *p, const tyb_pages_env *env, int seq, const void *k_slab, const void *v_slab, int row_capacity,
                             int rows, void *ws, void *stream);
 
 /* ---- attention ---------------------------------------------------------------------------- */
@@ -42,6 +48,7 @@ int tyb_pages_maps(const KVPages *p, void *maps);
 
 typedef struct {
     KVPages p;
+    tyb_pages_env env;
     const void *maps;
     int layer;
     const void *q;

@@ -6,16 +6,16 @@
 // element at most 16) once.  So the kernel is two CTAs per SM that stream equal shares of all the call's
 // rows, whatever the lengths: the key tiles of all (sequence, KV head) items, laid end to end,
 // are cut into gridDim.x equal runs.  One warp requests a run's tiles with TMA into a ring of stages,
-// crossing from item to item without a pause (item starts bring their query rows along).  Four warps
-// take 16 (BF16) or 8 (FP32) rows of each stage, with the running maximum and sum of an online softmax in
-// base 2, and at the item's end are joined through shared memory, while the SM's other CTA streams on.  An item that a run boundary cuts
+// crossing from item to item without a pause (item starts bring their query rows along).  Two teams of
+// two warps take the stages in turn, a warp 32 (BF16) or 16 (FP32) of its rows, with the running maximum
+// and sum of an online softmax in base 2; at the item's end the four are joined through shared memory,
+// while the SM's other CTA streams on.  (A stage is a chain of dependent steps, about a microsecond:
+// few keys per warp make it no shorter, so four of them at a time per SM keep up with the memory, two do not.)
+// An item that a run boundary cuts
 // is joined by the CTA that finishes it last (records in the workspace, a ticket per item); the order
 // of that sum is by run, not by arrival, so results repeat exactly.
 //
-//   BF16: mma.sync m16n8k16 from ldmatrix; P as a BF16 pair (value and remainder), so that the only
-//         roundings are the operands' own and the output's.  The products are far from the bound.
-//   FP32: mma.sync m16n8k8 on TF32 halves, x = hi + lo: hi.hi + hi.lo + lo.hi, a relative error of about
-//         2^-21 per product; sums in FP32.
+// The products (pages_mma.cuh) are mma.sync, with up to 16 query rows as columns.
 #define TYB_WHOLE_PROGRAM
 #include "pages_attn.cuh"
 #include "pages_mma.cuh"
@@ -23,16 +23,21 @@
 
 namespace tyb {
 
-constexpr int kTakers = 4;                       // warps that consume stages
+constexpr int kTeam = 2;                         // warps that share a stage
+constexpr int kTakers = 2 * kTeam;               // warps that consume stages: two teams, in turn
 constexpr int kTakerThreads = 32 * kTakers;
 constexpr int kStreamThreads = kTakerThreads + 32;  // + the requesting warp
 constexpr int kMaxStages = 10;
 constexpr int kStreamRuns = 2 * kSms;            // CTAs, at most
+// An item's start and end (its query, the join of the warps) cost a CTA about as much as this many stages:
+// runs are cut by stages plus this for each item.  Measured with 256 sequences of 1 .. 512 rows (4.6 stages on
+// average): 61 us against 84 us of runs with equal stages, whose run of one-stage items took twice the others.
+constexpr int kItemUnits = 2;
 
 template <typename T, int D>
 struct Stream {
-    static constexpr int kKeys = sizeof(T) == 2 ? 16 : 8;   // of a warp
-    static constexpr int kRows = kTakers * kKeys;           // of a stage
+    static constexpr int kKeys = sizeof(T) == 2 ? 32 : 16;  // of a warp
+    static constexpr int kRows = kTeam * kKeys;             // of a stage
     static constexpr int kBoxCols = 128 / (int)sizeof(T);   // columns of a 128-byte box
     static constexpr int kBoxes = D / kBoxCols;
     static constexpr int kBox = kRows * 128;                // bytes
@@ -43,7 +48,8 @@ struct Stream {
 
 // What the requesting warp tells the takers about a stage.
 struct Tile {
-    int first, last;  // of its item (in this CTA)
+    int first, last;  // of its item (in this run)
+    int end;          // of the run
     int k0;           // key of the stage's first row
     unsigned int seen;  // a bit per 8 rows: the page is there
     int shared;       // an item of the shared pass
@@ -57,7 +63,7 @@ struct StreamArgs {
     int layer;
     int tok_base;      // token (row of q) of this launch's first sequence
     int shared_tiles;  // row tiles of the shared pass in this launch (0: none)
-    int shared_units;  // stages of its rows
+    int shared_units;  // units of each: kItemUnits and the stages of its rows
     int out_slot;      // record slot of a.rec that receives the results; -1: they are the output
     int max_len;
     int stages, q_bytes, item_rows, buffers;
@@ -80,11 +86,12 @@ struct Runs {
         const unsigned int split = more * (base + 1);
         return u < split ? u / (base + 1) : more + (u - split) / base;
     }
-    // The runs c0 .. c1 that units [u0, u1) lie in, and which record of run c0 is theirs (0: its first item's,
-    // 1: its last's; in the later runs they are the first item).
+    // The runs c0 .. c1 that have stages of the item of units [u0, u1), and which record of run c0 is the item's
+    // (0: its first item's, 1: its last's, an earlier item having ended in the run; in the later runs it comes
+    // first).
     __device__ __forceinline__ void span(unsigned int u0, unsigned int u1, int& c0, int& c1, int& s0) const
     {
-        c0 = (int)of(u0);
+        c0 = (int)of(u0 + kItemUnits);
         c1 = (int)of(u1 - 1);
         s0 = start(c0) < u0;
     }
@@ -107,7 +114,7 @@ struct Gather {
     }
 };
 
-template <typename T, int D>
+template <typename T, int D, int kBlocks, bool kDup>
 __global__ void __launch_bounds__(kStreamThreads, 2)
     pages_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const StreamArgs sa)
 {
@@ -118,8 +125,8 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
     unsigned char* ring = smem;
     float* joins = reinterpret_cast<float*>(ring + sa.stages * S::kStage);  // [buffers][kTakers][item_rows][kPitch]
     float* split_q = joins + sa.buffers * kTakers * sa.item_rows * S::kPitch;  // FP32: hi and lo, [split_rows][kPitch] each
-    const int split_rows = sa.item_rows <= 8 ? 8 : 16;
-    unsigned char* qs = reinterpret_cast<unsigned char*>(split_q + (sizeof(T) == 4 ? 2 * split_rows * S::kPitch : 0));  // [stages][q_bytes]
+    constexpr int split_rows = sizeof(T) == 4 && !kDup ? 8 * kBlocks : 0;
+    unsigned char* qs = reinterpret_cast<unsigned char*>(split_q + 2 * split_rows * S::kPitch);  // [stages][q_bytes]
     int* cum = reinterpret_cast<int*>(qs + sa.stages * sa.q_bytes);        // units before each sequence
     int* lens = cum + a.batch + 1;
 
@@ -140,20 +147,31 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
         mbar_init(&met, kTakers);
         fence_barrier_init();
     }
-    // Units (stages) of each sequence's own rows: at least one, so that every output row has an owner.
+    // Units of each sequence's own rows: kItemUnits, then its stages, of which it has one at least, so that every
+    // output row has an owner.
     auto own_lo = [&](int len) { return a.window ? max(0, len - a.window) : min(a.prefix, len); };
+    // A thread takes consecutive sequences, so that all loads are in flight at once and one scan will do.
     long long before = 0;
-    for (int base = 0; base < a.batch; base += kStreamThreads) {
-        const int b = base + tid;
-        int len = 0, n = 0;
-        if (b < a.batch) {
-            len = checked_len(a.p, a.seqs[b], a.st);
-            if (len > sa.max_len) {
-                raise(a.st, TYB_STATUS_BAD_ARGUMENT);
-                len = 0;
+    {
+        constexpr int kPer = (kStreamSeqs + kStreamThreads - 1) / kStreamThreads;
+        const int each = (a.batch + kStreamThreads - 1) / kStreamThreads, b0 = tid * each;
+        int len[kPer], n = 0;
+#pragma unroll
+        for (int i = 0; i < kPer; i++) len[i] = i < each && b0 + i < a.batch ? a.seqs[b0 + i] : -1;
+#pragma unroll
+        for (int i = 0; i < kPer; i++)
+            if (i < each && b0 + i < a.batch) len[i] = checked_len(a.p, len[i], a.st);
+#pragma unroll
+        for (int i = 0; i < kPer; i++)
+            if (i < each && b0 + i < a.batch) {
+                if (len[i] > sa.max_len) {
+                    raise(a.st, TYB_STATUS_BAD_ARGUMENT);
+                    len[i] = 0;
+                }
+                lens[b0 + i] = len[i];
+                len[i] = kItemUnits + max(1, tiles_of(len[i] - 1, own_lo(len[i]), a.sinks, S::kRows).count());
+                n += len[i];
             }
-            n = max(1, tiles_of(len - 1, own_lo(len), a.sinks, S::kRows).count());
-        }
         int sum = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -162,16 +180,18 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
         }
         if (lane == 31) scan[warp] = sum;
         __syncthreads();
-        int add = (int)before;
+        int at = sum - n;
+#pragma unroll
         for (int w = 0; w < kStreamThreads / 32; w++) {
-            if (w < warp) add += scan[w];
+            if (w < warp) at += scan[w];
             before += scan[w];
         }
-        if (b < a.batch) {
-            cum[b] = add + sum - n;
-            lens[b] = len;
-        }
-        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kPer; i++)
+            if (i < each && b0 + i < a.batch) {
+                cum[b0 + i] = at;
+                at += len[i];
+            }
     }
     if (tid == 0) cum[a.batch] = (int)before;
     __syncthreads();
@@ -188,19 +208,26 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
 
     if (warp == kTakers) {
         // ---- requests
-        const int sub = min(a.p.page_size, S::kRows), subs = S::kRows / sub, shift = page_shift(a.p.page_size);
-        const unsigned int sub_bits = (1u << (sub / 8)) - 1u;
-        const size_t esize = a.io_bf16 ? 2 : 4;
+        // Lane (part, box, K or V): a stage's rows come from 1, 2 or 4 parts (pages, or one part of a page), each
+        // 128-byte column box of each as one copy.
+        const int part_rows = box_rows(a.p), parts = S::kRows / part_rows, shift = page_shift(a.p.page_size);
+        const int part = lane % parts, box = lane / parts % S::kBoxes, which = lane / parts / S::kBoxes;
+        const unsigned int part_bits = (1u << (part_rows / 8)) - 1u;
+        const int part_bytes = part_rows * 128;
+        const uint32_t q_row = (uint32_t)(a.group * D * (a.io_bf16 ? 2 : 4));
+        const int max_page = a.p.num_pages;
         Tile tile = {};
         Tiles list = {};
         const int* table = a.p.table;
-        unsigned int u = begin, u0 = 0, u1 = 0;  // the current item's units
-        int b = 0, st = 0;
+        unsigned int u = begin, u0 = 0, u1 = 0, sent = 0;  // u0, u1: the current item's units
+        int b = 0, st = 0, page = -1;
         uint32_t phase = 0;
-        bool ok = true;
-        for (; u < end; u++) {
-            const bool start = u == begin || u >= u1;
-            if (start) {  // the item that unit u lies in
+        bool ok = true, more = true;
+        // The next stage: what it holds, and the lane's page of it (requested here, so that its way from memory
+        // passes while the stage before waits for its place).  tile.end: none follows.
+        auto next = [&]() {
+            tile.first = u == begin || u >= u1;
+            if (tile.first) {  // the item that unit u lies in
                 if (u < shared_all) {
                     const unsigned int item = u / sa.shared_units;
                     u0 = item * sa.shared_units;
@@ -212,9 +239,9 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
                     tile.sinks = 0;
                     tile.lo = 0;
                     tile.pos = min(a.prefix, lens[0]) - 1;
-                    const int s = a.seqs[0];
-                    table = a.p.table + (size_t)(lens[0] ? s : 0) * a.p.max_pages;
+                    table = a.p.table + (size_t)(lens[0] ? a.seqs[0] : 0) * a.p.max_pages;
                 } else {
+                    bool other = true;
                     if (u == begin) {  // which sequence: cum[b] * heads <= u - shared_all
                         int lo = 0, hi = a.batch;
                         while (hi - lo > 1) {
@@ -225,72 +252,87 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
                         b = lo;
                     } else if (u - shared_all >= (unsigned int)(cum[b + 1] * heads)) {
                         b++;
+                    } else {
+                        other = tile.shared;
                     }
-                    const unsigned int units = cum[b + 1] - cum[b], at = u - shared_all - cum[b] * heads;
-                    tile.kvh = (int)(at / units);
-                    u0 = u - at % units;
+                    const unsigned int units = cum[b + 1] - cum[b];
+                    if (u == begin) {
+                        const unsigned int at = u - shared_all - cum[b] * heads;
+                        tile.kvh = (int)(at / units);
+                        u0 = u - at % units;
+                    } else {
+                        tile.kvh = other ? 0 : tile.kvh + 1;
+                        u0 = u;
+                    }
                     u1 = u0 + units;
-                    tile.shared = 0;
-                    tile.tok0 = b;
-                    tile.ntok = 1;
-                    tile.sinks = a.sinks;
-                    tile.pos = lens[b] - 1;
-                    tile.lo = own_lo(lens[b]);
-                    table = a.p.table + (size_t)(lens[b] ? a.seqs[b] : 0) * a.p.max_pages;
+                    if (other) {
+                        tile.shared = 0;
+                        tile.tok0 = b;
+                        tile.ntok = 1;
+                        tile.sinks = a.sinks;
+                        tile.pos = lens[b] - 1;
+                        tile.lo = own_lo(lens[b]);
+                        table = a.p.table + (size_t)(lens[b] ? a.seqs[b] : 0) * a.p.max_pages;
+                    }
                 }
-                cuts.span(u0, u1, tile.c0, tile.c1, tile.s0);
+                // items inside the run are whole: only its first and last may lie in others too
+                tile.c0 = tile.c1 = run;
+                tile.s0 = 0;
+                if (u == begin || u1 > end) cuts.span(u0, u1, tile.c0, tile.c1, tile.s0);
                 list = tiles_of(tile.pos, tile.lo, tile.sinks, S::kRows);
+                if (u < u0 + kItemUnits) u = min(u0 + kItemUnits, end);
             }
-            tile.first = start;
-            tile.last = u + 1 == u1 || u + 1 == end;
-            const int i = (int)(u - u0);
-            tile.k0 = i < list.count() ? list.at(i) * S::kRows : tile.pos + 1;
-            // lane l < subs: the page (or part of one) at rows l * sub of the stage
-            int page = -1;
-            const int key = tile.k0 + lane * sub;
-            if (lane < subs && i < list.count() && key <= tile.pos) {
-                page = table[key >> shift];
-                if (page >= a.p.num_pages) {
-                    raise(a.st, TYB_STATUS_BAD_ARGUMENT);
-                    page = -1;
-                }
-            }
-            const unsigned int have = __ballot_sync(0xffffffffu, page >= 0);
-            tile.seen = 0;
-            for (int l = 0; l < subs; l++)
-                if (have >> l & 1u) tile.seen |= sub_bits << (l * (sub / 8));
-            if (u - begin >= (unsigned int)sa.stages) {
+            const bool none = u == end;  // the run ends before the item's first stage
+            tile.first = tile.first && !none;
+            tile.last = !none && (u + 1 == u1 || u + 1 == end);
+            tile.end = none || (u + 1 == u1 ? u1 + kItemUnits : u + 1) >= end;
+            const int i = none ? list.count() : (int)(u - u0 - kItemUnits);
+            const bool real = i < list.count();
+            tile.k0 = real ? list.at(i) * S::kRows : tile.pos + 1;
+            const int key = tile.k0 + part * part_rows;
+            page = real && which < 2 && key <= tile.pos ? table[key >> shift] : -1;
+            u++;
+        };
+        next();
+        while (more) {
+            if (sent >= (unsigned int)sa.stages) {
                 ok = wait_for(&empty[st], phase ^ 1u, sa.wait_ns, a.st);
                 if (__any_sync(0xffffffffu, !ok)) break;
             }
-            const uint32_t q_row = (uint32_t)(a.group * D * esize);
+            if (page >= max_page) {
+                raise(a.st, TYB_STATUS_BAD_ARGUMENT);
+                page = -1;
+            }
+            const unsigned int have = __ballot_sync(0xffffffffu, page >= 0);
+            tile.seen = 0;
+            for (int l = 0; l < parts; l++)
+                if (have >> l & 1u) tile.seen |= part_bits << (l * (part_rows / 8));
             if (lane == 0) {
                 tiles_of_stage[st] = tile;
-                mbar_arrive_expect_tx(&full[st], (uint32_t)__popc(have) * (uint32_t)(sub * 128 * S::kBoxes * 2) +
-                                                     (start ? q_row * (uint32_t)tile.ntok : 0u));
+                mbar_arrive_expect_tx(&full[st], (uint32_t)(__popc(have) * part_bytes) + (tile.first ? q_row * (uint32_t)tile.ntok : 0u));
             }
             __syncwarp();
-            unsigned char* to = ring + st * S::kStage;
             if (page >= 0) {
-                const int row = ((sa.layer * a.p.num_pages + page) * heads + tile.kvh) * a.p.page_size + (key & (a.p.page_size - 1));
-#pragma unroll
-                for (int c = 0; c < S::kBoxes; c++) {
-                    tma_load_2d(to + c * S::kBox + lane * sub * 128, &map_k, c * S::kBoxCols, row, &full[st]);
-                    tma_load_2d(to + S::kHalf + c * S::kBox + lane * sub * 128, &map_v, c * S::kBoxCols, row, &full[st]);
-                }
+                const int row = ((sa.layer * a.p.num_pages + page) * heads + tile.kvh) * a.p.page_size +
+                                ((tile.k0 + part * part_rows) & (a.p.page_size - 1));
+                tma_load_2d(ring + st * S::kStage + which * S::kHalf + box * S::kBox + part * part_bytes, which ? &map_v : &map_k,
+                            box * S::kBoxCols, row, &full[st]);
             }
-            if (start && lane < tile.ntok)
+            if (tile.first && lane < tile.ntok)
                 bulk_g2s(qs + st * sa.q_bytes + lane * q_row,
-                         static_cast<const char*>(a.q) +
-                             ((size_t)(sa.tok_base + tile.tok0 + lane) * a.q_stride + (size_t)tile.kvh * a.group * D) * esize,
+                         static_cast<const char*>(a.q) + ((size_t)(sa.tok_base + tile.tok0 + lane) * a.q_stride + (size_t)tile.kvh * a.group * D) *
+                                                             (a.io_bf16 ? 2 : 4),
                          q_row, &full[st]);
+            sent++;
             if (++st == sa.stages) {
                 st = 0;
                 phase ^= 1u;
             }
+            more = !tile.end;
+            if (more) next();
         }
         if (__any_sync(0xffffffffu, !ok)) {  // a wait ran out: the copies requested still land in this CTA
-            const unsigned int sent = u - begin, stages = sa.stages;
+            const unsigned int stages = sa.stages;
             for (unsigned int n = sent > stages ? sent - stages : 0; n < sent; n++)
                 wait_for(&full[n % stages], n / stages & 1u, sa.wait_ns, a.st);
         }
@@ -298,10 +340,10 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
     }
 
     // ---- takers
-    const int g = lane >> 2, t = lane & 3, r0 = warp * S::kKeys;
-    Rows<T, D> w;
+    const int g = lane >> 2, t = lane & 3, team = warp / kTeam, r0 = warp % kTeam * S::kKeys;
+    Rows<T, D, kBlocks, kDup> w;
     w.clear();
-    int st = 0;
+    int st = 0, turn = 0;  // turn: whose stage it is
     uint32_t phase = 0;
     bool one_item = true;  // no item has ended in this run yet
     int buffer = 0;        // of the join rows: two, used in turn
@@ -341,27 +383,30 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
             sum.add(join_ml[x][row], *reinterpret_cast<const float4*>(join + (x * sa.item_rows + row) * S::kPitch + c));
         return sum;
     };
-    for (unsigned int u = begin; u < end; u++) {
+    for (bool more = true; more;) {
         const bool here = wait_for(&full[st], phase, sa.wait_ns, a.st);
         if (__any_sync(0xffffffffu, !here)) return;
         const Tile tile = tiles_of_stage[st];
         const int nrows = tile.ntok * a.group;
+        more = !tile.end;
         if (tile.first) {
-            w.load_q(qs + st * sa.q_bytes, nrows, a.io_bf16, g, t, split_q, split_rows, tid, kTakerThreads);
-            if (sizeof(T) == 4 && !meet()) return;
+            w.load_q(qs + st * sa.q_bytes, nrows, a.io_bf16, g, t, split_q, tid, kTakerThreads);
+            if (split_rows && !meet()) return;
         }
         const int j0 = tile.k0 + r0;
         unsigned char* rows_k = ring + st * S::kStage;
         unsigned char* rows_v = rows_k + S::kHalf;
         const unsigned int want = (1u << (S::kKeys / 8)) - 1u, seen = tile.seen >> (r0 / 8) & want;
-        // none of the warp's rows in sight: nothing to do
-        const bool any = seen && j0 <= tile.pos && (j0 + S::kKeys > tile.lo || j0 < tile.sinks);
+        // the other team's stage, or none of the warp's rows in sight: nothing to do
+        const bool any = turn == team && seen && j0 <= tile.pos && (j0 + S::kKeys > tile.lo || j0 < tile.sinks);
         if (any) {
-            unsigned int see = (1u << S::kKeys) - 1u;  // bit i: row j0 + i
+            unsigned int see = 0xffffffffu >> (32 - S::kKeys);  // bit i: row j0 + i
             if (seen != want || j0 + S::kKeys - 1 > tile.pos || (j0 < tile.lo && j0 + S::kKeys > tile.sinks)) {
                 auto under = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; };
-                unsigned int pages = seen & 1u ? 0xffu : 0u;
-                if (seen & 2u) pages |= 0xff00u;
+                unsigned int pages = 0;
+#pragma unroll
+                for (int i = 0; i < S::kKeys / 8; i++)
+                    if (seen >> i & 1u) pages |= 0xffu << (8 * i);
                 see &= pages & under(tile.pos + 1 - j0) & (~under(tile.lo - j0) | under(tile.sinks - j0));
                 // what lies in rows out of sight may be anything, and 0 * NaN is not 0
                 for (int i = 0; i < S::kKeys; i++)
@@ -374,6 +419,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty[st]);
+        turn ^= 1;
         if (++st == sa.stages) {
             st = 0;
             phase ^= 1u;
@@ -386,18 +432,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
         else if (!meet()) return;
         float* join = joins + buffer * kTakers * sa.item_rows * S::kPitch;
         float2(*join_ml)[16] = join_mls[buffer];
-        w.finish();
-        if (t == 0) {
-            join_ml[warp][g] = make_float2(w.m[0], w.l[0]);
-            join_ml[warp][g + 8] = make_float2(w.m[1], w.l[1]);
-        }
-#pragma unroll
-        for (int r = 0; r < 2; r++)
-            if (g + 8 * r < nrows)
-#pragma unroll
-                for (int c = 0; c < D / 8; c++)
-                    *reinterpret_cast<float2*>(join + (warp * sa.item_rows + g + 8 * r) * S::kPitch + 8 * c + 2 * t) =
-                        make_float2(w.o[c][2 * r], w.o[c][2 * r + 1]);
+        w.put(join + warp * sa.item_rows * S::kPitch, S::kPitch, join_ml[warp], nrows, g, t);
         w.clear();  // (and so not kept through what follows)
         if (!meet()) return;
         const bool cut = tile.c0 != tile.c1, direct = !cut && !sa.shared_tiles;
@@ -459,25 +494,38 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
             Tile sh, ow;
             spans(tok, sh, ow);
             const int ns = sh.c1 - sh.c0 + 1, n = ns + ow.c1 - ow.c0 + 1;
-            auto row_of = [&](int x) {
-                if (x < ns) return (ns == 1 ? shared_row(tok, tile.kvh) : part_row(sh.c0 + x, x ? 0 : sh.s0)) + tok % per * a.group + in_head;
-                x -= ns;
-                return (ow.c0 == ow.c1 ? own_row(tok, tile.kvh) : part_row(ow.c0 + x, x ? 0 : ow.s0)) + in_head;
-            };
+            // Each lane fetches the statistics of one of the warp's records; then all of a record's columns at a time.
             const int c = lane % (D / 4) * 4;  // D = 64: two lanes have the same columns
             Gather sum;
-            for (int x = part; x < n; x += 8 * teams) {
-                float2 ml[8];
-                float4 o[8];
-#pragma unroll
-                for (int y = 0; y < 8; y++) {
-                    const size_t at = row_of(min(x + y * teams, n - 1));
-                    ml[y] = __ldcg(&sa.rec_ml[at]);
-                    o[y] = __ldcg(reinterpret_cast<const float4*>(sa.rec_o + at * D + c));
+            for (int base = 0; part + base * teams < n; base += 32) {
+                const int x = part + (base + lane) * teams, y = x - ns;
+                size_t at = 0;
+                float2 ml = make_float2(-INFINITY, 0.f);
+                if (x < n) {
+                    at = x < ns ? (ns == 1 ? shared_row(tok, tile.kvh) : part_row(sh.c0 + x, x ? 0 : sh.s0)) + tok % per * a.group
+                                : ow.c0 == ow.c1 ? own_row(tok, tile.kvh) : part_row(ow.c0 + y, y ? 0 : ow.s0);
+                    at += in_head;
+                    ml = __ldcg(&sa.rec_ml[at]);
                 }
+                float top = ml.x;
 #pragma unroll
-                for (int y = 0; y < 8; y++)
-                    if (x + y * teams < n) sum.add(ml[y], o[y]);
+                for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                const float f = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - top);
+                float l = ml.y * f;
+#pragma unroll
+                for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+                float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+                const int here = min(32, (n - part - base * teams + teams - 1) / teams);
+#pragma unroll 8
+                for (int i = 0; i < here; i++) {
+                    const float fi = __shfl_sync(0xffffffffu, f, i);
+                    const float4 v = __ldcg(reinterpret_cast<const float4*>(sa.rec_o + __shfl_sync(0xffffffffu, at, i) * D + c));
+                    o.x = fmaf(v.x, fi, o.x);
+                    o.y = fmaf(v.y, fi, o.y);
+                    o.z = fmaf(v.z, fi, o.z);
+                    o.w = fmaf(v.w, fi, o.w);
+                }
+                sum.add(make_float2(top, l), o);
             }
             const size_t R = (size_t)(sa.tok_base + tok) * a.q_heads + tile.kvh * a.group + in_head;
             if (teams == 1) {
@@ -507,22 +555,19 @@ constexpr int kSmemMax = 227 * 1024, kSmemSm = 228 * 1024, kStaticMax = 2048;  /
 
 static int shared_tiles_of(const AttnArgs& a, int count) { return (count + 16 / a.group - 1) / (16 / a.group); }
 
-template <typename T, int D>
-static int launch_stream_t(StreamArgs sa, const void* maps, cudaStream_t stream)
+template <typename T, int D, int kBlocks, bool kDup>
+static int launch_rows_t(StreamArgs sa, const void* maps, cudaStream_t stream)
 {
     using S = Stream<T, D>;
     static bool ready[64];
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return (int)e;
+    const int dev = sa.a.device;
     if (dev < 0 || dev >= 64) return (int)cudaErrorInvalidDevice;
-    const int tokens = sa.shared_tiles ? 16 / sa.a.group : 1;  // of an item, at most
-    sa.q_bytes = (tokens * sa.a.group * D * (sa.a.io_bf16 ? 2 : 4) + 127) / 128 * 128;
-    sa.item_rows = tokens * sa.a.group;
+    cudaError_t e;
+    sa.q_bytes = (sa.item_rows * D * (sa.a.io_bf16 ? 2 : 4) + 127) / 128 * 128;
     // Two CTAs per SM where that leaves each two stages or more, else one.
     sa.buffers = sa.item_rows <= 4 ? 2 : 1;
     const int fixed = sa.buffers * kTakers * sa.item_rows * S::kPitch * 4 + (2 * sa.a.batch + 1) * 4 + 1024 +  // + alignment
-                      (sizeof(T) == 4 ? 2 * (sa.item_rows <= 8 ? 8 : 16) * S::kPitch * 4 : 0);
+                      (sizeof(T) == 4 && !kDup ? 2 * 8 * kBlocks * S::kPitch * 4 : 0);
     int ctas = 2, most = kSmemSm / 2 - 1024 - kStaticMax;
     if ((most - fixed) / (S::kStage + sa.q_bytes) < 2) {
         ctas = 1;
@@ -532,15 +577,25 @@ static int launch_stream_t(StreamArgs sa, const void* maps, cudaStream_t stream)
     if (sa.stages > kMaxStages) sa.stages = kMaxStages;
     const int bytes = sa.stages * (S::kStage + sa.q_bytes) + fixed;
     if (!ready[dev]) {
-        e = cudaFuncSetAttribute(pages_stream_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax - kStaticMax);
+        e = cudaFuncSetAttribute(pages_stream_kernel<T, D, kBlocks, kDup>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax - kStaticMax);
         if (e == cudaSuccess)
-            e = cudaFuncSetAttribute(pages_stream_kernel<T, D>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+            e = cudaFuncSetAttribute(pages_stream_kernel<T, D, kBlocks, kDup>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
         if (e != cudaSuccess) return (int)e;
         ready[dev] = true;
     }
     const CUtensorMap* m = static_cast<const CUtensorMap*>(maps);
-    pages_stream_kernel<T, D><<<ctas * kSms, kStreamThreads, bytes, stream>>>(m[0], m[1], sa);
+    pages_stream_kernel<T, D, kBlocks, kDup><<<ctas * kSms, kStreamThreads, bytes, stream>>>(m[0], m[1], sa);
     return (int)cudaGetLastError();
+}
+
+template <typename T, int D>
+static int launch_stream_t(StreamArgs sa, const void* maps, cudaStream_t stream)
+{
+    const int tokens = sa.shared_tiles ? min(sa.a.batch, 16 / sa.a.group) : 1;  // of an item, at most
+    sa.item_rows = tokens * sa.a.group;
+    if (sa.item_rows <= 4) return launch_rows_t<T, D, 1, true>(sa, maps, stream);
+    if (sa.item_rows <= 8) return launch_rows_t<T, D, 1, false>(sa, maps, stream);
+    return launch_rows_t<T, D, 2, false>(sa, maps, stream);
 }
 
 // Record rows of one launch for `count` sequences.
@@ -566,13 +621,13 @@ int launch_stream(const AttnArgs& a, int layer, int first, int count, bool share
     sa.tok_base = first;
     const int rows = a.p.kv_dtype == TYB_BF16 ? 64 : 32;  // of a stage
     sa.shared_tiles = shared ? shared_tiles_of(a, count) : 0;
-    sa.shared_units = shared ? (a.prefix + rows - 1) / rows : 0;
+    sa.shared_units = shared ? kItemUnits + (a.prefix + rows - 1) / rows : 0;
     sa.out_slot = out_slot;
     sa.max_len = max_len;
     sa.rec_o = static_cast<float*>(ws);
     sa.rec_ml = reinterpret_cast<float2*>(sa.rec_o + record_rows(a, count, shared) * D);
     sa.tickets = tickets;
-    sa.wait_ns = tyb_wait_limit();
+    sa.wait_ns = tyb_wait_limit_of(a.device);
     if (a.p.kv_dtype == TYB_BF16)
         return D == 128 ? launch_stream_t<__nv_bfloat16, 128>(sa, maps, stream) : launch_stream_t<__nv_bfloat16, 64>(sa, maps, stream);
     return D == 128 ? launch_stream_t<float, 128>(sa, maps, stream) : launch_stream_t<float, 64>(sa, maps, stream);

@@ -24,9 +24,12 @@ def _library():
 
 
 def _ints(x, what):
-    if x.dtype != torch.int32 or not x.is_contiguous():
+    if x.dtype is not torch.int32 or not x.is_contiguous():
         raise ValueError(f"{what}: a contiguous int32 tensor is wanted")
     return x
+
+
+_raw_stream = torch._C._cuda_getCurrentRawStream  # what torch.cuda.current_stream().cuda_stream is, without the objects
 
 
 class PagePool:
@@ -44,7 +47,8 @@ class PagePool:
             raise ValueError("k and v have to be contiguous")
         if table.dim() != 2 or length.shape != table.shape[:1] or ref.shape != k.shape[1:2]:
             raise ValueError("table [seqs][entries], length [seqs], ref [pages] are wanted")
-        self.device = k.device
+        self.device, self._index = k.device, k.device.index
+        self._codes = {torch.float32: pkg.ATTN_DT_F32, torch.bfloat16: pkg.ATTN_DT_BF16}
         layers, pages, self.kv_heads, page, self.head_dim = k.shape
         dtype = pkg.ATTN_KV_BF16 if k.dtype == torch.bfloat16 else pkg.ATTN_KV_F32
         with torch.cuda.device(self.device):
@@ -70,39 +74,38 @@ class PagePool:
             self._handle = None
 
     def _stream(self):
-        self.lib.attn_set_stream(torch.cuda.current_stream(self.device).cuda_stream)
+        self.lib.attn_set_stream(_raw_stream(self._index))
 
     def _call(self, fn, *args):
         if not self._handle:
             raise RuntimeError("the pool is closed")
-        self._stream()
+        self.lib.attn_set_stream(_raw_stream(self._index))
         if fn(*args):
             msg = _package().last_error(self.lib)
             self.lib.attn_clear_error()
             raise RuntimeError(msg)
 
     def _dtype(self, x):
-        pkg = _package()
-        if x.dtype == torch.bfloat16:
-            return pkg.ATTN_DT_BF16
-        if x.dtype == torch.float32:
-            return pkg.ATTN_DT_F32
-        raise ValueError(f"bfloat16 or float32 is wanted, not {x.dtype}")
+        code = self._codes.get(x.dtype)
+        if code is None:
+            raise ValueError(f"bfloat16 or float32 is wanted, not {x.dtype}")
+        return code
 
     def _tokens(self, x, heads, what):
         """Row stride, in elements, of [rows][heads][head_dim] (any row stride, as in a slice of a fused projection)."""
-        if x.dim() != 3 or x.shape[1] != heads or x.shape[2] != self.head_dim:
-            raise ValueError(f"{what}: [rows][{heads}][{self.head_dim}] is wanted, not {tuple(x.shape)}")
-        if x.stride(2) != 1 or x.stride(1) != self.head_dim:
+        shape, d = x.shape, self.head_dim
+        if len(shape) != 3 or shape[1] != heads or shape[2] != d:
+            raise ValueError(f"{what}: [rows][{heads}][{d}] is wanted, not {tuple(shape)}")
+        stride = x.stride()
+        if stride[2] != 1 or (stride[1] != d and heads > 1):
             raise ValueError(f"{what}: the heads of a row have to lie one after another")
-        return x.stride(0) if x.shape[0] > 1 else heads * self.head_dim
+        return stride[0] if shape[0] > 1 else heads * d
 
     # ---- maintenance ----------------------------------------------------------------------------
 
     def _list(self, x, what, n=None):
-        _ints(x, what)
-        if x.dim() != 1 or x.device != self.device or (n is not None and x.numel() != n):
-            raise ValueError(f"{what}: a list{'' if n is None else f' of {n}'} on {self.device} is wanted")
+        if x.dtype is not torch.int32 or x.dim() != 1 or not x.is_contiguous() or (n is not None and x.shape[0] != n):
+            raise ValueError(f"{what}: a contiguous int32 list{'' if n is None else f' of {n}'} is wanted")
         return x.data_ptr()
 
     def extend(self, seqs, counts):
@@ -148,25 +151,27 @@ class PagePool:
     def _output(self, q, out):
         if out is None:
             return torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
+        if out.shape != q.shape or out.dtype is not q.dtype or not out.is_contiguous():
             raise ValueError("out: contiguous, of q's shape and type, is wanted")
         return out
 
     def attend_prefix(self, q, layer, seqs, prefix_len, max_len, scale, out=None):
         """One token for each sequence, q [batch][q_heads][head_dim], their first prefix_len tokens shared."""
-        stride = self._tokens(q, q.shape[1], "q")
+        rows, heads = q.shape[0], q.shape[1]
+        stride = self._tokens(q, heads, "q")
         out = self._output(q, out)
         self._call(self.lib.attention_pages_prefix_gqa, q.data_ptr(), stride, self._handle, layer,
-                   self._list(seqs, "seqs", q.shape[0]), q.shape[0], q.shape[1], prefix_len, max_len, out.data_ptr(),
-                   self._dtype(q), scale)
+                   self._list(seqs, "seqs", rows), rows, heads, prefix_len, max_len, out.data_ptr(), self._dtype(q), scale)
         return out
 
     def attend_window(self, q, layer, seqs, starts, max_new, max_len, window, sinks, scale, out=None):
         """Causal attention of each sequence's last tokens, q [rows][q_heads][head_dim], through a window (0: none) with
         sinks; starts None: one token for each sequence."""
-        stride = self._tokens(q, q.shape[1], "q")
+        rows, heads = q.shape[0], q.shape[1]
+        stride = self._tokens(q, heads, "q")
         out = self._output(q, out)
+        batch = seqs.shape[0]
         self._call(self.lib.attention_pages_window_gqa, q.data_ptr(), stride, self._handle, layer, self._list(seqs, "seqs"),
-                   None if starts is None else self._list(starts, "starts", seqs.numel() + 1), seqs.numel(), q.shape[0],
-                   q.shape[1], max_new, max_len, window, sinks, out.data_ptr(), self._dtype(q), scale)
+                   None if starts is None else self._list(starts, "starts", batch + 1), batch, rows, heads, max_new, max_len,
+                   window, sinks, out.data_ptr(), self._dtype(q), scale)
         return out
