@@ -131,6 +131,7 @@ __global__ void __launch_bounds__(kPlanThreads)
     extern __shared__ unsigned int marks[];
     const Plan plan = plan_at(ws, n, p.num_pages);
     const int cap = p.max_pages * p.page_size;
+    after_predecessor();
     clear_marks(marks, p.max_seqs);
     int need = 0;
     bool bad = false;
@@ -193,6 +194,7 @@ __global__ void __launch_bounds__(kPlanThreads)
     const Plan plan = plan_at(ws, n, p.num_pages);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int cap = p.max_pages * p.page_size;
+    after_predecessor();
     clear_marks(marks, p.max_seqs);
     bool bad = false;
     for (int i = threadIdx.x; i < n; i += kPlanThreads) {
@@ -279,6 +281,7 @@ __global__ void __launch_bounds__(kApplyThreads)
     pages_fork_apply_kernel(const KVPages p, const int* src, const int* dst, int n, int deep, int row_bytes, void* ws)
 {
     const Plan plan = plan_at(ws, n, p.num_pages);
+    after_predecessor();
     if (!plan.head->ok) return;
     const int lane = threadIdx.x & 31;
     // Tables and counts: a warp per item.
@@ -316,6 +319,7 @@ __global__ void __launch_bounds__(kApplyThreads)
 __global__ void __launch_bounds__(128)
     pages_free_kernel(const KVPages p, const int* seqs, int trim, int window, int sinks, Status st)
 {
+    after_predecessor();
     const int s = seqs[blockIdx.x];
     if (s < 0 || s >= p.max_seqs) {
         if (threadIdx.x == 0) raise(st, TYB_STATUS_BAD_ARGUMENT);
@@ -339,6 +343,7 @@ __global__ void __launch_bounds__(128)
 __global__ void __launch_bounds__(kPlanThreads) pages_compact_plan_kernel(const KVPages p, int* live_out, void* ws)
 {
     const Plan plan = plan_at(ws, 0, p.num_pages);
+    after_predecessor();
     int live = 0;
     for (int i = threadIdx.x; i < p.num_pages; i += kPlanThreads) live += p.ref[i] > 0;
     int total;
@@ -366,6 +371,7 @@ __global__ void __launch_bounds__(kPlanThreads) pages_compact_plan_kernel(const 
 __global__ void __launch_bounds__(kApplyThreads) pages_compact_apply_kernel(const KVPages p, int row_bytes, void* ws)
 {
     const Plan plan = plan_at(ws, 0, p.num_pages);
+    after_predecessor();
     const int live = plan.head->live;
     const long long entries = (long long)p.max_seqs * p.max_pages;
     for (long long i = (long long)blockIdx.x * kApplyThreads + threadIdx.x; i < entries; i += (long long)gridDim.x * kApplyThreads) {
@@ -396,6 +402,7 @@ __global__ void __launch_bounds__(kApplyThreads)
                        const In* v_new, long long stride, Status st)
 {
     const int lane = threadIdx.x & 31;
+    after_predecessor();
     const int row_vecs = p.kv_heads * p.head_dim / 8, head_vecs = p.head_dim / 8;
     for (int w = (int)(blockIdx.x * (kApplyThreads / 32) + (threadIdx.x >> 5)); w < 2 * rows; w += (int)gridDim.x * (kApplyThreads / 32)) {
         const int t = w >> 1;
@@ -427,6 +434,7 @@ __global__ void __launch_bounds__(kApplyThreads)
     pages_import_kernel(const KVPages p, int seq, const char* k_slab, const char* v_slab, int row_capacity, int rows,
                         int row_bytes, const void* ws)
 {
+    after_predecessor();
     if (!static_cast<const PlanHead*>(ws)->ok) return;
     const int lt = p.num_layers * 2;
     const long long units = (long long)((rows + p.page_size - 1) / p.page_size) * lt * p.kv_heads;
@@ -466,87 +474,70 @@ using namespace tyb;
 
 extern "C" size_t tyb_pages_plan_bytes(const KVPages* p, int n) { return plan_bytes(n, p->num_pages); }
 
-extern "C" int tyb_pages_extend_launch(const KVPages* p, const tyb_pages_env* env, const int* seqs, const int* counts, int n, void* ws, void* stream)
+extern "C" int tyb_pages_extend_launch(const KVPages* p, const tyb_pages_env* env, const int* seqs, const int* counts, int n, void* ws,
+                                       void* stream)
 {
-    const Status st = status_of(env);
     size_t marks;
-    int e = marks_bytes(pages_extend_kernel, p, &marks);
+    const int e = marks_bytes(pages_extend_kernel, p, &marks);
     if (e) return e;
-    pages_extend_kernel<<<1, kPlanThreads, marks, (cudaStream_t)stream>>>(*p, seqs, counts, n, 0, 0, ws, st);
-    return (int)cudaGetLastError();
+    return launch_after(pages_extend_kernel, dim3(1), kPlanThreads, marks, (cudaStream_t)stream, *p, seqs, counts, n, 0, 0, ws, status_of(env));
 }
 
-extern "C" int tyb_pages_fork_launch(const KVPages* p, const tyb_pages_env* env, const int* src, const int* dst, int n, int deep, void* ws, void* stream)
+extern "C" int tyb_pages_fork_launch(const KVPages* p, const tyb_pages_env* env, const int* src, const int* dst, int n, int deep, void* ws,
+                                     void* stream)
 {
-    const Status st = status_of(env);
     size_t marks;
     int e = marks_bytes(pages_fork_plan_kernel, p, &marks);
+    if (!e) e = launch_after(pages_fork_plan_kernel, dim3(1), kPlanThreads, marks, (cudaStream_t)stream, *p, src, dst, n, deep, ws, status_of(env));
     if (e) return e;
-    pages_fork_plan_kernel<<<1, kPlanThreads, marks, (cudaStream_t)stream>>>(*p, src, dst, n, deep, ws, st);
-    e = (int)cudaGetLastError();
-    if (e) return e;
-    pages_fork_apply_kernel<<<kSms * 8, kApplyThreads, 0, (cudaStream_t)stream>>>(*p, src, dst, n, deep, row_bytes_of(p), ws);
-    return (int)cudaGetLastError();
+    return launch_after(pages_fork_apply_kernel, dim3(kSms * 8), kApplyThreads, 0, (cudaStream_t)stream, *p, src, dst, n, deep, row_bytes_of(p), ws);
 }
 
 extern "C" int tyb_pages_free_launch(const KVPages* p, const tyb_pages_env* env, const int* seqs, int n, void* stream)
 {
-    const Status st = status_of(env);
-    pages_free_kernel<<<n, 128, 0, (cudaStream_t)stream>>>(*p, seqs, 0, 0, 0, st);
-    return (int)cudaGetLastError();
+    return launch_after(pages_free_kernel, dim3(n), 128, 0, (cudaStream_t)stream, *p, seqs, 0, 0, 0, status_of(env));
 }
 
 extern "C" int tyb_pages_trim_launch(const KVPages* p, const tyb_pages_env* env, const int* seqs, int n, int window, int sinks, void* stream)
 {
-    const Status st = status_of(env);
-    pages_free_kernel<<<n, 128, 0, (cudaStream_t)stream>>>(*p, seqs, 1, window, sinks, st);
-    return (int)cudaGetLastError();
+    return launch_after(pages_free_kernel, dim3(n), 128, 0, (cudaStream_t)stream, *p, seqs, 1, window, sinks, status_of(env));
 }
 
 extern "C" int tyb_pages_compact_launch(const KVPages* p, int* live_out, void* ws, void* stream)
 {
-    pages_compact_plan_kernel<<<1, kPlanThreads, 0, (cudaStream_t)stream>>>(*p, live_out, ws);
-    const int e = (int)cudaGetLastError();
+    const int e = launch_after(pages_compact_plan_kernel, dim3(1), kPlanThreads, 0, (cudaStream_t)stream, *p, live_out, ws);
     if (e) return e;
-    pages_compact_apply_kernel<<<kSms * 8, kApplyThreads, 0, (cudaStream_t)stream>>>(*p, row_bytes_of(p), ws);
-    return (int)cudaGetLastError();
+    return launch_after(pages_compact_apply_kernel, dim3(kSms * 8), kApplyThreads, 0, (cudaStream_t)stream, *p, row_bytes_of(p), ws);
 }
 
-extern "C" int tyb_pages_write_launch(const KVPages* p, const tyb_pages_env* env, int layer, const int* seqs, const int* starts, int n, int rows,
-                                      const void* k_new, const void* v_new, int in_bf16, long long stride, void* stream)
+template <typename In, typename T>
+static int launch_write(const KVPages* p, const tyb_pages_env* env, int layer, const int* seqs, const int* starts, int n, int rows,
+                        const void* k_new, const void* v_new, long long stride, cudaStream_t stream)
 {
-    const Status st = status_of(env);
     const int per_cta = kApplyThreads / 32;
     const long long ctas = (2LL * rows + per_cta - 1) / per_cta;
-    const unsigned grid = (unsigned)(ctas < kSms * 16 ? ctas : kSms * 16);
-    cudaStream_t cs = (cudaStream_t)stream;
-    const bool bf = p->kv_dtype == TYB_BF16;
-    if (in_bf16 && bf)
-        pages_write_kernel<__nv_bfloat16, __nv_bfloat16><<<grid, kApplyThreads, 0, cs>>>(
-            *p, layer, seqs, starts, n, rows, (const __nv_bfloat16*)k_new, (const __nv_bfloat16*)v_new, stride, st);
-    else if (in_bf16)
-        pages_write_kernel<__nv_bfloat16, float><<<grid, kApplyThreads, 0, cs>>>(
-            *p, layer, seqs, starts, n, rows, (const __nv_bfloat16*)k_new, (const __nv_bfloat16*)v_new, stride, st);
-    else if (bf)
-        pages_write_kernel<float, __nv_bfloat16><<<grid, kApplyThreads, 0, cs>>>(
-            *p, layer, seqs, starts, n, rows, (const float*)k_new, (const float*)v_new, stride, st);
-    else
-        pages_write_kernel<float, float><<<grid, kApplyThreads, 0, cs>>>(*p, layer, seqs, starts, n, rows, (const float*)k_new,
-                                                                        (const float*)v_new, stride, st);
-    return (int)cudaGetLastError();
+    return launch_after(pages_write_kernel<In, T>, dim3((unsigned)(ctas < kSms * 16 ? ctas : kSms * 16)), kApplyThreads, 0, stream, *p, layer,
+                        seqs, starts, n, rows, static_cast<const In*>(k_new), static_cast<const In*>(v_new), stride, status_of(env));
 }
 
-extern "C" int tyb_pages_import_launch(const KVPages* p, const tyb_pages_env* env, int seq, const void* k_slab, const void* v_slab, int row_capacity,
-                                       int rows, void* ws, void* stream)
+extern "C" int tyb_pages_write_launch(const KVPages* p, const tyb_pages_env* env, int layer, const int* seqs, const int* starts, int n,
+                                      int rows, const void* k_new, const void* v_new, int in_bf16, long long stride, void* stream)
 {
-    const Status st = status_of(env);
+    typedef __nv_bfloat16 bf;
+    auto* launch = p->kv_dtype == TYB_BF16 ? (in_bf16 ? launch_write<bf, bf> : launch_write<float, bf>)
+                                           : (in_bf16 ? launch_write<bf, float> : launch_write<float, float>);
+    return launch(p, env, layer, seqs, starts, n, rows, k_new, v_new, stride, (cudaStream_t)stream);
+}
+
+extern "C" int tyb_pages_import_launch(const KVPages* p, const tyb_pages_env* env, int seq, const void* k_slab, const void* v_slab,
+                                       int row_capacity, int rows, void* ws, void* stream)
+{
     size_t marks;
     int e = marks_bytes(pages_extend_kernel, p, &marks);
+    if (!e)
+        e = launch_after(pages_extend_kernel, dim3(1), kPlanThreads, marks, (cudaStream_t)stream, *p, nullptr, nullptr, 1, seq, rows, ws,
+                         status_of(env));
     if (e) return e;
-    pages_extend_kernel<<<1, kPlanThreads, marks, (cudaStream_t)stream>>>(*p, nullptr, nullptr, 1, seq, rows, ws, st);
-    e = (int)cudaGetLastError();
-    if (e) return e;
-    pages_import_kernel<<<kSms * 8, kApplyThreads, 0, (cudaStream_t)stream>>>(*p, seq, (const char*)k_slab, (const char*)v_slab,
-                                                                             row_capacity, rows, row_bytes_of(p), ws);
-    return (int)cudaGetLastError();
+    return launch_after(pages_import_kernel, dim3(kSms * 8), kApplyThreads, 0, (cudaStream_t)stream, *p, seq, static_cast<const char*>(k_slab),
+                        static_cast<const char*>(v_slab), row_capacity, rows, row_bytes_of(p), ws);
 }

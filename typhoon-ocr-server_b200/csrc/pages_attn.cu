@@ -320,6 +320,7 @@ __global__ void __launch_bounds__(kThreads) pages_rows_kernel(const AttnArgs a)
     const int kvh = blockIdx.y, split = blockIdx.z;
     const int per = kRowsCta / a.group;
     int seq = 0, tok0, ntok, pos0;  // first token (row of q) of the tile, tokens, position of the first
+    after_predecessor();
     __shared__ int found[4];
     {
         // which sequence's tile this is: a warp scans the sequences' tile counts
@@ -420,6 +421,7 @@ __global__ void __launch_bounds__(kThreads) pages_join_kernel(const AttnArgs a)
 {
     const int lane = threadIdx.x & 31;
     const int R = (int)(blockIdx.x * kWarps + (threadIdx.x >> 5));
+    after_predecessor();
     if (R >= a.rec.rows) return;
     constexpr int kPer = D / 32;
     float top = -INFINITY;
@@ -540,8 +542,7 @@ static int launch_rows(const AttnArgs& a, int row_tiles, cudaStream_t stream)
         if (e != cudaSuccess) return (int)e;
         ready[dev] = true;
     }
-    pages_rows_kernel<float, D><<<dim3(row_tiles, a.p.kv_heads, a.splits), kThreads, rows, stream>>>(a);
-    return (int)cudaGetLastError();
+    return launch_after(pages_rows_kernel<float, D>, dim3(row_tiles, a.p.kv_heads, a.splits), kThreads, rows, stream, a);
 }
 
 }  // namespace tyb
@@ -586,9 +587,7 @@ extern "C" int tyb_pages_attn_launch(const tyb_pages_attn* c, void* ws, void* ti
     }
     if (records(l)) {
         const int grid = ceil_div(a.rec.rows, kWarps);
-        if (D == 128) pages_join_kernel<128><<<grid, kThreads, 0, st>>>(a);
-        else pages_join_kernel<64><<<grid, kThreads, 0, st>>>(a);
-        return (int)cudaGetLastError();
+        return launch_after(D == 128 ? pages_join_kernel<128> : pages_join_kernel<64>, dim3(grid), kThreads, 0, st, a);
     }
     return 0;
 }

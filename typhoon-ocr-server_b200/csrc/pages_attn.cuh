@@ -18,6 +18,31 @@ __device__ __forceinline__ void raise(const Status& s, unsigned int bits)
     flag_mirror(s.mirror);
 }
 
+// The kernels of the paged cache are launched as programmatic dependents (launch_after): a kernel may start while
+// its predecessor in the stream ends, sets itself up, and reads or writes nothing global before this wait.
+// Only then it lets the next one start, as the library's other kernels do and rely on.
+__device__ __forceinline__ void after_predecessor()
+{
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+template <typename... P, typename... A>
+int launch_after(void (*kernel)(P...), dim3 grid, int threads, size_t shared, cudaStream_t stream, A... args)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = shared;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return (int)cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+
 // Waits for phase `parity` of an mbarrier, at most limit_ns; false (and the status raised) when that ran
 // out.
 __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, uint64_t limit_ns, const Status& s)

@@ -147,6 +147,30 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int rows_item = ta.tall ? kRows : 2 * kRows;
     const int per = rows_item / a.group;  // tokens of an item
 
+    if (warp == 8) {
+        if (lane == 0) {
+            for (int i = 0; i < 2; i++) {
+                mbar_init(&k_full[i], 1);
+                mbar_init(&k_free[i], 1);
+                mbar_init(&v_full[i], 1);
+                mbar_init(&v_free[i], 1);
+                mbar_init(&v_clear[i], 32);
+                mbar_init(&s_full[i], 1);
+                mbar_init(&s_free[i], kRows);
+                mbar_init(&p_full[i], kRows);
+                mbar_init(&pv_done[i], 1);
+            }
+            mbar_init(q_full, kSoftThreads);
+            mbar_init(drain, 1);
+            fence_barrier_init();
+            fence_proxy_async_smem();
+        }
+        __syncwarp();
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        tc_fence_before();
+    }
+    after_predecessor();
     // Which tokens: item x of the batch (the last items, with the most keys to see, first).
     if (warp == 0 && !ta.shared_pass) {
         const int x = (int)(gridDim.x - 1 - blockIdx.x);
@@ -176,29 +200,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
             before += __shfl_sync(0xffffffffu, sum, 31);
         }
-    }
-    if (warp == 8) {
-        if (lane == 0) {
-            for (int i = 0; i < 2; i++) {
-                mbar_init(&k_full[i], 1);
-                mbar_init(&k_free[i], 1);
-                mbar_init(&v_full[i], 1);
-                mbar_init(&v_free[i], 1);
-                mbar_init(&v_clear[i], 32);
-                mbar_init(&s_full[i], 1);
-                mbar_init(&s_free[i], kRows);
-                mbar_init(&p_full[i], kRows);
-                mbar_init(&pv_done[i], 1);
-            }
-            mbar_init(q_full, kSoftThreads);
-            mbar_init(drain, 1);
-            fence_barrier_init();
-            fence_proxy_async_smem();
-        }
-        __syncwarp();
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-        tc_fence_before();
     }
     __syncthreads();
     tc_fence_after();
@@ -551,8 +552,7 @@ static int launch_tc(const TcArgs& ta, const void* maps, dim3 grid, cudaStream_t
         ready[dev] = true;
     }
     const CUtensorMap* m = static_cast<const CUtensorMap*>(maps);
-    pages_tc_kernel<D><<<grid, kTcThreads, Smem<D>::kBytes, stream>>>(m[0], m[1], ta);
-    return (int)cudaGetLastError();
+    return launch_after(pages_tc_kernel<D>, grid, kTcThreads, Smem<D>::kBytes, stream, m[0], m[1], ta);
 }
 
 int tc_launch(const AttnArgs& a, int layer, bool tall, bool shared_pass, int items, const void* maps, cudaStream_t stream)

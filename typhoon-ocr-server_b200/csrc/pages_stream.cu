@@ -147,6 +147,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
         mbar_init(&met, kTakers);
         fence_barrier_init();
     }
+    after_predecessor();
     // Units of each sequence's own rows: kItemUnits, then its stages, of which it has one at least, so that every
     // output row has an owner.
     auto own_lo = [&](int len) { return a.window ? max(0, len - a.window) : min(a.prefix, len); };
@@ -452,7 +453,6 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
 
         // Tickets: of each sequence that the item has rows of, this run's record is there; the last to come
         // joins that sequence's rows.
-        __threadfence();
         if (tid == 0) last_of = 0;
         if (!meet()) return;
         // the records of (token, KV head): where its shared ones and its own ones lie
@@ -472,7 +472,10 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
             spans(tile.tok0 + tid, sh, ow);
             const unsigned int count = (unsigned int)(ow.c1 - ow.c0 + 1 + sh.c1 - sh.c0 + 1);
             unsigned int* ticket = sa.tickets + (size_t)(tile.tok0 + tid) * heads + tile.kvh;
-            if (atomicAdd(ticket, 1u) == count - 1u) {
+            // releases what all the CTA's threads wrote before they met, and acquires what the others released
+            unsigned int before_me;
+            asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(before_me) : "l"(ticket) : "memory");
+            if (before_me == count - 1u) {
                 *ticket = 0u;
                 atomicOr(&last_of, 1u << tid);
             }
@@ -480,7 +483,6 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
         if (!meet()) return;
         const unsigned int mine = last_of;
         if (!mine) continue;
-        __threadfence();
         // The rows of all those sequences at once: `teams` warps a row, each with some of its records, eight
         // requested at a time; then the warps are joined.
         const int rows = __popc(mine) * a.group, teams = rows >= kTakers ? 1 : kTakers / rows;
@@ -516,14 +518,19 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
                 for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
                 float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
                 const int here = min(32, (n - part - base * teams + teams - 1) / teams);
-#pragma unroll 8
-                for (int i = 0; i < here; i++) {
-                    const float fi = __shfl_sync(0xffffffffu, f, i);
-                    const float4 v = __ldcg(reinterpret_cast<const float4*>(sa.rec_o + __shfl_sync(0xffffffffu, at, i) * D + c));
-                    o.x = fmaf(v.x, fi, o.x);
-                    o.y = fmaf(v.y, fi, o.y);
-                    o.z = fmaf(v.z, fi, o.z);
-                    o.w = fmaf(v.w, fi, o.w);
+                for (int i = 0; i < here; i += 8) {  // eight requested at a time
+                    float4 v[8];
+#pragma unroll
+                    for (int k = 0; k < 8; k++)
+                        v[k] = __ldcg(reinterpret_cast<const float4*>(sa.rec_o + __shfl_sync(0xffffffffu, at, min(i + k, here - 1)) * D + c));
+#pragma unroll
+                    for (int k = 0; k < 8; k++) {
+                        const float fk = i + k < here ? __shfl_sync(0xffffffffu, f, (i + k) & 31) : 0.f;
+                        o.x = fmaf(v[k].x, fk, o.x);
+                        o.y = fmaf(v[k].y, fk, o.y);
+                        o.z = fmaf(v[k].z, fk, o.z);
+                        o.w = fmaf(v[k].w, fk, o.w);
+                    }
                 }
                 sum.add(make_float2(top, l), o);
             }
@@ -584,8 +591,7 @@ static int launch_rows_t(StreamArgs sa, const void* maps, cudaStream_t stream)
         ready[dev] = true;
     }
     const CUtensorMap* m = static_cast<const CUtensorMap*>(maps);
-    pages_stream_kernel<T, D, kBlocks, kDup><<<ctas * kSms, kStreamThreads, bytes, stream>>>(m[0], m[1], sa);
-    return (int)cudaGetLastError();
+    return launch_after(pages_stream_kernel<T, D, kBlocks, kDup>, dim3(ctas * kSms), kStreamThreads, bytes, stream, m[0], m[1], sa);
 }
 
 template <typename T, int D>
