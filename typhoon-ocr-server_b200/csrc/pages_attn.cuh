@@ -47,17 +47,20 @@ int launch_after(void (*kernel)(P...), dim3 grid, int threads, size_t shared, cu
 // out.
 __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, uint64_t limit_ns, const Status& s)
 {
-    if (mbar_try_wait(bar, parity)) return true;
-    const uint64_t t0 = globaltimer_ns();
-    while (true) {
-#pragma unroll 1
-        for (int i = 0; i < 64; i++)
-            if (mbar_try_wait(bar, parity)) return true;
-        if (globaltimer_ns() - t0 > limit_ns) {
-            raise(s, TYB_STATUS_WAIT_TIMEOUT);
-            return false;
-        }
-    }
+    return mbar_wait_bounded_to(bar, parity, limit_ns, TYB_STATUS_WAIT_TIMEOUT, s.word, s.mirror);
+}
+
+// The same by all lanes of a warp, with one answer.
+__device__ __forceinline__ bool warp_wait_for(uint64_t* bar, uint32_t parity, uint64_t limit_ns, const Status& s)
+{
+    return !__any_sync(0xffffffffu, !wait_for(bar, parity, limit_ns, s));
+}
+
+// One arrival for the warp, after all its lanes have come here.
+__device__ __forceinline__ void warp_arrive(uint64_t* bar)
+{
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
 }
 
 // A query row at position `pos` sees key j when j <= pos and (j >= lo or j < sinks).  The four uses:

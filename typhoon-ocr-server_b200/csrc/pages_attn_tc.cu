@@ -3,20 +3,23 @@
 // decode batch.
 //
 // A CTA has query rows of one KV head (its q_heads / kv_heads query heads folded into the rows, so
-// that one K/V tile feeds them all) and a run of key tiles of 128.  Two streams of 128 rows alternate
-// on the tensor core, one's softmax overlapping the other's products:
-//   wide   256 rows, both streams take every tile (each K/V tile is loaded once for 256 rows);
-//   tall   at most 128 rows: the streams have the same rows and take the tiles in turn, and their
-//          results are joined like those of two splits.  Half the tensor work of a wide item that
-//          would be half empty, and twice the streams' tiles in flight.
+// that one K/V tile feeds them all) and a run of key tiles of 128, taken in halves.  Two streams of 128
+// rows alternate on the tensor core, one's softmax overlapping the other's products:
+//   wide   256 rows, both streams take every half (each K/V tile is loaded once for 256 rows);
+//   tall   at most 128 rows: the streams have the same rows and take a half each, and their results are
+//          joined like those of two splits.  Half the tensor work of a wide item that would be half empty.
 // A tile comes page by page: one TMA tensor copy per page and 64 columns, the 128-byte-swizzled
 // layout building up in shared memory as if it were one copy; the pages of a tile are issued by as
 // many lanes of the producer warp.  Rows of the tile that no row of the item sees (behind the
 // sequence's end, a page that is not there, before the window) may hold anything: their scores are
 // masked, and their V rows are cleared in shared memory before P.V, since 0 * NaN is not 0.
 //
-// Roles (12 warps): 0-3 and 4-7 the streams' softmax (one row per thread), 8 issues the MMAs, 9 the
-// copies, 10 clears V rows.  TMEM: S (128 columns, the streams in turn) | P0 | P1 (64 each) | O0 | O1.
+// Roles (12 warps): 0-3 and 4-7 the streams' softmax (one row per thread), 8 issues Q.K^T, 11 P.V, 9 the
+// copies, 10 clears V rows.  TMEM: S0 | S1 (64 columns each) | P of each stream, two buffers (32 each) |
+// O0 | O1.  The halves are what makes room for two P buffers beside an S for each stream: the softmax of a half
+// waits for neither the P.V of the one before nor the other stream, only for its own S, which is computed
+// while it works on the half before.  (One S of 128 columns for both and one P each: 2.6 us a tile of 256
+// rows x 128 keys; MMAs alone about 1.1 us, exponentials alone about as much.)
 // Every wait is bounded; a CTA whose wait ran out raises the status word, leaves its loops, frees its
 // TMEM and returns.
 #define TYB_WHOLE_PROGRAM
@@ -27,6 +30,7 @@ namespace tyb {
 
 constexpr int kRows = 128;   // rows of a stream (tensor-core M)
 constexpr int kKeys = 128;   // keys of a tile
+constexpr int kHalf = 64;    // and of a step: N of S, K of P.V
 constexpr int kSoftThreads = 256;
 constexpr int kTcThreads = kSoftThreads + 128;
 // Register split, as in the fused prefill: launched at kLaunchRegs, the issue warpgroup drops to
@@ -59,6 +63,28 @@ __host__ __device__ constexpr uint32_t idesc(int n, bool b_mn_major)
     return (1u << 4) | (1u << 7) | (1u << 10) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
 }
 
+// D[tmem] (+)= A . B^T, kind::f16, A from shared memory (mma_ss) or TMEM (mma_ts).  Issued by one elected lane of a
+// converged warp, so that descriptors and addresses stay in uniform registers: issued from a branch of one
+// lane, each product cost about 150 cycles in moving its operands there, more than twice its execution.
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t accumulate)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a),
+                 "l"(b), "r"(id), "r"(accumulate)
+                 : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t accumulate)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+                 "r"(a), "l"(b), "r"(id), "r"(accumulate)
+                 : "memory");
+}
+
 __device__ __forceinline__ float max3(float a, float b, float c)
 {
     float d;
@@ -69,17 +95,17 @@ __device__ __forceinline__ float max3(float a, float b, float c)
 // Columns [0, n) of 32, n clamped.
 __device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
 
-// Which of a tile's columns a row sees, 32 per word.
+// Which of a step's columns a row sees, 32 per word.
 struct Mask {
-    uint32_t w[4];
+    uint32_t w[kHalf / 32];
 };
 
 template <bool kMask>
-__device__ __forceinline__ float row_max(const float (&s)[kKeys], const Mask& mk)
+__device__ __forceinline__ float row_max(const float (&s)[kHalf], const Mask& mk)
 {
     float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-    for (int c = 0; c < kKeys; c += 2) {
+    for (int c = 0; c < kHalf; c += 2) {
         const float a = (!kMask || (mk.w[c >> 5] >> (c & 31) & 1u)) ? s[c] : -INFINITY;
         const float b = (!kMask || (mk.w[c >> 5] >> ((c + 1) & 31) & 1u)) ? s[c + 1] : -INFINITY;
         m[(c >> 1) & 3] = max3(m[(c >> 1) & 3], a, b);
@@ -90,13 +116,13 @@ __device__ __forceinline__ float row_max(const float (&s)[kKeys], const Mask& mk
 // p = exp2(s * scale + neg) on the visible columns (0 on the others) as BF16 pairs into the row's TMEM
 // columns at p_addr; returns the FP32 sum.  kTrack: *top receives the largest exponent.
 template <bool kMask, bool kTrack>
-__device__ __forceinline__ float row_exp(const float (&s)[kKeys], const Mask& mk, float scale, float neg, uint32_t p_addr, float* top)
+__device__ __forceinline__ float row_exp(const float (&s)[kHalf], const Mask& mk, float scale, float neg, uint32_t p_addr, float* top)
 {
     const float2 sc = make_float2(scale, scale), nm = make_float2(neg, neg);
     float2 acc0 = make_float2(0.f, 0.f), acc1 = make_float2(0.f, 0.f);
     float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
-    for (int q = 0; q < 4; q++) {
+    for (int q = 0; q < kHalf / 32; q++) {
         uint32_t pk[16];
 #pragma unroll
         for (int c = 0; c < 32; c += 4) {
@@ -136,11 +162,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     unsigned char *sQ = smem + S::kQ, *sK = smem + S::kK, *sV = smem + S::kV;
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBars);
-    uint64_t *k_full = bars, *k_free = bars + 2, *v_full = bars + 4, *v_free = bars + 6, *s_full = bars + 8, *s_free = bars + 10,
-             *p_full = bars + 12, *pv_done = bars + 14, *v_clear = bars + 16, *q_full = bars + 18, *drain = bars + 19;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 20);
-    int* found = reinterpret_cast<int*>(bars + 21);                      // [4]
-    volatile uint32_t* present = reinterpret_cast<uint32_t*>(bars + 23);  // [kSeen] a bit per 16 rows of the tile
+    uint64_t *k_full = bars, *k_free = bars + 2, *v_full = bars + 4, *v_free = bars + 6, *v_clear = bars + 8;  // [stage]
+    uint64_t *s_full = bars + 10, *s_free = bars + 12;    // [stream]
+    uint64_t *p_full = bars + 14, *pv_done = bars + 18;   // [stream][buffer]
+    uint64_t *q_full = bars + 22, *drain = bars + 23;  // drain: [2]
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 25);
+    int* found = reinterpret_cast<int*>(bars + 26);                      // [4]
+    volatile uint32_t* present = reinterpret_cast<uint32_t*>(bars + 28);  // [kSeen] a bit per 16 rows of the tile
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int kvh = blockIdx.y, split = blockIdx.z;
@@ -154,14 +182,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 mbar_init(&k_free[i], 1);
                 mbar_init(&v_full[i], 1);
                 mbar_init(&v_free[i], 1);
-                mbar_init(&v_clear[i], 32);
+                mbar_init(&v_clear[i], 1);
                 mbar_init(&s_full[i], 1);
-                mbar_init(&s_free[i], kRows);
-                mbar_init(&p_full[i], kRows);
+                mbar_init(&s_free[i], kRows / 32);
+            }
+            for (int i = 0; i < 4; i++) {
+                mbar_init(&p_full[i], kRows / 32);
                 mbar_init(&pv_done[i], 1);
             }
-            mbar_init(q_full, kSoftThreads);
-            mbar_init(drain, 1);
+            mbar_init(q_full, kSoftThreads / 32);
+            mbar_init(&drain[0], 1);
+            mbar_init(&drain[1], 1);
             fence_barrier_init();
             fence_proxy_async_smem();
         }
@@ -225,14 +256,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const Tiles tiles = tiles_of(ntok > 0 ? pos_max : -1, lo_min, sinks, kKeys);
     const int all = tiles.count();
     const int first = (int)((long long)all * split / a.splits), nt = (int)((long long)all * (split + 1) / a.splits) - first;
-    const int steps = ta.tall ? nt : 2 * nt;  // softmax steps of both streams; step i: stream i & 1
-    // Whether some row of the item does not see the whole tile (its pages aside), and whether the tile
+    constexpr uint32_t kTile16 = S::kTile >> 4, kHalf16 = (kHalf * 128) >> 4;  // in units of the operand descriptors
+    // Step i of both streams is stream i & 1's; its tile and half:
+    const int steps = ta.tall ? 2 * nt : 4 * nt;
+    auto tile_of = [&](int i) { return ta.tall ? i >> 1 : i >> 2; };
+    auto half_of = [&](int i) { return ta.tall ? i & 1 : i >> 1 & 1; };
+    // Whether some row of the item does not see the whole half (its pages aside), and whether the tile
     // has rows that none sees.
-    auto edge = [&](int k0) { return k0 + kKeys - 1 > pos0 || (k0 < lo_max && k0 + kKeys > sinks); };
+    auto edge = [&](int k0) { return k0 + kHalf - 1 > pos0 || (k0 < lo_max && k0 + kHalf > sinks); };
     auto loose = [&](int k0) { return k0 + kKeys - 1 > pos_max || (k0 < lo_min && k0 + kKeys > sinks); };
-    auto wait = [&](uint64_t* bar, uint32_t parity) {
-        return wait_for(bar, parity & 1u, ta.wait_ns, a.st);
-    };
+    auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_for(bar, parity & 1u, ta.wait_ns, a.st); };
+    auto warp_wait = [&](uint64_t* bar, uint32_t parity) { return warp_wait_for(bar, parity & 1u, ta.wait_ns, a.st); };
 
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
@@ -258,8 +292,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 const int row = page < 0 ? 0
                                          : ((ta.layer * a.p.num_pages + page) * a.p.kv_heads + kvh) * a.p.page_size + (key & (a.p.page_size - 1));
                 const uint32_t bytes = (uint32_t)__popc(have) * (uint32_t)(part_bytes * (D / 64));
-                if (t >= kStages) ok = wait(&k_free[st], (uint32_t)((t - kStages) >> 1));
-                if (__any_sync(0xffffffffu, !ok)) break;
+                if (t >= kStages) ok = warp_wait(&k_free[st], (uint32_t)((t - kStages) >> 1));
+                if (!ok) break;
                 if (lane == 0) {
                     uint32_t seen = 0;
                     for (int l = 0; l < per_tile; l++)
@@ -273,8 +307,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     for (int c = 0; c < D / 64; c++)
                         tma_load_2d(sK + st * S::kTile + c * kBox + lane * part_bytes, &map_k, 64 * c, row, &k_full[st]);
                 k_sent = t + 1;
-                if (t >= kStages) ok = wait(&v_free[st], (uint32_t)((t - kStages) >> 1));
-                if (__any_sync(0xffffffffu, !ok)) break;
+                if (t >= kStages) ok = warp_wait(&v_free[st], (uint32_t)((t - kStages) >> 1));
+                if (!ok) break;
                 if (lane == 0) mbar_arrive_expect_tx(&v_full[st], bytes);
                 __syncwarp();
                 if (page >= 0)
@@ -283,75 +317,71 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         tma_load_2d(sV + st * S::kTile + c * kBox + lane * part_bytes, &map_v, 64 * c, row, &v_full[st]);
                 v_sent = t + 1;
             }
-            if (__any_sync(0xffffffffu, !ok)) {  // a wait ran out: the copies requested still land in this CTA
-                for (int t = max(0, k_sent - kStages); t < k_sent; t++) wait(&k_full[t & 1], (uint32_t)(t >> 1));
-                for (int t = max(0, v_sent - kStages); t < v_sent; t++) wait(&v_full[t & 1], (uint32_t)(t >> 1));
+            if (!ok) {  // a wait ran out: the copies requested still land in this CTA
+                for (int t = max(0, k_sent - kStages); t < k_sent; t++) warp_wait(&k_full[t & 1], (uint32_t)(t >> 1));
+                for (int t = max(0, v_sent - kStages); t < v_sent; t++) warp_wait(&v_full[t & 1], (uint32_t)(t >> 1));
             }
         } else if (warp == 8) {
-            // ---- MMA issue (one thread): QK runs two steps ahead of P.V
-            if (lane == 0 && steps > 0) {
-                const uint64_t dq[2] = {umma_desc(smem_u32(sQ), 16), umma_desc(smem_u32(sQ) + (ta.tall ? 0 : S::kTile), 16)};
-                const uint64_t dk[2] = {umma_desc(smem_u32(sK), 16), umma_desc(smem_u32(sK) + S::kTile, 16)};
-                const uint64_t dv[2] = {umma_desc(smem_u32(sV), kBox), umma_desc(smem_u32(sV) + S::kTile, kBox)};
-                auto tile = [&](int i) { return ta.tall ? i : i >> 1; };
-                auto last_use = [&](int i) { return ta.tall || (i & 1); };
-                auto qk = [&](int i) {
-                    const int h = i & 1, t = tile(i), st = t & 1;
+            // ---- S = Q . K^T: a stream's next one goes out as soon as its S has been read
+            const uint64_t dq = umma_desc(smem_u32(sQ), 16), dk = umma_desc(smem_u32(sK), 16);
+            bool ok = steps == 0 || warp_wait(q_full, 0);
+            for (int i = 0; i < steps && ok; i++) {
+                const int h = i & 1, t = tile_of(i), st = t & 1;
+                if (i >= 2) ok = warp_wait(&s_free[h], (uint32_t)(i >> 1) - 1u);
+                if (ok && (i == 0 || tile_of(i - 1) != t)) ok = warp_wait(&k_full[st], (uint32_t)(t >> 1));
+                if (!ok) break;
+                tc_fence_after();
+                const uint64_t q = dq + (ta.tall ? 0u : h * kTile16), k = dk + (st * kTile16 + half_of(i) * kHalf16);
+                const bool last = i + 1 == steps || tile_of(i + 1) != t;
+                if (elect_one()) {
 #pragma unroll
                     for (int kk = 0; kk < D / 16; kk++) {
                         const uint32_t off = ((kk >> 2) * kBox + (kk & 3) * 32) >> 4;
-                        tc_mma(tmem, (h ? dq[1] : dq[0]) + off, (st ? dk[1] : dk[0]) + off, idesc(kKeys, false), kk > 0);
+                        mma_ss(tmem + h * kHalf, q + off, k + off, idesc(kHalf, false), kk > 0);
                     }
                     tc_commit(&s_full[h]);
-                    if (last_use(i)) tc_commit(&k_free[st]);
-                };
-                auto pv = [&](int i) {
-                    const int h = i & 1, t = tile(i), st = t & 1;
-#pragma unroll
-                    for (int kk = 0; kk < kKeys / 16; kk++)
-                        tc_mma_ts(tmem + 256 + h * D, tmem + 128 + h * 64 + kk * 8, (st ? dv[1] : dv[0]) + ((kk * 16 * 128) >> 4),
-                                  idesc(D, true), i > 1 || kk > 0);
-                    tc_commit(&pv_done[h]);
-                    if (last_use(i)) tc_commit(&v_free[st]);
-                };
-                auto step_ready = [&](int i) {  // S free (step i - 1 has read it) and K there
-                    const bool ok = (i == 0 || wait(&s_free[(i - 1) & 1], (uint32_t)((i - 1) >> 1))) &&
-                                    wait(&k_full[tile(i) & 1], (uint32_t)(tile(i) >> 1));
-                    tc_fence_after();
-                    return ok;
-                };
-                auto v_ready = [&](int i) {
-                    const int t = tile(i), st = t & 1;
-                    return wait(&v_full[st], (uint32_t)(t >> 1)) && wait(&v_clear[st], (uint32_t)(t >> 1));
-                };
-                bool ok = wait(q_full, 0) && step_ready(0);
-                if (ok) qk(0);
-                if (ok && steps > 1) {
-                    ok = step_ready(1);
-                    if (ok) qk(1);
+                    if (last) tc_commit(&k_free[st]);
                 }
-                for (int i = 0; i < steps && ok; i++) {
-                    if (i + 2 < steps) {
-                        ok = step_ready(i + 2);
-                        if (!ok) break;
-                        qk(i + 2);
-                    }
-                    ok = wait(&p_full[i & 1], (uint32_t)(i >> 1)) && v_ready(i);
-                    tc_fence_after();
-                    if (ok) pv(i);
-                }
-                if (!ok) {  // the products issued end before TMEM is given back
-                    tc_commit(drain);
-                    wait(drain, 0);
-                }
+                __syncwarp();
             }
-            __syncwarp();
+            if (!ok) {  // the products issued end before TMEM is given back
+                if (elect_one()) tc_commit(&drain[0]);
+                __syncwarp();
+                warp_wait(&drain[0], 0);
+            }
+        } else if (warp == 11) {
+            // ---- O += P . V, from a warp of its own: one warp's waits and issue for both took longer than the products
+            const uint64_t dv = umma_desc(smem_u32(sV), kBox);
+            bool ok = true;
+            for (int i = 0; i < steps && ok; i++) {
+                const int h = i & 1, t = tile_of(i), st = t & 1, buf = i >> 1 & 1;
+                if (i == 0 || tile_of(i - 1) != t) ok = warp_wait(&v_full[st], (uint32_t)(t >> 1)) && warp_wait(&v_clear[st], (uint32_t)(t >> 1));
+                if (ok) ok = warp_wait(&p_full[2 * h + buf], (uint32_t)(i >> 2));
+                if (!ok) break;
+                tc_fence_after();
+                const uint64_t v = dv + (st * kTile16 + half_of(i) * kHalf16);
+                const bool last = i + 1 == steps || tile_of(i + 1) != t;
+                if (elect_one()) {
+#pragma unroll
+                    for (int kk = 0; kk < kHalf / 16; kk++)
+                        mma_ts(tmem + 256 + h * D, tmem + 128 + (2 * h + buf) * 32 + kk * 8, v + ((kk * 16 * 128) >> 4), idesc(D, true),
+                               i > 1 || kk > 0);
+                    tc_commit(&pv_done[2 * h + buf]);
+                    if (last) tc_commit(&v_free[st]);
+                }
+                __syncwarp();
+            }
+            if (!ok) {
+                if (elect_one()) tc_commit(&drain[1]);
+                __syncwarp();
+                warp_wait(&drain[1], 0);
+            }
         } else if (warp == 10) {
             // ---- V rows that no row of the item sees.  Every tile passes here, so that this warp and the MMAs
             // stay within one phase of each other.
             for (int t = 0; t < nt; t++) {
                 const int st = t & 1, k0 = tiles.at(first + t) * kKeys;
-                if (__any_sync(0xffffffffu, !wait(&v_full[st], (uint32_t)(t >> 1)))) break;
+                if (!warp_wait(&v_full[st], (uint32_t)(t >> 1))) break;
                 const uint32_t seen = present[t & (kSeen - 1)];
                 if (loose(k0) || seen != 0xffu) {
                     for (int r = 0; r < kKeys; r++) {
@@ -363,7 +393,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     }
                     fence_proxy_async_smem();
                 }
-                mbar_arrive(&v_clear[st]);
+                warp_arrive(&v_clear[st]);
             }
         }
     } else {
@@ -372,30 +402,37 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         // over the same tokens.
         const int h = warp >> 2, r = 32 * (warp & 3) + lane;
         // ---- queries, BF16, into the swizzled layout: a warp per 32 rows, D / 8 lanes a row
-        if (!ta.tall || h == 0) {
-            constexpr int kLanes = D / 8, kAtOnce = 32 / kLanes;
+        // (rows that are not there repeat the last token's: nobody takes their results).  All of a warp's loads are in
+        // flight at once.
+        if (ntok > 0 && (!ta.tall || h == 0)) {
+            constexpr int kLanes = D / 8, kAtOnce = 32 / kLanes, kLoads = 32 / kAtOnce;
             unsigned char* tile = sQ + h * S::kTile;
-#pragma unroll 8
-            for (int i = 0; i < 32; i += kAtOnce) {
-                const int row = 32 * (warp & 3) + i + lane / kLanes, c = lane % kLanes * 8;
-                const int flat = ta.tall ? row : 2 * row + h;
-                const int tk = flat / a.group, hh = flat - tk * a.group;
-                float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                uint4 packed = make_uint4(0, 0, 0, 0);
-                if (tk < ntok) {
-                    const size_t off = (size_t)(tok0 + tk) * a.q_stride + (size_t)(kvh * a.group + hh) * D + c;
-                    if (a.io_bf16) {
-                        packed = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) + off);
-                    } else {
-                        load8(static_cast<const float*>(a.q) + off, x);
-                        packed = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
-                    }
-                }
-                *reinterpret_cast<uint4*>(tile + sw128_offset(row, c)) = packed;
+            const int c = lane % kLanes * 8;
+            size_t off[kLoads];
+#pragma unroll
+            for (int i = 0; i < kLoads; i++) {
+                const int row = 32 * (warp & 3) + i * kAtOnce + lane / kLanes, flat = ta.tall ? row : 2 * row + h;
+                const int tk = min(flat / a.group, ntok - 1), hh = flat % a.group;
+                off[i] = (size_t)(tok0 + tk) * a.q_stride + (size_t)(kvh * a.group + hh) * D + c;
             }
+            uint4 x[kLoads];
+            if (a.io_bf16) {
+#pragma unroll
+                for (int i = 0; i < kLoads; i++) x[i] = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) + off[i]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < kLoads; i++) {
+                    float f[8];
+                    load8(static_cast<const float*>(a.q) + off[i], f);
+                    x[i] = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kLoads; i++)
+                *reinterpret_cast<uint4*>(tile + sw128_offset(32 * (warp & 3) + i * kAtOnce + lane / kLanes, c)) = x[i];
         }
         fence_proxy_async_smem();
-        mbar_arrive(q_full);
+        warp_arrive(q_full);
 
         // ---- softmax: a row per thread
         const int flat = ta.tall ? r : 2 * r + h;
@@ -404,45 +441,46 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const int pos = ta.shared_pass ? pos0 : pos0 + min(tk, ntok - 1);
         const int lo = windowed ? max(0, pos - a.window + 1) : 0;
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-        const uint32_t s_addr = tmem + lanes, p_addr = tmem + lanes + 128 + h * 64, o_addr = tmem + lanes + 256 + h * D;
-        const int mine = ta.tall ? (nt + 1 - h) >> 1 : nt;  // steps of this stream
+        const uint32_t s_addr = tmem + lanes + h * kHalf, p_addr = tmem + lanes + 128 + h * 64, o_addr = tmem + lanes + 256 + h * D;
+        const int mine = steps >> 1;  // steps of this stream
         float m_run = -INFINITY, l_run = 0.f;
         bool ok = true;
-        auto warp_wait = [&](uint64_t* bar, uint32_t parity) { return !__any_sync(0xffffffffu, !wait(bar, parity)); };
+        auto pv_wait = [&](int j) { return warp_wait(&pv_done[2 * h + (j & 1)], (uint32_t)(j >> 1)); };
         for (int j = 0; j < mine; j++) {
-            const int t = ta.tall ? 2 * j + h : j;
+            const int i = 2 * j + h, t = tile_of(i);
             if (!warp_wait(&s_full[h], (uint32_t)j)) {
                 ok = false;
                 break;
             }
             tc_fence_after();
-            float sv[kKeys];
-            tmem_ld128(s_addr, sv);
+            float sv[kHalf];
+            tmem_ld64(s_addr, sv);
             tc_fence_before();
-            const uint32_t seen = present[t & (kSeen - 1)];
-            mbar_arrive(&s_free[h]);
-            if (j > 0) {  // P is the previous P.V's operand until that is done
-                if (!warp_wait(&pv_done[h], (uint32_t)(j - 1))) {
-                    ok = false;
-                    break;
-                }
-                tc_fence_after();
-            }
-            const int k0 = tiles.at(first + t) * kKeys;
-            const bool masked = edge(k0) || seen != 0xffu;
+            const uint32_t seen = present[t & (kSeen - 1)] >> (half_of(i) * 4) & 0xfu;
+            warp_arrive(&s_free[h]);
+            const int k0 = tiles.at(first + t) * kKeys + half_of(i) * kHalf;
+            const bool masked = edge(k0) || seen != 0xfu;
             Mask mk;
             if (masked) {
 #pragma unroll
-                for (int q = 0; q < 4; q++) {
+                for (int q = 0; q < kHalf / 32; q++) {
                     const int c0 = k0 + 32 * q;
                     const uint32_t pages = (seen >> (2 * q) & 1u ? 0xffffu : 0u) | (seen >> (2 * q) & 2u ? 0xffff0000u : 0u);
                     mk.w[q] = below(pos + 1 - c0) & (~below(lo - c0) | below(sinks - c0)) & pages;
                 }
             }
-            // The running maximum moves only when a tile's exceeds it by more than 2^8 (P stays within BF16's
+            if (j > 1) {  // the P buffer is the operand of P.V two steps back until that is done
+                if (!pv_wait(j - 2)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+            }
+            const uint32_t p = p_addr + (j & 1) * 32;
+            // The running maximum moves only when a step's exceeds it by more than 2^8 (P stays within BF16's
             // range and the FP32 sums do not mind), which spares most rescalings of O: exponentials against the
             // running maximum, tracking the largest exponent, and again if some row's passed 8.  Rows that have
-            // seen nothing yet take their tile's maximum first.
+            // seen nothing yet take their step's maximum first.
             float rowsum, alpha = 1.f;
             if (__any_sync(0xffffffffu, m_run == -INFINITY)) {
                 float m_new = m_run;
@@ -452,12 +490,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 alpha = m_run == -INFINITY ? 1.f : pt_exp2(m_run - m_new);  // nothing gathered: nothing to scale
                 m_run = m_new;
                 const float neg = m_run == -INFINITY ? 0.f : -m_run;
-                rowsum = masked ? row_exp<true, false>(sv, mk, a.scale_log2, neg, p_addr, nullptr)
-                                : row_exp<false, false>(sv, mk, a.scale_log2, neg, p_addr, nullptr);
+                rowsum = masked ? row_exp<true, false>(sv, mk, a.scale_log2, neg, p, nullptr)
+                                : row_exp<false, false>(sv, mk, a.scale_log2, neg, p, nullptr);
             } else {
                 float top;
-                rowsum = masked ? row_exp<true, true>(sv, mk, a.scale_log2, -m_run, p_addr, &top)
-                                : row_exp<false, true>(sv, mk, a.scale_log2, -m_run, p_addr, &top);
+                rowsum = masked ? row_exp<true, true>(sv, mk, a.scale_log2, -m_run, p, &top)
+                                : row_exp<false, true>(sv, mk, a.scale_log2, -m_run, p, &top);
                 const bool move = top > 8.f;
                 if (__any_sync(0xffffffffu, move)) {
                     float m_new = m_run;
@@ -466,11 +504,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         alpha = pt_exp2(m_run - m_new);
                     }
                     m_run = m_new;
-                    rowsum = masked ? row_exp<true, false>(sv, mk, a.scale_log2, -m_run, p_addr, nullptr)
-                                    : row_exp<false, false>(sv, mk, a.scale_log2, -m_run, p_addr, nullptr);
+                    rowsum = masked ? row_exp<true, false>(sv, mk, a.scale_log2, -m_run, p, nullptr)
+                                    : row_exp<false, false>(sv, mk, a.scale_log2, -m_run, p, nullptr);
                 }
             }
             if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+                if (!pv_wait(j - 1)) {  // O is at rest
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
 #pragma unroll
                 for (int q = 0; q < D / 32; q++) {
                     float ov[32];
@@ -483,13 +526,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
             l_run = l_run * alpha + rowsum;
             tc_fence_before();
-            mbar_arrive(&p_full[h]);
+            warp_arrive(&p_full[2 * h + (j & 1)]);
         }
         // ---- the row's output, or its record
         const int slot = a.slot0 + (ta.tall ? 2 * split + h : split);
         const size_t R = (size_t)(tok0 + tk) * a.q_heads + kvh * a.group + hh;
         const bool direct = a.rec.slots == 1;
-        if (ok && mine > 0) ok = warp_wait(&pv_done[h], (uint32_t)(mine - 1));
+        if (ok && mine > 0) ok = pv_wait(mine - 1);
         if (ok) {
             tc_fence_after();
             const float mul = !direct ? 1.f : l_run == 0.f ? 0.f : 1.f / l_run;

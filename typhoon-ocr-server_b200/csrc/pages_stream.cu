@@ -297,8 +297,8 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
         next();
         while (more) {
             if (sent >= (unsigned int)sa.stages) {
-                ok = wait_for(&empty[st], phase ^ 1u, sa.wait_ns, a.st);
-                if (__any_sync(0xffffffffu, !ok)) break;
+                ok = warp_wait_for(&empty[st], phase ^ 1u, sa.wait_ns, a.st);
+                if (!ok) break;
             }
             if (page >= max_page) {
                 raise(a.st, TYB_STATUS_BAD_ARGUMENT);
@@ -332,10 +332,10 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
             more = !tile.end;
             if (more) next();
         }
-        if (__any_sync(0xffffffffu, !ok)) {  // a wait ran out: the copies requested still land in this CTA
+        if (!ok) {  // a wait ran out: the copies requested still land in this CTA
             const unsigned int stages = sa.stages;
             for (unsigned int n = sent > stages ? sent - stages : 0; n < sent; n++)
-                wait_for(&full[n % stages], n / stages & 1u, sa.wait_ns, a.st);
+                warp_wait_for(&full[n % stages], n / stages & 1u, sa.wait_ns, a.st);
         }
         return;
     }
@@ -358,11 +358,10 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
     // wait ran out and left does not leave the others waiting.
     uint32_t meeting = 0;
     auto meet = [&]() {
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&met);
-        const bool ok = wait_for(&met, meeting, sa.wait_ns, a.st);
+        warp_arrive(&met);
+        const bool ok = warp_wait_for(&met, meeting, sa.wait_ns, a.st);
         meeting ^= 1u;
-        return !__any_sync(0xffffffffu, !ok);
+        return ok;
     };
     // A finished row block: the output, or its record for the join kernel.
     auto deliver = [&](size_t R, int c, const Gather& x) {
@@ -385,8 +384,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
         return sum;
     };
     for (bool more = true; more;) {
-        const bool here = wait_for(&full[st], phase, sa.wait_ns, a.st);
-        if (__any_sync(0xffffffffu, !here)) return;
+        if (!warp_wait_for(&full[st], phase, sa.wait_ns, a.st)) return;
         const Tile tile = tiles_of_stage[st];
         const int nrows = tile.ntok * a.group;
         more = !tile.end;
@@ -418,8 +416,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
             }
             w.step(rows_k, rows_v, S::kBox, r0, see, a.scale_log2, split_q, g, t, lane);
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&empty[st]);
+        warp_arrive(&empty[st]);
         turn ^= 1;
         if (++st == sa.stages) {
             st = 0;
