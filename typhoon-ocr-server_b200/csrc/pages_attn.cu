@@ -481,11 +481,11 @@ static Layout layout_of(const tyb_pages_attn* c)
     // Each of the sequences of a call ends in a tile of its own; no list has more tiles than this.
     l.row_tiles = l.tokens ? ceil_div(c->batch, per) : (int)((c->rows + (long long)c->batch * (per - 1)) / per);
     const long long keys = l.tokens ? c->prefix : c->window && c->window < c->max_len ? c->window + c->sinks : c->max_len;
-    const int tiles = ceil_div(keys, l.tc ? 128 : 8);
+    const int tiles = ceil_div(keys, l.tc ? 64 : 8);
     const long long ctas = (long long)l.row_tiles * c->p.kv_heads;
     if (l.tc) {
-        l.splits = (int)(kSms / ctas);  // one CTA fits an SM; a split has at least two tiles
-        if (l.splits > tiles / 2) l.splits = tiles / 2;
+        l.splits = (int)(kSms / ctas);  // one CTA fits an SM; a split has at least four tiles
+        if (l.splits > tiles / 4) l.splits = tiles / 4;
     } else {
         l.splits = ceil_div(3LL * kSms, ctas);
         if (l.splits > ceil_div(tiles, 8)) l.splits = ceil_div(tiles, 8);

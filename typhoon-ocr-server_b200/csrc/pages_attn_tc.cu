@@ -3,11 +3,11 @@
 // decode batch.
 //
 // A CTA has query rows of one KV head (its q_heads / kv_heads query heads folded into the rows, so
-// that one K/V tile feeds them all) and a run of key tiles of 128, taken in halves.  Two streams of 128
-// rows alternate on the tensor core, one's softmax overlapping the other's products:
-//   wide   256 rows, both streams take every half (each K/V tile is loaded once for 256 rows);
-//   tall   at most 128 rows: the streams have the same rows and take a half each, and their results are
-//          joined like those of two splits.  Half the tensor work of a wide item that would be half empty.
+// that one K/V tile feeds them all) and a run of key tiles of 64.  Two streams of 128 rows alternate on
+// the tensor core, one's softmax overlapping the other's products:
+//   wide   256 rows, both streams take every tile (each K/V tile is loaded once for 256 rows);
+//   tall   at most 128 rows: the streams have the same rows and take the tiles in turn, and their results
+//          are joined like those of two splits.  Half the tensor work of a wide item that would be half empty.
 // A tile comes page by page: one TMA tensor copy per page and 64 columns, the 128-byte-swizzled
 // layout building up in shared memory as if it were one copy; the pages of a tile are issued by as
 // many lanes of the producer warp.  Rows of the tile that no row of the item sees (behind the
@@ -16,10 +16,10 @@
 //
 // Roles (12 warps): 0-3 and 4-7 the streams' softmax (one row per thread), 8 issues Q.K^T, 11 P.V, 9 the
 // copies, 10 clears V rows.  TMEM: S0 | S1 (64 columns each) | P of each stream, two buffers (32 each) |
-// O0 | O1.  The halves are what makes room for two P buffers beside an S for each stream: the softmax of a half
-// waits for neither the P.V of the one before nor the other stream, only for its own S, which is computed
-// while it works on the half before.  (One S of 128 columns for both and one P each: 2.6 us a tile of 256
-// rows x 128 keys; MMAs alone about 1.1 us, exponentials alone about as much.)
+// O0 | O1.  Tiles of 64 keys are what makes room for two P buffers beside an S for each stream: the softmax of a
+// tile waits for neither the P.V of the one before nor the other stream, only for its own S, which is computed
+// while it works on the tile before.  (With tiles of 128, one S for both streams and one P each, 256 rows x 128
+// keys took 2.6 us; their products alone take 1.1 us and their exponentials as much.)
 // Every wait is bounded; a CTA whose wait ran out raises the status word, leaves its loops, frees its
 // TMEM and returns.
 #define TYB_WHOLE_PROGRAM
@@ -29,8 +29,7 @@
 namespace tyb {
 
 constexpr int kRows = 128;   // rows of a stream (tensor-core M)
-constexpr int kKeys = 128;   // keys of a tile
-constexpr int kHalf = 64;    // and of a step: N of S, K of P.V
+constexpr int kKeys = 64;    // keys of a tile: N of S, K of P.V
 constexpr int kSoftThreads = 256;
 constexpr int kTcThreads = kSoftThreads + 128;
 // Register split, as in the fused prefill: launched at kLaunchRegs, the issue warpgroup drops to
@@ -38,9 +37,10 @@ constexpr int kTcThreads = kSoftThreads + 128;
 constexpr int kLaunchRegs = 168, kIssueRegs = 112, kSoftRegs = 192;
 static_assert(kSoftThreads * kSoftRegs + 128 * kIssueRegs <= kTcThreads * kLaunchRegs, "register split");
 static_assert(2 * kSoftRegs + kIssueRegs <= 512, "register split of a sub-partition");
-constexpr int kBox = kTcBox;  // 128 rows x 64 columns of BF16
-constexpr int kStages = 2;
-constexpr int kSeen = 8;  // ring of page masks, one per tile: more than the tiles in flight
+constexpr int kBoxQ = kTcBox;        // 128 rows x 64 columns of BF16
+constexpr int kBox = kKeys * 128;    // a tile's rows x 64 columns
+constexpr int kStages = 5;           // of the K and V rings: 32 KB of 128-wide tiles each, all that fits beside Q
+constexpr int kSeen = 16;  // ring of page masks, one per tile: more than the tiles in flight
 
 struct TcArgs {
     AttnArgs a;
@@ -52,8 +52,8 @@ struct TcArgs {
 
 template <int D>
 struct Smem {
-    static constexpr int kTile = (D / 64) * kBox;
-    static constexpr int kQ = 0, kK = 2 * kTile, kV = kK + kStages * kTile, kBars = kV + kStages * kTile;
+    static constexpr int kTileQ = (D / 64) * kBoxQ, kTile = (D / 64) * kBox;
+    static constexpr int kQ = 0, kK = 2 * kTileQ, kV = kK + kStages * kTile, kBars = kV + kStages * kTile;
     static constexpr size_t kBytes = (size_t)kBars + 512 + 1024;  // + barriers + alignment slack
 };
 
@@ -95,17 +95,17 @@ __device__ __forceinline__ float max3(float a, float b, float c)
 // Columns [0, n) of 32, n clamped.
 __device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
 
-// Which of a step's columns a row sees, 32 per word.
+// Which of a tile's columns a row sees, 32 per word.
 struct Mask {
-    uint32_t w[kHalf / 32];
+    uint32_t w[kKeys / 32];
 };
 
 template <bool kMask>
-__device__ __forceinline__ float row_max(const float (&s)[kHalf], const Mask& mk)
+__device__ __forceinline__ float row_max(const float (&s)[kKeys], const Mask& mk)
 {
     float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-    for (int c = 0; c < kHalf; c += 2) {
+    for (int c = 0; c < kKeys; c += 2) {
         const float a = (!kMask || (mk.w[c >> 5] >> (c & 31) & 1u)) ? s[c] : -INFINITY;
         const float b = (!kMask || (mk.w[c >> 5] >> ((c + 1) & 31) & 1u)) ? s[c + 1] : -INFINITY;
         m[(c >> 1) & 3] = max3(m[(c >> 1) & 3], a, b);
@@ -116,13 +116,13 @@ __device__ __forceinline__ float row_max(const float (&s)[kHalf], const Mask& mk
 // p = exp2(s * scale + neg) on the visible columns (0 on the others) as BF16 pairs into the row's TMEM
 // columns at p_addr; returns the FP32 sum.  kTrack: *top receives the largest exponent.
 template <bool kMask, bool kTrack>
-__device__ __forceinline__ float row_exp(const float (&s)[kHalf], const Mask& mk, float scale, float neg, uint32_t p_addr, float* top)
+__device__ __forceinline__ float row_exp(const float (&s)[kKeys], const Mask& mk, float scale, float neg, uint32_t p_addr, float* top)
 {
     const float2 sc = make_float2(scale, scale), nm = make_float2(neg, neg);
     float2 acc0 = make_float2(0.f, 0.f), acc1 = make_float2(0.f, 0.f);
     float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
-    for (int q = 0; q < kHalf / 32; q++) {
+    for (int q = 0; q < kKeys / 32; q++) {
         uint32_t pk[16];
 #pragma unroll
         for (int c = 0; c < 32; c += 4) {
@@ -162,13 +162,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     unsigned char *sQ = smem + S::kQ, *sK = smem + S::kK, *sV = smem + S::kV;
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBars);
-    uint64_t *k_full = bars, *k_free = bars + 2, *v_full = bars + 4, *v_free = bars + 6, *v_clear = bars + 8;  // [stage]
-    uint64_t *s_full = bars + 10, *s_free = bars + 12;    // [stream]
-    uint64_t *p_full = bars + 14, *pv_done = bars + 18;   // [stream][buffer]
-    uint64_t *q_full = bars + 22, *drain = bars + 23;  // drain: [2]
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 25);
-    int* found = reinterpret_cast<int*>(bars + 26);                      // [4]
-    volatile uint32_t* present = reinterpret_cast<uint32_t*>(bars + 28);  // [kSeen] a bit per 16 rows of the tile
+    uint64_t *k_full = bars, *k_free = k_full + kStages, *v_full = k_free + kStages, *v_free = v_full + kStages,
+             *v_clear = v_free + kStages;                         // [stage]
+    uint64_t *s_full = v_clear + kStages, *s_free = s_full + 2;   // [stream]
+    uint64_t *p_full = s_free + 2, *pv_done = p_full + 4;         // [stream][buffer]
+    uint64_t *q_full = pv_done + 4, *drain = q_full + 1;          // drain: [2]
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
+    int* found = reinterpret_cast<int*>(drain + 3);                       // [4]
+    volatile uint32_t* present = reinterpret_cast<uint32_t*>(drain + 5);  // [kSeen] a bit per 16 rows of the tile
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int kvh = blockIdx.y, split = blockIdx.z;
@@ -177,12 +178,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 
     if (warp == 8) {
         if (lane == 0) {
-            for (int i = 0; i < 2; i++) {
+            for (int i = 0; i < kStages; i++) {
                 mbar_init(&k_full[i], 1);
                 mbar_init(&k_free[i], 1);
                 mbar_init(&v_full[i], 1);
                 mbar_init(&v_free[i], 1);
                 mbar_init(&v_clear[i], 1);
+            }
+            for (int i = 0; i < 2; i++) {
                 mbar_init(&s_full[i], 1);
                 mbar_init(&s_free[i], kRows / 32);
             }
@@ -256,14 +259,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const Tiles tiles = tiles_of(ntok > 0 ? pos_max : -1, lo_min, sinks, kKeys);
     const int all = tiles.count();
     const int first = (int)((long long)all * split / a.splits), nt = (int)((long long)all * (split + 1) / a.splits) - first;
-    constexpr uint32_t kTile16 = S::kTile >> 4, kHalf16 = (kHalf * 128) >> 4;  // in units of the operand descriptors
-    // Step i of both streams is stream i & 1's; its tile and half:
-    const int steps = ta.tall ? 2 * nt : 4 * nt;
-    auto tile_of = [&](int i) { return ta.tall ? i >> 1 : i >> 2; };
-    auto half_of = [&](int i) { return ta.tall ? i & 1 : i >> 1 & 1; };
-    // Whether some row of the item does not see the whole half (its pages aside), and whether the tile
+    constexpr uint32_t kTile16 = S::kTile >> 4, kTileQ16 = S::kTileQ >> 4;  // in units of the operand descriptors
+    // Step i of both streams is stream i & 1's; its tile:
+    const int steps = ta.tall ? nt : 2 * nt;
+    auto tile_of = [&](int i) { return ta.tall ? i : i >> 1; };
+    // Whether some row of the item does not see the whole tile (its pages aside), and whether the tile
     // has rows that none sees.
-    auto edge = [&](int k0) { return k0 + kHalf - 1 > pos0 || (k0 < lo_max && k0 + kHalf > sinks); };
+    auto edge = [&](int k0) { return k0 + kKeys - 1 > pos0 || (k0 < lo_max && k0 + kKeys > sinks); };
     auto loose = [&](int k0) { return k0 + kKeys - 1 > pos_max || (k0 < lo_min && k0 + kKeys > sinks); };
     auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_for(bar, parity & 1u, ta.wait_ns, a.st); };
     auto warp_wait = [&](uint64_t* bar, uint32_t parity) { return warp_wait_for(bar, parity & 1u, ta.wait_ns, a.st); };
@@ -271,15 +273,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
         if (warp == 9) {
-            // ---- copies: lane l < parts of a tile has the page, or the half page, at its rows l * part
+            // ---- copies: lane l < parts of a tile has the page (or its part) at rows l * part
             const int part = box_rows(a.p), shift = page_shift(a.p.page_size), per_tile = kKeys / part;
             const int* table = a.p.table + (size_t)max(0, min(seq, a.p.max_seqs - 1)) * a.p.max_pages;
             const uint32_t part_bits = (1u << (part / 16)) - 1u;
             const int part_bytes = part * 128;  // of a 64-column box
             bool ok = true;
             int k_sent = 0, v_sent = 0;  // tiles requested
+            int st = 0;
+            uint32_t phase = 1;  // of the last use of the stage
             for (int t = 0; t < nt && ok; t++) {
-                const int st = t & 1, key = tiles.at(first + t) * kKeys + lane * part;
+                const int key = tiles.at(first + t) * kKeys + lane * part;
                 int page = -1;
                 if (lane < per_tile && key <= pos_max) {
                     page = table[key >> shift];
@@ -292,7 +296,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 const int row = page < 0 ? 0
                                          : ((ta.layer * a.p.num_pages + page) * a.p.kv_heads + kvh) * a.p.page_size + (key & (a.p.page_size - 1));
                 const uint32_t bytes = (uint32_t)__popc(have) * (uint32_t)(part_bytes * (D / 64));
-                if (t >= kStages) ok = warp_wait(&k_free[st], (uint32_t)((t - kStages) >> 1));
+                if (t >= kStages) ok = warp_wait(&k_free[st], phase);
                 if (!ok) break;
                 if (lane == 0) {
                     uint32_t seen = 0;
@@ -307,7 +311,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     for (int c = 0; c < D / 64; c++)
                         tma_load_2d(sK + st * S::kTile + c * kBox + lane * part_bytes, &map_k, 64 * c, row, &k_full[st]);
                 k_sent = t + 1;
-                if (t >= kStages) ok = warp_wait(&v_free[st], (uint32_t)((t - kStages) >> 1));
+                if (t >= kStages) ok = warp_wait(&v_free[st], phase);
                 if (!ok) break;
                 if (lane == 0) mbar_arrive_expect_tx(&v_full[st], bytes);
                 __syncwarp();
@@ -316,33 +320,42 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     for (int c = 0; c < D / 64; c++)
                         tma_load_2d(sV + st * S::kTile + c * kBox + lane * part_bytes, &map_v, 64 * c, row, &v_full[st]);
                 v_sent = t + 1;
+                if (++st == kStages) {
+                    st = 0;
+                    phase ^= 1u;
+                }
             }
             if (!ok) {  // a wait ran out: the copies requested still land in this CTA
-                for (int t = max(0, k_sent - kStages); t < k_sent; t++) warp_wait(&k_full[t & 1], (uint32_t)(t >> 1));
-                for (int t = max(0, v_sent - kStages); t < v_sent; t++) warp_wait(&v_full[t & 1], (uint32_t)(t >> 1));
+                for (int t = max(0, k_sent - kStages); t < k_sent; t++) warp_wait(&k_full[t % kStages], (uint32_t)(t / kStages));
+                for (int t = max(0, v_sent - kStages); t < v_sent; t++) warp_wait(&v_full[t % kStages], (uint32_t)(t / kStages));
             }
         } else if (warp == 8) {
             // ---- S = Q . K^T: a stream's next one goes out as soon as its S has been read
             const uint64_t dq = umma_desc(smem_u32(sQ), 16), dk = umma_desc(smem_u32(sK), 16);
             bool ok = steps == 0 || warp_wait(q_full, 0);
+            int st = 0;
+            uint32_t phase = 0;
             for (int i = 0; i < steps && ok; i++) {
-                const int h = i & 1, t = tile_of(i), st = t & 1;
+                const int h = i & 1;
                 if (i >= 2) ok = warp_wait(&s_free[h], (uint32_t)(i >> 1) - 1u);
-                if (ok && (i == 0 || tile_of(i - 1) != t)) ok = warp_wait(&k_full[st], (uint32_t)(t >> 1));
+                if (ok && (ta.tall || h == 0)) ok = warp_wait(&k_full[st], phase);
                 if (!ok) break;
                 tc_fence_after();
-                const uint64_t q = dq + (ta.tall ? 0u : h * kTile16), k = dk + (st * kTile16 + half_of(i) * kHalf16);
-                const bool last = i + 1 == steps || tile_of(i + 1) != t;
+                const uint64_t q = dq + (ta.tall ? 0u : h * kTileQ16), k = dk + st * kTile16;
+                const bool last = ta.tall || h == 1;  // use of the tile
                 if (elect_one()) {
 #pragma unroll
-                    for (int kk = 0; kk < D / 16; kk++) {
-                        const uint32_t off = ((kk >> 2) * kBox + (kk & 3) * 32) >> 4;
-                        mma_ss(tmem + h * kHalf, q + off, k + off, idesc(kHalf, false), kk > 0);
-                    }
+                    for (int kk = 0; kk < D / 16; kk++)
+                        mma_ss(tmem + h * kKeys, q + (((kk >> 2) * kBoxQ + (kk & 3) * 32) >> 4), k + (((kk >> 2) * kBox + (kk & 3) * 32) >> 4),
+                               idesc(kKeys, false), kk > 0);
                     tc_commit(&s_full[h]);
                     if (last) tc_commit(&k_free[st]);
                 }
                 __syncwarp();
+                if (last && ++st == kStages) {
+                    st = 0;
+                    phase ^= 1u;
+                }
             }
             if (!ok) {  // the products issued end before TMEM is given back
                 if (elect_one()) tc_commit(&drain[0]);
@@ -353,23 +366,29 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             // ---- O += P . V, from a warp of its own: one warp's waits and issue for both took longer than the products
             const uint64_t dv = umma_desc(smem_u32(sV), kBox);
             bool ok = true;
+            int st = 0;
+            uint32_t phase = 0;
             for (int i = 0; i < steps && ok; i++) {
-                const int h = i & 1, t = tile_of(i), st = t & 1, buf = i >> 1 & 1;
-                if (i == 0 || tile_of(i - 1) != t) ok = warp_wait(&v_full[st], (uint32_t)(t >> 1)) && warp_wait(&v_clear[st], (uint32_t)(t >> 1));
+                const int h = i & 1, buf = i >> 1 & 1;
+                if (ta.tall || h == 0) ok = warp_wait(&v_full[st], phase) && warp_wait(&v_clear[st], phase);
                 if (ok) ok = warp_wait(&p_full[2 * h + buf], (uint32_t)(i >> 2));
                 if (!ok) break;
                 tc_fence_after();
-                const uint64_t v = dv + (st * kTile16 + half_of(i) * kHalf16);
-                const bool last = i + 1 == steps || tile_of(i + 1) != t;
+                const uint64_t v = dv + st * kTile16;
+                const bool last = ta.tall || h == 1;  // use of the tile
                 if (elect_one()) {
 #pragma unroll
-                    for (int kk = 0; kk < kHalf / 16; kk++)
+                    for (int kk = 0; kk < kKeys / 16; kk++)
                         mma_ts(tmem + 256 + h * D, tmem + 128 + (2 * h + buf) * 32 + kk * 8, v + ((kk * 16 * 128) >> 4), idesc(D, true),
                                i > 1 || kk > 0);
                     tc_commit(&pv_done[2 * h + buf]);
                     if (last) tc_commit(&v_free[st]);
                 }
                 __syncwarp();
+                if (last && ++st == kStages) {
+                    st = 0;
+                    phase ^= 1u;
+                }
             }
             if (!ok) {
                 if (elect_one()) tc_commit(&drain[1]);
@@ -379,21 +398,26 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         } else if (warp == 10) {
             // ---- V rows that no row of the item sees.  Every tile passes here, so that this warp and the MMAs
             // stay within one phase of each other.
+            int st = 0;
+            uint32_t phase = 0;
             for (int t = 0; t < nt; t++) {
-                const int st = t & 1, k0 = tiles.at(first + t) * kKeys;
-                if (!warp_wait(&v_full[st], (uint32_t)(t >> 1))) break;
+                const int k0 = tiles.at(first + t) * kKeys;
+                if (!warp_wait(&v_full[st], phase)) break;
                 const uint32_t seen = present[t & (kSeen - 1)];
-                if (loose(k0) || seen != 0xffu) {
-                    for (int r = 0; r < kKeys; r++) {
-                        const int j = k0 + r;
-                        if ((seen >> (r >> 4) & 1u) && j <= pos_max && (j >= lo_min || j < sinks)) continue;
-                        if (lane < 8 * (D / 64))
-                            *reinterpret_cast<uint4*>(sV + st * S::kTile + (lane >> 3) * kBox + r * 128 + (lane & 7) * 16) =
-                                make_uint4(0, 0, 0, 0);
+                if (loose(k0) || seen != 0xfu) {
+#pragma unroll 4
+                    for (int i = lane; i < kKeys * (D / 8); i += 32) {
+                        const int r = i / (D / 8), c = i % (D / 8), j = k0 + r;
+                        if (!((seen >> (r >> 4) & 1u) && j <= pos_max && (j >= lo_min || j < sinks)))
+                            *reinterpret_cast<uint4*>(sV + st * S::kTile + (c >> 3) * kBox + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
                     }
                     fence_proxy_async_smem();
                 }
                 warp_arrive(&v_clear[st]);
+                if (++st == kStages) {
+                    st = 0;
+                    phase ^= 1u;
+                }
             }
         }
     } else {
@@ -406,7 +430,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         // flight at once.
         if (ntok > 0 && (!ta.tall || h == 0)) {
             constexpr int kLanes = D / 8, kAtOnce = 32 / kLanes, kLoads = 32 / kAtOnce;
-            unsigned char* tile = sQ + h * S::kTile;
+            unsigned char* tile = sQ + h * S::kTileQ;
             const int c = lane % kLanes * 8;
             size_t off[kLoads];
 #pragma unroll
@@ -441,8 +465,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const int pos = ta.shared_pass ? pos0 : pos0 + min(tk, ntok - 1);
         const int lo = windowed ? max(0, pos - a.window + 1) : 0;
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-        const uint32_t s_addr = tmem + lanes + h * kHalf, p_addr = tmem + lanes + 128 + h * 64, o_addr = tmem + lanes + 256 + h * D;
-        const int mine = steps >> 1;  // steps of this stream
+        const uint32_t s_addr = tmem + lanes + h * kKeys, p_addr = tmem + lanes + 128 + h * 64, o_addr = tmem + lanes + 256 + h * D;
+        const int mine = (steps + 1 - h) >> 1;  // steps of this stream
         float m_run = -INFINITY, l_run = 0.f;
         bool ok = true;
         auto pv_wait = [&](int j) { return warp_wait(&pv_done[2 * h + (j & 1)], (uint32_t)(j >> 1)); };
@@ -453,17 +477,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 break;
             }
             tc_fence_after();
-            float sv[kHalf];
+            float sv[kKeys];
             tmem_ld64(s_addr, sv);
             tc_fence_before();
-            const uint32_t seen = present[t & (kSeen - 1)] >> (half_of(i) * 4) & 0xfu;
+            const uint32_t seen = present[t & (kSeen - 1)];
             warp_arrive(&s_free[h]);
-            const int k0 = tiles.at(first + t) * kKeys + half_of(i) * kHalf;
+            const int k0 = tiles.at(first + t) * kKeys;
             const bool masked = edge(k0) || seen != 0xfu;
             Mask mk;
             if (masked) {
 #pragma unroll
-                for (int q = 0; q < kHalf / 32; q++) {
+                for (int q = 0; q < kKeys / 32; q++) {
                     const int c0 = k0 + 32 * q;
                     const uint32_t pages = (seen >> (2 * q) & 1u ? 0xffffu : 0u) | (seen >> (2 * q) & 2u ? 0xffff0000u : 0u);
                     mk.w[q] = below(pos + 1 - c0) & (~below(lo - c0) | below(sinks - c0)) & pages;
