@@ -433,11 +433,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             unsigned char* tile = sQ + h * S::kTileQ;
             const int c = lane % kLanes * 8;
             size_t off[kLoads];
+            // row 32 (warp & 3) + lane / kLanes, then kAtOnce further each time; in flat rows twice that when wide
+            const int row0 = 32 * (warp & 3) + lane / kLanes, flat0 = ta.tall ? row0 : 2 * row0 + h, ahead = ta.tall ? kAtOnce : 2 * kAtOnce;
+            int tk = flat0 / a.group, hh = flat0 - tk * a.group;
+            const int tk_ahead = ahead / a.group, hh_ahead = ahead - tk_ahead * a.group;
 #pragma unroll
             for (int i = 0; i < kLoads; i++) {
-                const int row = 32 * (warp & 3) + i * kAtOnce + lane / kLanes, flat = ta.tall ? row : 2 * row + h;
-                const int tk = min(flat / a.group, ntok - 1), hh = flat % a.group;
-                off[i] = (size_t)(tok0 + tk) * a.q_stride + (size_t)(kvh * a.group + hh) * D + c;
+                off[i] = (size_t)(tok0 + min(tk, ntok - 1)) * a.q_stride + (size_t)(kvh * a.group + hh) * D + c;
+                tk += tk_ahead;
+                hh += hh_ahead;
+                if (hh >= a.group) {
+                    hh -= a.group;
+                    tk++;
+                }
             }
             uint4 x[kLoads];
             if (a.io_bf16) {
@@ -453,7 +461,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
 #pragma unroll
             for (int i = 0; i < kLoads; i++)
-                *reinterpret_cast<uint4*>(tile + sw128_offset(32 * (warp & 3) + i * kAtOnce + lane / kLanes, c)) = x[i];
+                *reinterpret_cast<uint4*>(tile + sw128_offset(row0 + i * kAtOnce, c)) = x[i];
         }
         fence_proxy_async_smem();
         warp_arrive(q_full);
@@ -552,39 +560,63 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             tc_fence_before();
             warp_arrive(&p_full[2 * h + (j & 1)]);
         }
-        // ---- the row's output, or its record
+        // ---- the rows' outputs, or their records: 64 columns at a time through shared memory (the stream's query
+        // tile, no longer needed), so that they leave in whole lines instead of 16 bytes of 32 rows at a time
         const int slot = a.slot0 + (ta.tall ? 2 * split + h : split);
-        const size_t R = (size_t)(tok0 + tk) * a.q_heads + kvh * a.group + hh;
         const bool direct = a.rec.slots == 1;
         if (ok && mine > 0) ok = pv_wait(mine - 1);
-        if (ok) {
-            tc_fence_after();
-            const float mul = !direct ? 1.f : l_run == 0.f ? 0.f : 1.f / l_run;
+        if (ta.tall) asm volatile("bar.sync 1, %0;" ::"n"(kSoftThreads) : "memory");  // the other stream is done with the queries too
+        const size_t R = (size_t)(tok0 + tk) * a.q_heads + kvh * a.group + hh;
+        const float mul = !direct ? 1.f : l_run == 0.f ? 0.f : 1.f / l_run;
+        if (!direct && here && ok) a.rec.ml[(size_t)slot * a.rec.rows + R] = make_float2(m_run, l_run);
+        tc_fence_after();
+        unsigned char* stage = sQ + h * S::kTileQ + (warp & 3) * (S::kTileQ / 4);  // 32 rows of 256 (FP32) or 128 bytes
+        const bool half = direct && a.io_bf16;
+        static_assert(S::kTileQ / 4 >= 32 * 128, "room for 32 rows");
+        constexpr int kCols = S::kTileQ / 4 >= 32 * 256 ? 64 : 32;  // columns that fit as FP32
+#pragma unroll 1
+        for (int c0 = 0; c0 < D; c0 += kCols) {
+            if (ok) {
 #pragma unroll
-            for (int c = 0; c < D / 32; c++) {
-                float v[32];
-                if (mine > 0) {
-                    tmem_ld32(o_addr + c * 32, v);
-                } else {
+                for (int c = 0; c < kCols; c += 32) {
+                    float v[32];
+                    if (mine > 0) {
+                        tmem_ld32(o_addr + c0 + c, v);
+                    } else {
 #pragma unroll
-                    for (int i = 0; i < 32; i++) v[i] = 0.f;
-                }
-                if (!here) continue;
+                        for (int i = 0; i < 32; i++) v[i] = 0.f;
+                    }
 #pragma unroll
-                for (int i = 0; i < 32; i++) v[i] = mul == 0.f ? 0.f : v[i] * mul;
-                if (direct && a.io_bf16) {
-                    __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.out) + R * D + c * 32;
+                    for (int i = 0; i < 32; i++) v[i] = mul == 0.f ? 0.f : v[i] * mul;
+                    // piece p of a row lies at p ^ (row % 8): no two rows' pieces of a phase in the same banks
+                    if (half) {
 #pragma unroll
-                    for (int i = 0; i < 32; i += 8)
-                        *reinterpret_cast<uint4*>(dst + i) = make_uint4(pack_bf16x2(v[i], v[i + 1]), pack_bf16x2(v[i + 2], v[i + 3]),
-                                                                       pack_bf16x2(v[i + 4], v[i + 5]), pack_bf16x2(v[i + 6], v[i + 7]));
-                } else {
-                    float* dst = direct ? static_cast<float*>(a.out) + R * D + c * 32 : a.rec.o + ((size_t)slot * a.rec.rows + R) * D + c * 32;
+                        for (int i = 0; i < 32; i += 8)
+                            *reinterpret_cast<uint4*>(stage + lane * (kCols * 2) + ((((c + i) >> 3) ^ (lane & (kCols / 8 - 1))) << 4)) =
+                                make_uint4(pack_bf16x2(v[i], v[i + 1]), pack_bf16x2(v[i + 2], v[i + 3]), pack_bf16x2(v[i + 4], v[i + 5]),
+                                           pack_bf16x2(v[i + 6], v[i + 7]));
+                    } else {
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(dst + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                        for (int i = 0; i < 32; i += 4)
+                            *reinterpret_cast<float4*>(stage + lane * (kCols * 4) + ((((c + i) >> 2) ^ (lane & 7)) << 4)) =
+                                make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                    }
                 }
             }
-            if (!direct && here) a.rec.ml[(size_t)slot * a.rec.rows + R] = make_float2(m_run, l_run);
+            __syncwarp();
+            // a row's pieces by neighbouring lanes; the row's address from the lane that has the row
+            const int per_row = half ? kCols / 8 : kCols / 4, rows_at_once = 32 / per_row;
+            for (int r0 = 0; r0 < 32; r0 += rows_at_once) {
+                const int row = r0 + lane / per_row, piece = lane % per_row;
+                const long long to = __shfl_sync(0xffffffffu, here && ok ? (long long)R : -1ll, row);
+                const uint4 x = *reinterpret_cast<const uint4*>(stage + row * (kCols * (half ? 2 : 4)) +
+                                                                ((piece ^ (row & (half ? kCols / 8 - 1 : 7))) << 4));
+                if (to < 0) continue;
+                if (half) *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) + to * D + c0 + piece * 8) = x;
+                else if (direct) *reinterpret_cast<uint4*>(static_cast<float*>(a.out) + to * D + c0 + piece * 4) = x;
+                else *reinterpret_cast<uint4*>(a.rec.o + ((size_t)slot * a.rec.rows + to) * D + c0 + piece * 4) = x;
+            }
+            __syncwarp();
         }
         tc_fence_before();
     }
@@ -654,10 +686,12 @@ extern "C" int tyb_pages_maps(const KVPages* p, void* maps)
     const cuuint64_t strides[1] = {(cuuint64_t)p->head_dim * (bf16 ? 2 : 4)};
     const cuuint32_t box[2] = {bf16 ? 64u : 32u, (cuuint32_t)box_rows(*p)};
     const cuuint32_t estr[2] = {1, 1};
-    for (int i = 0; i < 2; i++)
-        if (fn(static_cast<CUtensorMap*>(maps) + i, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, i ? p->v : p->k, dims, strides, box, estr,
-               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    for (int i = 0; i < 4; i++) {  // K, V; then in boxes of 16 rows
+        const cuuint32_t b[2] = {box[0], i < 2 ? box[1] : 16u};
+        if (fn(static_cast<CUtensorMap*>(maps) + i, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2,
+               i & 1 ? p->v : p->k, dims, strides, b, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
             return (int)cudaErrorInvalidValue;
+    }
     return 0;
 }

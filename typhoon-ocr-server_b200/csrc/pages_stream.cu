@@ -58,6 +58,10 @@ struct Tile {
     int c0, c1, s0;   // the runs that have part of the item, and which record of run c0 is its
 };
 
+struct Maps {
+    CUtensorMap m[4];  // K, V; K, V in boxes of 16 rows
+};
+
 struct StreamArgs {
     AttnArgs a;
     int layer;
@@ -116,7 +120,7 @@ struct Gather {
 
 template <typename T, int D, int kBlocks, bool kDup>
 __global__ void __launch_bounds__(kStreamThreads, 2)
-    pages_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const StreamArgs sa)
+    pages_stream_kernel(const __grid_constant__ Maps maps, const StreamArgs sa)
 {
     using S = Stream<T, D>;
     const AttnArgs& a = sa.a;
@@ -209,12 +213,12 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
 
     if (warp == kTakers) {
         // ---- requests
-        // Lane (part, box, K or V): a stage's rows come from 1, 2 or 4 parts (pages, or one part of a page), each
-        // 128-byte column box of each as one copy.
-        const int part_rows = box_rows(a.p), parts = S::kRows / part_rows, shift = page_shift(a.p.page_size);
-        const int part = lane % parts, box = lane / parts % S::kBoxes, which = lane / parts / S::kBoxes;
-        const unsigned int part_bits = (1u << (part_rows / 8)) - 1u;
-        const int part_bytes = part_rows * 128;
+        // Lane (part, box, K or V): a stage's rows come in 1, 2 or 4 parts (pages, or one part of a page; 16 rows each
+        // where not all of a stage is in sight, so that no more is read than that), each 128-byte column box of
+        // each as one copy.
+        const int shift = page_shift(a.p.page_size);
+        int part_rows = 0, parts = 1, part = 0, box = 0, which = 2;
+        bool fine = false;
         const uint32_t q_row = (uint32_t)(a.group * D * (a.io_bf16 ? 2 : 4));
         const int max_page = a.p.num_pages;
         Tile tile = {};
@@ -290,8 +294,14 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
             const int i = none ? list.count() : (int)(u - u0 - kItemUnits);
             const bool real = i < list.count();
             tile.k0 = real ? list.at(i) * S::kRows : tile.pos + 1;
+            fine = tile.k0 + S::kRows - 1 > tile.pos || (tile.k0 < tile.lo && tile.k0 + S::kRows > tile.sinks);
+            part_rows = fine ? 16 : box_rows(a.p);
+            parts = S::kRows / part_rows;
+            part = lane & (parts - 1);
+            box = lane / parts & (S::kBoxes - 1);
+            which = lane / (parts * S::kBoxes);
             const int key = tile.k0 + part * part_rows;
-            page = real && which < 2 && key <= tile.pos ? table[key >> shift] : -1;
+            page = real && which < 2 && key <= tile.pos && (key + part_rows > tile.lo || key < tile.sinks) ? table[key >> shift] : -1;
             u++;
         };
         next();
@@ -307,16 +317,16 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
             const unsigned int have = __ballot_sync(0xffffffffu, page >= 0);
             tile.seen = 0;
             for (int l = 0; l < parts; l++)
-                if (have >> l & 1u) tile.seen |= part_bits << (l * (part_rows / 8));
+                if (have >> l & 1u) tile.seen |= ((1u << (part_rows / 8)) - 1u) << (l * (part_rows / 8));
             if (lane == 0) {
                 tiles_of_stage[st] = tile;
-                mbar_arrive_expect_tx(&full[st], (uint32_t)(__popc(have) * part_bytes) + (tile.first ? q_row * (uint32_t)tile.ntok : 0u));
+                mbar_arrive_expect_tx(&full[st], (uint32_t)(__popc(have) * part_rows * 128) + (tile.first ? q_row * (uint32_t)tile.ntok : 0u));
             }
             __syncwarp();
             if (page >= 0) {
                 const int row = ((sa.layer * a.p.num_pages + page) * heads + tile.kvh) * a.p.page_size +
                                 ((tile.k0 + part * part_rows) & (a.p.page_size - 1));
-                tma_load_2d(ring + st * S::kStage + which * S::kHalf + box * S::kBox + part * part_bytes, which ? &map_v : &map_k,
+                tma_load_2d(ring + st * S::kStage + which * S::kHalf + box * S::kBox + part * part_rows * 128, &maps.m[2 * fine + which],
                             box * S::kBoxCols, row, &full[st]);
             }
             if (tile.first && lane < tile.ntok)
@@ -587,8 +597,7 @@ static int launch_rows_t(StreamArgs sa, const void* maps, cudaStream_t stream)
         if (e != cudaSuccess) return (int)e;
         ready[dev] = true;
     }
-    const CUtensorMap* m = static_cast<const CUtensorMap*>(maps);
-    return launch_after(pages_stream_kernel<T, D, kBlocks, kDup>, dim3(ctas * kSms), kStreamThreads, bytes, stream, m[0], m[1], sa);
+    return launch_after(pages_stream_kernel<T, D, kBlocks, kDup>, dim3(ctas * kSms), kStreamThreads, bytes, stream, *static_cast<const Maps*>(maps), sa);
 }
 
 template <typename T, int D>
