@@ -9,7 +9,7 @@
 // the plan's `ok` at 0 and the apply kernel does nothing.
 //
 // The row copies are bound by memory: each row is read once and written once, by 16-byte accesses,
-// a (page, layer, tensor, head) block of consecutive rows per CTA and turn.
+// a (page, layer, tensor, head) block of consecutive rows per warp and turn.
 #define TYB_WHOLE_PROGRAM
 #include "pages_attn.cuh"
 
@@ -133,29 +133,29 @@ __global__ void __launch_bounds__(kPlanThreads)
     const int cap = p.max_pages * p.page_size;
     after_predecessor();
     clear_marks(marks, p.max_seqs);
-    int need = 0;
+    int need = 0, s = 0, len = 0, mine = 0, at = 0;  // the thread's item of the last turn: the only one of most calls
     bool bad = false;
     for (int base = 0; base < n; base += kPlanThreads) {
         const int i = base + (int)threadIdx.x;
-        int mine = 0;
+        mine = 0;
         if (i < n) {
-            const int s = seqs ? seqs[i] : seq0, c = counts ? counts[i] : count0;
+            const int c = counts ? counts[i] : count0;
+            s = seqs ? seqs[i] : seq0;
             if (s < 0 || s >= p.max_seqs || c < 0 || !mark(marks, s)) {
                 bad = true;
             } else {
-                const int len = p.len[s];
-                if (len < 0 || len > cap || c > cap - len || (!seqs && len != 0))
-                    bad = true;
-                else
-                    mine = (len + c + p.page_size - 1) / p.page_size - (len + p.page_size - 1) / p.page_size;
+                len = p.len[s];
+                if (len < 0 || len > cap || c > cap - len || (!seqs && len != 0)) bad = true;
+                else mine = (len + c + p.page_size - 1) / p.page_size - (len + p.page_size - 1) / p.page_size;
+                len += c;
             }
         }
         // no list of valid items needs more pages than the pool has: the sum stays far below 2^31
         if (mine > p.num_pages) mine = p.num_pages + 1;
         if (__syncthreads_or(bad)) break;
         int total;
-        const int at = block_scan(mine, &total);
-        if (i < n) plan.first[i] = need + at;
+        at = need + block_scan(mine, &total);
+        if (i < n && n > kPlanThreads) plan.first[i] = at;
         need += total;
         if (need > p.num_pages) break;
     }
@@ -165,18 +165,35 @@ __global__ void __launch_bounds__(kPlanThreads)
     plan_done(plan.head, bad, short_of, 0, st);
     __syncthreads();
     if (bad || short_of) return;
-    // a warp per sequence
-    for (int i = (int)(threadIdx.x >> 5); i < n; i += kPlanWarps) {
-        const int s = seqs ? seqs[i] : seq0, c = counts ? counts[i] : count0;
-        const int len = p.len[s];
-        const int e0 = (len + p.page_size - 1) / p.page_size, e1 = (len + c + p.page_size - 1) / p.page_size;
-        for (int e = e0 + (int)(threadIdx.x & 31); e < e1; e += 32) {
-            const int page = plan.fresh[plan.first[i] + e - e0];
-            p.table[(size_t)s * p.max_pages + e] = page;
+    for (int base = 0; base < n; base += kPlanThreads) {
+        const int i = base + (int)threadIdx.x;
+        if (n > kPlanThreads && i < n) {  // not the thread's last item
+            s = seqs[i];
+            at = plan.first[i];
+            const int c = counts[i], old = p.len[s];
+            len = old + c;
+            mine = (len + p.page_size - 1) / p.page_size - (old + p.page_size - 1) / p.page_size;
+        }
+        if (i >= n) mine = 0;
+        const int e0 = (len + p.page_size - 1) / p.page_size - mine;
+        // a few pages by the sequence's own thread, many by its warp
+        const bool many = mine > 8;
+        for (int k = 0; !many && k < mine; k++) {
+            const int page = plan.fresh[at + k];
+            p.table[(size_t)s * p.max_pages + e0 + k] = page;
             p.ref[page] = 1;
         }
-        __syncwarp();
-        if ((threadIdx.x & 31) == 0) p.len[s] = len + c;
+        for (unsigned int left = __ballot_sync(0xffffffffu, many); left; left &= left - 1) {
+            const int l = __ffs(left) - 1;
+            const int s1 = __shfl_sync(0xffffffffu, s, l), at1 = __shfl_sync(0xffffffffu, at, l), e1 = __shfl_sync(0xffffffffu, e0, l),
+                      n1 = __shfl_sync(0xffffffffu, mine, l);
+            for (int k = threadIdx.x & 31; k < n1; k += 32) {
+                const int page = plan.fresh[at1 + k];
+                p.table[(size_t)s1 * p.max_pages + e1 + k] = page;
+                p.ref[page] = 1;
+            }
+        }
+        if (i < n) p.len[s] = len;
     }
 }
 
@@ -250,30 +267,37 @@ __global__ void __launch_bounds__(kPlanThreads)
     }
 }
 
-// The rows of a plan's moves, the CTA's share of (move, layer, tensor, head) blocks.
+// A block of `bytes` consecutive bytes (a multiple of 16, up to 64 KB) by one warp, eight 16-byte accesses a lane
+// requested at a time.
+__device__ __forceinline__ void copy_block(char* to, const char* from, int bytes, int lane)
+{
+    const uint4* f = reinterpret_cast<const uint4*>(from);
+    uint4* t = reinterpret_cast<uint4*>(to);
+    const int n = bytes / 16;
+    for (int i = lane; i < n; i += 8 * 32) {
+        uint4 x[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            if (i + j * 32 < n) x[j] = __ldcs(f + i + j * 32);
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            if (i + j * 32 < n) __stcs(t + i + j * 32, x[j]);
+    }
+}
+
+// The rows of a plan's moves: a (move, layer, tensor, head) block per warp and turn, neighbouring warps
+// neighbouring heads.  (A block per CTA and turn left two accesses a thread in flight: 113 us for 350 MB.)
 __device__ void copy_rows(const KVPages& p, const Plan& plan, int row_bytes)
 {
-    const int lt = p.num_layers * 2;
-    const long long units = (long long)plan.head->moves * lt * p.kv_heads;
-    for (long long u = blockIdx.x; u < units; u += gridDim.x) {
-        const int h = (int)(u % p.kv_heads);
-        const long long q = u / p.kv_heads;
-        const int layer = (int)(q % lt) >> 1;
-        const Move m = plan.moves[q / lt];
-        char* slab = static_cast<char*>((q & 1) ? p.v : p.k);
-        const size_t block = (size_t)p.page_size * row_bytes;
-        const uint4* from = reinterpret_cast<const uint4*>(slab + (((size_t)layer * p.num_pages + m.from) * p.kv_heads + h) * block);
-        uint4* to = reinterpret_cast<uint4*>(slab + (((size_t)layer * p.num_pages + m.to) * p.kv_heads + h) * block);
-        const int n = m.rows * (row_bytes / 16);
-        for (int i = threadIdx.x; i < n; i += 4 * kApplyThreads) {
-            uint4 x[4];
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-                if (i + j * kApplyThreads < n) x[j] = __ldcs(from + i + j * kApplyThreads);
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-                if (i + j * kApplyThreads < n) __stcs(to + i + j * kApplyThreads, x[j]);
-        }
+    const int lane = threadIdx.x & 31;
+    const unsigned int lt = p.num_layers * 2, per_move = lt * p.kv_heads;  // no pool has 2^32 blocks: it has fewer rows
+    const unsigned int units = (unsigned int)plan.head->moves * per_move, warps = gridDim.x * (kApplyThreads / 32);
+    const size_t block = (size_t)p.page_size * row_bytes;
+    for (unsigned int u = blockIdx.x * (kApplyThreads / 32) + (threadIdx.x >> 5); u < units; u += warps) {
+        const unsigned int move = u / per_move, in_move = u - move * per_move, q = in_move / p.kv_heads, h = in_move - q * p.kv_heads;
+        const Move m = plan.moves[move];
+        char* slab = static_cast<char*>((q & 1) ? p.v : p.k) + ((size_t)(q >> 1) * p.num_pages * p.kv_heads + h) * block;
+        copy_block(slab + (size_t)m.to * p.kv_heads * block, slab + (size_t)m.from * p.kv_heads * block, m.rows * row_bytes, lane);
     }
 }
 
@@ -436,20 +460,16 @@ __global__ void __launch_bounds__(kApplyThreads)
 {
     after_predecessor();
     if (!static_cast<const PlanHead*>(ws)->ok) return;
-    const int lt = p.num_layers * 2;
-    const long long units = (long long)((rows + p.page_size - 1) / p.page_size) * lt * p.kv_heads;
-    for (long long u = blockIdx.x; u < units; u += gridDim.x) {
-        const int h = (int)(u % p.kv_heads);
-        const long long q = u / p.kv_heads;
-        const int layer = (int)(q % lt) >> 1, e = (int)(q / lt);
+    const int lane = threadIdx.x & 31;
+    const unsigned int lt = p.num_layers * 2, per_entry = lt * p.kv_heads, warps = gridDim.x * (kApplyThreads / 32);
+    const unsigned int units = (unsigned int)((rows + p.page_size - 1) / p.page_size) * per_entry;
+    const size_t block = (size_t)p.page_size * row_bytes;
+    for (unsigned int u = blockIdx.x * (kApplyThreads / 32) + (threadIdx.x >> 5); u < units; u += warps) {
+        const unsigned int e = u / per_entry, in_entry = u - e * per_entry, q = in_entry / p.kv_heads, h = in_entry - q * p.kv_heads;
         const int page = p.table[(size_t)seq * p.max_pages + e];
-        const char* slab = (q & 1) ? v_slab : k_slab;
-        const uint4* from = reinterpret_cast<const uint4*>(
-            slab + (((size_t)layer * p.kv_heads + h) * row_capacity + (size_t)e * p.page_size) * row_bytes);
-        uint4* to = reinterpret_cast<uint4*>(static_cast<char*>((q & 1) ? p.v : p.k) +
-                                             (((size_t)layer * p.num_pages + page) * p.kv_heads + h) * p.page_size * row_bytes);
-        const int n = min(p.page_size, rows - e * p.page_size) * (row_bytes / 16);
-        for (int i = threadIdx.x; i < n; i += kApplyThreads) to[i] = from[i];
+        const char* from = ((q & 1) ? v_slab : k_slab) + (((size_t)(q >> 1) * p.kv_heads + h) * row_capacity + (size_t)e * p.page_size) * row_bytes;
+        char* to = static_cast<char*>((q & 1) ? p.v : p.k) + (((size_t)(q >> 1) * p.num_pages + page) * p.kv_heads + h) * block;
+        copy_block(to, from, min(p.page_size, rows - (int)e * p.page_size) * row_bytes, lane);
     }
 }
 
