@@ -139,6 +139,44 @@ struct AttnArgs {
 constexpr int kTcTall = 128, kTcWide = 256;
 int tc_launch(const AttnArgs& a, int layer, bool tall, bool shared_pass, int items, const void* maps, cudaStream_t stream);
 
+// The row form (pages_rows.cu) for the prompt chunks of an FP32 pool, row tiles of kRowsTile rows.
+constexpr int kRowsTile = 64;
+int rows_launch(const AttnArgs& a, int layer, int items, const void* maps, cudaStream_t stream);
+
+// Item x of a list of row tiles: sequence b's queries starts[b] .. starts[b + 1] in tiles of `per` tokens.
+// found: b (-1: no such item), its first query, its queries, and that query's place before the sequence's end
+// (its position is the length plus this).  By one warp.
+__device__ __forceinline__ void find_item(const AttnArgs& a, int x, int per, int* found)
+{
+    const int lane = threadIdx.x & 31;
+    int before = 0;
+    if (lane == 0) found[0] = -1;
+    __syncwarp();
+    for (int base = 0; base < a.batch && before <= x; base += 32) {
+        const int b = base + lane;
+        const int q0 = b < a.batch ? a.starts[b] : 0, q1 = b < a.batch ? a.starts[b + 1] : 0;
+        const int cnt = q1 > q0 ? (q1 - q0 + per - 1) / per : 0;
+        int sum = cnt;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += y;
+        }
+        const int lo = before + sum - cnt;
+        if (x >= lo && x < lo + cnt) {
+            if (q0 < 0 || q1 > a.rows) {
+                raise(a.st, TYB_STATUS_BAD_ARGUMENT);
+            } else {
+                found[0] = b;
+                found[1] = q0 + (x - lo) * per;
+                found[2] = min(per, q1 - q0 - (x - lo) * per);
+                found[3] = (x - lo) * per - (q1 - q0);
+            }
+        }
+        before += __shfl_sync(0xffffffffu, sum, 31);
+    }
+}
+
 // The streaming form (pages_stream.cu): the single tokens of sequences first .. first + count (at most
 // kStreamSeqs) of the call, with the shared pass over a.prefix rows in the same launch (`shared`); the
 // results are the output, or (out_slot >= 0) record slot out_slot of a.rec.  ws: stream_bytes; tickets: count * kv_heads words, zero (and left

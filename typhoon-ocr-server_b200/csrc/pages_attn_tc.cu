@@ -205,36 +205,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         tc_fence_before();
     }
     after_predecessor();
-    // Which tokens: item x of the batch (the last items, with the most keys to see, first).
-    if (warp == 0 && !ta.shared_pass) {
-        const int x = (int)(gridDim.x - 1 - blockIdx.x);
-        int before = 0;
-        if (lane == 0) found[0] = -1;
-        __syncwarp();
-        for (int base = 0; base < a.batch && before <= x; base += 32) {
-            const int b = base + lane;
-            const int q0 = b < a.batch ? a.starts[b] : 0, q1 = b < a.batch ? a.starts[b + 1] : 0;
-            const int cnt = q1 > q0 ? (q1 - q0 + per - 1) / per : 0;
-            int sum = cnt;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int y = __shfl_up_sync(0xffffffffu, sum, o);
-                if (lane >= o) sum += y;
-            }
-            const int lo = before + sum - cnt;
-            if (x >= lo && x < lo + cnt) {
-                if (q0 < 0 || q1 > a.rows) {
-                    raise(a.st, TYB_STATUS_BAD_ARGUMENT);
-                } else {
-                    found[0] = b;
-                    found[1] = q0 + (x - lo) * per;
-                    found[2] = min(per, q1 - q0 - (x - lo) * per);
-                    found[3] = (x - lo) * per - (q1 - q0);
-                }
-            }
-            before += __shfl_sync(0xffffffffu, sum, 31);
-        }
-    }
+    if (warp == 0 && !ta.shared_pass) find_item(a, (int)(gridDim.x - 1 - blockIdx.x), per, found);  // the last items, with the most keys, first
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;

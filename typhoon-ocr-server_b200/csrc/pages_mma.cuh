@@ -40,11 +40,13 @@ __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], 
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// x = hi + lo in TF32, the remainder below 2^-22 |x|.
+// x = hi + lo in TF32 to within 2^-22 |x|: hi the leading 11 significant bits, lo the exact rest, rounded (to nearest,
+// by half a unit of the last bit that the product reads: it ignores the 13 below).  In integer and FP32 operations of
+// full rate; the conversions to TF32 have a fraction of it.
 __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo)
 {
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(x - __uint_as_float(hi)));
+    hi = __float_as_uint(x) & 0xffffe000u;
+    lo = __float_as_uint(x - __uint_as_float(hi)) + 0x1000u;
 }
 
 __device__ __forceinline__ void ldsm(uint32_t (&r)[4], uint32_t at)
@@ -80,6 +82,14 @@ __device__ __forceinline__ void put_out(const AttnArgs& a, size_t at, float4 x, 
         *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
 }
 
+// What a tile's keys look like to rows that all see the same: bit i, key i.
+template <int kKeys>
+struct SameSight {
+    unsigned int see;
+    __device__ __forceinline__ bool all() const { return see == 0xffffffffu >> (32 - kKeys); }
+    __device__ __forceinline__ bool operator()(int, int, int i) const { return see >> i & 1u; }
+};
+
 // Column q of block n of the products is query row 8 n + q; with kDup (rows up to 4, one block) columns 4-7
 // are rows 0-3 again.  Lane (g, t) = (lane / 4, lane % 4).
 // O^T fragments: o[n][i][c] is dimension 16 i + g + 8 (c / 2) of column 2 t + c % 2; statistics per column.
@@ -99,20 +109,21 @@ struct Running {
         }
     }
 
-    // Scores s[n][e][c] (key 16 e + g + 8 (c / 2) of column 2 t + c % 2) become weights; bit i of `see`: key i
-    // is in sight of the rows.
-    template <int E>
-    __device__ __forceinline__ void weigh(float (&s)[kBlocks][E][4], unsigned int see, float scale, int g)
+    // Scores s[n][e][c] (key 16 e + g + 8 (c / 2) of column 2 t + c % 2) become weights.  sight.all(): every key
+    // is in sight of every row; else sight(n, c, i): key i is in sight of column 2 t + c of block n.
+    template <int E, typename Sight>
+    __device__ __forceinline__ void weigh(float (&s)[kBlocks][E][4], const Sight& sight, float scale, int g)
     {
-        if (see != 0xffffffffu >> (32 - 16 * E)) {
+        if (!sight.all()) {
 #pragma unroll
             for (int e = 0; e < E; e++)
 #pragma unroll
                 for (int hf = 0; hf < 2; hf++)
-                    if (!(see >> (16 * e + g + 8 * hf) & 1u)) {
 #pragma unroll
-                        for (int n = 0; n < kBlocks; n++) s[n][e][2 * hf] = s[n][e][2 * hf + 1] = -INFINITY;
-                    }
+                    for (int n = 0; n < kBlocks; n++)
+#pragma unroll
+                        for (int c = 0; c < 2; c++)
+                            if (!sight(n, c, 16 * e + g + 8 * hf)) s[n][e][2 * hf + c] = -INFINITY;
         }
         float top[kBlocks][2];
         bool rise = false;
@@ -214,7 +225,8 @@ struct Rows<__nv_bfloat16, D, kBlocks, kDup> : Running<D, kBlocks, kDup> {
     }
 
     // Rows r0 .. r0 + 32 of the tile.
-    __device__ __forceinline__ void step(const unsigned char* kt, const unsigned char* vt, int box, int r0, unsigned int see, float scale,
+    template <typename Sight>
+    __device__ __forceinline__ void step(const unsigned char* kt, const unsigned char* vt, int box, int r0, const Sight& see, float scale,
                                          const float*, int g, int t, int lane)
     {
         float s[kBlocks][2][4];
@@ -304,16 +316,17 @@ struct Rows<float, D, kBlocks, kDup> : Running<D, kBlocks, kDup> {
     }
 
     // Rows r0 .. r0 + 16 of the tile.
-    __device__ __forceinline__ void step(const unsigned char* kt, const unsigned char* vt, int box, int r0, unsigned int see, float scale,
+    template <typename Sight>
+    __device__ __forceinline__ void step(const unsigned char* kt, const unsigned char* vt, int box, int r0, const Sight& see, float scale,
                                          const float* split, int g, int t, int lane)
     {
-        // Even and odd steps, and the small terms, in accumulators of their own: shorter chains, and the small
-        // terms are not rounded away one by one.
-        float s[kBlocks][1][4], s2[kBlocks][4];
+        // The terms hi.hi, lo.hi and hi.lo in accumulators of their own: shorter chains, and the small terms are not
+        // rounded away one by one.
+        float s[kBlocks][1][4], s2[kBlocks][4], s3[kBlocks][4];
 #pragma unroll
         for (int b = 0; b < kBlocks; b++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) s[b][0][i] = s2[b][i] = 0.f;
+            for (int i = 0; i < 4; i++) s[b][0][i] = s2[b][i] = s3[b][i] = 0.f;
         {
             const int row = r0 + (lane & 15), half = lane >> 4;
             const uint32_t at = smem_u32(kt) + row * 128;
@@ -335,7 +348,7 @@ struct Rows<float, D, kBlocks, kDup> : Running<D, kBlocks, kDup> {
                         const uint32_t h0 = p[0], h1 = p[4], l0 = p[8 * kBlocks * kPitch], l1 = p[8 * kBlocks * kPitch + 4];
                         mma_tf32(s[b][0], hi, h0, h1);
                         mma_tf32(s2[b], lo, h0, h1);
-                        mma_tf32(s2[b], hi, l0, l1);
+                        mma_tf32(s3[b], hi, l0, l1);
                     }
                 }
             }
@@ -344,7 +357,7 @@ struct Rows<float, D, kBlocks, kDup> : Running<D, kBlocks, kDup> {
         for (int b = 0; b < kBlocks; b++)
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                s[b][0][i] += s2[b][i];
+                s[b][0][i] += s2[b][i] + s3[b][i];
                 if (kDup) s[b][0][i] += __shfl_xor_sync(0xffffffffu, s[b][0][i], 2);  // the columns of hi and of lo
             }
         this->template weigh<1>(s, see, scale, g);

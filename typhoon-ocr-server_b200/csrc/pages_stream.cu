@@ -58,6 +58,12 @@ struct Tile {
     int c0, c1, s0;   // the runs that have part of the item, and which record of run c0 is its
 };
 
+// Where the records of a (token, KV head) lie: in runs sh0 .. sh1 those of its shared item (none: sh1 < sh0), in runs
+// own0 .. own1 its own; *_second: whether that of the first such run is the run's second record.
+struct Parts {
+    int sh0, sh1, sh_second, own0, own1, own_second;
+};
+
 struct Maps {
     CUtensorMap m[4];  // K, V; K, V in boxes of 16 rows
 };
@@ -136,9 +142,10 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
 
     __shared__ uint64_t full[kMaxStages], empty[kMaxStages], met;
     __shared__ Tile tiles_of_stage[kMaxStages];
-    __shared__ float2 join_mls[2][kTakers][16];
+    __shared__ float2 join_mls[kTakers][16];  // (two buffers: of four rows each)
     __shared__ int scan[kStreamThreads / 32];
     __shared__ unsigned int last_of;  // tokens whose join is this CTA's
+    __shared__ Parts parts_of[16];    // and where their records lie
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int heads = a.p.kv_heads, run = blockIdx.x;
@@ -359,10 +366,10 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
     bool one_item = true;  // no item has ended in this run yet
     int buffer = 0;        // of the join rows: two, used in turn
     // Rows of the records: of a cut item's part in a run, of uncut own rows, of an uncut shared item.
-    auto part_row = [&](int run_of, int second) { return (size_t)(2 * run_of + second) * 16; };
-    auto own_row = [&](int tok, int kvh) { return (size_t)2 * kStreamRuns * 16 + (size_t)tok * a.q_heads + kvh * a.group; };
+    auto part_row = [&](int run_of, int second) { return (2 * run_of + second) * 16; };
+    auto own_row = [&](int tok, int kvh) { return 2 * kStreamRuns * 16 + tok * a.q_heads + kvh * a.group; };
     auto shared_row = [&](int tok, int kvh) {
-        return (size_t)2 * kStreamRuns * 16 + (size_t)a.batch * a.q_heads + ((size_t)(tok / per) * heads + kvh) * 16;
+        return 2 * kStreamRuns * 16 + a.batch * a.q_heads + (tok / per * heads + kvh) * 16;
     };
     // The takers meet at an mbarrier rather than a CTA barrier: its wait is bounded, so that a warp whose
     // wait ran out and left does not leave the others waiting.
@@ -386,11 +393,10 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
     // Four columns of a row, joined over the warps' shares in shared memory.
     auto over_warps = [&](int row, int c) {
         const float* join = joins + buffer * kTakers * sa.item_rows * S::kPitch;
-        const float2(*join_ml)[16] = join_mls[buffer];
         Gather sum;
 #pragma unroll
         for (int x = 0; x < kTakers; x++)
-            sum.add(join_ml[x][row], *reinterpret_cast<const float4*>(join + (x * sa.item_rows + row) * S::kPitch + c));
+            sum.add(join_mls[x][4 * buffer + row], *reinterpret_cast<const float4*>(join + (x * sa.item_rows + row) * S::kPitch + c));
         return sum;
     };
     for (bool more = true; more;) {
@@ -424,7 +430,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
                 fence_proxy_async_smem();
                 __syncwarp();
             }
-            w.step(rows_k, rows_v, S::kBox, r0, see, a.scale_log2, split_q, g, t, lane);
+            w.step(rows_k, rows_v, S::kBox, r0, SameSight<S::kKeys>{see}, a.scale_log2, split_q, g, t, lane);
         }
         warp_arrive(&empty[st]);
         turn ^= 1;
@@ -439,12 +445,11 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
         if (sa.buffers == 2) buffer ^= 1;
         else if (!meet()) return;
         float* join = joins + buffer * kTakers * sa.item_rows * S::kPitch;
-        float2(*join_ml)[16] = join_mls[buffer];
-        w.put(join + warp * sa.item_rows * S::kPitch, S::kPitch, join_ml[warp], nrows, g, t);
+        w.put(join + warp * sa.item_rows * S::kPitch, S::kPitch, &join_mls[warp][4 * buffer], nrows, g, t);
         w.clear();  // (and so not kept through what follows)
         if (!meet()) return;
         const bool cut = tile.c0 != tile.c1, direct = !cut && !sa.shared_tiles;
-        const size_t record = cut ? part_row(run, one_item ? 0 : 1) : tile.shared ? shared_row(tile.tok0, tile.kvh) : own_row(tile.tok0, tile.kvh);
+        const int record = cut ? part_row(run, one_item ? 0 : 1) : tile.shared ? shared_row(tile.tok0, tile.kvh) : own_row(tile.tok0, tile.kvh);
         one_item = false;
         for (int i = tid; i < nrows * (D / 4); i += kTakerThreads) {
             const int row = i / (D / 4), c = i % (D / 4) * 4;
@@ -452,7 +457,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
             if (direct) {
                 deliver((size_t)(sa.tok_base + tile.tok0) * a.q_heads + tile.kvh * a.group + row, c, sum);
             } else {
-                *reinterpret_cast<float4*>(sa.rec_o + (record + row) * D + c) = sum.o;
+                *reinterpret_cast<float4*>(sa.rec_o + (size_t)(record + row) * D + c) = sum.o;
                 if (c == 0) sa.rec_ml[record + row] = make_float2(sum.m, sum.l);
             }
         }
@@ -462,81 +467,81 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
         // joins that sequence's rows.
         if (tid == 0) last_of = 0;
         if (!meet()) return;
-        // the records of (token, KV head): where its shared ones and its own ones lie
-        auto spans = [&](int tok, Tile& sh, Tile& ow) {
-            ow = sh = tile;
+        if (tid < tile.ntok) {
+            const int tok = tile.tok0 + tid;
+            Parts p = {0, -1, 0, tile.c0, tile.c1, tile.s0};
             if (tile.shared) {
+                p.sh0 = tile.c0, p.sh1 = tile.c1, p.sh_second = tile.s0;
                 const unsigned int units = cum[tok + 1] - cum[tok], v0 = shared_all + cum[tok] * heads + tile.kvh * units;
-                cuts.span(v0, v0 + units, ow.c0, ow.c1, ow.s0);
+                cuts.span(v0, v0 + units, p.own0, p.own1, p.own_second);
             } else if (sa.shared_tiles) {
                 const unsigned int v0 = ((unsigned int)(tok / per) * heads + tile.kvh) * sa.shared_units;
-                cuts.span(v0, v0 + sa.shared_units, sh.c0, sh.c1, sh.s0);
+                cuts.span(v0, v0 + sa.shared_units, p.sh0, p.sh1, p.sh_second);
             }
-            if (!sa.shared_tiles) sh.c0 = 0, sh.c1 = -1;
-        };
-        if (tid < tile.ntok) {
-            Tile sh, ow;
-            spans(tile.tok0 + tid, sh, ow);
-            const unsigned int count = (unsigned int)(ow.c1 - ow.c0 + 1 + sh.c1 - sh.c0 + 1);
-            unsigned int* ticket = sa.tickets + (size_t)(tile.tok0 + tid) * heads + tile.kvh;
+            const unsigned int count = (unsigned int)(p.own1 - p.own0 + 1 + p.sh1 - p.sh0 + 1);
+            unsigned int* ticket = sa.tickets + (size_t)tok * heads + tile.kvh;
             // releases what all the CTA's threads wrote before they met, and acquires what the others released
             unsigned int before_me;
             asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(before_me) : "l"(ticket) : "memory");
             if (before_me == count - 1u) {
                 *ticket = 0u;
+                parts_of[tid] = p;
                 atomicOr(&last_of, 1u << tid);
             }
         }
         if (!meet()) return;
         const unsigned int mine = last_of;
         if (!mine) continue;
-        // The rows of all those sequences at once: `teams` warps a row, each with some of its records, eight
-        // requested at a time; then the warps are joined.
+        // The rows of all those sequences at once: `teams` warps a row, each with some of its records, a dozen (statistics
+        // and columns) requested at a time; then the warps are joined.
         const int rows = __popc(mine) * a.group, teams = rows >= kTakers ? 1 : kTakers / rows;
         auto token_of = [&](int k) {  // of the k-th sequence to join
             unsigned int left = mine;
             for (; k > 0; k--) left &= left - 1;
             return __ffs(left) - 1;
         };
+        constexpr int kDozen = 12;
+#pragma unroll 1
         for (int j = warp; j < rows * teams; j += kTakers) {
-            const int row = j / teams, part = j % teams, k = token_of(row / a.group), in_head = row % a.group, tok = tile.tok0 + k;
-            Tile sh, ow;
-            spans(tok, sh, ow);
-            const int ns = sh.c1 - sh.c0 + 1, n = ns + ow.c1 - ow.c0 + 1;
-            // Each lane fetches the statistics of one of the warp's records; then all of a record's columns at a time.
+            const int row = j / teams, part = j - row * teams, seq_of = row / a.group, in_head = row - seq_of * a.group;
+            const int k = token_of(seq_of), tok = tile.tok0 + k;
+            const Parts p = parts_of[k];
+            const int ns = p.sh1 - p.sh0 + 1, n = ns + p.own1 - p.own0 + 1, mine_n = (n - part + teams - 1) / teams;
             const int c = lane % (D / 4) * 4;  // D = 64: two lanes have the same columns
             Gather sum;
-            for (int base = 0; part + base * teams < n; base += 32) {
-                const int x = part + (base + lane) * teams, y = x - ns;
-                size_t at = 0;
-                float2 ml = make_float2(-INFINITY, 0.f);
-                if (x < n) {
-                    at = x < ns ? (ns == 1 ? shared_row(tok, tile.kvh) : part_row(sh.c0 + x, x ? 0 : sh.s0)) + tok % per * a.group
-                                : ow.c0 == ow.c1 ? own_row(tok, tile.kvh) : part_row(ow.c0 + y, y ? 0 : ow.s0);
-                    at += in_head;
-                    ml = __ldcg(&sa.rec_ml[at]);
-                }
+#pragma unroll 1
+            for (int base = 0; base < mine_n; base += kDozen) {
+                const int here = min(kDozen, mine_n - base);
+                // lane y: record base + y of the warp's
+                const int x = part + (base + min(lane, here - 1)) * teams, y = x - ns;
+                int at;
+                if (x < ns) at = (ns == 1 ? shared_row(tok, tile.kvh) : part_row(p.sh0 + x, x ? 0 : p.sh_second)) + (tok - tok / per * per) * a.group;
+                else at = p.own0 == p.own1 ? own_row(tok, tile.kvh) : part_row(p.own0 + y, y ? 0 : p.own_second);
+                at += in_head;
+                float2 ml = __ldcg(&sa.rec_ml[at]);
+                float4 v[kDozen];
+#pragma unroll
+                for (int i = 0; i < kDozen; i++)
+                    v[i] = __ldcg(reinterpret_cast<const float4*>(sa.rec_o + (size_t)__shfl_sync(0xffffffffu, at, i) * D + c));
+                if (lane >= here) ml = make_float2(-INFINITY, 0.f);
                 float top = ml.x;
 #pragma unroll
-                for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                for (int d = 8; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                top = __shfl_sync(0xffffffffu, top, 0);
                 const float f = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - top);
                 float l = ml.y * f;
 #pragma unroll
-                for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+                for (int d = 8; d; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+                l = __shfl_sync(0xffffffffu, l, 0);
                 float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-                const int here = min(32, (n - part - base * teams + teams - 1) / teams);
-                for (int i = 0; i < here; i += 8) {  // eight requested at a time
-                    float4 v[8];
 #pragma unroll
-                    for (int k = 0; k < 8; k++)
-                        v[k] = __ldcg(reinterpret_cast<const float4*>(sa.rec_o + __shfl_sync(0xffffffffu, at, min(i + k, here - 1)) * D + c));
-#pragma unroll
-                    for (int k = 0; k < 8; k++) {
-                        const float fk = i + k < here ? __shfl_sync(0xffffffffu, f, (i + k) & 31) : 0.f;
-                        o.x = fmaf(v[k].x, fk, o.x);
-                        o.y = fmaf(v[k].y, fk, o.y);
-                        o.z = fmaf(v[k].z, fk, o.z);
-                        o.w = fmaf(v[k].w, fk, o.w);
+                for (int i = 0; i < kDozen; i++) {
+                    const float fi = __shfl_sync(0xffffffffu, f, i);
+                    if (i < here) {
+                        o.x = fmaf(v[i].x, fi, o.x);
+                        o.y = fmaf(v[i].y, fi, o.y);
+                        o.z = fmaf(v[i].z, fi, o.z);
+                        o.w = fmaf(v[i].w, fi, o.w);
                     }
                 }
                 sum.add(make_float2(top, l), o);
@@ -546,7 +551,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
                 if (lane < D / 4) deliver(R, c, sum);
             } else if (lane < D / 4) {
                 *reinterpret_cast<float4*>(join + (part * sa.item_rows + row) * S::kPitch + c) = sum.o;
-                if (c == 0) join_ml[part][row] = make_float2(sum.m, sum.l);
+                if (c == 0) join_mls[part][4 * buffer + row] = make_float2(sum.m, sum.l);
             }
         }
         if (teams > 1) {
@@ -555,11 +560,11 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
                 const int row = i / (D / 4), c = i % (D / 4) * 4, tok = tile.tok0 + token_of(row / a.group);
                 Gather sum;
                 for (int x = 0; x < teams; x++)
-                    sum.add(join_ml[x][row], *reinterpret_cast<const float4*>(join + (x * sa.item_rows + row) * S::kPitch + c));
+                    sum.add(join_mls[x][4 * buffer + row], *reinterpret_cast<const float4*>(join + (x * sa.item_rows + row) * S::kPitch + c));
                 deliver((size_t)(sa.tok_base + tok) * a.q_heads + tile.kvh * a.group + row % a.group, c, sum);
             }
         }
-        // (the next item's meeting comes before these join rows are written again)
+        // (the next item's meeting comes before these join rows, or parts_of, are written again)
     }
 }
 
