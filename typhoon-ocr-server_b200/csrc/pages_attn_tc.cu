@@ -210,16 +210,65 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
 
-    int seq = -1, tok0 = 0, ntok = 0, pos0 = -1;
+    int tok0 = 0, ntok = 0;
     if (ta.shared_pass) {
         tok0 = (int)blockIdx.x * per;
         ntok = min(per, a.batch - tok0);
-        seq = a.seqs[0];
-        pos0 = min(a.prefix, checked_len(a.p, seq, a.st)) - 1;
     } else if (found[0] >= 0) {
-        seq = a.seqs[found[0]];
         tok0 = found[1];
         ntok = found[2];
+    }
+    // ---- queries, BF16, into the swizzled layout: a warp per 32 rows, D / 8 lanes a row
+    // (rows that are not there repeat the last token's: nobody takes their results).  All of a warp's loads are in
+    // flight at once.
+    if (warp < 8 && ntok > 0 && (!ta.tall || warp < 4)) {
+        const int h = warp >> 2;
+        constexpr int kLanes = D / 8, kAtOnce = 32 / kLanes, kLoads = 32 / kAtOnce;
+        unsigned char* tile = sQ + h * S::kTileQ;
+        const int c = lane % kLanes * 8;
+        size_t off[kLoads];
+        // row 32 (warp & 3) + lane / kLanes, then kAtOnce further each time; in flat rows twice that when wide
+        const int row0 = 32 * (warp & 3) + lane / kLanes, flat0 = ta.tall ? row0 : 2 * row0 + h, ahead = ta.tall ? kAtOnce : 2 * kAtOnce;
+        int tk = flat0 / a.group, hh = flat0 - tk * a.group;
+        const int tk_ahead = ahead / a.group, hh_ahead = ahead - tk_ahead * a.group;
+#pragma unroll
+        for (int i = 0; i < kLoads; i++) {
+            off[i] = (size_t)(tok0 + min(tk, ntok - 1)) * a.q_stride + (size_t)(kvh * a.group + hh) * D + c;
+            tk += tk_ahead;
+            hh += hh_ahead;
+            if (hh >= a.group) {
+                hh -= a.group;
+                tk++;
+            }
+        }
+        uint4 x[kLoads];
+        if (a.io_bf16) {
+#pragma unroll
+            for (int i = 0; i < kLoads; i++) x[i] = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) + off[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kLoads; i++) {
+                float f[8];
+                load8(static_cast<const float*>(a.q) + off[i], f);
+                x[i] = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kLoads; i++)
+            *reinterpret_cast<uint4*>(tile + sw128_offset(row0 + i * kAtOnce, c)) = x[i];
+    }
+    if (warp < 8) {
+        fence_proxy_async_smem();
+        warp_arrive(q_full);
+    }
+
+    // (after the queries' loads are out: the length is two loads deep)
+    int seq = -1, pos0 = -1;
+    if (ta.shared_pass) {
+        seq = a.seqs[0];
+        pos0 = min(a.prefix, checked_len(a.p, seq, a.st)) - 1;
+    } else if (ntok > 0) {
+        seq = a.seqs[found[0]];
         pos0 = checked_len(a.p, seq, a.st) + found[3];
         if (pos0 < 0 && tid == 0) raise(a.st, TYB_STATUS_BAD_ARGUMENT);  // more queries than tokens
     }
@@ -396,47 +445,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         // Row r of stream h is flat row 2 r + h of the item (r when tall), token-major: both streams reach
         // over the same tokens.
         const int h = warp >> 2, r = 32 * (warp & 3) + lane;
-        // ---- queries, BF16, into the swizzled layout: a warp per 32 rows, D / 8 lanes a row
-        // (rows that are not there repeat the last token's: nobody takes their results).  All of a warp's loads are in
-        // flight at once.
-        if (ntok > 0 && (!ta.tall || h == 0)) {
-            constexpr int kLanes = D / 8, kAtOnce = 32 / kLanes, kLoads = 32 / kAtOnce;
-            unsigned char* tile = sQ + h * S::kTileQ;
-            const int c = lane % kLanes * 8;
-            size_t off[kLoads];
-            // row 32 (warp & 3) + lane / kLanes, then kAtOnce further each time; in flat rows twice that when wide
-            const int row0 = 32 * (warp & 3) + lane / kLanes, flat0 = ta.tall ? row0 : 2 * row0 + h, ahead = ta.tall ? kAtOnce : 2 * kAtOnce;
-            int tk = flat0 / a.group, hh = flat0 - tk * a.group;
-            const int tk_ahead = ahead / a.group, hh_ahead = ahead - tk_ahead * a.group;
-#pragma unroll
-            for (int i = 0; i < kLoads; i++) {
-                off[i] = (size_t)(tok0 + min(tk, ntok - 1)) * a.q_stride + (size_t)(kvh * a.group + hh) * D + c;
-                tk += tk_ahead;
-                hh += hh_ahead;
-                if (hh >= a.group) {
-                    hh -= a.group;
-                    tk++;
-                }
-            }
-            uint4 x[kLoads];
-            if (a.io_bf16) {
-#pragma unroll
-                for (int i = 0; i < kLoads; i++) x[i] = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) + off[i]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < kLoads; i++) {
-                    float f[8];
-                    load8(static_cast<const float*>(a.q) + off[i], f);
-                    x[i] = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < kLoads; i++)
-                *reinterpret_cast<uint4*>(tile + sw128_offset(row0 + i * kAtOnce, c)) = x[i];
-        }
-        fence_proxy_async_smem();
-        warp_arrive(q_full);
-
         // ---- softmax: a row per thread
         const int flat = ta.tall ? r : 2 * r + h;
         const int tk = flat / a.group, hh = flat - tk * a.group;
