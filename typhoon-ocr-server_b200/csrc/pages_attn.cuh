@@ -56,6 +56,11 @@ __device__ __forceinline__ bool warp_wait_for(uint64_t* bar, uint32_t parity, ui
     return !__any_sync(0xffffffffu, !wait_for(bar, parity, limit_ns, s));
 }
 
+// The limit of the waits for a kernel's own copies and products in flight, at its end: a CTA whose other waits ran
+// out (whatever the limit set for those) must not leave before them.
+constexpr uint64_t kDrainNs = 500000000ull;
+__device__ __forceinline__ uint64_t drain_ns(uint64_t limit_ns) { return limit_ns > kDrainNs ? limit_ns : kDrainNs; }
+
 // One arrival for the warp, after all its lanes have come here.
 __device__ __forceinline__ void warp_arrive(uint64_t* bar)
 {

@@ -287,7 +287,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // has rows that none sees.
     auto edge = [&](int k0) { return k0 + kKeys - 1 > pos0 || (k0 < lo_max && k0 + kKeys > sinks); };
     auto loose = [&](int k0) { return k0 + kKeys - 1 > pos_max || (k0 < lo_min && k0 + kKeys > sinks); };
-    auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_for(bar, parity & 1u, ta.wait_ns, a.st); };
+    auto warp_drain = [&](uint64_t* bar, uint32_t parity) { return warp_wait_for(bar, parity & 1u, drain_ns(ta.wait_ns), a.st); };
     auto warp_wait = [&](uint64_t* bar, uint32_t parity) { return warp_wait_for(bar, parity & 1u, ta.wait_ns, a.st); };
 
     if (warp >= 8) {
@@ -345,10 +345,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     phase ^= 1u;
                 }
             }
-            if (!ok) {  // a wait ran out: the copies requested still land in this CTA
-                for (int t = max(0, k_sent - kStages); t < k_sent; t++) warp_wait(&k_full[t % kStages], (uint32_t)(t / kStages));
-                for (int t = max(0, v_sent - kStages); t < v_sent; t++) warp_wait(&v_full[t % kStages], (uint32_t)(t / kStages));
-            }
+            // The copies requested have landed before this warp, and with it the CTA, ends.
+            for (int t = max(0, k_sent - kStages); t < k_sent; t++) warp_drain(&k_full[t % kStages], (uint32_t)(t / kStages));
+            for (int t = max(0, v_sent - kStages); t < v_sent; t++) warp_drain(&v_full[t % kStages], (uint32_t)(t / kStages));
         } else if (warp == 8) {
             // ---- S = Q . K^T: a stream's next one goes out as soon as its S has been read
             const uint64_t dq = umma_desc(smem_u32(sQ), 16), dk = umma_desc(smem_u32(sK), 16);
@@ -377,11 +376,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     phase ^= 1u;
                 }
             }
-            if (!ok) {  // the products issued end before TMEM is given back
-                if (elect_one()) tc_commit(&drain[0]);
-                __syncwarp();
-                warp_wait(&drain[0], 0);
-            }
+            // The products issued have ended before this warp does, and TMEM is given back.
+            if (elect_one()) tc_commit(&drain[0]);
+            __syncwarp();
+            warp_drain(&drain[0], 0);
         } else if (warp == 11) {
             // ---- O += P . V, from a warp of its own: one warp's waits and issue for both took longer than the products
             const uint64_t dv = umma_desc(smem_u32(sV), kBox);
@@ -410,11 +408,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     phase ^= 1u;
                 }
             }
-            if (!ok) {
-                if (elect_one()) tc_commit(&drain[1]);
-                __syncwarp();
-                warp_wait(&drain[1], 0);
-            }
+            if (elect_one()) tc_commit(&drain[1]);
+            __syncwarp();
+            warp_drain(&drain[1], 0);
         } else if (warp == 10) {
             // ---- V rows that no row of the item sees.  Every tile passes here, so that this warp and the MMAs
             // stay within one phase of each other.

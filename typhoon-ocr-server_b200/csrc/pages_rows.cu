@@ -108,8 +108,8 @@ __global__ void __launch_bounds__(kRowThreads, 2) pages_rows_kernel(const __grid
                 phase ^= 1u;
             }
         }
-        if (!ok)  // a wait ran out: the copies requested still land in this CTA
-            for (int n = max(0, t - stages); n < t; n++) warp_wait_for(&full[n % stages], (uint32_t)(n / stages) & 1u, wait_ns, a.st);
+        // The copies requested have landed before this warp, and with it the CTA, ends.
+        for (int n = max(0, t - stages); n < t; n++) warp_wait_for(&full[n % stages], (uint32_t)(n / stages) & 1u, drain_ns(wait_ns), a.st);
         return;
     }
 

@@ -349,11 +349,10 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
             more = !tile.end;
             if (more) next();
         }
-        if (!ok) {  // a wait ran out: the copies requested still land in this CTA
-            const unsigned int stages = sa.stages;
-            for (unsigned int n = sent > stages ? sent - stages : 0; n < sent; n++)
-                warp_wait_for(&full[n % stages], n / stages & 1u, sa.wait_ns, a.st);
-        }
+        // The copies requested have landed before this warp, and with it the CTA, ends.
+        const unsigned int all_stages = sa.stages;
+        for (unsigned int n = sent > all_stages ? sent - all_stages : 0; n < sent; n++)
+            warp_wait_for(&full[n % all_stages], n / all_stages & 1u, drain_ns(sa.wait_ns), a.st);
         return;
     }
 
