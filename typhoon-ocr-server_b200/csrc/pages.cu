@@ -268,7 +268,8 @@ __global__ void __launch_bounds__(kPlanThreads)
 }
 
 // A block of `bytes` consecutive bytes (a multiple of 16, up to 64 KB) by one warp, eight 16-byte accesses a lane
-// requested at a time.
+// requested at a time.  kAgain: other blocks are copied from the same bytes, which had better stay in L2.
+template <bool kAgain>
 __device__ __forceinline__ void copy_block(char* to, const char* from, int bytes, int lane)
 {
     const uint4* f = reinterpret_cast<const uint4*>(from);
@@ -278,26 +279,30 @@ __device__ __forceinline__ void copy_block(char* to, const char* from, int bytes
         uint4 x[8];
 #pragma unroll
         for (int j = 0; j < 8; j++)
-            if (i + j * 32 < n) x[j] = __ldcs(f + i + j * 32);
+            if (i + j * 32 < n) x[j] = kAgain ? __ldg(f + i + j * 32) : __ldcs(f + i + j * 32);
 #pragma unroll
         for (int j = 0; j < 8; j++)
             if (i + j * 32 < n) __stcs(t + i + j * 32, x[j]);
     }
 }
 
-// The rows of a plan's moves: a (move, layer, tensor, head) block per warp and turn, neighbouring warps
-// neighbouring heads.  (A block per CTA and turn left two accesses a thread in flight: 113 us for 350 MB.)
+// The rows of a plan's moves: a (move, layer, tensor, head) block per warp and turn.  Neighbouring warps have
+// neighbouring heads of a page; with kAgain (branches: several moves from one page) neighbouring moves of a head, so
+// that the page's rows are read from memory once.  (A block per CTA and turn left two accesses a thread in flight:
+// 113 us for 350 MB.  The rows read as if for the only time, page by page: 88 us.)
+template <bool kAgain>
 __device__ void copy_rows(const KVPages& p, const Plan& plan, int row_bytes)
 {
     const int lane = threadIdx.x & 31;
     const unsigned int lt = p.num_layers * 2, per_move = lt * p.kv_heads;  // no pool has 2^32 blocks: it has fewer rows
-    const unsigned int units = (unsigned int)plan.head->moves * per_move, warps = gridDim.x * (kApplyThreads / 32);
+    const unsigned int moves = plan.head->moves, units = moves * per_move, warps = gridDim.x * (kApplyThreads / 32);
     const size_t block = (size_t)p.page_size * row_bytes;
     for (unsigned int u = blockIdx.x * (kApplyThreads / 32) + (threadIdx.x >> 5); u < units; u += warps) {
-        const unsigned int move = u / per_move, in_move = u - move * per_move, q = in_move / p.kv_heads, h = in_move - q * p.kv_heads;
+        const unsigned int major = u / (kAgain ? moves : per_move), minor = u - major * (kAgain ? moves : per_move);
+        const unsigned int move = kAgain ? minor : major, in_move = kAgain ? major : minor, q = in_move / p.kv_heads, h = in_move - q * p.kv_heads;
         const Move m = plan.moves[move];
         char* slab = static_cast<char*>((q & 1) ? p.v : p.k) + ((size_t)(q >> 1) * p.num_pages * p.kv_heads + h) * block;
-        copy_block(slab + (size_t)m.to * p.kv_heads * block, slab + (size_t)m.from * p.kv_heads * block, m.rows * row_bytes, lane);
+        copy_block<kAgain>(slab + (size_t)m.to * p.kv_heads * block, slab + (size_t)m.from * p.kv_heads * block, m.rows * row_bytes, lane);
     }
 }
 
@@ -332,7 +337,7 @@ __global__ void __launch_bounds__(kApplyThreads)
         }
         if (lane == 0) p.len[d] = len;
     }
-    copy_rows(p, plan, row_bytes);
+    copy_rows<true>(p, plan, row_bytes);
 }
 
 // ---- free and trim -----------------------------------------------------------------------------
@@ -402,7 +407,7 @@ __global__ void __launch_bounds__(kApplyThreads) pages_compact_apply_kernel(cons
         const int page = p.table[i];
         if (page >= live && page < p.num_pages) p.table[i] = plan.fresh[page];
     }
-    copy_rows(p, plan, row_bytes);
+    copy_rows<false>(p, plan, row_bytes);
 }
 
 // ---- rows --------------------------------------------------------------------------------------
@@ -469,7 +474,7 @@ __global__ void __launch_bounds__(kApplyThreads)
         const int page = p.table[(size_t)seq * p.max_pages + e];
         const char* from = ((q & 1) ? v_slab : k_slab) + (((size_t)(q >> 1) * p.kv_heads + h) * row_capacity + (size_t)e * p.page_size) * row_bytes;
         char* to = static_cast<char*>((q & 1) ? p.v : p.k) + (((size_t)(q >> 1) * p.num_pages + page) * p.kv_heads + h) * block;
-        copy_block(to, from, min(p.page_size, rows - (int)e * p.page_size) * row_bytes, lane);
+        copy_block<false>(to, from, min(p.page_size, rows - (int)e * p.page_size) * row_bytes, lane);
     }
 }
 
