@@ -55,10 +55,39 @@ struct Layout {
     bool shared;  // the streaming form takes the shared prefix along
     bool tc, tall;
     int row_tiles, splits, slots;
+    int beside;   // SMs of a shared pass that the own rows run beside; 0: after it
 };
 
 // Query rows of a KV head from which the shared prefix runs on the tcgen05 form.
 constexpr int kTcSharedRows = 65;
+
+// A shared pass on the tensor cores and the streaming of the sequences' own rows are bound by different things: they
+// run at the same time where that is estimated to be shorter.  In microseconds: a split of the pass its tiles; the
+// own rows (taken to be half of what max_len allows) what a CTA needs for a stage (an item's start and end take as
+// long as kItemUnits of them), or what the memory can deliver; each of the two 10 for its start and end.  That met what
+// was measured within a tenth, in turn / at the same time: 256 sequences behind 4,096 shared rows with up to 512
+// own ones 94 / 79, with up to 64 own ones 55 / 46, behind 1,024 85 / 68; 64 behind 4,096 60 / 36; 512 behind 2,048 with up
+// to 128 91 / 84 (and 101 with twice the SMs for the pass).
+static void share_sms(const tyb_pages_attn* c, int tiles, int ctas, Layout* l)
+{
+    const double tile_us = l->tall ? 0.7 : 1.25, unit_us = 1.15, fixed_us = 10.0, memory = 6.4e6;
+    const double rows = 0.5 * (c->max_len - c->prefix), items = (double)c->batch * c->p.kv_heads;
+    const double bytes = rows * items * c->p.head_dim * 4.0, units = items * (kItemUnits + 0.5 + rows / 64);  // K and V in BF16
+    auto pass_us = [&](int splits) { return fixed_us + (tiles + splits - 1) / splits * tile_us; };
+    auto own_us = [&](int sms) {
+        const double busy = units / (2 * sms) * unit_us, read = bytes / memory;
+        return fixed_us + (busy > read ? busy : read);
+    };
+    double best = pass_us(l->splits) + own_us(kSms);
+    for (int s = 1; s <= tiles / 4 && s * ctas <= kSms / 2; s++) {
+        const double us = pass_us(s) > own_us(kSms - s * ctas) ? pass_us(s) : own_us(kSms - s * ctas);
+        if (us < best) {
+            best = us;
+            l->splits = s;
+            l->beside = s * ctas;
+        }
+    }
+}
 
 static Layout layout_of(const tyb_pages_attn* c)
 {
@@ -86,6 +115,7 @@ static Layout layout_of(const tyb_pages_attn* c)
         if (l.splits > tiles / 2) l.splits = tiles / 2;
     }
     if (l.splits < 1) l.splits = 1;
+    if (l.tokens) share_sms(c, tiles, (int)ctas, &l);
     l.slots = l.splits * (l.tall ? 2 : 1) + l.tokens;  // the last one of a shared pass's call: the own rows
     return l;
 }
@@ -159,7 +189,7 @@ extern "C" int tyb_pages_attn_launch(const tyb_pages_attn* c, void* ws, void* ti
     if (l.tokens) {
         for (int first = 0; first < c->batch; first += kStreamSeqs) {
             const int count = c->batch - first < kStreamSeqs ? c->batch - first : kStreamSeqs;
-            const int e = launch_stream(a, c->layer, first, count, l.shared, l.tiles ? l.slots - 1 : -1, c->max_len, c->maps, more,
+            const int e = launch_stream(a, c->layer, first, count, l.shared, l.tiles ? l.slots - 1 : -1, first ? 0 : l.beside, c->max_len, c->maps, more,
                                         static_cast<unsigned int*>(tickets), st);
             if (e) return e;
         }

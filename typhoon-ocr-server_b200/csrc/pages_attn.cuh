@@ -27,6 +27,11 @@ __device__ __forceinline__ void after_predecessor()
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
+// The two halves apart, for a kernel that runs beside its predecessor (which has itself waited, before it let this
+// one start, for all that came before).
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_predecessor() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 template <typename... P, typename... A>
 int launch_after(void (*kernel)(P...), dim3 grid, int threads, size_t shared, cudaStream_t stream, A... args)
 {
@@ -184,11 +189,17 @@ __device__ __forceinline__ void find_item(const AttnArgs& a, int x, int per, int
 
 // The streaming form (pages_stream.cu): the single tokens of sequences first .. first + count (at most
 // kStreamSeqs) of the call, with the shared pass over a.prefix rows in the same launch (`shared`); the
-// results are the output, or (out_slot >= 0) record slot out_slot of a.rec.  ws: stream_bytes; tickets: count * kv_heads words, zero (and left
-// so).
+// results are the output, or (out_slot >= 0) record slot out_slot of a.rec.  beside: 0, or the SMs that the
+// shared pass launched just before keeps busy: the launch then runs on the others at the same time, and waits for the
+// pass (which has waited for all before it) only at its end.  ws: stream_bytes; tickets: count * kv_heads words,
+// zero (and left so).
 constexpr int kStreamSeqs = 1024;
+// An item's start and end (its query, the join of the warps) cost a CTA about as much as this many stages:
+// runs are cut by stages plus this for each item.  Measured with 256 sequences of 1 .. 512 rows (4.6 stages on
+// average): 61 us against 84 us of runs with equal stages, whose run of one-stage items took twice the others.
+constexpr int kItemUnits = 2;
 size_t stream_bytes(const AttnArgs& a, int count, bool shared);
-int launch_stream(const AttnArgs& a, int layer, int first, int count, bool shared, int out_slot, int max_len, const void* maps, void* ws,
+int launch_stream(const AttnArgs& a, int layer, int first, int count, bool shared, int out_slot, int beside, int max_len, const void* maps, void* ws,
                   unsigned int* tickets, cudaStream_t stream);
 
 constexpr int kSms = 148;
@@ -208,6 +219,15 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const void* map, int c0, 
     asm volatile(
         "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(dst)),
         "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(smem_u32(bar))
+        : "memory");
+}
+
+// Rows from c1 of its column boxes from c2.
+__device__ __forceinline__ void tma_load_3d(void* dst, const void* map, int c1, int c2, uint64_t* bar)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(c1), "r"(c2), "r"(smem_u32(bar))
         : "memory");
 }
 

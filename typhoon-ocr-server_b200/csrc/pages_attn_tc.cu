@@ -655,18 +655,18 @@ extern "C" int tyb_pages_maps(const KVPages* p, void* maps)
             return (int)cudaErrorNotSupported;
         fn = reinterpret_cast<EncodeTiledFn>(f);
     }
-    // Every row of every layer, page and head as a 2-D tensor; a box is 128 bytes of a page's rows.
+    // Every row of every layer, page and head.  K, V: as a 2-D tensor, a box is 128 bytes of a page's rows (at most a
+    // stage's).  For the streaming form as a 3-D one, columns in a box by rows by column boxes: K, V with boxes of those
+    // rows, all their columns where they fill a stage; K, V with boxes of 16 rows by 128 bytes.
     const bool bf16 = p->kv_dtype == TYB_BF16;
-    const cuuint64_t dims[2] = {(cuuint64_t)p->head_dim, (cuuint64_t)p->num_layers * p->num_pages * p->kv_heads * p->page_size};
-    const cuuint64_t strides[1] = {(cuuint64_t)p->head_dim * (bf16 ? 2 : 4)};
-    const cuuint32_t box[2] = {bf16 ? 64u : 32u, (cuuint32_t)box_rows(*p)};
-    const cuuint32_t estr[2] = {1, 1};
-    for (int i = 0; i < 4; i++) {  // K, V; then in boxes of 16 rows
-        const cuuint32_t b[2] = {box[0], i < 2 ? box[1] : 16u};
-        if (fn(static_cast<CUtensorMap*>(maps) + i, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2,
-               i & 1 ? p->v : p->k, dims, strides, b, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+    const cuuint32_t cols = bf16 ? 64 : 32, boxes = (cuuint32_t)p->head_dim / cols, rows = (cuuint32_t)box_rows(*p);
+    const cuuint64_t all = (cuuint64_t)p->num_layers * p->num_pages * p->kv_heads * p->page_size, pitch = (cuuint64_t)p->head_dim * (bf16 ? 2 : 4);
+    const cuuint64_t dims2[2] = {(cuuint64_t)p->head_dim, all}, dims3[3] = {cols, all, boxes}, strides[2] = {pitch, 128};
+    const cuuint32_t estr[3] = {1, 1, 1}, box[3][3] = {{cols, rows, 1}, {cols, rows, rows == (bf16 ? 64u : 32u) ? boxes : 1u}, {cols, 16, 1}};
+    for (int i = 0; i < 6; i++)
+        if (fn(static_cast<CUtensorMap*>(maps) + i, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, i < 2 ? 2 : 3,
+               i & 1 ? p->v : p->k, i < 2 ? dims2 : dims3, strides, box[i / 2], estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
             return (int)cudaErrorInvalidValue;
-    }
     return 0;
 }

@@ -42,9 +42,8 @@ int tyb_pages_import_launch(const KVPages *p, const tyb_pages_env *env, int seq,
                             int rows, void *ws, void *stream);
 
 /* ---- attention ---------------------------------------------------------------------------- */
-/* TMA tensor maps of a pool's K and V (64-byte aligned room), built once per handle: 128 bytes of a row by a
- * page's rows (at most a stage's), and by 16 rows. */
-#define TYB_PAGES_MAPS_BYTES 512
+/* TMA tensor maps of a pool's K and V (64-byte aligned room), built once per handle. */
+#define TYB_PAGES_MAPS_BYTES (6 * 128)
 int tyb_pages_maps(const KVPages *p, void *maps);
 
 typedef struct {

@@ -8,12 +8,16 @@
 // are cut into gridDim.x equal runs.  One warp requests a run's tiles with TMA into a ring of stages,
 // crossing from item to item without a pause (item starts bring their query rows along).  Two teams of
 // two warps take the stages in turn, a warp 32 (BF16) or 16 (FP32) of its rows, with the running maximum
-// and sum of an online softmax in base 2; at the item's end the four are joined through shared memory,
-// while the SM's other CTA streams on.  (A stage is a chain of dependent steps, about a microsecond:
-// few keys per warp make it no shorter, so four of them at a time per SM keep up with the memory, two do not.)
-// An item that a run boundary cuts
-// is joined by the CTA that finishes it last (records in the workspace, a ticket per item); the order
-// of that sum is by run, not by arrival, so results repeat exactly.
+// and sum of an online softmax in base 2; at an item's end each leaves its rows in shared memory and goes on, and
+// the last to do so joins the four.  (A stage is a chain of dependent steps, about a microsecond: few keys per
+// warp make it no shorter, so four of them at a time per SM keep up with the memory, two do not.)
+// An item that a run boundary cuts is joined by the CTA that finishes it last (records in the workspace, a
+// ticket per item); the order of that sum is by run, not by arrival, so results repeat exactly.
+//
+// Long items: 512 windows of 2,048 rows and 16 sinks in 611 us, 4.2 GB at the rate of a copy.  Short ones are bound by
+// the stage's round trip (request, arrival, two warps' products, release) over a ring of three: 1.15 us a stage,
+// 256 x 8 items of 4.6 stages in 66 us on 116 SMs.  That was 97 us while the requesting warp divided by variables and
+// sent a copy per column box.
 //
 // The products (pages_mma.cuh) are mma.sync, with up to 16 query rows as columns.
 #define TYB_WHOLE_PROGRAM
@@ -28,11 +32,8 @@ constexpr int kTakers = 2 * kTeam;               // warps that consume stages: t
 constexpr int kTakerThreads = 32 * kTakers;
 constexpr int kStreamThreads = kTakerThreads + 32;  // + the requesting warp
 constexpr int kMaxStages = 10;
+constexpr int kItemRing = 16;                    // > kMaxStages: a taker reads of an item while that many stages follow
 constexpr int kStreamRuns = 2 * kSms;            // CTAs, at most
-// An item's start and end (its query, the join of the warps) cost a CTA about as much as this many stages:
-// runs are cut by stages plus this for each item.  Measured with 256 sequences of 1 .. 512 rows (4.6 stages on
-// average): 61 us against 84 us of runs with equal stages, whose run of one-stage items took twice the others.
-constexpr int kItemUnits = 2;
 
 template <typename T, int D>
 struct Stream {
@@ -46,17 +47,21 @@ struct Stream {
     static constexpr int kPitch = D + 4;                    // floats; joins and FP32 queries
 };
 
-// What the requesting warp tells the takers about a stage.
-struct Tile {
-    int first, last;  // of its item (in this run)
-    int end;          // of the run
-    int k0;           // key of the stage's first row
-    unsigned int seen;  // a bit per 8 rows: the page is there
-    int shared;       // an item of the shared pass
+// What the requesting warp tells the takers: about an item,
+struct Item {
+    int shared;       // of the shared pass
     int tok0, ntok, kvh;
     int pos, lo, sinks;
-    int c0, c1, s0;   // the runs that have part of the item, and which record of run c0 is its
+    int c0, c1, s0;   // the runs that have part of it, and which record of run c0 is its
 };
+// about a stage: its first row's key, a bit per 8 rows whose page is there, and
+struct __align__(16) Stage {
+    int k0;
+    unsigned int seen;
+    int flags;
+    int more;
+};
+constexpr int kFirst = 1, kLast = 2, kEnd = 4;  // of its item (in this run), of its item, of the run
 
 // Where the records of a (token, KV head) lie: in runs sh0 .. sh1 those of its shared item (none: sh1 < sh0), in runs
 // own0 .. own1 its own; *_second: whether that of the first such run is the run's second record.
@@ -65,7 +70,7 @@ struct Parts {
 };
 
 struct Maps {
-    CUtensorMap m[4];  // K, V; K, V in boxes of 16 rows
+    CUtensorMap m[4];  // K, V; K, V in boxes of 16 rows by 128 bytes
 };
 
 struct StreamArgs {
@@ -75,8 +80,9 @@ struct StreamArgs {
     int shared_tiles;  // row tiles of the shared pass in this launch (0: none)
     int shared_units;  // units of each: kItemUnits and the stages of its rows
     int out_slot;      // record slot of a.rec that receives the results; -1: they are the output
+    int beside;        // runs at the same time as the kernel before
     int max_len;
-    int stages, q_bytes, item_rows, buffers;
+    int stages, q_bytes, item_rows;
     // Records of this launch: [2 * kStreamRuns][16] rows of items cut by a run boundary; with a shared pass, uncut
     // items too: [batch * q_heads] own rows, then [shared_tiles * kv_heads][16] shared ones.
     float* rec_o;
@@ -133,16 +139,18 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
     extern __shared__ __align__(1024) unsigned char raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     unsigned char* ring = smem;
-    float* joins = reinterpret_cast<float*>(ring + sa.stages * S::kStage);  // [buffers][kTakers][item_rows][kPitch]
-    float* split_q = joins + sa.buffers * kTakers * sa.item_rows * S::kPitch;  // FP32: hi and lo, [split_rows][kPitch] each
+    float* joins = reinterpret_cast<float*>(ring + sa.stages * S::kStage);  // [kTakers][item_rows][kPitch]
+    float* split_q = joins + kTakers * sa.item_rows * S::kPitch;  // FP32: hi and lo, [split_rows][kPitch] each
     constexpr int split_rows = sizeof(T) == 4 && !kDup ? 8 * kBlocks : 0;
     unsigned char* qs = reinterpret_cast<unsigned char*>(split_q + 2 * split_rows * S::kPitch);  // [stages][q_bytes]
     int* cum = reinterpret_cast<int*>(qs + sa.stages * sa.q_bytes);        // units before each sequence
     int* lens = cum + a.batch + 1;
 
-    __shared__ uint64_t full[kMaxStages], empty[kMaxStages], met;
-    __shared__ Tile tiles_of_stage[kMaxStages];
-    __shared__ float2 join_mls[kTakers][16];  // (two buffers: of four rows each)
+    __shared__ uint64_t full[kMaxStages], empty[kMaxStages], met, joined;
+    __shared__ int left_rows;  // warps whose rows of the item lie in the join rows
+    __shared__ Stage stages_of[kMaxStages];
+    __shared__ Item items[kItemRing];
+    __shared__ float2 join_mls[kTakers][16];
     __shared__ int scan[kStreamThreads / 32];
     __shared__ unsigned int last_of;  // tokens whose join is this CTA's
     __shared__ Parts parts_of[16];    // and where their records lie
@@ -156,9 +164,16 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
             mbar_init(&empty[i], kTakers);
         }
         mbar_init(&met, kTakers);
+        mbar_init(&joined, 1);
+        left_rows = 0;
         fence_barrier_init();
     }
-    after_predecessor();
+    if (sa.beside) {
+        let_next_start();
+        __threadfence();  // nothing read before by this SM is taken for the page table's or the lengths' state
+    } else {
+        after_predecessor();
+    }
     // Units of each sequence's own rows: kItemUnits, then its stages, of which it has one at least, so that every
     // output row has an owner.
     auto own_lo = [&](int len) { return a.window ? max(0, len - a.window) : min(a.prefix, len); };
@@ -220,37 +235,54 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
 
     if (warp == kTakers) {
         // ---- requests
-        // Lane (part, box, K or V): a stage's rows come in 1, 2 or 4 parts (pages, or one part of a page; 16 rows each
-        // where not all of a stage is in sight, so that no more is read than that), each 128-byte column box of
-        // each as one copy.
-        const int shift = page_shift(a.p.page_size);
-        int part_rows = 0, parts = 1, part = 0, box = 0, which = 2;
+        // Lane (part, box, K or V): a stage's rows come as one copy of whole rows, or in 2 or 4 parts (pages; 16 rows
+        // each where not all of the stage is in sight, so that no more is read than that), each 128-byte column box
+        // of each as a copy.
+        const int shift = page_shift(a.p.page_size), whole = max(0, page_shift(S::kRows) - shift);
+        struct Lane {
+            int parts, rows, part, box, which, to;
+            uint32_t bytes;
+        };
+        auto lane_of = [&](int parts_log2, bool all_boxes) {
+            Lane l;
+            const int other = lane >> parts_log2;  // lane / parts
+            l.parts = 1 << parts_log2;
+            l.rows = S::kRows >> parts_log2;
+            l.part = lane & (l.parts - 1);
+            l.box = all_boxes ? 0 : other % S::kBoxes;
+            l.which = all_boxes ? other : other / S::kBoxes;
+            l.to = l.which * S::kHalf + l.box * S::kBox + l.part * l.rows * 128;
+            l.bytes = (uint32_t)(l.rows * 128 * (all_boxes ? S::kBoxes : 1));
+            return l;
+        };
+        const Lane coarse = lane_of(whole, whole == 0), finer = lane_of(page_shift(S::kRows) - 4, false);
+        Lane mine = coarse;
         bool fine = false;
         const uint32_t q_row = (uint32_t)(a.group * D * (a.io_bf16 ? 2 : 4));
         const int max_page = a.p.num_pages;
-        Tile tile = {};
+        Item item = {};
         Tiles list = {};
         const int* table = a.p.table;
         unsigned int u = begin, u0 = 0, u1 = 0, sent = 0;  // u0, u1: the current item's units
-        int b = 0, st = 0, page = -1;
+        int b = 0, st = 0, page = -1, item_at = kItemRing - 1, k0 = 0, flags = 0;
         uint32_t phase = 0;
         bool ok = true, more = true;
         // The next stage: what it holds, and the lane's page of it (requested here, so that its way from memory
-        // passes while the stage before waits for its place).  tile.end: none follows.
+        // passes while the stage before waits for its place).  kEnd: none follows.
         auto next = [&]() {
-            tile.first = u == begin || u >= u1;
-            if (tile.first) {  // the item that unit u lies in
+            const bool first = u == begin || u >= u1;
+            if (first) {  // the item that unit u lies in
                 if (u < shared_all) {
-                    const unsigned int item = u / sa.shared_units;
-                    u0 = item * sa.shared_units;
+                    const unsigned int n = u / sa.shared_units;
+                    u0 = n * sa.shared_units;
                     u1 = u0 + sa.shared_units;
-                    tile.shared = 1;
-                    tile.kvh = (int)(item % heads);
-                    tile.tok0 = (int)(item / heads) * per;
-                    tile.ntok = min(per, a.batch - tile.tok0);
-                    tile.sinks = 0;
-                    tile.lo = 0;
-                    tile.pos = min(a.prefix, lens[0]) - 1;
+                    item.shared = 1;
+                    item.kvh = (int)(n % heads);
+                    item.tok0 = (int)(n / heads) * per;
+                    item.ntok = min(per, a.batch - item.tok0);
+                    item.sinks = 0;
+                    item.lo = 0;
+                    item.pos = min(a.prefix, lens[0]) - 1;
                     table = a.p.table + (size_t)(lens[0] ? a.seqs[0] : 0) * a.p.max_pages;
                 } else {
                     bool other = true;
@@ -265,50 +297,45 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
                     } else if (u - shared_all >= (unsigned int)(cum[b + 1] * heads)) {
                         b++;
                     } else {
-                        other = tile.shared;
+                        other = item.shared;
                     }
                     const unsigned int units = cum[b + 1] - cum[b];
                     if (u == begin) {
                         const unsigned int at = u - shared_all - cum[b] * heads;
-                        tile.kvh = (int)(at / units);
+                        item.kvh = (int)(at / units);
                         u0 = u - at % units;
                     } else {
-                        tile.kvh = other ? 0 : tile.kvh + 1;
+                        item.kvh = other ? 0 : item.kvh + 1;
                         u0 = u;
                     }
                     u1 = u0 + units;
                     if (other) {
-                        tile.shared = 0;
-                        tile.tok0 = b;
-                        tile.ntok = 1;
-                        tile.sinks = a.sinks;
-                        tile.pos = lens[b] - 1;
-                        tile.lo = own_lo(lens[b]);
+                        item.shared = 0;
+                        item.tok0 = b;
+                        item.ntok = 1;
+                        item.sinks = a.sinks;
+                        item.pos = lens[b] - 1;
+                        item.lo = own_lo(lens[b]);
                         table = a.p.table + (size_t)(lens[b] ? a.seqs[b] : 0) * a.p.max_pages;
                     }
                 }
                 // items inside the run are whole: only its first and last may lie in others too
-                tile.c0 = tile.c1 = run;
-                tile.s0 = 0;
-                if (u == begin || u1 > end) cuts.span(u0, u1, tile.c0, tile.c1, tile.s0);
-                list = tiles_of(tile.pos, tile.lo, tile.sinks, S::kRows);
+                item.c0 = item.c1 = run;
+                item.s0 = 0;
+                if (u == begin || u1 > end) cuts.span(u0, u1, item.c0, item.c1, item.s0);
+                list = tiles_of(item.pos, item.lo, item.sinks, S::kRows);
                 if (u < u0 + kItemUnits) u = min(u0 + kItemUnits, end);
             }
             const bool none = u == end;  // the run ends before the item's first stage
-            tile.first = tile.first && !none;
-            tile.last = !none && (u + 1 == u1 || u + 1 == end);
-            tile.end = none || (u + 1 == u1 ? u1 + kItemUnits : u + 1) >= end;
+            flags = (none ? 0 : (first ? kFirst : 0) | (u + 1 == u1 || u + 1 == end ? kLast : 0)) |
+                    (none || (u + 1 == u1 ? u1 + kItemUnits : u + 1) >= end ? kEnd : 0);
             const int i = none ? list.count() : (int)(u - u0 - kItemUnits);
             const bool real = i < list.count();
-            tile.k0 = real ? list.at(i) * S::kRows : tile.pos + 1;
-            fine = tile.k0 + S::kRows - 1 > tile.pos || (tile.k0 < tile.lo && tile.k0 + S::kRows > tile.sinks);
-            part_rows = fine ? 16 : box_rows(a.p);
-            parts = S::kRows / part_rows;
-            part = lane & (parts - 1);
-            box = lane / parts & (S::kBoxes - 1);
-            which = lane / (parts * S::kBoxes);
-            const int key = tile.k0 + part * part_rows;
-            page = real && which < 2 && key <= tile.pos && (key + part_rows > tile.lo || key < tile.sinks) ? table[key >> shift] : -1;
+            k0 = real ? list.at(i) * S::kRows : item.pos + 1;
+            fine = k0 + S::kRows - 1 > item.pos || (k0 < item.lo && k0 + S::kRows > item.sinks);
+            mine = fine ? finer : coarse;
+            const int key = k0 + mine.part * mine.rows;
+            page = real && mine.which < 2 && key <= item.pos && (key + mine.rows > item.lo || key < item.sinks) ? table[key >> shift] : -1;
             u++;
         };
         next();
@@ -322,23 +349,25 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
                 page = -1;
             }
             const unsigned int have = __ballot_sync(0xffffffffu, page >= 0);
-            tile.seen = 0;
-            for (int l = 0; l < parts; l++)
-                if (have >> l & 1u) tile.seen |= ((1u << (part_rows / 8)) - 1u) << (l * (part_rows / 8));
+            if (flags & kFirst) {
+                if (++item_at == kItemRing) item_at = 0;
+                if (lane == 0) items[item_at] = item;
+            }
             if (lane == 0) {
-                tiles_of_stage[st] = tile;
-                mbar_arrive_expect_tx(&full[st], (uint32_t)(__popc(have) * part_rows * 128) + (tile.first ? q_row * (uint32_t)tile.ntok : 0u));
+                unsigned int seen = 0;
+                for (int l = 0; l < mine.parts; l++)
+                    if (have >> l & 1u) seen |= (0xffu >> (8 - mine.rows / 8)) << (l * (mine.rows / 8));
+                stages_of[st] = Stage{k0, seen, flags, 0};
+                mbar_arrive_expect_tx(&full[st], __popc(have) * mine.bytes + (flags & kFirst ? q_row * (uint32_t)item.ntok : 0u));
             }
             __syncwarp();
             if (page >= 0) {
-                const int row = ((sa.layer * a.p.num_pages + page) * heads + tile.kvh) * a.p.page_size +
-                                ((tile.k0 + part * part_rows) & (a.p.page_size - 1));
-                tma_load_2d(ring + st * S::kStage + which * S::kHalf + box * S::kBox + part * part_rows * 128, &maps.m[2 * fine + which],
-                            box * S::kBoxCols, row, &full[st]);
+                const int row = ((sa.layer * a.p.num_pages + page) * heads + item.kvh) * a.p.page_size + ((k0 + mine.part * mine.rows) & (a.p.page_size - 1));
+                tma_load_3d(ring + st * S::kStage + mine.to, &maps.m[2 * fine + mine.which], row, mine.box, &full[st]);
             }
-            if (tile.first && lane < tile.ntok)
+            if ((flags & kFirst) && lane < item.ntok)
                 bulk_g2s(qs + st * sa.q_bytes + lane * q_row,
-                         static_cast<const char*>(a.q) + ((size_t)(sa.tok_base + tile.tok0 + lane) * a.q_stride + (size_t)tile.kvh * a.group * D) *
+                         static_cast<const char*>(a.q) + ((size_t)(sa.tok_base + item.tok0 + lane) * a.q_stride + (size_t)item.kvh * a.group * D) *
                                                              (a.io_bf16 ? 2 : 4),
                          q_row, &full[st]);
             sent++;
@@ -346,13 +375,14 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
                 st = 0;
                 phase ^= 1u;
             }
-            more = !tile.end;
+            more = !(flags & kEnd);
             if (more) next();
         }
         // The copies requested have landed before this warp, and with it the CTA, ends.
         const unsigned int all_stages = sa.stages;
         for (unsigned int n = sent > all_stages ? sent - all_stages : 0; n < sent; n++)
             warp_wait_for(&full[n % all_stages], n / all_stages & 1u, drain_ns(sa.wait_ns), a.st);
+        if (sa.beside) wait_for_predecessor();  // so that the end of this kernel is the end of that one as well
         return;
     }
 
@@ -362,8 +392,9 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
     w.clear();
     int st = 0, turn = 0;  // turn: whose stage it is
     uint32_t phase = 0;
+    int item_at = kItemRing - 1;
     bool one_item = true;  // no item has ended in this run yet
-    int buffer = 0;        // of the join rows: two, used in turn
+    int direct_items = 0;
     // Rows of the records: of a cut item's part in a run, of uncut own rows, of an uncut shared item.
     auto part_row = [&](int run_of, int second) { return (2 * run_of + second) * 16; };
     auto own_row = [&](int tok, int kvh) { return 2 * kStreamRuns * 16 + tok * a.q_heads + kvh * a.group; };
@@ -391,26 +422,27 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
     };
     // Four columns of a row, joined over the warps' shares in shared memory.
     auto over_warps = [&](int row, int c) {
-        const float* join = joins + buffer * kTakers * sa.item_rows * S::kPitch;
         Gather sum;
 #pragma unroll
         for (int x = 0; x < kTakers; x++)
-            sum.add(join_mls[x][4 * buffer + row], *reinterpret_cast<const float4*>(join + (x * sa.item_rows + row) * S::kPitch + c));
+            sum.add(join_mls[x][row], *reinterpret_cast<const float4*>(joins + (x * sa.item_rows + row) * S::kPitch + c));
         return sum;
     };
     for (bool more = true; more;) {
         if (!warp_wait_for(&full[st], phase, sa.wait_ns, a.st)) return;
-        const Tile tile = tiles_of_stage[st];
+        const Stage stage = stages_of[st];
+        if ((stage.flags & kFirst) && ++item_at == kItemRing) item_at = 0;
+        const Item& tile = items[item_at];
         const int nrows = tile.ntok * a.group;
-        more = !tile.end;
-        if (tile.first) {
+        more = !(stage.flags & kEnd);
+        if (stage.flags & kFirst) {
             w.load_q(qs + st * sa.q_bytes, nrows, a.io_bf16, g, t, split_q, tid, kTakerThreads);
             if (split_rows && !meet()) return;
         }
-        const int j0 = tile.k0 + r0;
+        const int j0 = stage.k0 + r0;
         unsigned char* rows_k = ring + st * S::kStage;
         unsigned char* rows_v = rows_k + S::kHalf;
-        const unsigned int want = (1u << (S::kKeys / 8)) - 1u, seen = tile.seen >> (r0 / 8) & want;
+        const unsigned int want = (1u << (S::kKeys / 8)) - 1u, seen = stage.seen >> (r0 / 8) & want;
         // the other team's stage, or none of the warp's rows in sight: nothing to do
         const bool any = turn == team && seen && j0 <= tile.pos && (j0 + S::kKeys > tile.lo || j0 < tile.sinks);
         if (any) {
@@ -437,19 +469,42 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
             st = 0;
             phase ^= 1u;
         }
-        if (!tile.last) continue;
+        if (!(stage.flags & kLast)) continue;
+        const bool first_item = one_item;
+        one_item = false;
 
-        // ---- the item's end in this run: join the warps.  With two buffers the next item's join rows are the
-        // other one's, and these are written again only after all have met there; with one, they meet first.
-        if (sa.buffers == 2) buffer ^= 1;
-        else if (!meet()) return;
-        float* join = joins + buffer * kTakers * sa.item_rows * S::kPitch;
-        w.put(join + warp * sa.item_rows * S::kPitch, S::kPitch, &join_mls[warp][4 * buffer], nrows, g, t);
+        // ---- the item's end in this run: join the warps
+        const bool cut = tile.c0 != tile.c1, direct = !cut && !sa.shared_tiles;
+        if (direct && !split_rows) {
+            // An item to itself: each warp leaves its rows and goes on to the next item; the last to do so joins them.
+            if (direct_items > 0 && !warp_wait_for(&joined, (uint32_t)(direct_items - 1) & 1u, sa.wait_ns, a.st)) return;
+            direct_items++;
+            w.put(joins + warp * sa.item_rows * S::kPitch, S::kPitch, join_mls[warp], nrows, g, t);
+            w.clear();
+            __syncwarp();
+            int before_me = 0;
+            if (lane == 0) {
+                __threadfence_block();
+                before_me = atomicAdd(&left_rows, 1);
+                __threadfence_block();
+            }
+            before_me = __shfl_sync(0xffffffffu, before_me, 0);
+            __syncwarp();
+            if (before_me != kTakers - 1) continue;
+            if (lane == 0) left_rows = 0;
+            for (int i = lane; i < nrows * (D / 4); i += 32) {
+                const int row = i / (D / 4), c = i % (D / 4) * 4;
+                deliver((size_t)(sa.tok_base + tile.tok0) * a.q_heads + tile.kvh * a.group + row, c, over_warps(row, c));
+            }
+            warp_arrive(&joined);
+            continue;
+        }
+        // Others by all four together, once nobody needs the join rows.
+        if (!meet()) return;
+        w.put(joins + warp * sa.item_rows * S::kPitch, S::kPitch, join_mls[warp], nrows, g, t);
         w.clear();  // (and so not kept through what follows)
         if (!meet()) return;
-        const bool cut = tile.c0 != tile.c1, direct = !cut && !sa.shared_tiles;
-        const int record = cut ? part_row(run, one_item ? 0 : 1) : tile.shared ? shared_row(tile.tok0, tile.kvh) : own_row(tile.tok0, tile.kvh);
-        one_item = false;
+        const int record = cut ? part_row(run, first_item ? 0 : 1) : tile.shared ? shared_row(tile.tok0, tile.kvh) : own_row(tile.tok0, tile.kvh);
         for (int i = tid; i < nrows * (D / 4); i += kTakerThreads) {
             const int row = i / (D / 4), c = i % (D / 4) * 4;
             const Gather sum = over_warps(row, c);
@@ -490,7 +545,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
         }
         if (!meet()) return;
         const unsigned int mine = last_of;
-        if (!mine) continue;
+        if (!mine) continue;  // (and the join rows were read before the meeting)
         // The rows of all those sequences at once: `teams` warps a row, each with some of its records, a dozen (statistics
         // and columns) requested at a time; then the warps are joined.
         const int rows = __popc(mine) * a.group, teams = rows >= kTakers ? 1 : kTakers / rows;
@@ -549,8 +604,8 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
             if (teams == 1) {
                 if (lane < D / 4) deliver(R, c, sum);
             } else if (lane < D / 4) {
-                *reinterpret_cast<float4*>(join + (part * sa.item_rows + row) * S::kPitch + c) = sum.o;
-                if (c == 0) join_mls[part][4 * buffer + row] = make_float2(sum.m, sum.l);
+                *reinterpret_cast<float4*>(joins + (part * sa.item_rows + row) * S::kPitch + c) = sum.o;
+                if (c == 0) join_mls[part][row] = make_float2(sum.m, sum.l);
             }
         }
         if (teams > 1) {
@@ -559,11 +614,12 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
                 const int row = i / (D / 4), c = i % (D / 4) * 4, tok = tile.tok0 + token_of(row / a.group);
                 Gather sum;
                 for (int x = 0; x < teams; x++)
-                    sum.add(join_mls[x][4 * buffer + row], *reinterpret_cast<const float4*>(join + (x * sa.item_rows + row) * S::kPitch + c));
+                    sum.add(join_mls[x][row], *reinterpret_cast<const float4*>(joins + (x * sa.item_rows + row) * S::kPitch + c));
                 deliver((size_t)(sa.tok_base + tok) * a.q_heads + tile.kvh * a.group + row % a.group, c, sum);
             }
         }
-        // (the next item's meeting comes before these join rows, or parts_of, are written again)
+        // (these join rows, and parts_of, are written again only after another meeting, or by a direct item:)
+        if (!meet()) return;
     }
 }
 
@@ -583,8 +639,7 @@ static int launch_rows_t(StreamArgs sa, const void* maps, cudaStream_t stream)
     cudaError_t e;
     sa.q_bytes = (sa.item_rows * D * (sa.a.io_bf16 ? 2 : 4) + 127) / 128 * 128;
     // Two CTAs per SM where that leaves each two stages or more, else one.
-    sa.buffers = sa.item_rows <= 4 ? 2 : 1;
-    const int fixed = sa.buffers * kTakers * sa.item_rows * S::kPitch * 4 + (2 * sa.a.batch + 1) * 4 + 1024 +  // + alignment
+    const int fixed = kTakers * sa.item_rows * S::kPitch * 4 + (2 * sa.a.batch + 1) * 4 + 1024 +  // + alignment
                       (sizeof(T) == 4 && !kDup ? 2 * 8 * kBlocks * S::kPitch * 4 : 0);
     int ctas = 2, most = kSmemSm / 2 - 1024 - kStaticMax;
     if ((most - fixed) / (S::kStage + sa.q_bytes) < 2) {
@@ -601,7 +656,7 @@ static int launch_rows_t(StreamArgs sa, const void* maps, cudaStream_t stream)
         if (e != cudaSuccess) return (int)e;
         ready[dev] = true;
     }
-    return launch_after(pages_stream_kernel<T, D, kBlocks, kDup>, dim3(ctas * kSms), kStreamThreads, bytes, stream, *static_cast<const Maps*>(maps), sa);
+    return launch_after(pages_stream_kernel<T, D, kBlocks, kDup>, dim3(ctas * (kSms - sa.beside)), kStreamThreads, bytes, stream, *reinterpret_cast<const Maps*>(static_cast<const CUtensorMap*>(maps) + 2), sa);
 }
 
 template <typename T, int D>
@@ -625,7 +680,7 @@ size_t stream_bytes(const AttnArgs& a, int count, bool shared)
     return record_rows(a, count, shared) * (a.p.head_dim * sizeof(float) + sizeof(float2));
 }
 
-int launch_stream(const AttnArgs& a, int layer, int first, int count, bool shared, int out_slot, int max_len, const void* maps, void* ws,
+int launch_stream(const AttnArgs& a, int layer, int first, int count, bool shared, int out_slot, int beside, int max_len, const void* maps, void* ws,
                   unsigned int* tickets, cudaStream_t stream)
 {
     const int D = a.p.head_dim;
@@ -640,6 +695,7 @@ int launch_stream(const AttnArgs& a, int layer, int first, int count, bool share
     sa.shared_units = shared ? kItemUnits + (a.prefix + rows - 1) / rows : 0;
     sa.out_slot = out_slot;
     sa.max_len = max_len;
+    sa.beside = beside;
     sa.rec_o = static_cast<float*>(ws);
     sa.rec_ml = reinterpret_cast<float2*>(sa.rec_o + record_rows(a, count, shared) * D);
     sa.tickets = tickets;
