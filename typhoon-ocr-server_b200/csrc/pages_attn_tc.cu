@@ -115,8 +115,9 @@ __device__ __forceinline__ float row_max(const float (&s)[kKeys], const Mask& mk
 
 // p = exp2(s * scale + neg) on the visible columns (0 on the others) as BF16 pairs into the row's TMEM
 // columns at p_addr; returns the FP32 sum.  kTrack: *top receives the largest exponent.
-template <bool kMask, bool kTrack>
-__device__ __forceinline__ float row_exp(const float (&s)[kKeys], const Mask& mk, float scale, float neg, uint32_t p_addr, float* top)
+template <bool kMask, bool kTrack, typename Ready>
+__device__ __forceinline__ float row_exp(const float (&s)[kKeys], const Mask& mk, float scale, float neg, uint32_t p_addr, float* top,
+                                         Ready ready)
 {
     const float2 sc = make_float2(scale, scale), nm = make_float2(neg, neg);
     float2 acc0 = make_float2(0.f, 0.f), acc1 = make_float2(0.f, 0.f);
@@ -145,6 +146,7 @@ __device__ __forceinline__ float row_exp(const float (&s)[kKeys], const Mask& mk
             pk[c / 2] = pack_bf16x2(e0.x, e0.y);
             pk[c / 2 + 1] = pack_bf16x2(e1.x, e1.y);
         }
+        if (q == 0) ready();
         tmem_st16u(p_addr + q * 16, pk);
     }
     tmem_wait_st();
@@ -476,13 +478,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     mk.w[q] = below(pos + 1 - c0) & (~below(lo - c0) | below(sinks - c0)) & pages;
                 }
             }
-            if (j > 1) {  // the P buffer is the operand of P.V two steps back until that is done
-                if (!pv_wait(j - 2)) {
-                    ok = false;
-                    break;
+            // The P buffer is the operand of P.V two steps back until that is done: looked at when the first half of the
+            // exponentials is on its way.
+            auto ready = [&]() {
+                if (j > 1) {
+                    ok = ok && pv_wait(j - 2);
+                    tc_fence_after();
                 }
-                tc_fence_after();
-            }
+            };
             const uint32_t p = p_addr + (j & 1) * 32;
             // The running maximum moves only when a step's exceeds it by more than 2^8 (P stays within BF16's
             // range and the FP32 sums do not mind), which spares most rescalings of O: exponentials against the
@@ -497,12 +500,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 alpha = m_run == -INFINITY ? 1.f : pt_exp2(m_run - m_new);  // nothing gathered: nothing to scale
                 m_run = m_new;
                 const float neg = m_run == -INFINITY ? 0.f : -m_run;
-                rowsum = masked ? row_exp<true, false>(sv, mk, a.scale_log2, neg, p, nullptr)
-                                : row_exp<false, false>(sv, mk, a.scale_log2, neg, p, nullptr);
+                rowsum = masked ? row_exp<true, false>(sv, mk, a.scale_log2, neg, p, nullptr, ready)
+                                : row_exp<false, false>(sv, mk, a.scale_log2, neg, p, nullptr, ready);
             } else {
                 float top;
-                rowsum = masked ? row_exp<true, true>(sv, mk, a.scale_log2, -m_run, p, &top)
-                                : row_exp<false, true>(sv, mk, a.scale_log2, -m_run, p, &top);
+                rowsum = masked ? row_exp<true, true>(sv, mk, a.scale_log2, -m_run, p, &top, ready)
+                                : row_exp<false, true>(sv, mk, a.scale_log2, -m_run, p, &top, ready);
                 const bool move = top > 8.f;
                 if (__any_sync(0xffffffffu, move)) {
                     float m_new = m_run;
@@ -511,10 +514,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         alpha = pt_exp2(m_run - m_new);
                     }
                     m_run = m_new;
-                    rowsum = masked ? row_exp<true, false>(sv, mk, a.scale_log2, -m_run, p, nullptr)
-                                    : row_exp<false, false>(sv, mk, a.scale_log2, -m_run, p, nullptr);
+                    rowsum = masked ? row_exp<true, false>(sv, mk, a.scale_log2, -m_run, p, nullptr, ready)
+                                    : row_exp<false, false>(sv, mk, a.scale_log2, -m_run, p, nullptr, ready);
                 }
             }
+            if (!ok) break;
             if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
                 if (!pv_wait(j - 1)) {  // O is at rest
                     ok = false;
