@@ -253,3 +253,23 @@ def test_repeatable_and_on_another_stream(pkg, lib, pages):
         assert torch.equal(a, b)
     lib.attn_set_stream(None)
     assert synced(pkg, lib) == ""
+
+
+@pytest.mark.parametrize("dtype", [BF, F])
+@pytest.mark.parametrize("hq,h,d", [(16, 8, 128), (8, 8, 64), (12, 4, 64), (32, 2, 64)])
+@pytest.mark.parametrize("batch", [3, 8, 20])
+def test_a_shared_prefix_repeats_exactly(pkg, lib, pages, dtype, hq, h, d, batch):
+    # Which sequences a run joins together is a matter of timing; the sums are not.
+    prefix, page = 1500, 64
+    pool = filled(pages, [prefix], page, h, d, dtype, 30, spare=batch)
+    big = pages.PagePool(pool.k, pool.v, torch.full((batch + 1, pool.table.shape[1] + 1), -1, dtype=torch.int32, device="cuda"),
+                         torch.zeros(batch + 1, dtype=torch.int32, device="cuda"), pool.ref)
+    big.table[0, :pool.table.shape[1]] = pool.table[0]
+    big.len[0] = prefix
+    big.fork(ints([0] * batch), ints(list(range(1, batch + 1))))
+    seqs = ints(list(range(1, batch + 1)))
+    q, _ = queries(batch, hq, d, dtype, pool, 31)
+    want = big.attend_prefix(q, 0, seqs, 1472, prefix, d**-0.5)
+    for _ in range(20):
+        assert torch.equal(big.attend_prefix(q, 0, seqs, 1472, prefix, d**-0.5), want)
+    assert synced(pkg, lib) == ""

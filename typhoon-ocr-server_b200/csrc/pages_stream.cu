@@ -122,11 +122,12 @@ struct Gather {
         // a record that saw nothing has l = 0, o = 0 and m = -inf: its factor is 0
         const float top = fmaxf(m, ml.x), f = m == -INFINITY ? 0.f : fast_exp2(m - top), e = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - top);
         m = top;
-        l = l * f + ml.y * e;
-        o.x = o.x * f + x.x * e;
-        o.y = o.y * f + x.y * e;
-        o.z = o.z * f + x.z * e;
-        o.w = o.w * f + x.w * e;
+        // (which product is rounded is spelled out, so that every place where this is inlined gives the same bits)
+        l = fmaf(l, f, __fmul_rn(ml.y, e));
+        o.x = fmaf(o.x, f, __fmul_rn(x.x, e));
+        o.y = fmaf(o.y, f, __fmul_rn(x.y, e));
+        o.z = fmaf(o.z, f, __fmul_rn(x.z, e));
+        o.w = fmaf(o.w, f, __fmul_rn(x.w, e));
     }
 };
 
@@ -546,9 +547,12 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
         if (!meet()) return;
         const unsigned int mine = last_of;
         if (!mine) continue;  // (and the join rows were read before the meeting)
-        // The rows of all those sequences at once: `teams` warps a row, each with some of its records, a dozen (statistics
-        // and columns) requested at a time; then the warps are joined.
-        const int rows = __popc(mine) * a.group, teams = rows >= kTakers ? 1 : kTakers / rows;
+        // The rows of all those sequences at once: a row's records in `shares`, each a dozen (statistics and columns)
+        // requested at a time; then the shares are joined.  Few rows: a warp per share, else all of a row's by one warp.
+        // (The shares depend on the group alone: how many sequences come together here is a matter of timing, and must not
+        // change the order of a sum.)
+        const int rows = __popc(mine) * a.group, shares = a.group >= kTakers ? 1 : kTakers / a.group;
+        const bool spread = shares > 1 && rows < kTakers;
         auto token_of = [&](int k) {  // of the k-th sequence to join
             unsigned int left = mine;
             for (; k > 0; k--) left &= left - 1;
@@ -556,64 +560,72 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
         };
         constexpr int kDozen = 12;
 #pragma unroll 1
-        for (int j = warp; j < rows * teams; j += kTakers) {
-            const int row = j / teams, part = j - row * teams, seq_of = row / a.group, in_head = row - seq_of * a.group;
+        for (int j = warp; j < (spread ? rows * shares : rows); j += kTakers) {
+            const int row = spread ? j / shares : j, seq_of = row / a.group, in_head = row - seq_of * a.group;
             const int k = token_of(seq_of), tok = tile.tok0 + k;
             const Parts p = parts_of[k];
-            const int ns = p.sh1 - p.sh0 + 1, n = ns + p.own1 - p.own0 + 1, mine_n = (n - part + teams - 1) / teams;
+            const int ns = p.sh1 - p.sh0 + 1, n = ns + p.own1 - p.own0 + 1;
             const int c = lane % (D / 4) * 4;  // D = 64: two lanes have the same columns
+            const int part0 = spread ? j - row * shares : 0, part1 = spread ? part0 + 1 : shares;
             Gather sum;
 #pragma unroll 1
-            for (int base = 0; base < mine_n; base += kDozen) {
-                const int here = min(kDozen, mine_n - base);
-                // lane y: record base + y of the warp's
-                const int x = part + (base + min(lane, here - 1)) * teams, y = x - ns;
-                int at;
-                if (x < ns) at = (ns == 1 ? shared_row(tok, tile.kvh) : part_row(p.sh0 + x, x ? 0 : p.sh_second)) + (tok - tok / per * per) * a.group;
-                else at = p.own0 == p.own1 ? own_row(tok, tile.kvh) : part_row(p.own0 + y, y ? 0 : p.own_second);
-                at += in_head;
-                float2 ml = __ldcg(&sa.rec_ml[at]);
-                float4 v[kDozen];
+            for (int part = part0; part < part1; part++) {
+                const int mine_n = (n - part + shares - 1) / shares;
+                Gather share;
+#pragma unroll 1
+                for (int base = 0; base < mine_n; base += kDozen) {
+                    const int here = min(kDozen, mine_n - base);
+                    // lane y: record base + y of the warp's
+                    const int x = part + (base + min(lane, here - 1)) * shares, y = x - ns;
+                    int at;
+                    if (x < ns) at = (ns == 1 ? shared_row(tok, tile.kvh) : part_row(p.sh0 + x, x ? 0 : p.sh_second)) + (tok - tok / per * per) * a.group;
+                    else at = p.own0 == p.own1 ? own_row(tok, tile.kvh) : part_row(p.own0 + y, y ? 0 : p.own_second);
+                    at += in_head;
+                    float2 ml = __ldcg(&sa.rec_ml[at]);
+                    float4 v[kDozen];
 #pragma unroll
-                for (int i = 0; i < kDozen; i++)
-                    v[i] = __ldcg(reinterpret_cast<const float4*>(sa.rec_o + (size_t)__shfl_sync(0xffffffffu, at, i) * D + c));
-                if (lane >= here) ml = make_float2(-INFINITY, 0.f);
-                float top = ml.x;
+                    for (int i = 0; i < kDozen; i++)
+                        v[i] = __ldcg(reinterpret_cast<const float4*>(sa.rec_o + (size_t)__shfl_sync(0xffffffffu, at, i) * D + c));
+                    if (lane >= here) ml = make_float2(-INFINITY, 0.f);
+                    float top = ml.x;
 #pragma unroll
-                for (int d = 8; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-                top = __shfl_sync(0xffffffffu, top, 0);
-                const float f = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - top);
-                float l = ml.y * f;
+                    for (int d = 8; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                    top = __shfl_sync(0xffffffffu, top, 0);
+                    const float f = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - top);
+                    float l = ml.y * f;
 #pragma unroll
-                for (int d = 8; d; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
-                l = __shfl_sync(0xffffffffu, l, 0);
-                float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+                    for (int d = 8; d; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+                    l = __shfl_sync(0xffffffffu, l, 0);
+                    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-                for (int i = 0; i < kDozen; i++) {
-                    const float fi = __shfl_sync(0xffffffffu, f, i);
-                    if (i < here) {
-                        o.x = fmaf(v[i].x, fi, o.x);
-                        o.y = fmaf(v[i].y, fi, o.y);
-                        o.z = fmaf(v[i].z, fi, o.z);
-                        o.w = fmaf(v[i].w, fi, o.w);
+                    for (int i = 0; i < kDozen; i++) {
+                        const float fi = __shfl_sync(0xffffffffu, f, i);
+                        if (i < here) {
+                            o.x = fmaf(v[i].x, fi, o.x);
+                            o.y = fmaf(v[i].y, fi, o.y);
+                            o.z = fmaf(v[i].z, fi, o.z);
+                            o.w = fmaf(v[i].w, fi, o.w);
+                        }
                     }
+                    share.add(make_float2(top, l), o);
                 }
-                sum.add(make_float2(top, l), o);
+                sum.add(make_float2(share.m, share.l), share.o);
             }
-            const size_t R = (size_t)(sa.tok_base + tok) * a.q_heads + tile.kvh * a.group + in_head;
-            if (teams == 1) {
-                if (lane < D / 4) deliver(R, c, sum);
-            } else if (lane < D / 4) {
-                *reinterpret_cast<float4*>(joins + (part * sa.item_rows + row) * S::kPitch + c) = sum.o;
-                if (c == 0) join_mls[part][row] = make_float2(sum.m, sum.l);
+            if (lane < D / 4) {
+                if (spread) {
+                    *reinterpret_cast<float4*>(joins + (part0 * sa.item_rows + row) * S::kPitch + c) = sum.o;
+                    if (c == 0) join_mls[part0][row] = make_float2(sum.m, sum.l);
+                } else {
+                    deliver((size_t)(sa.tok_base + tok) * a.q_heads + tile.kvh * a.group + in_head, c, sum);
+                }
             }
         }
-        if (teams > 1) {
+        if (spread) {
             if (!meet()) return;
             for (int i = tid; i < rows * (D / 4); i += kTakerThreads) {
                 const int row = i / (D / 4), c = i % (D / 4) * 4, tok = tile.tok0 + token_of(row / a.group);
                 Gather sum;
-                for (int x = 0; x < teams; x++)
+                for (int x = 0; x < shares; x++)
                     sum.add(join_mls[x][row], *reinterpret_cast<const float4*>(joins + (x * sa.item_rows + row) * S::kPitch + c));
                 deliver((size_t)(sa.tok_base + tok) * a.q_heads + tile.kvh * a.group + row % a.group, c, sum);
             }
