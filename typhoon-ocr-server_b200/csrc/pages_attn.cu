@@ -84,7 +84,7 @@ static void share_sms(const tyb_pages_attn* c, int tiles, int ctas, Layout* l)
         if (us < best) {
             best = us;
             l->splits = s;
-            l->beside = s * ctas;
+            l->beside = (s * ctas + 1) / 2 * 2;
         }
     }
 }
@@ -182,7 +182,7 @@ extern "C" int tyb_pages_attn_launch(const tyb_pages_attn* c, void* ws, void* ti
     }
     void* more = static_cast<char*>(ws) + (record_bytes(a, l) + 255) / 256 * 256;
     if (l.tiles) {
-        const int e = l.tc ? tc_launch(a, c->layer, l.tall, l.tokens, l.row_tiles, c->maps, st)
+        const int e = l.tc ? tc_launch(a, c->layer, l.tall, l.tokens, l.beside > 0, l.row_tiles, c->maps, st)
                            : rows_launch(a, c->layer, l.row_tiles, c->maps, st);
         if (e) return e;
     }

@@ -32,20 +32,29 @@ __device__ __forceinline__ void after_predecessor()
 __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_predecessor() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+// In clusters of `cluster` CTAs.
 template <typename... P, typename... A>
-int launch_after(void (*kernel)(P...), dim3 grid, int threads, size_t shared, cudaStream_t stream, A... args)
+int launch_after_in(int cluster, void (*kernel)(P...), dim3 grid, int threads, size_t shared, cudaStream_t stream, A... args)
 {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = shared;
     cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
     return (int)cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+template <typename... P, typename... A>
+int launch_after(void (*kernel)(P...), dim3 grid, int threads, size_t shared, cudaStream_t stream, A... args)
+{
+    return launch_after_in(1, kernel, grid, threads, shared, stream, args...);
 }
 
 // Waits for phase `parity` of an mbarrier, at most limit_ns; false (and the status raised) when that ran
@@ -147,7 +156,7 @@ struct AttnArgs {
 // The tcgen05 form (pages_attn_tc.cu) for the query rows of a BF16 pool, `items` row tiles: tall, of at
 // most 128 rows each, with two record slots a split; else of 256 rows.
 constexpr int kTcTall = 128, kTcWide = 256;
-int tc_launch(const AttnArgs& a, int layer, bool tall, bool shared_pass, int items, const void* maps, cudaStream_t stream);
+int tc_launch(const AttnArgs& a, int layer, bool tall, bool shared_pass, bool beside, int items, const void* maps, cudaStream_t stream);
 
 // The row form (pages_rows.cu) for the prompt chunks of an FP32 pool, row tiles of kRowsTile rows.
 constexpr int kRowsTile = 64;

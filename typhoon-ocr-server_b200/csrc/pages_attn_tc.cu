@@ -26,6 +26,8 @@
 #include "pages_attn.cuh"
 #include "tcgen05.cuh"
 
+#include <type_traits>
+
 namespace tyb {
 
 constexpr int kRows = 128;   // rows of a stream (tensor-core M)
@@ -46,6 +48,7 @@ struct TcArgs {
     AttnArgs a;
     int layer;
     int tall;        // the streams share their rows
+    int row_tiles;
     int shared_pass; // the rows are the batch's single tokens against the first sequence's leading rows
     unsigned long long wait_ns;
 };
@@ -174,7 +177,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     volatile uint32_t* present = reinterpret_cast<uint32_t*>(drain + 5);  // [kSeen] a bit per 16 rows of the tile
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int kvh = blockIdx.y, split = blockIdx.z;
+    // CTA: a row tile's KV heads next to each other, then its splits (16,384 tokens through 4,096 in 485 us, with
+    // a head's row tiles next to each other 505 us).
+    const int kvh = (int)blockIdx.x % a.p.kv_heads, split = (int)blockIdx.x / a.p.kv_heads % a.splits,
+              row_tile = (int)blockIdx.x / (a.p.kv_heads * a.splits);
+    if (row_tile >= ta.row_tiles) return;  // (one CTA, of a grid rounded up to pairs)
     const int rows_item = ta.tall ? kRows : 2 * kRows;
     const int per = rows_item / a.group;  // tokens of an item
 
@@ -207,14 +214,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         tc_fence_before();
     }
     after_predecessor();
-    if (warp == 0 && !ta.shared_pass) find_item(a, (int)(gridDim.x - 1 - blockIdx.x), per, found);  // the last items, with the most keys, first
+    if (warp == 0 && !ta.shared_pass) find_item(a, ta.row_tiles - 1 - row_tile, per, found);  // the last items, with the most keys, first
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
 
     int tok0 = 0, ntok = 0;
     if (ta.shared_pass) {
-        tok0 = (int)blockIdx.x * per;
+        tok0 = row_tile * per;
         ntok = min(per, a.batch - tok0);
     } else if (found[0] >= 0) {
         tok0 = found[1];
@@ -539,7 +546,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             tc_fence_before();
             warp_arrive(&p_full[2 * h + (j & 1)]);
         }
-        // ---- the rows' outputs, or their records: 64 columns at a time through shared memory (the stream's query
+        // ---- the rows' outputs, or their records: some columns at a time through shared memory (the stream's query
         // tile, no longer needed), so that they leave in whole lines instead of 16 bytes of 32 rows at a time
         const int slot = a.slot0 + (ta.tall ? 2 * split + h : split);
         const bool direct = a.rec.slots == 1;
@@ -549,54 +556,59 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const float mul = !direct ? 1.f : l_run == 0.f ? 0.f : 1.f / l_run;
         if (!direct && here && ok) a.rec.ml[(size_t)slot * a.rec.rows + R] = make_float2(m_run, l_run);
         tc_fence_after();
-        unsigned char* stage = sQ + h * S::kTileQ + (warp & 3) * (S::kTileQ / 4);  // 32 rows of 256 (FP32) or 128 bytes
-        const bool half = direct && a.io_bf16;
+        unsigned char* stage = sQ + h * S::kTileQ + (warp & 3) * (S::kTileQ / 4);
         static_assert(S::kTileQ / 4 >= 32 * 128, "room for 32 rows");
-        constexpr int kCols = S::kTileQ / 4 >= 32 * 256 ? 64 : 32;  // columns that fit as FP32
+        constexpr int kWide = S::kTileQ / 4 >= 32 * 256 ? 64 : 32;  // columns that fit as FP32
+        auto leave = [&](auto as_half) {
+            constexpr bool kHalf = decltype(as_half)::value;
+            constexpr int kCols = kHalf ? 64 : kWide, kPitch = kCols * (kHalf ? 2 : 4), kPieces = kPitch / 16, kSwap = kPieces < 8 ? kPieces - 1 : 7;
 #pragma unroll 1
-        for (int c0 = 0; c0 < D; c0 += kCols) {
-            if (ok) {
+            for (int c0 = 0; c0 < D; c0 += kCols) {
+                if (ok) {
 #pragma unroll
-                for (int c = 0; c < kCols; c += 32) {
-                    float v[32];
-                    if (mine > 0) {
-                        tmem_ld32(o_addr + c0 + c, v);
-                    } else {
+                    for (int c = 0; c < kCols; c += 32) {
+                        float v[32];
+                        if (mine > 0) {
+                            tmem_ld32(o_addr + c0 + c, v);
+                        } else {
 #pragma unroll
-                        for (int i = 0; i < 32; i++) v[i] = 0.f;
-                    }
+                            for (int i = 0; i < 32; i++) v[i] = 0.f;
+                        }
 #pragma unroll
-                    for (int i = 0; i < 32; i++) v[i] = mul == 0.f ? 0.f : v[i] * mul;
-                    // piece p of a row lies at p ^ (row % 8): no two rows' pieces of a phase in the same banks
-                    if (half) {
+                        for (int i = 0; i < 32; i++) v[i] = mul == 0.f ? 0.f : v[i] * mul;
+                        // piece p of a row lies at p ^ (row % 8): no two rows' pieces of a phase in the same banks
+                        if (kHalf) {
 #pragma unroll
-                        for (int i = 0; i < 32; i += 8)
-                            *reinterpret_cast<uint4*>(stage + lane * (kCols * 2) + ((((c + i) >> 3) ^ (lane & (kCols / 8 - 1))) << 4)) =
-                                make_uint4(pack_bf16x2(v[i], v[i + 1]), pack_bf16x2(v[i + 2], v[i + 3]), pack_bf16x2(v[i + 4], v[i + 5]),
-                                           pack_bf16x2(v[i + 6], v[i + 7]));
-                    } else {
+                            for (int i = 0; i < 32; i += 8)
+                                *reinterpret_cast<uint4*>(stage + lane * kPitch + ((((c + i) >> 3) ^ (lane & kSwap)) << 4)) =
+                                    make_uint4(pack_bf16x2(v[i], v[i + 1]), pack_bf16x2(v[i + 2], v[i + 3]), pack_bf16x2(v[i + 4], v[i + 5]),
+                                               pack_bf16x2(v[i + 6], v[i + 7]));
+                        } else {
 #pragma unroll
-                        for (int i = 0; i < 32; i += 4)
-                            *reinterpret_cast<float4*>(stage + lane * (kCols * 4) + ((((c + i) >> 2) ^ (lane & 7)) << 4)) =
-                                make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                            for (int i = 0; i < 32; i += 4)
+                                *reinterpret_cast<float4*>(stage + lane * kPitch + ((((c + i) >> 2) ^ (lane & kSwap)) << 4)) =
+                                    make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                        }
                     }
                 }
+                __syncwarp();
+                // a row's pieces by neighbouring lanes; the row's address from the lane that has the row
+                constexpr int kAtOnce = 32 / kPieces;
+#pragma unroll
+                for (int r0 = 0; r0 < 32; r0 += kAtOnce) {
+                    const int row = r0 + lane / kPieces, piece = lane % kPieces;
+                    const long long to = __shfl_sync(0xffffffffu, here && ok ? (long long)R : -1ll, row);
+                    const uint4 x = *reinterpret_cast<const uint4*>(stage + row * kPitch + ((piece ^ (row & kSwap)) << 4));
+                    if (to < 0) continue;
+                    if (kHalf) *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) + to * D + c0 + piece * 8) = x;
+                    else if (direct) *reinterpret_cast<uint4*>(static_cast<float*>(a.out) + to * D + c0 + piece * 4) = x;
+                    else *reinterpret_cast<uint4*>(a.rec.o + ((size_t)slot * a.rec.rows + to) * D + c0 + piece * 4) = x;
+                }
+                __syncwarp();
             }
-            __syncwarp();
-            // a row's pieces by neighbouring lanes; the row's address from the lane that has the row
-            const int per_row = half ? kCols / 8 : kCols / 4, rows_at_once = 32 / per_row;
-            for (int r0 = 0; r0 < 32; r0 += rows_at_once) {
-                const int row = r0 + lane / per_row, piece = lane % per_row;
-                const long long to = __shfl_sync(0xffffffffu, here && ok ? (long long)R : -1ll, row);
-                const uint4 x = *reinterpret_cast<const uint4*>(stage + row * (kCols * (half ? 2 : 4)) +
-                                                                ((piece ^ (row & (half ? kCols / 8 - 1 : 7))) << 4));
-                if (to < 0) continue;
-                if (half) *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) + to * D + c0 + piece * 8) = x;
-                else if (direct) *reinterpret_cast<uint4*>(static_cast<float*>(a.out) + to * D + c0 + piece * 4) = x;
-                else *reinterpret_cast<uint4*>(a.rec.o + ((size_t)slot * a.rec.rows + to) * D + c0 + piece * 4) = x;
-            }
-            __syncwarp();
-        }
+        };
+        if (direct && a.io_bf16) leave(std::true_type());
+        else leave(std::false_type());
         tc_fence_before();
     }
     __syncthreads();
@@ -613,7 +625,7 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t,
                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
 template <int D>
-static int launch_tc(const TcArgs& ta, const void* maps, dim3 grid, cudaStream_t stream)
+static int launch_tc(const TcArgs& ta, const void* maps, int grid, int pair, cudaStream_t stream)
 {
     static bool ready[64];
     const int dev = ta.a.device;
@@ -630,10 +642,10 @@ static int launch_tc(const TcArgs& ta, const void* maps, dim3 grid, cudaStream_t
         ready[dev] = true;
     }
     const CUtensorMap* m = static_cast<const CUtensorMap*>(maps);
-    return launch_after(pages_tc_kernel<D>, grid, kTcThreads, Smem<D>::kBytes, stream, m[0], m[1], ta);
+    return launch_after_in(pair, pages_tc_kernel<D>, dim3(grid), kTcThreads, Smem<D>::kBytes, stream, m[0], m[1], ta);
 }
 
-int tc_launch(const AttnArgs& a, int layer, bool tall, bool shared_pass, int items, const void* maps, cudaStream_t stream)
+int tc_launch(const AttnArgs& a, int layer, bool tall, bool shared_pass, bool beside, int items, const void* maps, cudaStream_t stream)
 {
     TcArgs ta;
     ta.a = a;
@@ -641,8 +653,11 @@ int tc_launch(const AttnArgs& a, int layer, bool tall, bool shared_pass, int ite
     ta.tall = tall;
     ta.shared_pass = shared_pass;
     ta.wait_ns = tyb_wait_limit_of(a.device);
-    const dim3 grid(items, a.p.kv_heads, a.splits);
-    return a.p.head_dim == 128 ? launch_tc<128>(ta, maps, grid, stream) : launch_tc<64>(ta, maps, grid, stream);
+    ta.row_tiles = items;
+    // Beside the own rows in pairs, which lie on the two SMs of a TPC: one of these CTAs and one of the streaming form's
+    // on the two slowed the latter (256 questions: the run there took 68 us on average, the others 53).
+    const int pair = beside ? 2 : 1, ctas = items * a.p.kv_heads * a.splits, grid = (ctas + pair - 1) / pair * pair;
+    return a.p.head_dim == 128 ? launch_tc<128>(ta, maps, grid, pair, stream) : launch_tc<64>(ta, maps, grid, pair, stream);
 }
 
 }  // namespace tyb
