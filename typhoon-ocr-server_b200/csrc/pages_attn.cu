@@ -58,19 +58,22 @@ struct Layout {
     int beside;   // SMs of a shared pass that the own rows run beside; 0: after it
 };
 
-// Query rows of a KV head from which the shared prefix runs on the tcgen05 form.
-constexpr int kTcSharedRows = 65;
+// Query rows of a KV head, and their product with the shared keys, from which a shared prefix runs on the tcgen05 form
+// rather than in the streaming one.  With 2 rows a sequence and up to 50 own rows, streaming / tcgen05 in microseconds:
+// 48 rows x 200 keys 20.5 / 23.5, 96 x 200 21.5 / 25.6; 16 x 1,024 20.1 / 17.4, 32 x 1,024 21.9 / 19.3, 96 x 1,024 28.2 /
+// 20.0; 32 x 4,096 25.8 / 24.2, 96 x 4,096 38.9 / 24.8; 12 x 16,384 34.6 / 38.7, 32 x 16,384 42.1 / 42.2, 48 x 16,384 59.9 / 42.5.
+constexpr int kTcSharedRows = 32, kTcSharedWork = 24576;
 
 // A shared pass on the tensor cores and the streaming of the sequences' own rows are bound by different things: they
 // run at the same time where that is estimated to be shorter.  In microseconds: a split of the pass its tiles; the
 // own rows (taken to be half of what max_len allows) what a CTA needs for a stage (an item's start and end take as
-// long as kItemUnits of them), or what the memory can deliver; each of the two 10 for its start and end.  That met what
-// was measured within a tenth, in turn / at the same time: 256 sequences behind 4,096 shared rows with up to 512
-// own ones 94 / 79, with up to 64 own ones 55 / 46, behind 1,024 85 / 68; 64 behind 4,096 60 / 36; 512 behind 2,048 with up
-// to 128 91 / 84 (and 101 with twice the SMs for the pass).
+// long as kItemUnits of them), or what the memory can deliver; each of the two 10 for its start and end.  Of the splits
+// tried, that picked the fastest or one within 1 % of it.  Measured, in turn / at the same time: 256 sequences behind 4,096
+// shared rows with up to 512 own ones 94 / 72, with up to 64 own ones 55 / 41, behind 1,024 85 / 68; 64 behind 4,096
+// 61 / 35; 512 behind 2,048 with up to 128 91 / 77; 128 behind 4,096 with up to 1,500 110 / 82.
 static void share_sms(const tyb_pages_attn* c, int tiles, int ctas, Layout* l)
 {
-    const double tile_us = l->tall ? 0.7 : 1.25, unit_us = 1.15, fixed_us = 10.0, memory = 6.4e6;
+    const double tile_us = l->tall ? 0.7 : 1.0, unit_us = 1.0, fixed_us = 10.0, memory = 6.4e6;
     const double rows = 0.5 * (c->max_len - c->prefix), items = (double)c->batch * c->p.kv_heads;
     const double bytes = rows * items * c->p.head_dim * 4.0, units = items * (kItemUnits + 0.5 + rows / 64);  // K and V in BF16
     auto pass_us = [&](int splits) { return fixed_us + (tiles + splits - 1) / splits * tile_us; };
@@ -96,7 +99,8 @@ static Layout layout_of(const tyb_pages_attn* c)
     const int group = c->q_heads / c->p.kv_heads;
     l.tokens = c->max_new == 1 && c->rows == c->batch;
     const bool prefix = l.tokens && c->prefix > 0;
-    l.tiles = !l.tokens || (prefix && bf16 && (long long)c->batch * group >= kTcSharedRows);
+    const long long shared_rows = (long long)c->batch * group;
+    l.tiles = !l.tokens || (prefix && bf16 && shared_rows >= kTcSharedRows && shared_rows * c->prefix >= kTcSharedWork);
     l.shared = prefix && !l.tiles;
     if (!l.tiles) return l;
     l.tc = bf16;
