@@ -115,7 +115,10 @@ static Layout layout_of(const tyb_pages_attn* c)
         l.splits = (int)(kSms / ctas);  // one CTA fits an SM; a split has at least four tiles
         if (l.splits > tiles / 4) l.splits = tiles / 4;
     } else {
-        l.splits = (int)(4 * kSms / ctas);  // two CTAs fit an SM; a split has at least two tiles
+        // Splits for twice as many CTAs as fit, each of at least two tiles (3 chunks of 37 .. 733 tokens through 301: with
+        // heads of 64 as many as fit 43 us, twice 45, three times 45; 12 of up to 300 through 1,200: 204, 141, 133; the first
+        // with heads of 128: as many as fit and half as many again 97, twice 98, three times 112).
+        l.splits = (int)(2 * rows_ctas(c->p.head_dim) * kSms / ctas);
         if (l.splits > tiles / 2) l.splits = tiles / 2;
     }
     if (l.splits < 1) l.splits = 1;

@@ -160,6 +160,8 @@ int tc_launch(const AttnArgs& a, int layer, bool tall, bool shared_pass, bool be
 
 // The row form (pages_rows.cu) for the prompt chunks of an FP32 pool, row tiles of kRowsTile rows.
 constexpr int kRowsTile = 64;
+// CTAs on an SM: what the registers allow.  (40 chunks of 200 .. 900 tokens with heads of 64: 412 us, with two 455 us.)
+__host__ __device__ constexpr int rows_ctas(int head_dim) { return head_dim == 64 ? 3 : 2; }
 int rows_launch(const AttnArgs& a, int layer, int items, const void* maps, cudaStream_t stream);
 
 // Item x of a list of row tiles: sequence b's queries starts[b] .. starts[b + 1] in tiles of `per` tokens.

@@ -42,7 +42,7 @@ struct ColumnSight {
 };
 
 template <int D>
-__global__ void __launch_bounds__(kRowThreads, 2) pages_rows_kernel(const __grid_constant__ RowMaps maps, const AttnArgs a, int layer, int stages,
+__global__ void __launch_bounds__(kRowThreads, rows_ctas(D)) pages_rows_kernel(const __grid_constant__ RowMaps maps, const AttnArgs a, int layer, int stages,
                                                                    unsigned long long wait_ns)
 {
     using R = RowTile<D>;
@@ -220,9 +220,9 @@ static int launch(const AttnArgs& a, int layer, int items, const void* maps, cud
     static bool ready[64];
     const int dev = a.device;
     if (dev < 0 || dev >= 64) return (int)cudaErrorInvalidDevice;
-    // as many stages as leave room for a second CTA on the SM, or two
+    // as many stages as leave room for rows_ctas(D) CTAs on the SM, or two
     const int fixed = kRowWarps * R::kSplit + 1024;
-    int stages = (228 * 1024 / 2 - 1024 - 1024 - fixed) / R::kStage;
+    int stages = (228 * 1024 / rows_ctas(D) - 1024 - 1024 - fixed) / R::kStage;
     stages = stages < 2 ? 2 : stages > kRowStagesMax ? kRowStagesMax : stages;
     const int bytes = stages * R::kStage + fixed;
     if (!ready[dev]) {
