@@ -273,3 +273,53 @@ def test_a_shared_prefix_repeats_exactly(pkg, lib, pages, dtype, hq, h, d, batch
     for _ in range(20):
         assert torch.equal(big.attend_prefix(q, 0, seqs, 1472, prefix, d**-0.5), want)
     assert synced(pkg, lib) == ""
+
+
+@pytest.mark.parametrize("hq,h,d,batch,prefix,own", [(4, 2, 64, 1100, 700, 20), (16, 8, 128, 70, 2000, 300), (9, 3, 64, 200, 3000, 30),
+                                                     (14, 7, 128, 33, 1000, 90)])
+def test_a_large_batch_in_a_graph(pkg, lib, pages, hq, h, d, batch, prefix, own):
+    # Shared rows on the tensor cores with the own rows beside them: more sequences than one launch has, odd numbers of
+    # KV heads, and replays back to back, each of which overwrites what the one before left.
+    page = 16
+    pool = filled(pages, [prefix], page, h, d, BF, 40, spare=batch * (own // page + 3))
+    big = pages.PagePool(pool.k, pool.v, torch.full((batch + 1, prefix // page + own // page + 3), -1, dtype=torch.int32, device="cuda"),
+                         torch.zeros(batch + 1, dtype=torch.int32, device="cuda"), pool.ref)
+    w = min(pool.table.shape[1], big.table.shape[1])
+    big.table[0, :w] = pool.table[0, :w]
+    big.len[0] = prefix
+    seqs = ints(list(range(1, batch + 1)))
+    big.fork(ints([0] * batch), seqs)
+    counts = [1 + 7 * i % own for i in range(batch)]
+    starts = [0]
+    for c in counts:
+        starts.append(starts[-1] + c)
+    g = torch.Generator().manual_seed(41)
+    k, v = (torch.randn((starts[-1], h, d), generator=g).to("cuda", BF) for _ in range(2))
+    big.extend(seqs, ints(counts))
+    big.write(0, seqs, ints(starts), k, v)
+    q, q64 = queries(batch, hq, d, BF, pool, 42)
+    other = torch.randn_like(q)
+    scale = d**-0.5
+    want = big.attend_prefix(q, 0, seqs, prefix, prefix + own, scale)
+    want_other = big.attend_prefix(other, 0, seqs, prefix, prefix + own, scale)
+    assert synced(pkg, lib) == ""
+    for b in (0, 1, batch // 2, batch - 1):
+        kk, vv, there = rows_of(big, 0, b + 1)
+        close(want[b:b + 1], attention(q64[b:b + 1], kk, vv, there[None], scale), big, BF)
+    side, graph, out, out_other = torch.cuda.Stream(), torch.cuda.CUDAGraph(), torch.empty_like(q), torch.empty_like(q)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        big.attend_prefix(q, 0, seqs, prefix, prefix + own, scale, out=out)
+    side.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        big.attend_prefix(q, 0, seqs, prefix, prefix + own, scale, out=out)
+        big.attend_prefix(other, 0, seqs, prefix, prefix + own, scale, out=out_other)
+    for _ in range(5):
+        out.zero_()
+        out_other.zero_()
+        for _ in range(4):
+            graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(out_other, want_other)
+    lib.attn_set_stream(None)
+    assert synced(pkg, lib) == ""

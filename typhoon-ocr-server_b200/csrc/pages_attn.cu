@@ -131,10 +131,6 @@ static AttnArgs args_of(const tyb_pages_attn* c, const Layout& l)
 {
     AttnArgs a = {};
     a.p = c->p;
-    const size_t layer = (size_t)c->layer * c->p.num_pages * c->p.kv_heads * c->p.page_size * c->p.head_dim *
-                         (c->p.kv_dtype == TYB_BF16 ? 2 : 4);
-    a.k = static_cast<const char*>(c->p.k) + layer;
-    a.v = static_cast<const char*>(c->p.v) + layer;
     a.q = c->q;
     a.q_stride = c->q_stride;
     a.out = c->out;

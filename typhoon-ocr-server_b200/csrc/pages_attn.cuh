@@ -134,8 +134,6 @@ __device__ __forceinline__ int checked_len(const KVPages& p, int s, const Status
 
 struct AttnArgs {
     KVPages p;
-    const void* k;  // the layer's pages
-    const void* v;
     const void* q;
     long long q_stride;
     void* out;
@@ -147,8 +145,8 @@ struct AttnArgs {
     int prefix;      // leading rows left to (or handled by) the shared pass
     int window, sinks;
     float scale_log2;
-    int splits, slot0;  // this launch's splits, and the record slot of its first
-    Records rec;        // slots == 1: the output is written directly
+    int splits;   // a record slot each
+    Records rec;  // slots == 1: the output is written directly
     Status st;
     int device;
 };

@@ -548,7 +548,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         // ---- the rows' outputs, or their records: some columns at a time through shared memory (the stream's query
         // tile, no longer needed), so that they leave in whole lines instead of 16 bytes of 32 rows at a time
-        const int slot = a.slot0 + (ta.tall ? 2 * split + h : split);
+        const int slot = ta.tall ? 2 * split + h : split;
         const bool direct = a.rec.slots == 1;
         if (ok && mine > 0) ok = pv_wait(mine - 1);
         if (ta.tall) asm volatile("bar.sync 1, %0;" ::"n"(kSoftThreads) : "memory");  // the other stream is done with the queries too

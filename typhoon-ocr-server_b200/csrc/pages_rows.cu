@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(kRowThreads, rows_ctas(D)) pages_rows_kernel(c
         if (a.rec.slots == 1) {
             put_out(a, out * D + c, v, ml.y);
         } else {
-            const size_t at = (size_t)(a.slot0 + split) * a.rec.rows + out;
+            const size_t at = (size_t)split * a.rec.rows + out;
             *reinterpret_cast<float4*>(a.rec.o + at * D + c) = v;
             if (c == 0) a.rec.ml[at] = ml;
         }

@@ -226,6 +226,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
     const unsigned long long all = ((unsigned long long)sa.shared_tiles * sa.shared_units + before) * heads;
     if (all >= 1ull << 31) {  // only tables that name pages over and over
         if (tid == 0) raise(a.st, TYB_STATUS_BAD_ARGUMENT);
+        if (sa.beside) wait_for_predecessor();
         return;
     }
     const Runs cuts((unsigned int)all, min(gridDim.x, (unsigned int)all));
