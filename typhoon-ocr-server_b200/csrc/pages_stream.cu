@@ -502,7 +502,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
             continue;
         }
         // Others by all four together, once nobody needs the join rows.
-        if (!meet()) return;
+        if (!first_item && !meet()) return;
         w.put(joins + warp * sa.item_rows * S::kPitch, S::kPitch, join_mls[warp], nrows, g, t);
         w.clear();  // (and so not kept through what follows)
         if (!meet()) return;
@@ -632,7 +632,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
             }
         }
         // (these join rows, and parts_of, are written again only after another meeting, or by a direct item:)
-        if (!meet()) return;
+        if (more && !meet()) return;
     }
 }
 
