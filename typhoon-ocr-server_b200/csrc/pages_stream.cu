@@ -560,24 +560,27 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
             return __ffs(left) - 1;
         };
         constexpr int kDozen = 12;
+        // (with 64 columns a row needs half a warp: two at a time)
+        constexpr int kLanes = D / 4, kAtOnce = 32 / kLanes;
+        const int half = kAtOnce > 1 ? lane / kLanes : 0, in_half = lane - half * kLanes, c = in_half * 4, jobs = spread ? rows * shares : rows;
+        auto of_half = [&](auto x, int from) { return __shfl_sync(0xffffffffu, x, half * kLanes + from); };
 #pragma unroll 1
-        for (int j = warp; j < (spread ? rows * shares : rows); j += kTakers) {
-            const int row = spread ? j / shares : j, seq_of = row / a.group, in_head = row - seq_of * a.group;
+        for (int j0 = warp * kAtOnce; j0 < jobs; j0 += kTakers * kAtOnce) {
+            const int j = min(j0 + half, jobs - 1), row = spread ? j / shares : j, seq_of = row / a.group, in_head = row - seq_of * a.group;
             const int k = token_of(seq_of), tok = tile.tok0 + k;
             const Parts p = parts_of[k];
             const int ns = p.sh1 - p.sh0 + 1, n = ns + p.own1 - p.own0 + 1;
-            const int c = lane % (D / 4) * 4;  // D = 64: two lanes have the same columns
-            const int part0 = spread ? j - row * shares : 0, part1 = spread ? part0 + 1 : shares;
+            const int part0 = spread ? j - row * shares : 0, parts = spread ? 1 : shares;
             Gather sum;
 #pragma unroll 1
-            for (int part = part0; part < part1; part++) {
-                const int mine_n = (n - part + shares - 1) / shares;
+            for (int part = part0; part < part0 + parts; part++) {
+                const int mine_n = (n - part + shares - 1) / shares, most_n = max(mine_n, __shfl_xor_sync(0xffffffffu, mine_n, 16));
                 Gather share;
 #pragma unroll 1
-                for (int base = 0; base < mine_n; base += kDozen) {
-                    const int here = min(kDozen, mine_n - base);
-                    // lane y: record base + y of the warp's
-                    const int x = part + (base + min(lane, here - 1)) * shares, y = x - ns;
+                for (int base = 0; base < most_n; base += kDozen) {
+                    const int here = min(kDozen, mine_n - base);  // (0 or less: only the other half of the warp has any)
+                    // lane y: record base + y of the share
+                    const int x = min(part + (base + min(in_half, max(here, 1) - 1)) * shares, n - 1), y = x - ns;
                     int at;
                     if (x < ns) at = (ns == 1 ? shared_row(tok, tile.kvh) : part_row(p.sh0 + x, x ? 0 : p.sh_second)) + (tok - tok / per * per) * a.group;
                     else at = p.own0 == p.own1 ? own_row(tok, tile.kvh) : part_row(p.own0 + y, y ? 0 : p.own_second);
@@ -585,22 +588,21 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
                     float2 ml = __ldcg(&sa.rec_ml[at]);
                     float4 v[kDozen];
 #pragma unroll
-                    for (int i = 0; i < kDozen; i++)
-                        v[i] = __ldcg(reinterpret_cast<const float4*>(sa.rec_o + (size_t)__shfl_sync(0xffffffffu, at, i) * D + c));
-                    if (lane >= here) ml = make_float2(-INFINITY, 0.f);
+                    for (int i = 0; i < kDozen; i++) v[i] = __ldcg(reinterpret_cast<const float4*>(sa.rec_o + (size_t)of_half(at, i) * D + c));
+                    if (in_half >= here) ml = make_float2(-INFINITY, 0.f);
                     float top = ml.x;
 #pragma unroll
                     for (int d = 8; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-                    top = __shfl_sync(0xffffffffu, top, 0);
+                    top = of_half(top, 0);
                     const float f = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - top);
                     float l = ml.y * f;
 #pragma unroll
                     for (int d = 8; d; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
-                    l = __shfl_sync(0xffffffffu, l, 0);
+                    l = of_half(l, 0);
                     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
                     for (int i = 0; i < kDozen; i++) {
-                        const float fi = __shfl_sync(0xffffffffu, f, i);
+                        const float fi = of_half(f, i);
                         if (i < here) {
                             o.x = fmaf(v[i].x, fi, o.x);
                             o.y = fmaf(v[i].y, fi, o.y);
@@ -608,17 +610,16 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
                             o.w = fmaf(v[i].w, fi, o.w);
                         }
                     }
-                    share.add(make_float2(top, l), o);
+                    if (here > 0) share.add(make_float2(top, l), o);
                 }
                 sum.add(make_float2(share.m, share.l), share.o);
             }
-            if (lane < D / 4) {
-                if (spread) {
-                    *reinterpret_cast<float4*>(joins + (part0 * sa.item_rows + row) * S::kPitch + c) = sum.o;
-                    if (c == 0) join_mls[part0][row] = make_float2(sum.m, sum.l);
-                } else {
-                    deliver((size_t)(sa.tok_base + tok) * a.q_heads + tile.kvh * a.group + in_head, c, sum);
-                }
+            if (j0 + half >= jobs) continue;
+            if (spread) {
+                *reinterpret_cast<float4*>(joins + (part0 * sa.item_rows + row) * S::kPitch + c) = sum.o;
+                if (c == 0) join_mls[part0][row] = make_float2(sum.m, sum.l);
+            } else {
+                deliver((size_t)(sa.tok_base + tok) * a.q_heads + tile.kvh * a.group + in_head, c, sum);
             }
         }
         if (spread) {
