@@ -5,12 +5,14 @@
 #define TYB_WHOLE_PROGRAM
 #include "pages_mma.cuh"
 
+#include <type_traits>
+
 namespace tyb {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 
-// Joins the split records of each output row: a warp per row.
+// Joins the split records of each output row: a warp per row, four records (statistics and values) requested at a time.
 template <int D>
 __global__ void __launch_bounds__(kThreads) pages_join_kernel(const AttnArgs a)
 {
@@ -18,21 +20,35 @@ __global__ void __launch_bounds__(kThreads) pages_join_kernel(const AttnArgs a)
     const int R = (int)(blockIdx.x * kWarps + (threadIdx.x >> 5));
     after_predecessor();
     if (R >= a.rec.rows) return;
-    constexpr int kPer = D / 32;
-    float top = -INFINITY;
-    for (int s = lane; s < a.rec.slots; s += 32) top = fmaxf(top, a.rec.ml[(size_t)s * a.rec.rows + R].x);
+    constexpr int kPer = D / 32, kAtOnce = 4;
+    using Values = typename std::conditional<kPer == 4, float4, float2>::type;
+    float top = -INFINITY, acc[kPer] = {}, l = 0.f;
+    for (int s0 = 0; s0 < a.rec.slots; s0 += kAtOnce) {
+        float2 ml[kAtOnce];
+        Values o[kAtOnce];
 #pragma unroll
-    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    float acc[kPer] = {}, l = 0.f;
-#pragma unroll 4
-    for (int s = 0; s < a.rec.slots; s++) {
-        const float2 ml = a.rec.ml[(size_t)s * a.rec.rows + R];
-        const float f = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - top);
-        l = fmaf(ml.y, f, l);
-        const float* o = a.rec.o + ((size_t)s * a.rec.rows + R) * D + lane * kPer;
-        if (f != 0.f) {
+        for (int i = 0; i < kAtOnce; i++) {
+            const size_t at = (size_t)min(s0 + i, a.rec.slots - 1) * a.rec.rows + R;
+            ml[i] = a.rec.ml[at];
+            o[i] = *reinterpret_cast<const Values*>(a.rec.o + at * D + lane * kPer);
+        }
+        const float before = top;
 #pragma unroll
-            for (int i = 0; i < kPer; i++) acc[i] = fmaf(o[i], f, acc[i]);
+        for (int i = 0; i < kAtOnce; i++) {
+            if (s0 + i >= a.rec.slots) ml[i] = make_float2(-INFINITY, 0.f);
+            top = fmaxf(top, ml[i].x);
+        }
+        const float g = before == -INFINITY ? 0.f : fast_exp2(before - top);
+        l *= g;
+#pragma unroll
+        for (int x = 0; x < kPer; x++) acc[x] *= g;
+#pragma unroll
+        for (int i = 0; i < kAtOnce; i++) {
+            const float f = ml[i].x == -INFINITY ? 0.f : fast_exp2(ml[i].x - top);
+            l = fmaf(ml[i].y, f, l);
+            const float* v = reinterpret_cast<const float*>(&o[i]);
+#pragma unroll
+            for (int x = 0; x < kPer; x++) acc[x] = f == 0.f ? acc[x] : fmaf(v[x], f, acc[x]);  // (a record of nothing: no matter what lies there)
         }
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
