@@ -131,9 +131,9 @@ static Layout layout_of(const tyb_pages_attn* c)
         l.splits = (int)(kSms / ctas);  // one CTA fits an SM; a split has at least four tiles
         if (l.splits > tiles / 4) l.splits = tiles / 4;
     } else {
-        // Splits for twice as many CTAs as fit, each of at least two tiles (3 chunks of 37 .. 733 tokens through 301: with
-        // heads of 64 as many as fit 43 us, twice 45, three times 45; 12 of up to 300 through 1,200: 204, 141, 133; the first
-        // with heads of 128: as many as fit and half as many again 97, twice 98, three times 112).
+        // Splits for twice as many CTAs as fit, each of at least 64 keys.  As many as fit, twice, three times as many: 3 chunks of
+        // 37 .. 733 tokens through 301, heads of 64, 42, 44, 44 us; with heads of 128 80, 68, 75; 12 of up to 300 through 1,200,
+        // heads of 64, 204, 141, 131; one of 400 with 32 heads of 128 on 4 71, 72, 77.
         l.splits = (int)(2 * rows_ctas(c->p.head_dim) * kSms / ctas);
         if (l.splits > tiles / 2) l.splits = tiles / 2;
     }

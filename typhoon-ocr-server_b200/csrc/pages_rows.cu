@@ -1,5 +1,5 @@
 // pages_rows.cu -- prompt chunks over an FP32 paged cache, through a window with sinks: 64 query rows a CTA
-// (the q_heads / kv_heads heads of a KV head folded into the rows) against key tiles of 32.
+// (the q_heads / kv_heads heads of a KV head folded into the rows) against key tiles of 32 or 16.
 //
 // A requesting warp brings the tiles by TMA into a ring of stages; four warps with 16 query rows each take
 // every tile, with the running maximum and sum of an online softmax in base 2 (pages_mma.cuh: products on
@@ -13,18 +13,21 @@ namespace tyb {
 
 constexpr int kRowWarps = kRowsTile / 16;
 constexpr int kRowThreads = 32 * (kRowWarps + 1);
-constexpr int kTileKeys = 32;
 constexpr int kRowStagesMax = 6;
 
 template <int D>
 struct RowTile {
-    static constexpr int kBoxes = D / 32, kBox = kTileKeys * 128, kHalf = kBoxes * kBox, kStage = 2 * kHalf;
+    // Heads of 128: tiles of 16 keys, with which two CTAs fit an SM (3 chunks of 37 .. 733 tokens through 301: 68 us, with tiles of 32 96; 20 of 200 .. 900: 390, 552).  Heads
+    // of 64, where three fit either way: 44 / 42 us, 40 chunks 409 / 411.
+    static constexpr int kKeys = D == 64 ? 32 : 16;
+    static constexpr unsigned int kAll = 0xffffffffu >> (32 - kKeys);
+    static constexpr int kBoxes = D / 32, kBox = kKeys * 128, kHalf = kBoxes * kBox, kStage = 2 * kHalf;
     static constexpr int kPitch = D + 4;
     static constexpr int kSplit = 2 * 16 * kPitch * 4;  // a warp's query rows, hi and lo; at the end its output rows
 };
 
 struct RowMaps {
-    CUtensorMap m[2];  // K, V
+    CUtensorMap m[2];  // K, V; for tiles of 16 keys in boxes of 16 rows
 };
 
 // A lane's four columns of query rows: where they stand, and what of the tile at j0 they see.
@@ -71,19 +74,19 @@ __global__ void __launch_bounds__(kRowThreads, rows_ctas(D)) pages_rows_kernel(c
     if (pos0 < 0 && tid == 0) raise(a.st, TYB_STATUS_BAD_ARGUMENT);  // more queries than tokens
     auto lo_of_pos = [&](int pos) { return a.window ? max(0, pos - a.window + 1) : 0; };
     const int lo_min = lo_of_pos(pos0);
-    const Tiles tiles = tiles_of(pos_max, lo_min, a.sinks, kTileKeys);
+    const Tiles tiles = tiles_of(pos_max, lo_min, a.sinks, R::kKeys);
     const int all = tiles.count(), first = (int)((long long)all * split / a.splits), nt = (int)((long long)all * (split + 1) / a.splits) - first;
 
     if (warp == kRowWarps) {
         // ---- requests: lane (part, 128-byte column box, K or V)
-        const int part_rows = box_rows(a.p), parts = kTileKeys / part_rows, shift = page_shift(a.p.page_size);
+        const int part_rows = min(box_rows(a.p), R::kKeys), parts = R::kKeys / part_rows, shift = page_shift(a.p.page_size);
         const int part = lane & (parts - 1), box = lane / parts & (R::kBoxes - 1), which = lane / (parts * R::kBoxes);
         const int* table = a.p.table + (size_t)max(0, min(seq, a.p.max_seqs - 1)) * a.p.max_pages;
         int st = 0, t = 0;
         uint32_t phase = 0;
         bool ok = true;
         for (; t < nt; t++) {
-            const int key = tiles.at(first + t) * kTileKeys + part * part_rows;
+            const int key = tiles.at(first + t) * R::kKeys + part * part_rows;
             int page = which < 2 && key <= pos_max ? table[key >> shift] : -1;
             if (page >= a.p.num_pages) {
                 raise(a.st, TYB_STATUS_BAD_ARGUMENT);
@@ -100,9 +103,12 @@ __global__ void __launch_bounds__(kRowThreads, rows_ctas(D)) pages_rows_kernel(c
                 mbar_arrive_expect_tx(&full[st], (uint32_t)(__popc(have) * part_rows * 128));
             }
             __syncwarp();
-            if (page >= 0)
-                tma_load_2d(ring + st * R::kStage + which * R::kHalf + box * R::kBox + part * part_rows * 128, &maps.m[which], box * 32,
-                            ((layer * a.p.num_pages + page) * a.p.kv_heads + kvh) * a.p.page_size + (key & (a.p.page_size - 1)), &full[st]);
+            if (page >= 0) {
+                const int row = ((layer * a.p.num_pages + page) * a.p.kv_heads + kvh) * a.p.page_size + (key & (a.p.page_size - 1));
+                unsigned char* to = ring + st * R::kStage + which * R::kHalf + box * R::kBox + part * part_rows * 128;
+                if (R::kKeys == 16) tma_load_3d(to, &maps.m[which], row, box, &full[st]);
+                else tma_load_2d(to, &maps.m[which], box * 32, row, &full[st]);
+            }
             if (++st == stages) {
                 st = 0;
                 phase ^= 1u;
@@ -163,14 +169,14 @@ __global__ void __launch_bounds__(kRowThreads, rows_ctas(D)) pages_rows_kernel(c
     for (int i = 0; i < nt; i++) {
         ok = warp_wait_for(&full[st], phase, wait_ns, a.st);
         if (!ok) break;
-        const int k0 = tiles.at(first + i) * kTileKeys;
+        const int k0 = tiles.at(first + i) * R::kKeys;
         const unsigned int seen = seen_of[st];
         unsigned char *rows_k = ring + st * R::kStage, *rows_v = rows_k + R::kHalf;
         // Rows that no query of the CTA sees may hold anything, and 0 * NaN is not 0.  (Every warp clears them for
         // itself: the others write the same zeros.)
-        if (seen != 0xffffffffu || k0 + kTileKeys - 1 > pos_max || (k0 < lo_min && k0 + kTileKeys > a.sinks)) {
+        if (seen != R::kAll || k0 + R::kKeys - 1 > pos_max || (k0 < lo_min && k0 + R::kKeys > a.sinks)) {
 #pragma unroll 4
-            for (int x = lane; x < kTileKeys * (D / 4); x += 32) {
+            for (int x = lane; x < R::kKeys * (D / 4); x += 32) {
                 const int r = x / (D / 4), c = x % (D / 4), j = k0 + r;
                 if (!((seen >> r & 1u) && j <= pos_max && (j >= lo_min || j < a.sinks)))
                     *reinterpret_cast<uint4*>(rows_v + (c >> 3) * R::kBox + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
@@ -179,7 +185,7 @@ __global__ void __launch_bounds__(kRowThreads, rows_ctas(D)) pages_rows_kernel(c
             __syncwarp();
         }
 #pragma unroll 1
-        for (int r0 = 0; r0 < kTileKeys; r0 += 16) {
+        for (int r0 = 0; r0 < R::kKeys; r0 += 16) {
             sight.j0 = k0 + r0;
             sight.seen = seen >> r0 & 0xffffu;
             if (!sight.seen || sight.j0 > wpos_max || (sight.j0 + 16 <= wlo_min && sight.j0 >= a.sinks)) continue;  // nothing in sight
@@ -232,7 +238,7 @@ static int launch(const AttnArgs& a, int layer, int items, const void* maps, cud
         if (e != cudaSuccess) return (int)e;
         ready[dev] = true;
     }
-    return launch_after(pages_rows_kernel<D>, dim3(items, a.p.kv_heads, a.splits), kRowThreads, bytes, stream, *static_cast<const RowMaps*>(maps), a,
+    return launch_after(pages_rows_kernel<D>, dim3(items, a.p.kv_heads, a.splits), kRowThreads, bytes, stream, *reinterpret_cast<const RowMaps*>(static_cast<const CUtensorMap*>(maps) + (R::kKeys == 16 ? 4 : 0)), a,
                         layer, stages, tyb_wait_limit_of(dev));
 }
 
