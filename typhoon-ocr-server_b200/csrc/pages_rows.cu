@@ -17,8 +17,9 @@ constexpr int kRowStagesMax = 6;
 
 template <int D>
 struct RowTile {
-    // Heads of 128: tiles of 16 keys, with which two CTAs fit an SM (3 chunks of 37 .. 733 tokens through 301: 68 us, with tiles of 32 96; 20 of 200 .. 900: 390, 552).  Heads
-    // of 64, where three fit either way: 44 / 42 us, 40 chunks 409 / 411.
+    // Heads of 128: tiles of 16 keys, with which two CTAs fit an SM (3 chunks of 37 .. 733 tokens through 301: 68 us, with
+    // tiles of 32 96; 20 of 200 .. 900: 390 and 552).  Heads of 64, of which three fit either way: tiles of 32 (3 chunks
+    // 44 us, with 16 42; 40 chunks 409 and 411; 12 through 1,200 rows 140 and 141).
     static constexpr int kKeys = D == 64 ? 32 : 16;
     static constexpr unsigned int kAll = 0xffffffffu >> (32 - kKeys);
     static constexpr int kBoxes = D / 32, kBox = kKeys * 128, kHalf = kBoxes * kBox, kStage = 2 * kHalf;

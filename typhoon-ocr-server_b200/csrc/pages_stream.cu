@@ -14,10 +14,9 @@
 // An item that a run boundary cuts is joined by the CTA that finishes it last (records in the workspace, a
 // ticket per item); the order of that sum is by run, not by arrival, so results repeat exactly.
 //
-// Long items: 512 windows of 2,048 rows and 16 sinks in 611 us, 4.2 GB at the rate of a copy.  Short ones are bound by
-// the stage's round trip (request, arrival, two warps' products, release) over a ring of three: 1.15 us a stage,
-// 256 x 8 items of 4.6 stages in 66 us on 116 SMs.  That was 97 us while the requesting warp divided by variables and
-// sent a copy per column box.
+// Long items: 512 windows of 2,048 rows and 16 sinks in 610 us, 4.2 GB at the rate of a copy.  Short ones are bound by
+// the stage's round trip (request, arrival, two warps' products, release) over a ring of three: 1.0 us a stage,
+// 256 x 8 items of 4.6 stages in 60 us on 116 SMs.
 //
 // The products (pages_mma.cuh) are mma.sync, with up to 16 query rows as columns.
 #define TYB_WHOLE_PROGRAM
