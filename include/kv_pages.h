@@ -8,14 +8,16 @@
  * them), so that requests about one document hold its rows once.  Everything the calls below
  * read and write is DEVICE memory, bookkeeping included: a call queues work on the library stream
  * (attn_set_stream) and returns; nothing is read back.  A call may be captured in a CUDA graph
- * once a call of the same sizes has run on that stream (it sizes the stream's workspace).
+ * once a call of the same sizes has been made on that pool (it sizes the pool's workspace; a captured
+ * call that would need more is refused).  Later calls of any size leave such a graph valid.
  *
  * Errors: what the host can see is refused with a nonzero return and attn_last_error().  What only
  * the device can see raises a bit that the next attn_sync() reports: a sequence, page or length
  * outside its bounds ("index check failed"), or a pool without enough free pages ("out of
  * pages").  A maintenance call that raises one changes nothing.
  *
- * A pool is driven from one stream at a time.
+ * A pool is driven from one stream at a time, replays of the graphs captured from it among the work
+ * that this counts.
  */
 #pragma once
 #include "kv_cache.h"
@@ -40,7 +42,8 @@ KVPages *kv_pages_alloc(int num_layers, int num_pages, int page_size, int kv_hea
  * bookkeeping is; kv_pages_release leaves that memory alone. */
 KVPages *kv_pages_attach(void *k, void *v, int *table, int *len, int *ref, int num_layers, int num_pages,
                          int page_size, int kv_heads, int head_dim, int max_seqs, int max_pages, int kv_dtype);
-/* Waits for the library stream, then frees the handle (and the memory that kv_pages_alloc made). */
+/* Waits for the library stream, then frees the handle, its workspace (what a captured call was given of
+ * that is kept until exit) and the memory that kv_pages_alloc made. */
 void     kv_pages_release(KVPages *p);
 
 /* ---- maintenance ------------------------------------------------------------------------

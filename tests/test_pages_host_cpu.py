@@ -1,0 +1,130 @@
+"""The host side of the paged cache (csrc/pages.c) over a CUDA runtime that only keeps books
+(pages_host_fake.c): what becomes of a pool's workspace, and what reaches a launch."""
+
+import ctypes
+import shutil
+import subprocess
+from pathlib import Path
+
+import pytest
+
+ROOT = Path(__file__).resolve().parents[1]
+VP = ctypes.c_void_p
+
+
+def cuda_headers():
+    for at in ("/usr/local/cuda/include",):
+        if (Path(at) / "cuda_runtime_api.h").exists():
+            return at
+    pytest.skip("no CUDA headers")
+
+
+@pytest.fixture(scope="module")
+def built(tmp_path_factory):
+    cc = shutil.which("gcc", path="/usr/bin") or shutil.which("gcc")
+    if not cc:
+        pytest.skip("no C compiler")
+    out = tmp_path_factory.mktemp("host") / "pages_host.so"
+    subprocess.run([cc, "-shared", "-fPIC", "-std=gnu11", "-w", "-g", "-I", str(ROOT / "include"), "-I", str(ROOT / "typhoon-ocr-server_b200" / "csrc"),
+                    "-I", cuda_headers(), str(ROOT / "typhoon-ocr-server_b200" / "csrc" / "pages.c"), str(ROOT / "tests" / "pages_host_fake.c"),
+                    "-o", str(out), "-Wl,-Bsymbolic", "-lpthread"], check=True)
+    return ctypes.CDLL(str(out))
+
+
+class Host:
+    def __init__(self, lib):
+        self.lib = lib
+        self.buf = (ctypes.c_char * 4096)()
+        self.at = (ctypes.addressof(self.buf) + 63) & ~63
+        lib.kv_pages_attach.restype = VP
+        lib.fake_error.restype = ctypes.c_char_p
+
+    def get(self, name, kind=ctypes.c_int):
+        return kind.in_dll(self.lib, name).value
+
+    def set(self, name, value):
+        ctypes.c_int.in_dll(self.lib, name).value = value
+
+    def pool(self, pages=8, entries=4):
+        a = VP(self.at)
+        h = self.lib.kv_pages_attach(a, a, a, a, a, 1, pages, 16, 2, 64, 3, entries, 1)
+        assert h, self.lib.fake_error()
+        return VP(h)
+
+    def attend(self, h, batch, window=0, sinks=0):
+        a = VP(self.at)
+        return self.lib.attention_pages_window_gqa(a, ctypes.c_longlong(128), h, 0, a, None, batch, batch, 2, 1, 64, window, sinks, a, 1,
+                                                   ctypes.c_float(1.0))
+
+    def ws(self):
+        return self.get("fake_ws", VP)
+
+    def tickets(self):
+        return self.get("fake_tickets", VP)
+
+    def live(self, p):
+        return bool(self.lib.fake_is_live(VP(p)))
+
+
+@pytest.fixture
+def host(built):
+    h = Host(built)
+    h.set("fake_capturing", 0)
+    h.lib.fake_stream(VP(0))
+    return h
+
+
+def test_what_a_captured_call_was_given_stays(host):
+    """A graph keeps the addresses of its calls: no later call, larger or on another stream, frees them."""
+    pool = host.pool()
+    assert host.attend(pool, 4) == 0
+    host.set("fake_capturing", 1)
+    assert host.attend(pool, 4) == 0
+    ws, tickets = host.ws(), host.tickets()
+    host.set("fake_capturing", 0)
+    assert host.attend(pool, 256) == 0
+    assert host.ws() != ws
+    assert host.live(ws) and host.live(tickets)
+    for s in range(1, 70):  # more streams than anything is kept for
+        host.lib.fake_stream(VP(64 * s))
+        assert host.attend(pool, 4) == 0
+        assert host.live(ws) and host.live(tickets)
+    assert host.lib.kv_pages_compact(pool, None) == 0
+    host.lib.kv_pages_release(pool)
+    assert host.live(ws) and host.live(tickets)
+
+
+def test_a_pools_workspace_is_its_own(host):
+    """Two pools driven on two streams, through graphs captured on one: no scratch, no tickets in common."""
+    a, b = host.pool(), host.pool()
+    given = []
+    for p in (a, b):
+        assert host.attend(p, 4) == 0
+        given += [host.ws(), host.tickets()]
+    assert len(set(given)) == 4
+    host.lib.kv_pages_release(a)
+    host.lib.kv_pages_release(b)
+
+
+def test_growing_and_releasing_leave_nothing_behind(host):
+    before = host.lib.fake_live()
+    pool = host.pool()
+    for n in (1, 30, 300, 2):
+        assert host.attend(pool, n) == 0
+    assert host.lib.fake_live() == before + 2
+    host.lib.kv_pages_release(pool)
+    assert host.lib.fake_live() == before
+
+
+def test_a_capture_is_refused_what_it_would_have_to_allocate(host):
+    pool = host.pool()
+    assert host.attend(pool, 4) == 0
+    host.set("fake_capturing", 1)
+    mallocs, syncs, memsets, launches = (host.get("fake_" + x) for x in ("mallocs", "syncs", "memsets", "launches"))
+    assert host.attend(pool, 400) != 0
+    assert b"captured" in host.lib.fake_error()
+    assert [host.get("fake_" + x) for x in ("mallocs", "syncs", "memsets", "launches")] == [mallocs, syncs, memsets, launches]
+    assert host.attend(pool, 4) == 0  # what fits goes on
+    host.set("fake_capturing", 0)
+    assert host.attend(pool, 400) == 0
+    host.lib.kv_pages_release(pool)

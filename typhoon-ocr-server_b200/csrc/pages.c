@@ -18,80 +18,81 @@
 
 #define TYB_PAGES_MAGIC 0x54594250u /* "TYBP" */
 
+enum { WS_SCRATCH, WS_TICKETS, WS_KINDS };
+
 typedef struct {
     KVPages pub; /* first: the KVPages* handed out converts back */
     uint32_t magic;
     int owned;
     tyb_pages_env env;
+    pthread_mutex_t lock;
+    struct {
+        void *p;
+        size_t bytes;
+        int captured;          /* a captured call was given it */
+        unsigned int timeouts; /* tickets: tyb_timeouts() when they were last known to be zero */
+    } ws[WS_KINDS];
     _Alignas(64) unsigned char maps[TYB_PAGES_MAPS_BYTES];
 } tyb_pages;
 
 /* ---- workspace ----------------------------------------------------------------------------
- * One buffer per (device, stream), so that calls on different streams never share one; work on one
- * stream uses it in turn.  Grown on demand (after waiting for the device), kept until exit. */
-#define TYB_PAGES_STREAMS 32
-static pthread_mutex_t g_lock = PTHREAD_MUTEX_INITIALIZER;
-enum { WS_SCRATCH, WS_TICKETS, WS_KINDS };
-static struct {
-    int used, device;
-    void *stream, *p[WS_KINDS];
-    size_t bytes[WS_KINDS];
-    unsigned int timeouts; /* tyb_timeouts() when the tickets were last known to be zero */
-} g_ws[TYB_PAGES_STREAMS];
-static int g_next;
+ * A pool has its own, since a pool is driven from one stream at a time: work queued by its calls, and
+ * the graphs captured from them, use it in turn, and calls on other pools never touch it.  It grows on
+ * demand (after waiting for the device), but not while the stream is captured, where an allocation
+ * would spoil the capture.  A buffer that a captured call was given is never freed or handed on: a graph
+ * may name it for as long as the process lives.  (Each is at least half as large again as the one it
+ * replaced, so those kept are at most twice the largest.) */
 
-/* The calling stream's buffer of a kind; tickets are zero when handed out.  NULL on failure (error set). */
-static void *workspace(int device, int kind, size_t bytes, const char *what)
+static int capturing(void)
 {
-    void *st = tyb_stream(), *p = NULL;
-    int at = -1;
-    pthread_mutex_lock(&g_lock);
-    for (int i = 0; i < TYB_PAGES_STREAMS && at < 0; i++)
-        if (g_ws[i].used && g_ws[i].device == device && g_ws[i].stream == st) at = i;
-    if (at < 0) { /* a slot of its own: a free one, else the one taken longest ago on this device */
-        for (int i = 0; i < TYB_PAGES_STREAMS && at < 0; i++)
-            if (!g_ws[i].used) at = i;
-        for (int i = 0; i < TYB_PAGES_STREAMS && at < 0; i++, g_next++)
-            if (g_ws[g_next % TYB_PAGES_STREAMS].device == device) at = g_next % TYB_PAGES_STREAMS;
-        if (at >= 0 && g_ws[at].used) {
-            cudaDeviceSynchronize(); /* it may still be in use */
-            for (int k = 0; k < WS_KINDS; k++) cudaFree(g_ws[at].p[k]);
-        }
-        if (at >= 0) {
-            memset(&g_ws[at], 0, sizeof g_ws[at]);
-            g_ws[at].used = 1;
-            g_ws[at].device = device;
-            g_ws[at].stream = st;
-        }
+    enum cudaStreamCaptureStatus state = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing((cudaStream_t)tyb_stream(), &state) != cudaSuccess) {
+        cudaGetLastError(); /* the default stream beside another's capture: the launch will say so */
+        return 0;
     }
-    if (at < 0) {
-        tyb_set_error("%s: workspaces of %d streams in use on other devices", what, TYB_PAGES_STREAMS);
-    } else {
-        if (g_ws[at].bytes[kind] < bytes) {
-            if (g_ws[at].p[kind]) {
-                cudaDeviceSynchronize();
-                cudaFree(g_ws[at].p[kind]);
-                g_ws[at].p[kind] = NULL;
-                g_ws[at].bytes[kind] = 0;
-            }
-            size_t want = 1 << 18;
+    return state != cudaStreamCaptureStatusNone;
+}
+
+static void give_back(tyb_pages *t, int kind)
+{
+    if (t->ws[kind].p && !t->ws[kind].captured) {
+        cudaDeviceSynchronize(); /* it may still be in use */
+        cudaFree(t->ws[kind].p);
+    }
+    memset(&t->ws[kind], 0, sizeof t->ws[kind]);
+}
+
+/* The pool's buffer of a kind; tickets are zero when handed out.  NULL on failure (error set). */
+static void *workspace(tyb_pages *t, int kind, size_t bytes, const char *what)
+{
+    void *p = NULL;
+    pthread_mutex_lock(&t->lock);
+    const int in_graph = capturing();
+    if (t->ws[kind].bytes < bytes) {
+        if (in_graph) {
+            tyb_set_error("%s: the pool's workspace is too small for this call, and cannot grow while the stream is captured: "
+                          "make a call of these sizes before", what);
+        } else {
+            size_t want = t->ws[kind].bytes ? t->ws[kind].bytes : 1 << 18;
             while (want < bytes) want += want / 2;
-            if (tyb_dev_alloc(&g_ws[at].p[kind], want, what)) {
-                g_ws[at].bytes[kind] = want;
-                if (kind == WS_TICKETS) g_ws[at].timeouts = tyb_timeouts() - 1; /* not zero yet */
-            }
-        }
-        p = g_ws[at].p[kind];
-        if (p && kind == WS_TICKETS && g_ws[at].timeouts != tyb_timeouts()) {
-            /* new, or a kernel gave up in mid-call since: it may not have put its tickets back */
-            g_ws[at].timeouts = tyb_timeouts();
-            if (!tyb_cuda_ok(cudaMemsetAsync(p, 0, g_ws[at].bytes[kind], (cudaStream_t)st), what)) {
-                g_ws[at].timeouts--;
-                p = NULL;
+            give_back(t, kind);
+            if (tyb_dev_alloc(&t->ws[kind].p, want, what)) {
+                t->ws[kind].bytes = want;
+                if (kind == WS_TICKETS) t->ws[kind].timeouts = tyb_timeouts() - 1; /* not zero yet */
             }
         }
     }
-    pthread_mutex_unlock(&g_lock);
+    if (t->ws[kind].bytes >= bytes) p = t->ws[kind].p;
+    if (p && in_graph) t->ws[kind].captured = 1;
+    if (p && kind == WS_TICKETS && t->ws[kind].timeouts != tyb_timeouts()) {
+        /* new, or a kernel gave up in mid-call since: it may not have put its tickets back */
+        t->ws[kind].timeouts = tyb_timeouts();
+        if (!tyb_cuda_ok(cudaMemsetAsync(p, 0, t->ws[kind].bytes, (cudaStream_t)tyb_stream()), what)) {
+            t->ws[kind].timeouts--;
+            p = NULL;
+        }
+    }
+    pthread_mutex_unlock(&t->lock);
     return p;
 }
 
@@ -157,6 +158,19 @@ static size_t slab_bytes(const KVPages *p)
            (p->kv_dtype == ATTN_KV_BF16 ? 2 : 4);
 }
 
+static void destroy(tyb_pages *t)
+{
+    if (t->owned) {
+        cudaFree(t->pub.k);
+        cudaFree(t->pub.v);
+        cudaFree(t->pub.table); /* table, len and ref are one allocation */
+    }
+    for (int k = 0; k < WS_KINDS; k++) give_back(t, k);
+    pthread_mutex_destroy(&t->lock);
+    t->magic = 0;
+    free(t);
+}
+
 static tyb_pages *make(const KVPages *dims, int owned, const char *what)
 {
     tyb_pages *t = (tyb_pages *)aligned_alloc(64, sizeof *t); /* the maps' alignment */
@@ -168,8 +182,9 @@ static tyb_pages *make(const KVPages *dims, int owned, const char *what)
     t->pub = *dims;
     t->magic = TYB_PAGES_MAGIC;
     t->owned = owned;
+    pthread_mutex_init(&t->lock, NULL);
     if (!tyb_cuda_ok(cudaGetDevice(&t->env.device), what)) {
-        free(t);
+        destroy(t);
         return NULL;
     }
     if (tyb_status_mirror_setup() != 0) cudaGetLastError(); /* as in kv_cache_alloc_ex */
@@ -177,21 +192,10 @@ static tyb_pages *make(const KVPages *dims, int owned, const char *what)
     t->env.mirror = tyb_status_mirror_device();
     if (!t->env.status) {
         tyb_set_error("%s: no status word on device %d", what, t->env.device);
-        free(t);
+        destroy(t);
         return NULL;
     }
     return t;
-}
-
-static void destroy(tyb_pages *t)
-{
-    if (t->owned) {
-        cudaFree(t->pub.k);
-        cudaFree(t->pub.v);
-        cudaFree(t->pub.table); /* table, len and ref are one allocation */
-    }
-    t->magic = 0;
-    free(t);
 }
 
 KVPages *kv_pages_alloc(int num_layers, int num_pages, int page_size, int kv_heads, int head_dim, int max_seqs,
@@ -278,7 +282,7 @@ int kv_pages_extend(KVPages *p, const int *seqs, const int *counts, int n)
     if (!t) return 1;
     if (!list_ready(seqs, n, "seqs", &rc, what)) return rc;
     if (!on_device(counts, 4, "counts", what)) return 1;
-    void *ws = workspace(t->env.device, WS_SCRATCH, tyb_pages_plan_bytes(p, n), what);
+    void *ws = workspace(t, WS_SCRATCH, tyb_pages_plan_bytes(p, n), what);
     return ws ? launched(tyb_pages_extend_launch(p, &t->env, seqs, counts, n, ws, tyb_stream()), what) : 1;
 }
 
@@ -289,7 +293,7 @@ static int fork_or_copy(KVPages *p, const int *src, const int *dst, int n, int d
     if (!t) return 1;
     if (!list_ready(src, n, "src", &rc, what)) return rc;
     if (!on_device(dst, 4, "dst", what)) return 1;
-    void *ws = workspace(t->env.device, WS_SCRATCH, tyb_pages_plan_bytes(p, n), what);
+    void *ws = workspace(t, WS_SCRATCH, tyb_pages_plan_bytes(p, n), what);
     return ws ? launched(tyb_pages_fork_launch(p, &t->env, src, dst, n, deep, ws, tyb_stream()), what) : 1;
 }
 
@@ -326,7 +330,7 @@ int kv_pages_compact(KVPages *p, int *live_out)
     const char *what = "kv_pages_compact";
     tyb_pages *t = pages_from(p, what);
     if (!t || (live_out && !on_device(live_out, 4, "live_out", what))) return 1;
-    void *ws = workspace(t->env.device, WS_SCRATCH, tyb_pages_plan_bytes(p, 0), what);
+    void *ws = workspace(t, WS_SCRATCH, tyb_pages_plan_bytes(p, 0), what);
     return ws ? launched(tyb_pages_compact_launch(p, live_out, ws, tyb_stream()), what) : 1;
 }
 
@@ -398,7 +402,7 @@ int kv_pages_import(KVPages *p, int seq, const KVCache *cache)
     for (int l = 0; l < KV_NUM_LAYERS; l++)
         if (!tyb_flush_pending(c, l, what)) return 1;
     if (rows == 0) return 0;
-    void *ws = workspace(t->env.device, WS_SCRATCH, tyb_pages_plan_bytes(p, 1), what);
+    void *ws = workspace(t, WS_SCRATCH, tyb_pages_plan_bytes(p, 1), what);
     if (!ws) return 1;
     return launched(tyb_pages_import_launch(p, &t->env, seq, c->k_slab, c->v_slab, cache->max_seq_len, rows, ws, tyb_stream()), what);
 }
@@ -436,8 +440,8 @@ static int attend(const KVPages *p, tyb_pages_attn *a, const char *what)
     a->env = t->env;
     size_t bytes, ticket_bytes;
     tyb_pages_attn_bytes(a, &bytes, &ticket_bytes);
-    void *ws = bytes ? workspace(t->env.device, WS_SCRATCH, bytes, what) : NULL;
-    void *tickets = ticket_bytes ? workspace(t->env.device, WS_TICKETS, ticket_bytes, what) : NULL;
+    void *ws = bytes ? workspace(t, WS_SCRATCH, bytes, what) : NULL;
+    void *tickets = ticket_bytes ? workspace(t, WS_TICKETS, ticket_bytes, what) : NULL;
     if ((bytes && !ws) || (ticket_bytes && !tickets)) return 1;
     return launched(tyb_pages_attn_launch(a, ws, tickets, tyb_stream()), what);
 }

@@ -31,6 +31,8 @@ def _ints(x, what):
 
 _raw_stream = torch._C._cuda_getCurrentRawStream  # what torch.cuda.current_stream().cuda_stream is, without the objects
 
+_dropped = []  # (library, handle, device) of pools that nobody closed
+
 
 class PagePool:
     """k, v [layers][pages][kv_heads][page_size][head_dim] (bfloat16 or float32); table [seqs][entries],
@@ -51,6 +53,10 @@ class PagePool:
         self._codes = {torch.float32: pkg.ATTN_DT_F32, torch.bfloat16: pkg.ATTN_DT_BF16}
         layers, pages, self.kv_heads, page, self.head_dim = k.shape
         dtype = pkg.ATTN_KV_BF16 if k.dtype == torch.bfloat16 else pkg.ATTN_KV_F32
+        while _dropped and not torch.cuda.is_current_stream_capturing():
+            old, handle, device = _dropped.pop()
+            with torch.cuda.device(device):
+                old.kv_pages_release(handle)
         with torch.cuda.device(self.device):
             self._handle = self.lib.kv_pages_attach(k.data_ptr(), v.data_ptr(), table.data_ptr(), length.data_ptr(),
                                                     ref.data_ptr(), layers, pages, page, self.kv_heads, self.head_dim,
@@ -69,12 +75,15 @@ class PagePool:
     def close(self):
         """Gives the handle back (after waiting for the stream); the tensors stay the caller's."""
         if self._handle:
-            self._stream()
-            self.lib.kv_pages_release(self._handle)
-            self._handle = None
+            handle, self._handle = self._handle, None
+            with torch.cuda.device(self.device):
+                self.lib.attn_set_stream(_raw_stream(self._index))
+                self.lib.kv_pages_release(handle)
 
-    def _stream(self):
-        self.lib.attn_set_stream(_raw_stream(self._index))
+    def __del__(self, dropped=_dropped):
+        # The collector may run anywhere, in a capture too, so this calls no CUDA: the next pool made gives the handle back.
+        if getattr(self, "_handle", None):
+            dropped.append((self.lib, self._handle, self.device))
 
     def _call(self, fn, *args):
         if not self._handle:
