@@ -8,6 +8,7 @@
 #include <stdio.h>
 #include <stdlib.h>
 #include <string.h>
+#include <unistd.h>
 
 #include "attn_ext.h"
 #include "host_internal.h"
@@ -21,6 +22,8 @@ char fake_foreign[64];
 int fake_syncs, fake_mallocs, fake_memsets, fake_launches;
 void *fake_ws, *fake_tickets;        /* what the last launch was given */
 int fake_window, fake_sinks;         /* of the last trim or attention launch */
+int fake_launch_us;                  /* how long a launch takes */
+int fake_overlaps, fake_lost;        /* launches while another one was on its way; that found their workspace freed */
 static void *g_stream;
 static char g_err[512];
 
@@ -119,6 +122,11 @@ int tyb_pages_maps(const KVPages *p, void *maps) { return 0; }
 size_t tyb_pages_plan_bytes(const KVPages *p, int n) { return 64 + 4u * (size_t)n + 16u * (size_t)p->num_pages; }
 static int launch(void *ws, void *tickets)
 {
+    static int inside;
+    if (__atomic_add_fetch(&inside, 1, __ATOMIC_SEQ_CST) > 1) __atomic_add_fetch(&fake_overlaps, 1, __ATOMIC_SEQ_CST);
+    if (fake_launch_us) usleep(fake_launch_us);
+    if ((ws && !fake_is_live(ws)) || (tickets && !fake_is_live(tickets))) __atomic_add_fetch(&fake_lost, 1, __ATOMIC_SEQ_CST);
+    __atomic_sub_fetch(&inside, 1, __ATOMIC_SEQ_CST);
     fake_ws = ws;
     fake_tickets = tickets;
     fake_launches++;

@@ -4,6 +4,7 @@
 import ctypes
 import shutil
 import subprocess
+import threading
 from pathlib import Path
 
 import pytest
@@ -127,4 +128,28 @@ def test_a_capture_is_refused_what_it_would_have_to_allocate(host):
     assert host.attend(pool, 4) == 0  # what fits goes on
     host.set("fake_capturing", 0)
     assert host.attend(pool, 400) == 0
+    host.lib.kv_pages_release(pool)
+
+
+def test_threads_that_share_a_pool_queue_whole_calls(host):
+    """A call may be several launches with one workspace: another thread's call on the pool comes before or after."""
+    pool = host.pool()
+    for x in ("overlaps", "lost"):
+        host.set("fake_" + x, 0)
+    host.set("fake_launch_us", 300)
+    a, n = VP(host.at), [0]
+    calls = [lambda i: host.lib.kv_pages_fork(pool, a, a, 1 + 100000 * i), lambda i: host.lib.kv_pages_compact(pool, None),
+             lambda i: host.attend(pool, 1 + 10 * i), lambda i: host.lib.kv_pages_free(pool, a, 1)]
+
+    def go(call):
+        for i in range(40):
+            n[0] += call(i) != 0
+
+    threads = [threading.Thread(target=go, args=(c,)) for c in calls]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    host.set("fake_launch_us", 0)
+    assert (n[0], host.get("fake_overlaps"), host.get("fake_lost")) == (0, 0, 0)
     host.lib.kv_pages_release(pool)

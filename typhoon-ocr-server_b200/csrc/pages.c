@@ -25,7 +25,7 @@ typedef struct {
     uint32_t magic;
     int owned;
     tyb_pages_env env;
-    pthread_mutex_t lock;
+    pthread_mutex_t lock; /* held from a call's workspace to its last launch */
     struct {
         void *p;
         size_t bytes;
@@ -37,7 +37,9 @@ typedef struct {
 
 /* ---- workspace ----------------------------------------------------------------------------
  * A pool has its own, since a pool is driven from one stream at a time: work queued by its calls, and
- * the graphs captured from them, use it in turn, and calls on other pools never touch it.  It grows on
+ * the graphs captured from them, use it in turn, and calls on other pools never touch it.  Its lock is held
+ * until a call's last launch, so that host threads that share the stream queue whole calls, and none loses
+ * to another's growth the buffer that it was just given.  It grows on
  * demand (after waiting for the device), but not while the stream is captured, where an allocation
  * would spoil the capture.  A buffer that a captured call was given is never freed or handed on: a graph
  * may name it for as long as the process lives.  (Each is at least half as large again as the one it
@@ -62,11 +64,11 @@ static void give_back(tyb_pages *t, int kind)
     memset(&t->ws[kind], 0, sizeof t->ws[kind]);
 }
 
-/* The pool's buffer of a kind; tickets are zero when handed out.  NULL on failure (error set). */
+/* The pool's buffer of a kind, its lock being held; tickets are zero when handed out.  NULL on failure
+ * (error set). */
 static void *workspace(tyb_pages *t, int kind, size_t bytes, const char *what)
 {
     void *p = NULL;
-    pthread_mutex_lock(&t->lock);
     const int in_graph = capturing();
     if (t->ws[kind].bytes < bytes) {
         if (in_graph) {
@@ -92,7 +94,6 @@ static void *workspace(tyb_pages *t, int kind, size_t bytes, const char *what)
             p = NULL;
         }
     }
-    pthread_mutex_unlock(&t->lock);
     return p;
 }
 
@@ -268,10 +269,18 @@ static int list_ready(const int *list, int n, const char *name, int *rc, const c
     return on_device(list, 4, name, what);
 }
 
-static int launched(int err, const char *what)
+/* Ends a call that holds the pool's lock. */
+static int launched(tyb_pages *t, int err, const char *what)
 {
-    if (!tyb_cuda_ok(err, what)) return 1;
-    return 0;
+    pthread_mutex_unlock(&t->lock);
+    return tyb_cuda_ok(err, what) ? 0 : 1;
+}
+
+/* The same for a call that was not given its workspace (error set). */
+static int not_launched(tyb_pages *t)
+{
+    pthread_mutex_unlock(&t->lock);
+    return 1;
 }
 
 int kv_pages_extend(KVPages *p, const int *seqs, const int *counts, int n)
@@ -282,8 +291,9 @@ int kv_pages_extend(KVPages *p, const int *seqs, const int *counts, int n)
     if (!t) return 1;
     if (!list_ready(seqs, n, "seqs", &rc, what)) return rc;
     if (!on_device(counts, 4, "counts", what)) return 1;
+    pthread_mutex_lock(&t->lock);
     void *ws = workspace(t, WS_SCRATCH, tyb_pages_plan_bytes(p, n), what);
-    return ws ? launched(tyb_pages_extend_launch(p, &t->env, seqs, counts, n, ws, tyb_stream()), what) : 1;
+    return ws ? launched(t, tyb_pages_extend_launch(p, &t->env, seqs, counts, n, ws, tyb_stream()), what) : not_launched(t);
 }
 
 static int fork_or_copy(KVPages *p, const int *src, const int *dst, int n, int deep, const char *what)
@@ -293,8 +303,9 @@ static int fork_or_copy(KVPages *p, const int *src, const int *dst, int n, int d
     if (!t) return 1;
     if (!list_ready(src, n, "src", &rc, what)) return rc;
     if (!on_device(dst, 4, "dst", what)) return 1;
+    pthread_mutex_lock(&t->lock);
     void *ws = workspace(t, WS_SCRATCH, tyb_pages_plan_bytes(p, n), what);
-    return ws ? launched(tyb_pages_fork_launch(p, &t->env, src, dst, n, deep, ws, tyb_stream()), what) : 1;
+    return ws ? launched(t, tyb_pages_fork_launch(p, &t->env, src, dst, n, deep, ws, tyb_stream()), what) : not_launched(t);
 }
 
 int kv_pages_fork(KVPages *p, const int *src, const int *dst, int n) { return fork_or_copy(p, src, dst, n, 0, "kv_pages_fork"); }
@@ -308,7 +319,8 @@ int kv_pages_free(KVPages *p, const int *seqs, int n)
     tyb_pages *t = pages_from(p, what);
     if (!t) return 1;
     if (!list_ready(seqs, n, "seqs", &rc, what)) return rc;
-    return launched(tyb_pages_free_launch(p, &t->env, seqs, n, tyb_stream()), what);
+    pthread_mutex_lock(&t->lock);
+    return launched(t, tyb_pages_free_launch(p, &t->env, seqs, n, tyb_stream()), what);
 }
 
 int kv_pages_trim(KVPages *p, const int *seqs, int n, int window, int sinks)
@@ -322,7 +334,8 @@ int kv_pages_trim(KVPages *p, const int *seqs, int n, int window, int sinks)
         return 1;
     }
     if (!list_ready(seqs, n, "seqs", &rc, what)) return rc;
-    return launched(tyb_pages_trim_launch(p, &t->env, seqs, n, window, sinks, tyb_stream()), what);
+    pthread_mutex_lock(&t->lock);
+    return launched(t, tyb_pages_trim_launch(p, &t->env, seqs, n, window, sinks, tyb_stream()), what);
 }
 
 int kv_pages_compact(KVPages *p, int *live_out)
@@ -330,8 +343,9 @@ int kv_pages_compact(KVPages *p, int *live_out)
     const char *what = "kv_pages_compact";
     tyb_pages *t = pages_from(p, what);
     if (!t || (live_out && !on_device(live_out, 4, "live_out", what))) return 1;
+    pthread_mutex_lock(&t->lock);
     void *ws = workspace(t, WS_SCRATCH, tyb_pages_plan_bytes(p, 0), what);
-    return ws ? launched(tyb_pages_compact_launch(p, live_out, ws, tyb_stream()), what) : 1;
+    return ws ? launched(t, tyb_pages_compact_launch(p, live_out, ws, tyb_stream()), what) : not_launched(t);
 }
 
 static int check_layer(const KVPages *p, int layer, const char *what)
@@ -373,7 +387,8 @@ int kv_pages_write(KVPages *p, int layer, const int *seqs, const int *starts, in
     if (!on_device(starts, 4, "starts", what) || !check_rows(k_new, in_dtype, stride, width, "k_new", what) ||
         !check_rows(v_new, in_dtype, stride, width, "v_new", what))
         return 1;
-    return launched(tyb_pages_write_launch(p, &t->env, layer, seqs, starts, n, rows, k_new, v_new, in_dtype == ATTN_DT_BF16, stride,
+    pthread_mutex_lock(&t->lock);
+    return launched(t, tyb_pages_write_launch(p, &t->env, layer, seqs, starts, n, rows, k_new, v_new, in_dtype == ATTN_DT_BF16, stride,
                                            tyb_stream()),
                     what);
 }
@@ -402,9 +417,10 @@ int kv_pages_import(KVPages *p, int seq, const KVCache *cache)
     for (int l = 0; l < KV_NUM_LAYERS; l++)
         if (!tyb_flush_pending(c, l, what)) return 1;
     if (rows == 0) return 0;
+    pthread_mutex_lock(&t->lock);
     void *ws = workspace(t, WS_SCRATCH, tyb_pages_plan_bytes(p, 1), what);
-    if (!ws) return 1;
-    return launched(tyb_pages_import_launch(p, &t->env, seq, c->k_slab, c->v_slab, cache->max_seq_len, rows, ws, tyb_stream()), what);
+    if (!ws) return not_launched(t);
+    return launched(t, tyb_pages_import_launch(p, &t->env, seq, c->k_slab, c->v_slab, cache->max_seq_len, rows, ws, tyb_stream()), what);
 }
 
 /* ---- attention ------------------------------------------------------------------------------ */
@@ -440,10 +456,11 @@ static int attend(const KVPages *p, tyb_pages_attn *a, const char *what)
     a->env = t->env;
     size_t bytes, ticket_bytes;
     tyb_pages_attn_bytes(a, &bytes, &ticket_bytes);
+    pthread_mutex_lock(&t->lock);
     void *ws = bytes ? workspace(t, WS_SCRATCH, bytes, what) : NULL;
     void *tickets = ticket_bytes ? workspace(t, WS_TICKETS, ticket_bytes, what) : NULL;
-    if ((bytes && !ws) || (ticket_bytes && !tickets)) return 1;
-    return launched(tyb_pages_attn_launch(a, ws, tickets, tyb_stream()), what);
+    if ((bytes && !ws) || (ticket_bytes && !tickets)) return not_launched(t);
+    return launched(t, tyb_pages_attn_launch(a, ws, tickets, tyb_stream()), what);
 }
 
 static int io_type(int io_dtype, const char *what)

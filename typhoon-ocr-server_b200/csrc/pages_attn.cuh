@@ -200,7 +200,9 @@ __device__ __forceinline__ void find_item(const AttnArgs& a, int x, int per, int
 // kStreamSeqs) of the call, with the shared pass over a.prefix rows in the same launch (`shared`); the
 // results are the output, or (out_slot >= 0) record slot out_slot of a.rec.  beside: 0, or the SMs that the
 // shared pass launched just before keeps busy: the launch then runs on the others at the same time, and waits for the
-// pass (which has waited for all before it) only at its end.  ws: stream_bytes; tickets: count * kv_heads words,
+// pass (which has waited for all before it) only at its end.  (A kernel that another host thread queues between the two
+// changes nothing of that: it has itself waited for the pass before it lets this launch start, and this one ends after
+// it.)  ws: stream_bytes; tickets: count * kv_heads words,
 // zero (and left so).
 constexpr int kStreamSeqs = 1024;
 // An item's start and end (its query, the join of the warps) cost a CTA about as much as this many stages:
