@@ -14,7 +14,9 @@
  * Errors: what the host can see is refused with a nonzero return and attn_last_error().  What only
  * the device can see raises a bit that the next attn_sync() reports: a sequence, page or length
  * outside its bounds ("index check failed"), or a pool without enough free pages ("out of
- * pages").  A maintenance call that raises one changes nothing.
+ * pages").  A maintenance call that raises one changes nothing.  A wait that ran out ("wait timed
+ * out") in a single-token attention call is raised again by those that follow on its pool, replays
+ * among them, until attn_sync() has reported it; from then on they are right.
  *
  * A pool is driven from one stream at a time, replays of the graphs captured from it among the work
  * that this counts.

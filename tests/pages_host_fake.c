@@ -65,7 +65,12 @@ cudaError_t cudaFree(void *p)
         }
     return cudaSuccess;
 }
-cudaError_t cudaMemset(void *p, int v, size_t n) { return fake_memsets++, cudaSuccess; }
+cudaError_t cudaMemset(void *p, int v, size_t n)
+{
+    fake_memsets++;
+    memset(p, v, n < 4096 ? n : 4096);
+    return cudaSuccess;
+}
 cudaError_t cudaMemsetAsync(void *p, int v, size_t n, cudaStream_t s) { return fake_memsets++, cudaSuccess; }
 cudaError_t cudaMemcpy(void *d, const void *s, size_t n, enum cudaMemcpyKind k) { return memcpy(d, s, n), cudaSuccess; }
 cudaError_t cudaDeviceSynchronize(void) { return fake_syncs++, cudaSuccess; }
@@ -108,7 +113,6 @@ int tyb_dev_alloc(void **p, size_t bytes, const char *what)
     *p = NULL;
     return tyb_cuda_ok(cudaMalloc(p, bytes), what);
 }
-unsigned int tyb_timeouts(void) { return 0; }
 static unsigned int g_word;
 int tyb_status_mirror_setup(void) { return 0; }
 unsigned int *tyb_status_word(void) { return &g_word; }
@@ -146,11 +150,12 @@ int tyb_pages_write_launch(const KVPages *p, const tyb_pages_env *env, int layer
                            const void *k_new, const void *v_new, int in_bf16, long long stride, void *stream) { return launch(0, 0); }
 int tyb_pages_import_launch(const KVPages *p, const tyb_pages_env *env, int seq, const void *k_slab, const void *v_slab, int row_capacity,
                             int rows, void *ws, void *stream) { return launch(ws, 0); }
-/* as much scratch as there are rows, a ticket for each (sequence, KV head) */
-void tyb_pages_attn_bytes(const tyb_pages_attn *a, size_t *ws, size_t *tickets)
+/* as much scratch as there are rows */
+size_t tyb_pages_ticket_bytes(const KVPages *p) { return 4096; }
+size_t tyb_pages_attn_bytes(const tyb_pages_attn *a, int *uses_tickets)
 {
-    *ws = 65536u * (size_t)a->rows;
-    *tickets = 4u * (size_t)a->batch * (size_t)a->p.kv_heads;
+    *uses_tickets = 1;
+    return 65536u * (size_t)a->rows;
 }
 int tyb_pages_attn_launch(const tyb_pages_attn *a, void *ws, void *tickets, void *stream)
 {

@@ -153,3 +153,23 @@ def test_threads_that_share_a_pool_queue_whole_calls(host):
     host.set("fake_launch_us", 0)
     assert (n[0], host.get("fake_overlaps"), host.get("fake_lost")) == (0, 0, 0)
     host.lib.kv_pages_release(pool)
+
+
+def test_tickets_after_a_wait_that_ran_out(host):
+    """Those of the pool whose kernel gave up are cleared, its mark too; another pool's, perhaps in use, are left."""
+    a, b = host.pool(), host.pool()
+    words = []
+    for p in (a, b):
+        assert host.attend(p, 4) == 0
+        words.append(ctypes.cast(host.tickets(), ctypes.POINTER(ctypes.c_uint32)))
+    for w in words:
+        w[16], w[40] = 3, 1
+    words[0][0] = 1
+    host.lib.tyb_pages_after_timeout()
+    assert [words[0][i] for i in (0, 16, 40)] == [0, 0, 0]
+    assert [words[1][i] for i in (0, 16, 40)] == [0, 3, 1]
+    words[1][0] = 1
+    host.lib.kv_pages_release(a)
+    host.lib.tyb_pages_after_timeout()
+    assert [words[1][i] for i in (0, 16, 40)] == [0, 0, 0]
+    host.lib.kv_pages_release(b)

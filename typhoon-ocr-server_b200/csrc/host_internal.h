@@ -173,9 +173,9 @@ int tyb_prefill_sharded(const void *q_raw, const void *k_raw, const void *v_raw,
                         int layer_idx, void *own_slot, int seq_len, float scale, float eps, int kv_head0, int kv_heads,
                         const void *xchg_dev, const void *xchg_maps, unsigned int epoch, const char *what);
 
-/* How many times a wait that ran out has been reported: after one, counters that kernels leave at zero
- * between launches may not be. */
-unsigned int tyb_timeouts(void);
+/* After a report of a wait that ran out: puts right what the kernels of page pools that gave up left half
+ * done (csrc/pages.c). */
+void tyb_pages_after_timeout(void);
 
 /* Wait for `stream`, then check the device status word.  1 when all is well;
  * otherwise 0 with the error set. */

@@ -18,9 +18,9 @@
 
 #define TYB_PAGES_MAGIC 0x54594250u /* "TYBP" */
 
-enum { WS_SCRATCH, WS_TICKETS, WS_KINDS };
+enum { WS_SCRATCH, WS_TICKETS, WS_KINDS }; /* tickets: tyb_pages_ticket_bytes, the same for every call of a pool */
 
-typedef struct {
+typedef struct tyb_pages_s {
     KVPages pub; /* first: the KVPages* handed out converts back */
     uint32_t magic;
     int owned;
@@ -29,9 +29,9 @@ typedef struct {
     struct {
         void *p;
         size_t bytes;
-        int captured;          /* a captured call was given it */
-        unsigned int timeouts; /* tickets: tyb_timeouts() when they were last known to be zero */
+        int captured; /* a captured call was given it */
     } ws[WS_KINDS];
+    struct tyb_pages_s *next; /* in g_pools */
     _Alignas(64) unsigned char maps[TYB_PAGES_MAPS_BYTES];
 } tyb_pages;
 
@@ -64,8 +64,8 @@ static void give_back(tyb_pages *t, int kind)
     memset(&t->ws[kind], 0, sizeof t->ws[kind]);
 }
 
-/* The pool's buffer of a kind, its lock being held; tickets are zero when handed out.  NULL on failure
- * (error set). */
+/* The pool's buffer of a kind, its lock being held; tickets are zero to begin with.  NULL on failure (error
+ * set). */
 static void *workspace(tyb_pages *t, int kind, size_t bytes, const char *what)
 {
     void *p = NULL;
@@ -80,21 +80,45 @@ static void *workspace(tyb_pages *t, int kind, size_t bytes, const char *what)
             give_back(t, kind);
             if (tyb_dev_alloc(&t->ws[kind].p, want, what)) {
                 t->ws[kind].bytes = want;
-                if (kind == WS_TICKETS) t->ws[kind].timeouts = tyb_timeouts() - 1; /* not zero yet */
+                if (kind == WS_TICKETS &&
+                    !tyb_cuda_ok(cudaMemsetAsync(t->ws[kind].p, 0, want, (cudaStream_t)tyb_stream()), what))
+                    give_back(t, kind);
             }
         }
     }
     if (t->ws[kind].bytes >= bytes) p = t->ws[kind].p;
     if (p && in_graph) t->ws[kind].captured = 1;
-    if (p && kind == WS_TICKETS && t->ws[kind].timeouts != tyb_timeouts()) {
-        /* new, or a kernel gave up in mid-call since: it may not have put its tickets back */
-        t->ws[kind].timeouts = tyb_timeouts();
-        if (!tyb_cuda_ok(cudaMemsetAsync(p, 0, t->ws[kind].bytes, (cudaStream_t)tyb_stream()), what)) {
-            t->ws[kind].timeouts--;
-            p = NULL;
-        }
-    }
     return p;
+}
+
+/* The pools that there are, for tyb_pages_after_timeout. */
+static pthread_mutex_t g_pools_lock = PTHREAD_MUTEX_INITIALIZER;
+static tyb_pages *g_pools;
+
+/* A kernel whose wait ran out leaves tickets half counted, and says so in their first word; until that is
+ * zero again, kernels that would use them raise the same status instead.  Called when the status has been
+ * reported: clears those tickets, and of the other pools nothing (they may be in use on other streams).  The
+ * word goes last: a launch that is on its way meanwhile finds it set in some of its CTAs, which set it
+ * again, or in none, and then the tickets are all zero. */
+void tyb_pages_after_timeout(void)
+{
+    int dev = -1;
+    if (cudaGetDevice(&dev) != cudaSuccess) return;
+    pthread_mutex_lock(&g_pools_lock);
+    for (tyb_pages *t = g_pools; t; t = t->next) {
+        pthread_mutex_lock(&t->lock);
+        char *tickets = (char *)t->ws[WS_TICKETS].p;
+        unsigned int gave_up = 0;
+        if (tickets && t->env.device == dev && cudaDeviceSynchronize() == cudaSuccess &&
+            cudaMemcpy(&gave_up, tickets, sizeof gave_up, cudaMemcpyDeviceToHost) == cudaSuccess && gave_up) {
+            const size_t head = TYB_PAGES_TICKET_HEAD;
+            if (cudaMemset(tickets + head, 0, t->ws[WS_TICKETS].bytes - head) == cudaSuccess && cudaDeviceSynchronize() == cudaSuccess &&
+                cudaMemset(tickets, 0, head) == cudaSuccess)
+                cudaDeviceSynchronize();
+        }
+        pthread_mutex_unlock(&t->lock);
+    }
+    pthread_mutex_unlock(&g_pools_lock);
 }
 
 /* ---- handles ------------------------------------------------------------------------------- */
@@ -161,6 +185,13 @@ static size_t slab_bytes(const KVPages *p)
 
 static void destroy(tyb_pages *t)
 {
+    pthread_mutex_lock(&g_pools_lock);
+    for (tyb_pages **at = &g_pools; *at; at = &(*at)->next)
+        if (*at == t) {
+            *at = t->next;
+            break;
+        }
+    pthread_mutex_unlock(&g_pools_lock);
     if (t->owned) {
         cudaFree(t->pub.k);
         cudaFree(t->pub.v);
@@ -196,6 +227,10 @@ static tyb_pages *make(const KVPages *dims, int owned, const char *what)
         destroy(t);
         return NULL;
     }
+    pthread_mutex_lock(&g_pools_lock);
+    t->next = g_pools;
+    g_pools = t;
+    pthread_mutex_unlock(&g_pools_lock);
     return t;
 }
 
@@ -454,12 +489,12 @@ static int attend(const KVPages *p, tyb_pages_attn *a, const char *what)
     a->p = *p;
     a->maps = t->maps;
     a->env = t->env;
-    size_t bytes, ticket_bytes;
-    tyb_pages_attn_bytes(a, &bytes, &ticket_bytes);
+    int uses_tickets;
+    const size_t bytes = tyb_pages_attn_bytes(a, &uses_tickets);
     pthread_mutex_lock(&t->lock);
     void *ws = bytes ? workspace(t, WS_SCRATCH, bytes, what) : NULL;
-    void *tickets = ticket_bytes ? workspace(t, WS_TICKETS, ticket_bytes, what) : NULL;
-    if ((bytes && !ws) || (ticket_bytes && !tickets)) return not_launched(t);
+    void *tickets = uses_tickets ? workspace(t, WS_TICKETS, tyb_pages_ticket_bytes(p), what) : NULL;
+    if ((bytes && !ws) || (uses_tickets && !tickets)) return not_launched(t);
     return launched(t, tyb_pages_attn_launch(a, ws, tickets, tyb_stream()), what);
 }
 

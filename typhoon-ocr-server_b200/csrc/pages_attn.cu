@@ -177,13 +177,15 @@ static size_t record_bytes(const AttnArgs& a, const Layout& l)
 
 using namespace tyb;
 
-extern "C" void tyb_pages_attn_bytes(const tyb_pages_attn* c, size_t* ws, size_t* tickets)
+extern "C" size_t tyb_pages_ticket_bytes(const KVPages* p) { return TYB_PAGES_TICKET_HEAD + (size_t)kStreamSeqs * p->kv_heads * sizeof(unsigned int); }
+
+extern "C" size_t tyb_pages_attn_bytes(const tyb_pages_attn* c, int* uses_tickets)
 {
     const Layout l = layout_of(c);
     const AttnArgs a = args_of(c, l);
     const int count = c->batch < kStreamSeqs ? c->batch : kStreamSeqs;
-    *ws = (record_bytes(a, l) + 255) / 256 * 256 + (l.tokens ? stream_bytes(a, count, l.shared) : 0);
-    *tickets = l.tokens ? (size_t)count * c->p.kv_heads * sizeof(unsigned int) : 0;
+    *uses_tickets = l.tokens;
+    return (record_bytes(a, l) + 255) / 256 * 256 + (l.tokens ? stream_bytes(a, count, l.shared) : 0);
 }
 
 extern "C" int tyb_pages_attn_launch(const tyb_pages_attn* c, void* ws, void* tickets, void* stream)

@@ -202,8 +202,8 @@ __device__ __forceinline__ void find_item(const AttnArgs& a, int x, int per, int
 // shared pass launched just before keeps busy: the launch then runs on the others at the same time, and waits for the
 // pass (which has waited for all before it) only at its end.  (A kernel that another host thread queues between the two
 // changes nothing of that: it has itself waited for the pass before it lets this launch start, and this one ends after
-// it.)  ws: stream_bytes; tickets: count * kv_heads words,
-// zero (and left so).
+// it.)  ws: stream_bytes; tickets: the pool's, its head
+// first (zero between launches unless one gave up).
 constexpr int kStreamSeqs = 1024;
 // An item's start and end (its query, the join of the warps) cost a CTA about as much as this many stages:
 // runs are cut by stages plus this for each item.  Measured with 256 sequences of 1 .. 512 rows (4.6 stages on

@@ -68,9 +68,12 @@ typedef struct {
     float scale;
 } tyb_pages_attn;
 
-/* Bytes of workspace and of tickets (words that are zero between launches; a launch that ended in a
- * status may leave them otherwise) of a call. */
-void tyb_pages_attn_bytes(const tyb_pages_attn *a, size_t *ws, size_t *tickets);
+/* Bytes of workspace of a call, and whether it uses the pool's tickets. */
+size_t tyb_pages_attn_bytes(const tyb_pages_attn *a, int *uses_tickets);
+/* Tickets of a pool: a head, whose first word is set by a kernel that gave up (its tickets may then be half
+ * counted: tyb_pages_after_timeout), then words that are zero between launches. */
+#define TYB_PAGES_TICKET_HEAD 64
+size_t tyb_pages_ticket_bytes(const KVPages *p);
 int tyb_pages_attn_launch(const tyb_pages_attn *a, void *ws, void *tickets, void *stream);
 
 #ifdef __cplusplus

@@ -86,6 +86,7 @@ struct StreamArgs {
     // items too: [batch * q_heads] own rows, then [shared_tiles * kv_heads][16] shared ones.
     float* rec_o;
     float2* rec_ml;
+    unsigned int* gave_up;  // not zero: a wait ran out in a launch before, whose tickets may be half counted
     unsigned int* tickets;  // [batch * kv_heads], zero between launches
     unsigned long long wait_ns;
 };
@@ -174,6 +175,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
     } else {
         after_predecessor();
     }
+    unsigned int gave_up = __ldcg(sa.gave_up);  // (wanted further down, with the lengths)
     // Units of each sequence's own rows: kItemUnits, then its stages, of which it has one at least, so that every
     // output row has an owner.
     auto own_lo = [&](int len) { return a.window ? max(0, len - a.window) : min(a.prefix, len); };
@@ -206,7 +208,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
             if (lane >= o) sum += y;
         }
         if (lane == 31) scan[warp] = sum;
-        __syncthreads();
+        gave_up = __syncthreads_or((int)gave_up);
         int at = sum - n;
 #pragma unroll
         for (int w = 0; w < kStreamThreads / 32; w++) {
@@ -222,6 +224,14 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
     }
     if (tid == 0) cum[a.batch] = (int)before;
     __syncthreads();
+    if (gave_up) {
+        if (tid == 0) {
+            atomicOr(sa.gave_up, 1u);
+            raise(a.st, TYB_STATUS_WAIT_TIMEOUT);
+        }
+        if (sa.beside) wait_for_predecessor();
+        return;
+    }
     const unsigned long long all = ((unsigned long long)sa.shared_tiles * sa.shared_units + before) * heads;
     if (all >= 1ull << 31) {  // only tables that name pages over and over
         if (tid == 0) raise(a.st, TYB_STATUS_BAD_ARGUMENT);
@@ -233,6 +243,13 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
     const unsigned int shared_all = (unsigned int)sa.shared_tiles * sa.shared_units * heads;
     const unsigned int begin = cuts.start(run), end = cuts.start(run + 1);
     const int per = 16 / a.group;  // tokens of a shared row tile
+
+    // A wait, by all lanes of a warp.
+    auto waited = [&](uint64_t* bar, uint32_t parity, uint64_t limit_ns) {
+        const bool ok = warp_wait_for(bar, parity, limit_ns, a.st);
+        if (!ok && lane == 0) atomicOr(sa.gave_up, 1u);
+        return ok;
+    };
 
     if (warp == kTakers) {
         // ---- requests
@@ -342,7 +359,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
         next();
         while (more) {
             if (sent >= (unsigned int)sa.stages) {
-                ok = warp_wait_for(&empty[st], phase ^ 1u, sa.wait_ns, a.st);
+                ok = waited(&empty[st], phase ^ 1u, sa.wait_ns);
                 if (!ok) break;
             }
             if (page >= max_page) {
@@ -382,7 +399,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
         // The copies requested have landed before this warp, and with it the CTA, ends.
         const unsigned int all_stages = sa.stages;
         for (unsigned int n = sent > all_stages ? sent - all_stages : 0; n < sent; n++)
-            warp_wait_for(&full[n % all_stages], n / all_stages & 1u, drain_ns(sa.wait_ns), a.st);
+            waited(&full[n % all_stages], n / all_stages & 1u, drain_ns(sa.wait_ns));
         if (sa.beside) wait_for_predecessor();  // so that the end of this kernel is the end of that one as well
         return;
     }
@@ -407,7 +424,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
     uint32_t meeting = 0;
     auto meet = [&]() {
         warp_arrive(&met);
-        const bool ok = warp_wait_for(&met, meeting, sa.wait_ns, a.st);
+        const bool ok = waited(&met, meeting, sa.wait_ns);
         meeting ^= 1u;
         return ok;
     };
@@ -430,7 +447,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
         return sum;
     };
     for (bool more = true; more;) {
-        if (!warp_wait_for(&full[st], phase, sa.wait_ns, a.st)) return;
+        if (!waited(&full[st], phase, sa.wait_ns)) return;
         const Stage stage = stages_of[st];
         if ((stage.flags & kFirst) && ++item_at == kItemRing) item_at = 0;
         const Item& tile = items[item_at];
@@ -478,7 +495,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
         const bool cut = tile.c0 != tile.c1, direct = !cut && !sa.shared_tiles;
         if (direct && !split_rows) {
             // An item to itself: each warp leaves its rows and goes on to the next item; the last to do so joins them.
-            if (direct_items > 0 && !warp_wait_for(&joined, (uint32_t)(direct_items - 1) & 1u, sa.wait_ns, a.st)) return;
+            if (direct_items > 0 && !waited(&joined, (uint32_t)(direct_items - 1) & 1u, sa.wait_ns)) return;
             direct_items++;
             w.put(joins + warp * sa.item_rows * S::kPitch, S::kPitch, join_mls[warp], nrows, g, t);
             w.clear();
@@ -711,7 +728,8 @@ int launch_stream(const AttnArgs& a, int layer, int first, int count, bool share
     sa.beside = beside;
     sa.rec_o = static_cast<float*>(ws);
     sa.rec_ml = reinterpret_cast<float2*>(sa.rec_o + record_rows(a, count, shared) * D);
-    sa.tickets = tickets;
+    sa.gave_up = tickets;
+    sa.tickets = tickets + TYB_PAGES_TICKET_HEAD / sizeof(unsigned int);
     sa.wait_ns = tyb_wait_limit_of(a.device);
     if (a.p.kv_dtype == TYB_BF16)
         return D == 128 ? launch_stream_t<__nv_bfloat16, 128>(sa, maps, stream) : launch_stream_t<__nv_bfloat16, 64>(sa, maps, stream);

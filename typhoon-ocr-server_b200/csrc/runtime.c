@@ -287,10 +287,6 @@ int tyb_prefetch_rows(const void *cache, int layer, int rows)
 
 /* ---- synchronisation + status ----------------------------------------------------- */
 
-static unsigned int g_timeouts;
-
-unsigned int tyb_timeouts(void) { return __atomic_load_n(&g_timeouts, __ATOMIC_RELAXED); }
-
 int tyb_finish(void *stream, const char *what)
 {
     unsigned int bits = 0;
@@ -308,7 +304,7 @@ int tyb_finish(void *stream, const char *what)
     int e = tyb_status_fetch(&bits, stream);
     if (!tyb_cuda_ok(e, what)) return 0;
     if (g_last_write.stream == stream) g_last_write.valid = 0; /* everything queued is done */
-    if (bits & TYB_STATUS_WAIT_TIMEOUT) __atomic_add_fetch(&g_timeouts, 1, __ATOMIC_RELAXED);
+    if (bits & TYB_STATUS_WAIT_TIMEOUT) tyb_pages_after_timeout();
     if (bits) {
         tyb_set_error("%s: device status 0x%x (%s%s%s)", what, bits,
                       (bits & TYB_STATUS_WAIT_TIMEOUT) ? "wait timed out " : "",
