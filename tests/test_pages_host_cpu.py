@@ -173,3 +173,15 @@ def test_tickets_after_a_wait_that_ran_out(host):
     host.lib.tyb_pages_after_timeout()
     assert [words[1][i] for i in (0, 16, 40)] == [0, 0, 0]
     host.lib.kv_pages_release(b)
+
+
+@pytest.mark.parametrize("sinks", [2**31 - 1, 2**31 - 16, 65, 64])
+def test_sinks_beyond_a_table_reach_no_kernel(host, sinks):
+    """A kernel rounds the sinks up to pages in 32 bits: past 2^31 - page_size that would be a row far before the table."""
+    pool = host.pool(entries=4)
+    a = VP(host.at)
+    assert host.lib.kv_pages_trim(pool, a, 1, 1, sinks) == 0
+    assert host.get("fake_sinks") == 4 * 16
+    assert host.lib.kv_pages_trim(pool, a, 1, 2**31 - 1, 5) == 0
+    assert (host.get("fake_window"), host.get("fake_sinks")) == (2**31 - 1, 5)
+    host.lib.kv_pages_release(pool)

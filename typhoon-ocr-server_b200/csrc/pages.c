@@ -369,6 +369,8 @@ int kv_pages_trim(KVPages *p, const int *seqs, int n, int window, int sinks)
         return 1;
     }
     if (!list_ready(seqs, n, "seqs", &rc, what)) return rc;
+    /* more than a sequence can have keeps it all; the kernel rounds it up to pages in 32 bits */
+    if (sinks > p->max_pages * p->page_size) sinks = p->max_pages * p->page_size;
     pthread_mutex_lock(&t->lock);
     return launched(t, tyb_pages_trim_launch(p, &t->env, seqs, n, window, sinks, tyb_stream()), what);
 }

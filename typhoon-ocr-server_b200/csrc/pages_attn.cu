@@ -124,7 +124,8 @@ static Layout layout_of(const tyb_pages_attn* c)
     const int per = (l.tall ? kTcTall : l.tc ? kTcWide : kRowsTile) / group;
     // Each of the sequences of a call ends in a tile of its own; no list has more tiles than this.
     l.row_tiles = l.tokens ? ceil_div(c->batch, per) : (int)((c->rows + (long long)c->batch * (per - 1)) / per);
-    const long long keys = l.tokens ? c->prefix : c->window && c->window < c->max_len ? c->window + c->sinks : c->max_len;
+    const long long in_view = c->window ? (long long)c->window + c->sinks : c->max_len;
+    const long long keys = l.tokens ? c->prefix : in_view < c->max_len ? in_view : c->max_len;
     const int tiles = ceil_div(keys, l.tc ? 64 : 32);
     const long long ctas = (long long)l.row_tiles * c->p.kv_heads;
     if (l.tc) {
