@@ -138,8 +138,9 @@ static int launch(void *ws, void *tickets)
 }
 int tyb_pages_extend_launch(const KVPages *p, const tyb_pages_env *env, const int *seqs, const int *counts, int n, void *ws, void *stream) { return launch(ws, 0); }
 int tyb_pages_fork_launch(const KVPages *p, const tyb_pages_env *env, const int *src, const int *dst, int n, int deep, void *ws, void *stream) { return launch(ws, 0); }
-int tyb_pages_free_launch(const KVPages *p, const tyb_pages_env *env, const int *seqs, int n, void *stream) { return launch(0, 0); }
-int tyb_pages_trim_launch(const KVPages *p, const tyb_pages_env *env, const int *seqs, int n, int window, int sinks, void *stream)
+size_t tyb_pages_release_bytes(int n) { return n > 256 ? 1024 : 0; }
+int tyb_pages_free_launch(const KVPages *p, const tyb_pages_env *env, const int *seqs, int n, void *ws, void *stream) { return launch(ws, 0); }
+int tyb_pages_trim_launch(const KVPages *p, const tyb_pages_env *env, const int *seqs, int n, int window, int sinks, void *ws, void *stream)
 {
     fake_window = window;
     fake_sinks = sinks;

@@ -1,0 +1,109 @@
+"""A maintenance call that a single entry of its list makes wrong changes nothing, wherever that entry stands."""
+
+import importlib
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+BF = torch.bfloat16
+
+
+@pytest.fixture(scope="module")
+def pages(pkg, lib):
+    return importlib.import_module(pkg.__name__ + ".pages")
+
+
+def ints(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def outcome(pkg, lib):
+    rc = lib.attn_sync()
+    msg = pkg.last_error(lib) if rc else ""
+    lib.attn_clear_error()
+    return msg
+
+
+PAGE = 16
+
+
+def pool_of(pages, seqs, entries=20):
+    """`seqs` sequences of 3 .. 300 tokens, and two that are not in use."""
+    lens = [3 + 31 * i % 298 for i in range(seqs)]
+    pool = pages.PagePool.empty(1, sum(-(-n // PAGE) for n in lens) + 50, PAGE, 1, 64, seqs + 2, entries, BF)
+    pool.extend(ints(list(range(seqs))), ints(lens))
+    return pool
+
+
+def books(pool):
+    return [x.clone() for x in (pool.table, pool.len, pool.ref)]
+
+
+def same(a, b):
+    return all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+CALLS = {"free": lambda pool, s: pool.free(s), "trim": lambda pool, s: pool.trim(s, 20, 17)}
+
+
+@pytest.mark.parametrize("call", list(CALLS))
+@pytest.mark.parametrize("seqs", [2, 7, 255, 256, 257, 700])
+@pytest.mark.parametrize("bad", [-1, 10**6, -(2**31), 2**31 - 1])
+def test_a_number_that_is_no_sequence(pkg, lib, pages, call, seqs, bad):
+    pool = pool_of(pages, seqs)
+    before = books(pool)
+    for at in {0, 1, seqs // 2, seqs - 1}:
+        wrong = list(range(seqs))
+        wrong[at] = bad
+        CALLS[call](pool, ints(wrong))
+        assert "index check failed" in outcome(pkg, lib)
+        assert same(books(pool), before), at
+    CALLS[call](pool, ints(list(range(seqs))))
+    assert outcome(pkg, lib) == ""
+    assert same(books(pool), before) == (call == "trim" and seqs == 2)  # (3 and 34 tokens: nothing to trim)
+
+
+@pytest.mark.parametrize("call", list(CALLS))
+@pytest.mark.parametrize("seqs", [1, 7, 256, 700])
+def test_a_table_that_names_no_page(pkg, lib, pages, call, seqs):
+    pool = pool_of(pages, seqs)
+    last = seqs - 1
+    pool.len[last] = 20 * PAGE
+    for entry in (2, 9, 17):  # of those that either call would take
+        keep = int(pool.table[last, entry])
+        for bad in (pool.ref.numel(), 2**31 - 1):
+            pool.table[last, entry] = bad
+            before = books(pool)
+            CALLS[call](pool, ints(list(range(seqs))))
+            assert "index check failed" in outcome(pkg, lib)
+            assert same(books(pool), before)
+        pool.table[last, entry] = keep
+    CALLS[call](pool, ints(list(range(seqs))))
+    assert outcome(pkg, lib) == ""
+
+
+@pytest.mark.parametrize("seqs", [3, 300])
+@pytest.mark.parametrize("bad", [-1, 20 * PAGE + 1, -(2**31), 2**31 - 1])
+def test_a_length_that_is_none(pkg, lib, pages, seqs, bad):
+    """Trim goes by it and refuses; free does not, and puts it right."""
+    pool = pool_of(pages, seqs)
+    pool.len[1] = bad
+    before, all_of = books(pool), ints(list(range(seqs)))
+    pool.trim(all_of, 20, 17)
+    assert "index check failed" in outcome(pkg, lib)
+    assert same(books(pool), before)
+    pool.free(all_of)
+    assert outcome(pkg, lib) == ""
+    assert int(pool.ref.abs().sum()) == 0 and int(pool.len.abs().sum()) == 0 and bool((pool.table == -1).all())
+
+
+@pytest.mark.parametrize("seqs", [1, 3, 100, 256, 300])
+def test_a_sequence_named_often_is_freed_once(pkg, lib, pages, seqs):
+    pool = pool_of(pages, 3)
+    pool.fork(ints([0]), ints([3]))
+    pool.free(ints([0] * seqs))
+    assert outcome(pkg, lib) == ""
+    assert pool.len.tolist()[0] == 0
+    named = pool.table[pool.table >= 0].long()
+    assert torch.equal(torch.bincount(named, minlength=pool.ref.numel()).to(torch.int32), pool.ref)

@@ -355,7 +355,10 @@ int kv_pages_free(KVPages *p, const int *seqs, int n)
     if (!t) return 1;
     if (!list_ready(seqs, n, "seqs", &rc, what)) return rc;
     pthread_mutex_lock(&t->lock);
-    return launched(t, tyb_pages_free_launch(p, &t->env, seqs, n, tyb_stream()), what);
+    const size_t bytes = tyb_pages_release_bytes(n);
+    void *ws = bytes ? workspace(t, WS_SCRATCH, bytes, what) : NULL;
+    if (bytes && !ws) return not_launched(t);
+    return launched(t, tyb_pages_free_launch(p, &t->env, seqs, n, ws, tyb_stream()), what);
 }
 
 int kv_pages_trim(KVPages *p, const int *seqs, int n, int window, int sinks)
@@ -372,7 +375,10 @@ int kv_pages_trim(KVPages *p, const int *seqs, int n, int window, int sinks)
     /* more than a sequence can have keeps it all; the kernel rounds it up to pages in 32 bits */
     if (sinks > p->max_pages * p->page_size) sinks = p->max_pages * p->page_size;
     pthread_mutex_lock(&t->lock);
-    return launched(t, tyb_pages_trim_launch(p, &t->env, seqs, n, window, sinks, tyb_stream()), what);
+    const size_t bytes = tyb_pages_release_bytes(n);
+    void *ws = bytes ? workspace(t, WS_SCRATCH, bytes, what) : NULL;
+    if (bytes && !ws) return not_launched(t);
+    return launched(t, tyb_pages_trim_launch(p, &t->env, seqs, n, window, sinks, ws, tyb_stream()), what);
 }
 
 int kv_pages_compact(KVPages *p, int *live_out)

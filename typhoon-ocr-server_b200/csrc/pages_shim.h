@@ -31,8 +31,9 @@ typedef struct {
 size_t tyb_pages_plan_bytes(const KVPages *p, int n);
 int tyb_pages_extend_launch(const KVPages *p, const tyb_pages_env *env, const int *seqs, const int *counts, int n, void *ws, void *stream);
 int tyb_pages_fork_launch(const KVPages *p, const tyb_pages_env *env, const int *src, const int *dst, int n, int deep, void *ws, void *stream);
-int tyb_pages_free_launch(const KVPages *p, const tyb_pages_env *env, const int *seqs, int n, void *stream);
-int tyb_pages_trim_launch(const KVPages *p, const tyb_pages_env *env, const int *seqs, int n, int window, int sinks, void *stream);
+size_t tyb_pages_release_bytes(int n); /* workspace of the next two */
+int tyb_pages_free_launch(const KVPages *p, const tyb_pages_env *env, const int *seqs, int n, void *ws, void *stream);
+int tyb_pages_trim_launch(const KVPages *p, const tyb_pages_env *env, const int *seqs, int n, int window, int sinks, void *ws, void *stream);
 int tyb_pages_compact_launch(const KVPages *p, int *live_out, void *ws, void *stream);
 int tyb_pages_write_launch(const KVPages *p, const tyb_pages_env *env, int layer, const int *seqs, const int *starts, int n, int rows,
                            const void *k_new, const void *v_new, int in_bf16, long long stride, void *stream);
