@@ -107,3 +107,27 @@ def test_a_sequence_named_often_is_freed_once(pkg, lib, pages, seqs):
     assert pool.len.tolist()[0] == 0
     named = pool.table[pool.table >= 0].long()
     assert torch.equal(torch.bincount(named, minlength=pool.ref.numel()).to(torch.int32), pool.ref)
+
+
+@pytest.mark.parametrize("deep", [False, True])
+@pytest.mark.parametrize("children,at", [(1, 0), (5, 4), (40, 33), (70, 69)])
+@pytest.mark.parametrize("entry", [0, 1, 37, 61, 62])
+def test_a_branch_of_a_table_that_names_no_page(pkg, lib, pages, deep, children, at, entry):
+    """Among the entries that the branch would share, or copy, of one source of the list."""
+    pool = pages.PagePool.empty(1, 70 * 63 + 200, PAGE, 1, 64, 80, 70, BF)
+    pool.extend(ints([0, 1]), ints([62 * PAGE + 5, 62 * PAGE + 3]))
+    src = [0] * children
+    src[at] = 1
+    src, dst = ints(src), ints(list(range(2, 2 + children)))
+    keep = int(pool.table[1, entry])
+    for bad in (pool.ref.numel(), 2**31 - 1):
+        pool.table[1, entry] = bad
+        before = books(pool)
+        (pool.copy if deep else pool.fork)(src, dst)
+        assert "index check failed" in outcome(pkg, lib)
+        assert same(books(pool), before)
+    pool.table[1, entry] = keep
+    (pool.copy if deep else pool.fork)(src, dst)
+    assert outcome(pkg, lib) == ""
+    named = pool.table[pool.table >= 0].long()
+    assert torch.equal(torch.bincount(named, minlength=pool.ref.numel()).to(torch.int32), pool.ref)

@@ -223,17 +223,20 @@ __global__ void __launch_bounds__(kPlanThreads)
     for (int i = threadIdx.x; !bad && i < n; i += kPlanThreads)
         if (marks[src[i] >> 5] >> (src[i] & 31) & 1u) bad = true;  // a source that the call also makes
     bad = __syncthreads_or(bad);
-    // How many pages each item takes (a warp per item), then where its first one stands.
-    for (int i = warp; !bad && i < n; i += kPlanWarps) {
-        const int s = src[i], len = p.len[s], e1 = entries_of(p, len);
+    // How many pages each item takes (a warp per item), then where its first one stands.  Entries that a branch shares are
+    // looked at too, once where a warp's items have the same source: they are to name pages that the pool has.
+    for (int i = warp, before = -1; !bad && i < n; i += kPlanWarps) {
+        const int s = src[i], len = p.len[s], e1 = entries_of(p, len), own = first_own_entry(p, len, deep);
         const int* row = p.table + (size_t)s * p.max_pages;
         int mine = 0;
         bool off = false;
-        for (int e = first_own_entry(p, len, deep) + lane; e < e1; e += 32) {
+#pragma unroll 4
+        for (int e = (s == before ? own : 0) + lane; e < e1; e += 32) {
             const int page = row[e];
-            mine += page >= 0;
+            mine += page >= 0 && e >= own;
             off |= page >= p.num_pages;
         }
+        before = s;
         bad |= __any_sync(0xffffffffu, off);
         mine = __reduce_add_sync(0xffffffffu, mine);
         if (lane == 0) plan.first[i] = mine;
@@ -328,7 +331,7 @@ __global__ void __launch_bounds__(kApplyThreads)
                 if (e >= own) {
                     page = plan.fresh[at + __popc(fresh & ((1u << lane) - 1u))];
                     p.ref[page] = 1;
-                } else if (page < p.num_pages) {
+                } else {
                     atomicAdd(&p.ref[page], 1);
                 }
             }
