@@ -14,9 +14,10 @@
  * Errors: what the host can see is refused with a nonzero return and attn_last_error().  What only
  * the device can see raises a bit that the next attn_sync() reports: a sequence, page or length
  * outside its bounds ("index check failed"), or a pool without enough free pages ("out of
- * pages").  A maintenance call that raises one changes nothing.  A wait that ran out ("wait timed
- * out") in a single-token attention call is raised again by those that follow on its pool, replays
- * among them, until attn_sync() has reported it; from then on they are right.
+ * pages").  A maintenance call that raises one changes nothing, except kv_pages_write: it writes the
+ * rows whose places are there, and raises one for the others.  A wait that ran out ("wait timed out")
+ * in a single-token attention call is raised again by those that follow on its pool, replays among
+ * them, until attn_sync() has reported it; from then on they are right.
  *
  * A pool is driven from one stream at a time, replays of the graphs captured from it among the work
  * that this counts.
@@ -56,7 +57,9 @@ void     kv_pages_release(KVPages *p);
  * rows are then written, layer by layer, with kv_pages_write).  A sequence appears once. */
 int kv_pages_extend(KVPages *p, const int *seqs, const int *counts, int n);
 /* The last starts[i + 1] - starts[i] rows of each sequence, from rows starts[i].. of k_new and v_new
- * [rows][kv_heads][head_dim] in `in_dtype` (ATTN_DT_*), rows `stride` elements apart; starts[n] = rows. */
+ * [rows][kv_heads][head_dim] in `in_dtype` (ATTN_DT_*), rows `stride` elements apart; starts[n] = rows.
+ * Each row is placed by itself: one without a place (no such sequence, not so long, its page given back)
+ * is reported and the others are written.  Table, lengths and counts stay as they are. */
 int kv_pages_write(KVPages *p, int layer, const int *seqs, const int *starts, int n, int rows, const void *k_new,
                    const void *v_new, int in_dtype, long long stride);
 /* Rows [0, cache->seq_len) of all 28 layers of a static cache become sequence `seq` (not in use

@@ -1,4 +1,5 @@
-"""A maintenance call that a single entry of its list makes wrong changes nothing, wherever that entry stands."""
+"""A maintenance call that a single entry of its list makes wrong changes nothing, wherever that entry stands; a write
+places row by row."""
 
 import importlib
 
@@ -131,3 +132,39 @@ def test_a_branch_of_a_table_that_names_no_page(pkg, lib, pages, deep, children,
     assert outcome(pkg, lib) == ""
     named = pool.table[pool.table >= 0].long()
     assert torch.equal(torch.bincount(named, minlength=pool.ref.numel()).to(torch.int32), pool.ref)
+
+
+@pytest.mark.parametrize("wrong", ["sequence", "length", "page given back", "page beyond the pool", "first start"])
+def test_a_write_places_what_has_a_place(pkg, lib, pages, wrong):
+    pool = pages.PagePool.empty(1, 12, PAGE, 2, 64, 4, 5, BF)
+    pool.extend(ints([0, 1, 2]), ints([40, 20, 33]))
+    for t in (pool.k, pool.v):
+        t.fill_(7)
+    k, v = (torch.randn((15, 2, 64), device="cuda").to(BF) for _ in range(2))
+    seqs, starts, placed = [0, 1, 2], [0, 5, 10, 15], [0, 2]  # items whose rows have places
+    if wrong == "sequence":
+        seqs[1] = 4
+    elif wrong == "length":
+        pool.len[1] = 4
+        placed = [0, (1, 1), 2]  # all but the first of its five rows
+    elif wrong == "page given back":
+        pool.table[1, 0] = -1  # rows 15 .. 19: row 15 lies in it
+        placed = [0, (1, 1), 2]
+    elif wrong == "page beyond the pool":
+        pool.table[1, 1] = 12  # and rows 16 .. 19 in this one
+        placed = [0, (1, 0, 1), 2]
+    else:
+        starts[0] = 2
+        placed = [(0, 2), 1, 2]
+    before, want = books(pool), [pool.k.clone(), pool.v.clone()]
+    pool.write(0, ints(seqs), ints(starts), k, v)
+    assert "index check failed" in outcome(pkg, lib)
+    for x in placed:
+        i, lo, hi = x if isinstance(x, tuple) and len(x) == 3 else (*x, 5) if isinstance(x, tuple) else (x, 0, 5)
+        for r in range(lo, hi):
+            at = int(before[1][seqs[i]]) - 5 + r
+            page = int(before[0][seqs[i], at // PAGE])
+            for t, new in zip(want, (k, v)):
+                t[0, page, :, at % PAGE] = new[5 * i + r]
+    assert torch.equal(pool.k, want[0]) and torch.equal(pool.v, want[1])
+    assert same(books(pool), before)

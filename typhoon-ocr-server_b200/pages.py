@@ -123,7 +123,8 @@ class PagePool:
                    seqs.numel())
 
     def write(self, layer, seqs, starts, k_new, v_new):
-        """The last starts[i + 1] - starts[i] rows of sequence seqs[i], from [rows][kv_heads][head_dim]."""
+        """The last starts[i + 1] - starts[i] rows of sequence seqs[i], from [rows][kv_heads][head_dim]; a row without a
+        place is reported by ``attn_sync`` and the others are written."""
         stride = self._tokens(k_new, self.kv_heads, "k_new")
         if v_new.shape != k_new.shape or v_new.dtype != k_new.dtype or self._tokens(v_new, self.kv_heads, "v_new") != stride:
             raise ValueError("v_new has to be like k_new")
