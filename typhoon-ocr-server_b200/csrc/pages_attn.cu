@@ -48,7 +48,8 @@ __global__ void __launch_bounds__(kThreads) pages_join_kernel(const AttnArgs a)
             l = fmaf(ml[i].y, f, l);
             const float* v = reinterpret_cast<const float*>(&o[i]);
 #pragma unroll
-            for (int x = 0; x < kPer; x++) acc[x] = f == 0.f ? acc[x] : fmaf(v[x], f, acc[x]);  // (a record of nothing: no matter what lies there)
+            for (int x = 0; x < kPer; x++) acc[x] = ml[i].x == -INFINITY ? acc[x] : fmaf(v[x], f, acc[x]);
+            // (what lies in a record of nothing does not matter; in one that only weighs nothing, rows may not be finite)
         }
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
