@@ -95,7 +95,9 @@ int kv_pages_compact(KVPages *p, int *live_out);
  * One token for each of `batch` sequences (their last one, its row written) that hold the same
  * first prefix_len tokens, in the same pages as far as those are full (what kv_pages_fork leaves):
  * the shared pages are read and multiplied once for all sequences, every sequence's further rows
- * by themselves, and the two parts joined.  All of len[seqs[b]] is seen. */
+ * by themselves, and the two parts joined.  All of len[seqs[b]] is seen.  A sequence that is shorter
+ * than the shared pages is reported ("index check failed"); one not in use may fill up a batch, though
+ * not as the first of any 1,024, and its output means nothing. */
 int attention_pages_prefix_gqa(const void *q, long long q_stride, const KVPages *p, int layer, const int *seqs,
                                int batch, int q_heads, int prefix_len, int max_len, void *output, int io_dtype,
                                float scale);

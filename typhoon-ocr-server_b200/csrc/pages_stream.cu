@@ -193,7 +193,9 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
 #pragma unroll
         for (int i = 0; i < kPer; i++)
             if (i < each && b0 + i < a.batch) {
-                if (len[i] > sa.max_len) {
+                // too long for the call's split, or without all of the shared rows (a sequence not in use aside, whose row means
+                // nothing, unless the shared rows are to be found by it)
+                if (len[i] > sa.max_len || (len[i] < a.prefix && (len[i] > 0 || b0 + i == 0))) {
                     raise(a.st, TYB_STATUS_BAD_ARGUMENT);
                     len[i] = 0;
                 }
