@@ -6,8 +6,8 @@
  * A pool holds `num_pages` pages of `page_size` rows for every layer; a sequence is a row of the
  * table that names its pages in order, and a page may be named by several sequences (ref counts
  * them), so that requests about one document hold its rows once.  Everything the calls below
- * read and write is DEVICE memory, bookkeeping included: a call queues work on the library stream
- * (attn_set_stream) and returns; nothing is read back.  A call may be captured in a CUDA graph
+ * read and write is memory of the pool's DEVICE, bookkeeping included (another device's is refused): a
+ * call queues work on the library stream (attn_set_stream) and returns; nothing is read back.  A call may be captured in a CUDA graph
  * once a call of the same sizes has been made on that pool (it sizes the pool's workspace; a captured
  * call that would need more is refused).  Later calls of any size leave such a graph valid.
  *

@@ -185,3 +185,39 @@ def test_sinks_beyond_a_table_reach_no_kernel(host, sinks):
     assert host.lib.kv_pages_trim(pool, a, 1, 2**31 - 1, 5) == 0
     assert (host.get("fake_window"), host.get("fake_sinks")) == (2**31 - 1, 5)
     host.lib.kv_pages_release(pool)
+
+
+def test_memory_of_another_device_is_refused(host):
+    """Every pointer of every call, before anything is launched."""
+    lib, a = host.lib, VP(host.at)
+    foreign = VP((ctypes.addressof((ctypes.c_char * 64).in_dll(lib, "fake_foreign")) + 15) & ~15)
+    pool, launches = host.pool(), host.get("fake_launches")
+    one, scale = ctypes.c_longlong(128), ctypes.c_float(1.0)
+
+    def each(call, *names):
+        """call(*pointers) with each pointer in turn on the other device."""
+        for i, name in enumerate(names):
+            args = [a] * len(names)
+            args[i] = foreign
+            assert call(*args), name
+            assert f"{name} is on device 1".encode() in lib.fake_error()
+        assert host.get("fake_launches") == launches
+        assert not call(*[a] * len(names))
+        host.set("fake_launches", launches)
+
+    each(lambda s, c: lib.kv_pages_extend(pool, s, c, 1), "seqs", "counts")
+    each(lambda s, d: lib.kv_pages_fork(pool, s, d, 1), "src", "dst")
+    each(lambda s, d: lib.kv_pages_copy(pool, s, d, 1), "src", "dst")
+    each(lambda s: lib.kv_pages_free(pool, s, 1), "seqs")
+    each(lambda s: lib.kv_pages_trim(pool, s, 1, 1, 0), "seqs")
+    each(lambda s: lib.kv_pages_compact(pool, s), "live_out")
+    each(lambda s, t, k, v: lib.kv_pages_write(pool, 0, s, t, 1, 1, k, v, 1, one), "seqs", "starts", "k_new", "v_new")
+    each(lambda q, s, o: lib.attention_pages_prefix_gqa(q, one, pool, 0, s, 2, 2, 0, 64, o, 1, scale), "q", "seqs", "output")
+    each(lambda q, s, t, o: lib.attention_pages_window_gqa(q, one, pool, 0, s, t, 1, 2, 2, 2, 64, 0, 0, o, 1, scale), "q", "seqs", "starts",
+         "output")
+    for i, name in enumerate(("k", "v", "table", "len", "ref")):
+        args = [a] * 5
+        args[i] = foreign
+        assert not lib.kv_pages_attach(*args, 1, 8, 16, 2, 64, 3, 4, 1)
+        assert f"{name} is on device 1".encode() in lib.fake_error()
+    lib.kv_pages_release(pool)

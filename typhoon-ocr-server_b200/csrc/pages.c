@@ -144,8 +144,10 @@ static tyb_pages *pages_from(const KVPages *p, const char *what)
     return t;
 }
 
-/* Device memory, `align` bytes aligned; 1 when so. */
-static int on_device(const void *p, size_t align, const char *name, const char *what)
+/* Memory of `device` (TYB_CURRENT: the current one), `align` bytes aligned; 1 when so.  (Another device's would be a fault, or a way over the
+ * link for every access.) */
+#define TYB_CURRENT (-1)
+static int on_device(const void *p, size_t align, int device, const char *name, const char *what)
 {
     if (!p) {
         tyb_set_error("%s: NULL %s", what, name);
@@ -155,9 +157,23 @@ static int on_device(const void *p, size_t align, const char *name, const char *
         tyb_set_error("%s: %s %p is not %zu-byte aligned", what, name, p, align);
         return 0;
     }
-    const int d = tyb_is_device_ptr(p);
-    if (d == 0) tyb_set_error("%s: %s is not device memory", what, name);
-    return d == 1;
+    if (device == TYB_CURRENT && !tyb_cuda_ok(cudaGetDevice(&device), what)) return 0;
+    struct cudaPointerAttributes at;
+    const cudaError_t e = cudaPointerGetAttributes(&at, p);
+    if (e != cudaSuccess) {
+        cudaGetLastError(); /* not for later calls */
+        tyb_set_error("%s: %s: %s", what, name, cudaGetErrorString(e));
+        return 0;
+    }
+    if (at.type != cudaMemoryTypeDevice && at.type != cudaMemoryTypeManaged) {
+        tyb_set_error("%s: %s is not device memory", what, name);
+        return 0;
+    }
+    if (at.type == cudaMemoryTypeDevice && at.device != device) {
+        tyb_set_error("%s: %s is on device %d, the pool on device %d", what, name, at.device, device);
+        return 0;
+    }
+    return 1;
 }
 
 static int check_dims(const KVPages *p, const char *what)
@@ -267,8 +283,9 @@ KVPages *kv_pages_attach(void *k, void *v, int *table, int *len, int *ref, int n
     const char *what = "kv_pages_attach";
     const KVPages d = {k, v, table, len, ref, num_layers, num_pages, page_size, kv_heads, head_dim, max_seqs, max_pages,
                        kv_dtype};
-    if (!check_dims(&d, what) || !on_device(k, 16, "k", what) || !on_device(v, 16, "v", what) ||
-        !on_device(table, 4, "table", what) || !on_device(len, 4, "len", what) || !on_device(ref, 4, "ref", what))
+    if (!check_dims(&d, what) || !on_device(k, 16, TYB_CURRENT, "k", what) || !on_device(v, 16, TYB_CURRENT, "v", what) ||
+        !on_device(table, 4, TYB_CURRENT, "table", what) || !on_device(len, 4, TYB_CURRENT, "len", what) ||
+        !on_device(ref, 4, TYB_CURRENT, "ref", what))
         return NULL;
     tyb_pages *t = make(&d, 0, what);
     if (t && !tyb_cuda_ok(tyb_pages_maps(&t->pub, t->maps), what)) {
@@ -290,7 +307,7 @@ void kv_pages_release(KVPages *p)
 /* ---- maintenance --------------------------------------------------------------------------- */
 
 /* A list of n device ints; 1 when there is one to work on, 0 when the call is done (*rc says how). */
-static int list_ready(const int *list, int n, const char *name, int *rc, const char *what)
+static int list_ready(const tyb_pages *t, const int *list, int n, const char *name, int *rc, const char *what)
 {
     *rc = 1;
     if (n < 0) {
@@ -301,7 +318,7 @@ static int list_ready(const int *list, int n, const char *name, int *rc, const c
         *rc = 0;
         return 0;
     }
-    return on_device(list, 4, name, what);
+    return on_device(list, 4, t->env.device, name, what);
 }
 
 /* Ends a call that holds the pool's lock. */
@@ -324,8 +341,8 @@ int kv_pages_extend(KVPages *p, const int *seqs, const int *counts, int n)
     int rc;
     tyb_pages *t = pages_from(p, what);
     if (!t) return 1;
-    if (!list_ready(seqs, n, "seqs", &rc, what)) return rc;
-    if (!on_device(counts, 4, "counts", what)) return 1;
+    if (!list_ready(t, seqs, n, "seqs", &rc, what)) return rc;
+    if (!on_device(counts, 4, t->env.device, "counts", what)) return 1;
     pthread_mutex_lock(&t->lock);
     void *ws = workspace(t, WS_SCRATCH, tyb_pages_plan_bytes(p, n), what);
     return ws ? launched(t, tyb_pages_extend_launch(p, &t->env, seqs, counts, n, ws, tyb_stream()), what) : not_launched(t);
@@ -336,8 +353,8 @@ static int fork_or_copy(KVPages *p, const int *src, const int *dst, int n, int d
     int rc;
     tyb_pages *t = pages_from(p, what);
     if (!t) return 1;
-    if (!list_ready(src, n, "src", &rc, what)) return rc;
-    if (!on_device(dst, 4, "dst", what)) return 1;
+    if (!list_ready(t, src, n, "src", &rc, what)) return rc;
+    if (!on_device(dst, 4, t->env.device, "dst", what)) return 1;
     pthread_mutex_lock(&t->lock);
     void *ws = workspace(t, WS_SCRATCH, tyb_pages_plan_bytes(p, n), what);
     return ws ? launched(t, tyb_pages_fork_launch(p, &t->env, src, dst, n, deep, ws, tyb_stream()), what) : not_launched(t);
@@ -353,7 +370,7 @@ int kv_pages_free(KVPages *p, const int *seqs, int n)
     int rc;
     tyb_pages *t = pages_from(p, what);
     if (!t) return 1;
-    if (!list_ready(seqs, n, "seqs", &rc, what)) return rc;
+    if (!list_ready(t, seqs, n, "seqs", &rc, what)) return rc;
     pthread_mutex_lock(&t->lock);
     const size_t bytes = tyb_pages_release_bytes(n);
     void *ws = bytes ? workspace(t, WS_SCRATCH, bytes, what) : NULL;
@@ -371,7 +388,7 @@ int kv_pages_trim(KVPages *p, const int *seqs, int n, int window, int sinks)
         tyb_set_error("%s: window %d must be at least 1 and sinks %d not negative", what, window, sinks);
         return 1;
     }
-    if (!list_ready(seqs, n, "seqs", &rc, what)) return rc;
+    if (!list_ready(t, seqs, n, "seqs", &rc, what)) return rc;
     /* more than a sequence can have keeps it all; the kernel rounds it up to pages in 32 bits */
     if (sinks > p->max_pages * p->page_size) sinks = p->max_pages * p->page_size;
     pthread_mutex_lock(&t->lock);
@@ -385,7 +402,7 @@ int kv_pages_compact(KVPages *p, int *live_out)
 {
     const char *what = "kv_pages_compact";
     tyb_pages *t = pages_from(p, what);
-    if (!t || (live_out && !on_device(live_out, 4, "live_out", what))) return 1;
+    if (!t || (live_out && !on_device(live_out, 4, t->env.device, "live_out", what))) return 1;
     pthread_mutex_lock(&t->lock);
     void *ws = workspace(t, WS_SCRATCH, tyb_pages_plan_bytes(p, 0), what);
     return ws ? launched(t, tyb_pages_compact_launch(p, live_out, ws, tyb_stream()), what) : not_launched(t);
@@ -399,7 +416,7 @@ static int check_layer(const KVPages *p, int layer, const char *what)
 }
 
 /* Rows of `width` elements, `stride` apart, in dtype: 16-byte accesses have to fit. */
-static int check_rows(const void *x, int dtype, long long stride, long long width, const char *name, const char *what)
+static int check_rows(const tyb_pages *t, const void *x, int dtype, long long stride, long long width, const char *name, const char *what)
 {
     if (dtype != ATTN_DT_F32 && dtype != ATTN_DT_BF16) {
         tyb_set_error("%s: unknown element type %d", what, dtype);
@@ -410,7 +427,7 @@ static int check_rows(const void *x, int dtype, long long stride, long long widt
                       stride, width);
         return 0;
     }
-    return on_device(x, 16, name, what);
+    return on_device(x, 16, t->env.device, name, what);
 }
 
 int kv_pages_write(KVPages *p, int layer, const int *seqs, const int *starts, int n, int rows, const void *k_new,
@@ -424,11 +441,11 @@ int kv_pages_write(KVPages *p, int layer, const int *seqs, const int *starts, in
         tyb_set_error("%s: rows %d out of range", what, rows);
         return 1;
     }
-    if (!list_ready(seqs, n, "seqs", &rc, what)) return rc;
+    if (!list_ready(t, seqs, n, "seqs", &rc, what)) return rc;
     if (rows == 0) return 0;
     const long long width = (long long)p->kv_heads * p->head_dim;
-    if (!on_device(starts, 4, "starts", what) || !check_rows(k_new, in_dtype, stride, width, "k_new", what) ||
-        !check_rows(v_new, in_dtype, stride, width, "v_new", what))
+    if (!on_device(starts, 4, t->env.device, "starts", what) || !check_rows(t, k_new, in_dtype, stride, width, "k_new", what) ||
+        !check_rows(t, v_new, in_dtype, stride, width, "v_new", what))
         return 1;
     pthread_mutex_lock(&t->lock);
     return launched(t, tyb_pages_write_launch(p, &t->env, layer, seqs, starts, n, rows, k_new, v_new, in_dtype == ATTN_DT_BF16, stride,
@@ -489,9 +506,11 @@ static int attend(const KVPages *p, tyb_pages_attn *a, const char *what)
         return 1;
     }
     if (a->batch == 0 || a->rows == 0) return 0;
-    if (!check_rows(a->q, a->io_bf16 ? ATTN_DT_BF16 : ATTN_DT_F32, a->q_stride, (long long)a->q_heads * p->head_dim, "q", what) ||
-        !on_device(a->out, 16, "output", what) || !on_device(a->seqs, 4, "seqs", what))
+    if (!check_rows(t, a->q, a->io_bf16 ? ATTN_DT_BF16 : ATTN_DT_F32, a->q_stride, (long long)a->q_heads * p->head_dim, "q", what) ||
+        !on_device(a->out, 16, t->env.device, "output", what) || !on_device(a->seqs, 4, t->env.device, "seqs", what))
         return 1;
+    const int tokens = a->max_new == 1 && a->rows == a->batch; /* one each: no starts */
+    if (!tokens && !on_device(a->starts, 4, t->env.device, "starts", what)) return 1;
     /* The shared pass takes whole pages: each sequence has its own copy of a partly filled one. */
     a->prefix -= a->prefix % p->page_size;
     a->p = *p;
@@ -535,8 +554,6 @@ int attention_pages_window_gqa(const void *q, long long q_stride, const KVPages 
 {
     const char *what = "attention_pages_window_gqa";
     if (!io_type(io_dtype, what)) return 1;
-    const int tokens = max_new == 1 && rows == batch;
-    if (!tokens && batch > 0 && rows > 0 && !on_device(starts, 4, "starts", what)) return 1;
     tyb_pages_attn a = {.layer = layer, .q = q, .q_stride = q_stride, .out = output, .io_bf16 = io_dtype == ATTN_DT_BF16,
                         .q_heads = q_heads, .seqs = seqs, .starts = starts, .batch = batch, .rows = rows,
                         .max_new = max_new, .max_len = max_len, .window = window, .sinks = sinks, .scale = scale};
