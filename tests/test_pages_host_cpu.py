@@ -107,14 +107,46 @@ def test_a_pools_workspace_is_its_own(host):
     host.lib.kv_pages_release(b)
 
 
-def test_growing_and_releasing_leave_nothing_behind(host):
-    before = host.lib.fake_live()
+def test_what_pools_give_back_serves_the_next(host):
+    """Outgrown and released buffers: some are kept for pools to come, after all work has ended, and no more than that."""
     pool = host.pool()
-    for n in (1, 30, 300, 2):
-        assert host.attend(pool, n) == 0
-    assert host.lib.fake_live() == before + 2
+    assert host.attend(pool, 4) == 0
+    mallocs, syncs = host.get("fake_mallocs"), host.get("fake_syncs")
     host.lib.kv_pages_release(pool)
-    assert host.lib.fake_live() == before
+    assert host.get("fake_syncs") > syncs
+    for _ in range(100):
+        pool, memsets = host.pool(), host.get("fake_memsets")
+        assert host.attend(pool, 4) == 0
+        assert host.get("fake_mallocs") == mallocs
+        assert host.get("fake_memsets") == memsets + 1  # the tickets
+        host.lib.kv_pages_release(pool)
+    pools = [host.pool() for _ in range(100)]  # all at once
+    for i, p in enumerate(pools):
+        assert host.attend(p, 1 + 5 * i) == 0
+    assert len({p.value for p in pools}) == 100 and host.lib.fake_live() >= 200
+    for p in pools:
+        host.lib.kv_pages_release(p)
+    left = host.lib.fake_live()
+    assert left < 40  # (what earlier tests captured is kept too)
+    for n in (1, 30, 300, 3000, 2, 9000):  # one that grows: its former buffers do not pile up
+        pool = host.pool()
+        assert host.attend(pool, n) == 0 and host.attend(pool, 2 * n) == 0
+        host.lib.kv_pages_release(pool)
+    assert host.lib.fake_live() <= left
+
+
+def test_a_spare_buffer_is_not_in_use_twice(host):
+    pools = [host.pool() for _ in range(6)]
+    for _ in range(3):
+        given = []
+        for p in pools:
+            assert host.attend(p, 4) == 0
+            given += [host.ws(), host.tickets()]
+        assert len(set(given)) == 12
+        host.lib.kv_pages_release(pools.pop())
+        pools.append(host.pool())
+    for p in pools:
+        host.lib.kv_pages_release(p)
 
 
 def test_a_capture_is_refused_what_it_would_have_to_allocate(host):

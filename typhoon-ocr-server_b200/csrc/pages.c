@@ -55,13 +55,81 @@ static int capturing(void)
     return state != cudaStreamCaptureStatusNone;
 }
 
+/* Buffers that no pool has any more, for the next one that needs such (an allocation and its return cost
+ * a new pool's first call about a millisecond).  No work uses them. */
+#define TYB_PAGES_SPARES 16
+#define TYB_PAGES_SPARE_BYTES ((size_t)256 << 20) /* in all */
+static pthread_mutex_t g_spare_lock = PTHREAD_MUTEX_INITIALIZER;
+static struct {
+    int device, kind;
+    void *p;
+    size_t bytes;
+} g_spare[TYB_PAGES_SPARES];
+static int g_spares;
+static size_t g_spare_bytes;
+
 static void give_back(tyb_pages *t, int kind)
 {
-    if (t->ws[kind].p && !t->ws[kind].captured) {
+    void *p = t->ws[kind].p;
+    if (p && !t->ws[kind].captured) {
         cudaDeviceSynchronize(); /* it may still be in use */
-        cudaFree(t->ws[kind].p);
+        pthread_mutex_lock(&g_spare_lock);
+        if (g_spares < TYB_PAGES_SPARES && g_spare_bytes + t->ws[kind].bytes <= TYB_PAGES_SPARE_BYTES) {
+            g_spare[g_spares].device = t->env.device;
+            g_spare[g_spares].kind = kind;
+            g_spare[g_spares].p = p;
+            g_spare[g_spares++].bytes = t->ws[kind].bytes;
+            g_spare_bytes += t->ws[kind].bytes;
+            p = NULL;
+        }
+        pthread_mutex_unlock(&g_spare_lock);
+        cudaFree(p);
     }
     memset(&t->ws[kind], 0, sizeof t->ws[kind]);
+}
+
+/* The smallest spare buffer of `bytes` to eight times as many for the pool; 0: there is none. */
+static int take_spare(tyb_pages *t, int kind, size_t bytes)
+{
+    int at = -1;
+    pthread_mutex_lock(&g_spare_lock);
+    for (int i = 0; i < g_spares; i++)
+        if (g_spare[i].device == t->env.device && g_spare[i].kind == kind && g_spare[i].bytes >= bytes && g_spare[i].bytes / 8 <= bytes &&
+            (at < 0 || g_spare[i].bytes < g_spare[at].bytes))
+            at = i;
+    if (at >= 0) {
+        t->ws[kind].p = g_spare[at].p;
+        t->ws[kind].bytes = g_spare[at].bytes;
+        g_spare_bytes -= g_spare[at].bytes;
+        g_spare[at] = g_spare[--g_spares];
+    }
+    pthread_mutex_unlock(&g_spare_lock);
+    return at >= 0;
+}
+
+/* Frees the current device's spare buffers; 0: there were none. */
+static int free_spares(int device)
+{
+    int freed = 0;
+    pthread_mutex_lock(&g_spare_lock);
+    for (int i = g_spares - 1; i >= 0; i--)
+        if (g_spare[i].device == device) {
+            cudaFree(g_spare[i].p);
+            g_spare_bytes -= g_spare[i].bytes;
+            g_spare[i] = g_spare[--g_spares];
+            freed = 1;
+        }
+    pthread_mutex_unlock(&g_spare_lock);
+    return freed;
+}
+
+/* A buffer of `bytes` for a pool that has none of the kind.  (What is spare may be what an allocation lacks.) */
+static int fetch(tyb_pages *t, int kind, size_t bytes, const char *what)
+{
+    if (take_spare(t, kind, bytes)) return 1;
+    if (!tyb_dev_alloc(&t->ws[kind].p, bytes, what) && !(free_spares(t->env.device) && tyb_dev_alloc(&t->ws[kind].p, bytes, what))) return 0;
+    t->ws[kind].bytes = bytes;
+    return 1;
 }
 
 /* The pool's buffer of a kind, its lock being held; tickets are zero to begin with.  NULL on failure (error
@@ -78,12 +146,9 @@ static void *workspace(tyb_pages *t, int kind, size_t bytes, const char *what)
             size_t want = t->ws[kind].bytes ? t->ws[kind].bytes : 1 << 18;
             while (want < bytes) want += want / 2;
             give_back(t, kind);
-            if (tyb_dev_alloc(&t->ws[kind].p, want, what)) {
-                t->ws[kind].bytes = want;
-                if (kind == WS_TICKETS &&
-                    !tyb_cuda_ok(cudaMemsetAsync(t->ws[kind].p, 0, want, (cudaStream_t)tyb_stream()), what))
-                    give_back(t, kind);
-            }
+            if (fetch(t, kind, want, what) && kind == WS_TICKETS &&
+                !tyb_cuda_ok(cudaMemsetAsync(t->ws[kind].p, 0, t->ws[kind].bytes, (cudaStream_t)tyb_stream()), what))
+                give_back(t, kind);
         }
     }
     if (t->ws[kind].bytes >= bytes) p = t->ws[kind].p;
