@@ -81,7 +81,8 @@ int kv_pages_trim(KVPages *p, const int *seqs, int n, int window, int sinks);
 int kv_pages_compact(KVPages *p, int *live_out);
 
 /* ---- attention --------------------------------------------------------------------------
- * Query head h reads KV head h / (q_heads / kv_heads); q_heads is a multiple of kv_heads, at most
+ * Queries and the rows in the pool are taken as they are: normalised and rotated by the caller where the
+ * model asks for it.  Query head h reads KV head h / (q_heads / kv_heads); q_heads is a multiple of kv_heads, at most
  * 16 times it.  q: token rows [..][q_heads][head_dim], rows q_stride elements apart; output
  * [..][q_heads][head_dim], contiguous; both in io_dtype (ATTN_DT_*).  Scores are scale * q . k; sums
  * and softmax statistics are FP32.  An ATTN_KV_BF16 pool multiplies BF16 operands (an FP32 query is

@@ -79,13 +79,15 @@ struct Layout {
 // rather than in the streaming one.  With 2 rows a sequence and up to 50 own rows, streaming / tcgen05 in microseconds:
 // 48 rows x 200 keys 20.5 / 23.5, 96 x 200 21.5 / 25.6; 16 x 1,024 20.1 / 17.4, 32 x 1,024 21.9 / 19.3, 96 x 1,024 28.2 /
 // 20.0; 32 x 4,096 25.8 / 24.2, 96 x 4,096 38.9 / 24.8; 12 x 16,384 34.6 / 38.7, 32 x 16,384 42.1 / 42.2, 48 x 16,384 59.9 / 42.5.
+// (The rule takes the shorter of the two everywhere but at 16 x 1,024.)
 constexpr int kTcSharedRows = 32, kTcSharedWork = 24576;
 
 // A shared pass on the tensor cores and the streaming of the sequences' own rows are bound by different things: they
 // run at the same time where that is estimated to be shorter.  In microseconds: a split of the pass its tiles; the
 // own rows (taken to be half of what max_len allows) what a CTA needs for a stage (an item's start and end take as
 // long as kItemUnits of them), or what the memory can deliver; each of the two 10 for its start and end.  Of the splits
-// tried, that picked the fastest or one within 1 % of it.  Measured, in turn / at the same time: 256 sequences behind 4,096
+// tried, that picked the fastest or one within 1 % of it.  (The prices are those of heads of 128 with two rows a sequence;
+// for others the split may not be the best.)  Measured, in turn / at the same time: 256 sequences behind 4,096
 // shared rows with up to 512 own ones 94 / 72, with up to 64 own ones 55 / 41, behind 1,024 85 / 68; 64 behind 4,096
 // 61 / 35; 512 behind 2,048 with up to 128 91 / 77; 128 behind 4,096 with up to 1,500 110 / 82.
 static void share_sms(const tyb_pages_attn* c, int tiles, int ctas, Layout* l)

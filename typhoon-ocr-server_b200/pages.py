@@ -1,8 +1,9 @@
 """The paged KV cache over torch tensors (include/kv_pages.h has the rules).
 
 A ``PagePool`` names tensors that the caller holds; every call queues work on torch's current
-stream (which becomes the calling thread's library stream) and returns.  ``attn_sync`` reports what
-only the device can see, a pool without enough free pages among it.
+stream (which becomes the calling thread's library stream, and stays it: static calls that belong on
+another set that again) and returns.  ``attn_sync`` reports what only the device can see, a pool
+without enough free pages among it.
 """
 
 from __future__ import annotations
