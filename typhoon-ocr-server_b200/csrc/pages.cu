@@ -396,21 +396,24 @@ struct Release {
 // A short list by one cluster: the CTAs look at all of it, tell each other whether it is right, and only then change
 // anything.  `team` warps to a sequence.  Up to as many sequences as it has warps; in one launch / in two, in microseconds
 // on the device: trim of 4, 32 and 256 sequences that has nothing to take 2.6, 2.8, 2.6 / 3.5, 3.6, 3.9; free of 32 and of 256
-// with up to 64 pages 2.8, 3.4 / 3.3, 4.0, of one with 4,096 3.1 / 6.0, of 256 with up to 512 5.8 / 4.0.
+// with up to 64 pages 2.9, 3.6 / 3.3, 4.0, of one with 4,096 3.3 / 6.0, of 256 with up to 512 6.0 / 4.0.
 constexpr int kTogether = 256;  // sequences, at most
 constexpr int kClusterCtas = 8, kClusterThreads = kTogether / kClusterCtas * 32;
 __global__ void __launch_bounds__(kClusterThreads) pages_release_kernel(const KVPages p, const int* seqs, int n, int team, const Release what, Status st)
 {
     __shared__ int wrong[kClusterCtas];
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // this CTA's shared memory is there
     after_predecessor();
     const int warp = (int)((blockIdx.x * kClusterThreads + threadIdx.x) >> 5), item = warp / team, first = warp % team * 32 + (int)(threadIdx.x & 31);
     const int s = item < n ? seqs[item] : -1;
     const int bad = __syncthreads_or(item < n && !what.right(p, s, first, team * 32));
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // and so is the others'
     if (threadIdx.x < kClusterCtas) {  // into every CTA's array
         uint32_t at;
         asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(&wrong[blockIdx.x])), "r"(threadIdx.x));
         asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(bad) : "memory");
     }
+    __syncwarp();  // (the barrier's aligned form wants the warp together)
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     int any = 0;
 #pragma unroll
